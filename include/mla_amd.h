@@ -322,6 +322,83 @@ int mla_q_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, int32
                     int32_t interleaved, void *pe_out, int64_t pe_stride_t, int64_t pe_stride_h,
                     void *nope_out, int64_t nope_stride_t, int64_t nope_stride_h, void *stream);
 
+/*
+ * Attention with per-head K and V of equal width, q_heads a multiple of kv_heads: query head h reads KV head
+ * h / (q_heads / kv_heads). bf16 in, fp32 accumulate, bf16 out plus fp32 natural-log LSE; head_dim 64 or 128. Query i of
+ * a request with E queries and L keys attends keys j <= L - E + i; one that attends no key gives out 0 and LSE -inf.
+ * Replaces the attention call of BaseAttnBackend.forward (python/minisgl/attention/base.py:19-22; FA template
+ * python/minisgl/attention/fa.py:48-65,157-182) for models with grouped heads.
+ *   q    [total_q, q_heads, head_dim] strides (q_stride_t, q_stride_h), 16-byte aligned, multiples of 8
+ *   k, v token row r, KV head h at k + r * k_row_stride + h * k_head_stride (v likewise), 16-byte aligned, non-negative
+ *        multiples of 8
+ *   out  [total_q, q_heads, head_dim] strides (out_stride_t, out_stride_h), 8-byte aligned, multiples of 4, either order
+ *   lse  [total_q, q_heads] fp32 (row stride lse_stride_t) or NULL
+ *   cu_seqlens_q [batch + 1], seq_lens_k [batch] int32 device arrays; offsets past total_q, lengths past the page
+ *        table's pt_cols * page_size tokens and page ids outside [0, num_pages) are cut or clamped, never followed.
+ *        Rows of q behind the last request are not read, and those of out and lse stay as they are.
+ * A value that no query of its request attends is never read (cache rows past a length may hold anything). Every value
+ * that one query of a request attends is multiplied into the others' rows with weight zero: it has to be finite.
+ *
+ * mla_gqa_prompt_bf16: whole prompts; k and v are packed like q (row cu_seqlens[b] + j), as many keys as queries.
+ */
+int mla_gqa_prompt_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_row_stride,
+                        int64_t k_head_stride, const void *v, int64_t v_row_stride, int64_t v_head_stride,
+                        const int32_t *cu_seqlens, int32_t batch, int32_t total_q, int32_t q_heads, int32_t kv_heads,
+                        int32_t head_dim, float scale, void *out, int64_t out_stride_t, int64_t out_stride_h,
+                        float *lse, int64_t lse_stride_t, void *stream);
+
+/*
+ * mla_gqa_chunk_bf16: each request's last E tokens (E from cu_seqlens_q, at most max_q; queries past max_q are left
+ * out) over its seq_lens_k[b] keys in a paged cache, any power-of-two page_size; row of key j: page_table[b, j /
+ * page_size] * page_size + j % page_size, for row strides that hold for the whole pool. Keys are split over the chip
+ * where there are few rows: `workspace` (16-byte aligned) holds the partial results, mla_gqa_workspace_bytes of it.
+ * Calls that overlap in time need workspaces of their own; nothing in one has to be kept or cleared between calls.
+ *
+ * mla_gqa_decode_bf16: the same with one token a request (query b is request b's last token).
+ */
+int mla_gqa_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t *bytes);
+
+int mla_gqa_chunk_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k_pool, int64_t k_row_stride,
+                       int64_t k_head_stride, const void *v_pool, int64_t v_row_stride, int64_t v_head_stride,
+                       int32_t num_pages, int32_t page_size, const int32_t *page_table, int32_t pt_cols,
+                       int64_t pt_stride, const int32_t *cu_seqlens_q, const int32_t *seq_lens_k, int32_t batch,
+                       int32_t total_q, int32_t max_q, int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale,
+                       void *workspace, int64_t workspace_bytes, void *out, int64_t out_stride_t, int64_t out_stride_h,
+                       float *lse, int64_t lse_stride_t, void *stream);
+
+int mla_gqa_decode_bf16(const void *q, int64_t q_stride_b, int64_t q_stride_h, const void *k_pool, int64_t k_row_stride,
+                        int64_t k_head_stride, const void *v_pool, int64_t v_row_stride, int64_t v_head_stride,
+                        int32_t num_pages, int32_t page_size, const int32_t *page_table, int32_t pt_cols,
+                        int64_t pt_stride, const int32_t *seq_lens, int32_t batch, int32_t q_heads, int32_t kv_heads,
+                        int32_t head_dim, float scale, void *workspace, int64_t workspace_bytes, void *out,
+                        int64_t out_stride_b, int64_t out_stride_h, float *lse, int64_t lse_stride_b, void *stream);
+
+/*
+ * The tables of a scheduler step from its requests' lengths, bit-exact, in one launch. Request b owns row table_idx[b]
+ * of the token table ([rows, cols] int32, one token location per column) and grows from cached_lens[b] = c to
+ * device_lens[b] = d tokens (cut to 0 <= c <= d <= cols). The first alloc_reqs requests take, in batch order, one entry
+ * of free_slots (page-aligned token locations) for each page first = ceil(c / page_size) .. ceil(d / page_size) - 1 of
+ * their row; the others (padding, whose rows are filled already) take none. Rows of requests that take pages are
+ * distinct. Written:
+ *   token_table[row, j * page_size + i] = slot + i of each page j taken (i < page_size, while inside cols)
+ *   page_table[b, j] = token_table[row, j * page_size] / page_size for j < ceil(d / page_size), 0 for further j < pt_cols
+ *   cu_seqlens_q[b] = sum over requests before b of d - c, and their sum in cu_seqlens_q[batch]
+ *   out_loc[cu_seqlens_q[b] + i] = token_table[row, c + i], positions[...] = c + i, for i < d - c (entries at and past
+ *                      total_new are not written)
+ *   *pages_taken = the free slots needed; if they are more than num_free, only this and cu_seqlens_q are written.
+ * max_extend bounds d - c (tokens past it may be left out), pt_cols * page_size should hold the longest d. Any
+ * page_size. Replaces CacheManager.allocate_paged and the scheduler's slot and position gathers
+ * (python/minisgl/scheduler/cache.py:42-53,119-161, scheduler/scheduler.py:198-214) with the page table of
+ * python/minisgl/attention/fa.py:84-97.
+ */
+int mla_page_tables_from_lengths(int32_t *token_table, int32_t token_table_rows, int32_t token_table_cols,
+                                 int64_t token_table_stride, const int32_t *table_idx, const int32_t *cached_lens,
+                                 const int32_t *device_lens, int32_t batch, int32_t alloc_reqs,
+                                 const int32_t *free_slots, int32_t num_free, int32_t page_size, int32_t max_extend,
+                                 int32_t *page_table, int32_t pt_cols, int64_t pt_stride, int32_t *out_loc,
+                                 int32_t *positions, int32_t total_new, int32_t *cu_seqlens_q, int32_t *pages_taken,
+                                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

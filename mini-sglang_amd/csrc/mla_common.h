@@ -152,4 +152,27 @@ hipError_t launch_q_rope(const void* q, int64_t qst, int64_t qsh, int32_t tokens
                          const float* cos_sin, int32_t max_pos, int32_t interleaved, void* pe, int64_t pst, int64_t psh,
                          void* nope, int64_t nst, int64_t nsh, hipStream_t stream);
 
+// Tables of a scheduler step (mla_tables.hip).
+struct PageTablesParams {
+  int32_t* token_table;
+  int32_t tt_rows, tt_cols;
+  int64_t tt_stride;
+  const int32_t* table_idx;
+  const int32_t* cached_lens;
+  const int32_t* device_lens;
+  int32_t batch, alloc_reqs;
+  const int32_t* free_slots;
+  int32_t num_free;
+  int32_t page_size, log2_ps;  // log2_ps < 0: not a power of two
+  int32_t* page_table;
+  int32_t pt_cols;
+  int64_t pt_stride;
+  int32_t* out_loc;
+  int32_t* positions;
+  int32_t total_new;
+  int32_t* cu_seqlens_q;
+  int32_t* pages_taken;
+};
+hipError_t launch_page_tables(const PageTablesParams& p, int32_t max_extend, hipStream_t stream);
+
 }  // namespace mla

@@ -1,0 +1,240 @@
+// extern "C" entry points of the grouped-head attention and of the step's tables (declared in include/mla_amd.h):
+// argument checks, the choice of kernel, and launches.
+#include <math.h>
+
+#include "mla_gqa.h"
+
+namespace mla {
+namespace {
+
+int done(hipError_t e, const char* who) {
+  if (e != hipSuccess) return api_error(MLA_ERR_HIP, "%s: %s", who, hipGetErrorString(e));
+  api_error(MLA_OK, "%s", "");
+  return MLA_OK;
+}
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
+
+// Requests of up to this many rows (tokens times group) are streamed: their attention is bound by reading K and V.
+constexpr int kStreamRows = 64;
+// Items that a batch is cut into (mla_gqa.h), about: of a streamed batch, and of one in blocks of 128 rows.
+constexpr int kStreamTarget = 1024;
+constexpr int kRowsTarget = 512;
+// A chunk batch of at least this many blocks fills the chip without cutting keys.
+constexpr int kRowsEnough = 1024;
+constexpr int kRowsBlock = 128;
+
+int stream_rows(int64_t most) { return most <= 16 ? 16 : most <= 32 ? 32 : 64; }
+
+int64_t workspace_floats(int64_t most, int dim) {
+  const bool stream = most <= kStreamRows;
+  return 2 * (int64_t)(stream ? kStreamTarget : kRowsTarget) * (stream ? stream_rows(most) : kRowsBlock) * (dim + 1);
+}
+
+int check_heads(const char* who, int32_t q_heads, int32_t kv_heads, int32_t dim) {
+  if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: %d query heads are no multiple of %d KV heads", who, q_heads, kv_heads);
+  if (dim != 64 && dim != 128) return api_error(MLA_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128, got %d", who, dim);
+  return MLA_OK;
+}
+
+// What all three attention entry points check; fills p but for the keys' addressing.
+int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                     int64_t k_row_stride, int64_t k_head_stride, const void* v, int64_t v_row_stride,
+                     int64_t v_head_stride, int32_t batch, int32_t total_q, int32_t q_heads, int32_t kv_heads,
+                     int32_t dim, float scale, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                     int64_t lse_stride_t) {
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: q, k and v must be 16-byte and out 8-byte aligned", who);
+  if (q_stride_t % 8 || q_stride_h % 8 || q_stride_t < 0 || q_stride_h < 0)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: q strides (%lld, %lld) must be non-negative multiples of 8", who,
+                     (long long)q_stride_t, (long long)q_stride_h);
+  if (k_row_stride % 8 || k_head_stride % 8 || v_row_stride % 8 || v_head_stride % 8 || k_row_stride < 0 ||
+      k_head_stride < 0 || v_row_stride < 0 || v_head_stride < 0)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: k and v strides must be non-negative multiples of 8", who);
+  // rows of out must not overlap, tokens outside heads or heads outside tokens
+  const bool by_token = (q_heads == 1 || out_stride_h >= dim) && (total_q == 1 || out_stride_t >= (q_heads - 1) * out_stride_h + dim);
+  const bool by_head = (total_q == 1 || out_stride_t >= dim) && (q_heads == 1 || out_stride_h >= (total_q - 1) * out_stride_t + dim);
+  if (out_stride_t % 4 || out_stride_h % 4 || out_stride_t < 0 || out_stride_h < 0 || !(by_token || by_head))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: out strides (%lld, %lld) must be multiples of 4 and hold %d tokens of %d heads of %d",
+                     who, (long long)out_stride_t, (long long)out_stride_h, total_q, q_heads, dim);
+  if (lse != nullptr && total_q > 1 && lse_stride_t < q_heads)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: lse_stride_t %lld < %d heads", who, (long long)lse_stride_t, q_heads);
+  if (!(scale > 0.f) || !isfinite(scale)) return api_error(MLA_ERR_INVALID_ARG, "%s: bad scale", who);
+  if ((int64_t)total_q * q_heads > 0x7fffffff) return api_error(MLA_ERR_UNSUPPORTED, "%s: total_q * q_heads passes 2^31", who);
+  p.q = static_cast<const __bf16*>(q);
+  p.q_stride_t = q_stride_t;
+  p.q_stride_h = q_stride_h;
+  p.k = static_cast<const __bf16*>(k);
+  p.k_row_stride = k_row_stride;
+  p.k_head_stride = k_head_stride;
+  p.v = static_cast<const __bf16*>(v);
+  p.v_row_stride = v_row_stride;
+  p.v_head_stride = v_head_stride;
+  p.batch = batch;
+  p.total_q = total_q;
+  p.kv_heads = kv_heads;
+  p.group = q_heads / kv_heads;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.out = static_cast<__bf16*>(out);
+  p.out_stride_t = out_stride_t;
+  p.out_stride_h = out_stride_h;
+  p.lse = lse;
+  p.lse_stride_t = lse_stride_t;
+  return MLA_OK;
+}
+
+int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
+          int64_t k_row_stride, int64_t k_head_stride, const void* v_pool, int64_t v_row_stride, int64_t v_head_stride,
+          int32_t num_pages, int32_t page_size, const int32_t* page_table, int32_t pt_cols, int64_t pt_stride,
+          const int32_t* cu_seqlens_q, const int32_t* seq_lens_k, int32_t batch, int32_t total_q, int32_t max_q,
+          int32_t q_heads, int32_t kv_heads, int32_t dim, float scale, void* workspace, int64_t workspace_bytes,
+          void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse, int64_t lse_stride_t, void* stream) {
+  if (batch < 0 || total_q < 0 || max_q < 0)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: batch %d, total_q %d, max_q %d", who, batch, total_q, max_q);
+  if (int rc = check_heads(who, q_heads, kv_heads, dim)) return rc;
+  if (batch == 0 || total_q == 0 || max_q == 0) return done(hipSuccess, who);
+  if (page_table == nullptr || seq_lens_k == nullptr || workspace == nullptr)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (!is_pow2(page_size)) return api_error(MLA_ERR_UNSUPPORTED, "%s: page_size %d must be a power of two", who, page_size);
+  if (num_pages < 1 || pt_cols < 1 || (batch > 1 && pt_stride < pt_cols))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: num_pages %d, pt_cols %d, pt_stride %lld", who, num_pages, pt_cols, (long long)pt_stride);
+  GqaParams p = {};
+  if (int rc = attention_params(who, p, q, q_stride_t, q_stride_h, k_pool, k_row_stride, k_head_stride, v_pool,
+                                v_row_stride, v_head_stride, batch, total_q, q_heads, kv_heads, dim, scale, out,
+                                out_stride_t, out_stride_h, lse, lse_stride_t))
+    return rc;
+  const int64_t most = (int64_t)max_q * p.group;  // rows of a request and KV head
+  const int64_t need = 4 * workspace_floats(most, dim);
+  if (!aligned(workspace, 16) || workspace_bytes < need)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
+                     (long long)need, (long long)workspace_bytes);
+  p.num_pages = num_pages;
+  for (p.log2_ps = 0; (1 << p.log2_ps) < page_size;) ++p.log2_ps;
+  p.page_table = page_table;
+  p.pt_stride = pt_stride;
+  const int64_t keys = (int64_t)pt_cols * page_size;
+  p.max_keys = (int32_t)(keys < 0x7fff0000 ? keys : 0x7fff0000);
+  p.cu_seqlens_q = cu_seqlens_q;
+  p.seq_lens_k = seq_lens_k;
+  p.max_q = max_q;
+  const bool stream_kernel = most <= kStreamRows;
+  const int64_t blocks = ((int64_t)total_q * p.group + kRowsBlock - 1) / kRowsBlock * kv_heads;
+  p.target = stream_kernel ? kStreamTarget : blocks >= kRowsEnough ? 0 : kRowsTarget;
+  p.ws_o = static_cast<float*>(workspace);
+  p.ws_lse = p.ws_o + workspace_floats(most, dim) / (dim + 1) * dim;
+  return done(stream_kernel ? launch_gqa_stream(p, dim, (hipStream_t)stream) : launch_gqa_rows(p, dim, (hipStream_t)stream), who);
+}
+
+}  // namespace
+}  // namespace mla
+
+extern "C" {
+
+int mla_gqa_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int64_t* bytes) {
+  const char* who = "mla_gqa_workspace_bytes";
+  if (bytes == nullptr || max_q < 0) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: bytes is null or max_q %d < 0", who, max_q);
+  if (int rc = mla::check_heads(who, q_heads, kv_heads, head_dim)) return rc;
+  *bytes = 4 * mla::workspace_floats((int64_t)max_q * (q_heads / kv_heads), head_dim);
+  return mla::done(hipSuccess, who);
+}
+
+int mla_gqa_prompt_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_row_stride,
+                        int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride,
+                        const int32_t* cu_seqlens, int32_t batch, int32_t total_q, int32_t q_heads, int32_t kv_heads,
+                        int32_t head_dim, float scale, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                        int64_t lse_stride_t, void* stream) {
+  const char* who = "mla_gqa_prompt_bf16";
+  if (batch < 0 || total_q < 0) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: batch %d, total_q %d", who, batch, total_q);
+  if (int rc = mla::check_heads(who, q_heads, kv_heads, head_dim)) return rc;
+  if (batch == 0 || total_q == 0) return mla::done(hipSuccess, who);
+  if (cu_seqlens == nullptr) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  mla::GqaParams p = {};
+  if (int rc = mla::attention_params(who, p, q, q_stride_t, q_stride_h, k, k_row_stride, k_head_stride, v, v_row_stride,
+                                     v_head_stride, batch, total_q, q_heads, kv_heads, head_dim, scale, out,
+                                     out_stride_t, out_stride_h, lse, lse_stride_t))
+    return rc;
+  p.max_keys = total_q;
+  p.cu_seqlens_q = cu_seqlens;
+  p.max_q = total_q;
+  return mla::done(mla::launch_gqa_rows(p, head_dim, (hipStream_t)stream), who);
+}
+
+int mla_gqa_chunk_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool, int64_t k_row_stride,
+                       int64_t k_head_stride, const void* v_pool, int64_t v_row_stride, int64_t v_head_stride,
+                       int32_t num_pages, int32_t page_size, const int32_t* page_table, int32_t pt_cols,
+                       int64_t pt_stride, const int32_t* cu_seqlens_q, const int32_t* seq_lens_k, int32_t batch,
+                       int32_t total_q, int32_t max_q, int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale,
+                       void* workspace, int64_t workspace_bytes, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                       float* lse, int64_t lse_stride_t, void* stream) {
+  const char* who = "mla_gqa_chunk_bf16";
+  if (batch > 0 && total_q > 0 && max_q > 0 && cu_seqlens_q == nullptr)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  return mla::paged(who, q, q_stride_t, q_stride_h, k_pool, k_row_stride, k_head_stride, v_pool, v_row_stride,
+                    v_head_stride, num_pages, page_size, page_table, pt_cols, pt_stride, cu_seqlens_q, seq_lens_k, batch,
+                    total_q, max_q < total_q ? max_q : total_q, q_heads, kv_heads, head_dim, scale, workspace,
+                    workspace_bytes, out, out_stride_t, out_stride_h, lse, lse_stride_t, stream);
+}
+
+int mla_gqa_decode_bf16(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_pool, int64_t k_row_stride,
+                        int64_t k_head_stride, const void* v_pool, int64_t v_row_stride, int64_t v_head_stride,
+                        int32_t num_pages, int32_t page_size, const int32_t* page_table, int32_t pt_cols,
+                        int64_t pt_stride, const int32_t* seq_lens, int32_t batch, int32_t q_heads, int32_t kv_heads,
+                        int32_t head_dim, float scale, void* workspace, int64_t workspace_bytes, void* out,
+                        int64_t out_stride_b, int64_t out_stride_h, float* lse, int64_t lse_stride_b, void* stream) {
+  return mla::paged("mla_gqa_decode_bf16", q, q_stride_b, q_stride_h, k_pool, k_row_stride, k_head_stride, v_pool,
+                    v_row_stride, v_head_stride, num_pages, page_size, page_table, pt_cols, pt_stride, nullptr, seq_lens,
+                    batch, batch, 1, q_heads, kv_heads, head_dim, scale, workspace, workspace_bytes, out, out_stride_b,
+                    out_stride_h, lse, lse_stride_b, stream);
+}
+
+int mla_page_tables_from_lengths(int32_t* token_table, int32_t token_table_rows, int32_t token_table_cols,
+                                 int64_t token_table_stride, const int32_t* table_idx, const int32_t* cached_lens,
+                                 const int32_t* device_lens, int32_t batch, int32_t alloc_reqs,
+                                 const int32_t* free_slots, int32_t num_free, int32_t page_size, int32_t max_extend,
+                                 int32_t* page_table, int32_t pt_cols, int64_t pt_stride, int32_t* out_loc,
+                                 int32_t* positions, int32_t total_new, int32_t* cu_seqlens_q, int32_t* pages_taken,
+                                 void* stream) {
+  const char* who = "mla_page_tables_from_lengths";
+  if (batch < 1 || batch > 65535 || alloc_reqs < 0 || alloc_reqs > batch || num_free < 0 || max_extend < 0 || total_new < 0 || pt_cols < 0)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: batch %d (1 to 65535), alloc_reqs %d, num_free %d, max_extend %d, total_new %d, pt_cols %d",
+                          who, batch, alloc_reqs, num_free, max_extend, total_new, pt_cols);
+  if (page_size < 1 || page_size > (1 << 20)) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: page_size %d must be in [1, 2^20]", who, page_size);
+  if (token_table == nullptr || table_idx == nullptr || cached_lens == nullptr || device_lens == nullptr ||
+      cu_seqlens_q == nullptr || pages_taken == nullptr || (num_free > 0 && free_slots == nullptr) ||
+      (pt_cols > 0 && page_table == nullptr) || (total_new > 0 && (out_loc == nullptr || positions == nullptr)))
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (token_table_rows < 1 || token_table_cols < 1 || token_table_cols > (1 << 30) || token_table_stride < token_table_cols)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: token table of %d x %d, stride %lld", who, token_table_rows,
+                          token_table_cols, (long long)token_table_stride);
+  if (batch > 1 && pt_stride < pt_cols)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: pt_stride %lld < %d columns", who, (long long)pt_stride, pt_cols);
+  mla::PageTablesParams p;
+  p.token_table = token_table;
+  p.tt_rows = token_table_rows;
+  p.tt_cols = token_table_cols;
+  p.tt_stride = token_table_stride;
+  p.table_idx = table_idx;
+  p.cached_lens = cached_lens;
+  p.device_lens = device_lens;
+  p.batch = batch;
+  p.alloc_reqs = alloc_reqs;
+  p.free_slots = free_slots;
+  p.num_free = num_free;
+  p.page_size = page_size;
+  p.log2_ps = -1;
+  if (mla::is_pow2(page_size)) for (p.log2_ps = 0; (1 << p.log2_ps) < page_size;) ++p.log2_ps;
+  p.page_table = page_table;
+  p.pt_cols = pt_cols;
+  p.pt_stride = pt_stride;
+  p.out_loc = out_loc;
+  p.positions = positions;
+  p.total_new = total_new;
+  p.cu_seqlens_q = cu_seqlens_q;
+  p.pages_taken = pages_taken;
+  return mla::done(mla::launch_page_tables(p, max_extend, (hipStream_t)stream), who);
+}
+
+}  // extern "C"

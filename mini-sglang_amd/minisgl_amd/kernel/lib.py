@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
-from typing import Tuple
+from typing import NamedTuple, Tuple
 
 import numpy as np
 
@@ -75,6 +75,27 @@ SIGNATURES = {
     "mla_q_rope_bf16": (
         ctypes.c_int,
         [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp],
+    ),
+    "mla_gqa_prompt_bf16": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i32, ctypes.c_float,
+         _vp, _i64, _i64, _vp, _i64, _vp],
+    ),
+    "mla_gqa_workspace_bytes": (ctypes.c_int, [_i32, _i32, _i32, _i32, ctypes.POINTER(_i64)]),
+    "mla_gqa_chunk_bf16": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i32, _i64, _vp, _vp, _i32, _i32, _i32,
+         _i32, _i32, _i32, ctypes.c_float, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
+    ),
+    "mla_gqa_decode_bf16": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i32, _i64, _vp, _i32, _i32, _i32, _i32,
+         ctypes.c_float, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
+    ),
+    "mla_page_tables_from_lengths": (
+        ctypes.c_int,
+        [_vp, _i32, _i32, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _i32, _i64, _vp, _vp, _i32,
+         _vp, _vp, _vp],
     ),
 }
 
@@ -494,3 +515,182 @@ def qkv_a_rows(qkv, q_rank: int, q_norm_weight, kv_norm_weight, positions, cos_s
         "mla_qkv_a_rows_bf16",
     )
     return out
+
+
+def _on_device(t, call):
+    """``call()`` with the device of tensor ``t`` current (launches and the current stream go by it)."""
+    import torch
+
+    if t.device.index == torch.cuda.current_device():
+        return call()
+    with torch.cuda.device(t.device):
+        return call()
+
+
+def _check_tensors(device, dtype, **tensors) -> None:
+    for name, t in tensors.items():
+        assert t.device == device and t.is_cuda, f"{name} must be on {device}, the other tensors' GPU"
+        assert t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}"
+
+
+def _check_gqa(q, k, v, heads_dim: int, out, lse) -> None:
+    import torch
+
+    assert q.dim() == 3 and k.dim() == v.dim() == heads_dim + 2, "q is [T, Hq, D]; k and v end in [Hkv, D]"
+    T, Hq, D = q.shape
+    Hkv = k.shape[-2]
+    assert k.shape == v.shape and k.shape[-1] == D and Hkv > 0 and Hq % Hkv == 0, "k, v: D as q's, heads that divide q's"
+    _check_tensors(q.device, torch.bfloat16, q=q, k=k, v=v, out=out)
+    assert q.stride(-1) == 1 and k.stride(-1) == 1 and v.stride(-1) == 1 and out.stride(-1) == 1, "rows must be contiguous"
+    assert out.shape == q.shape
+    if lse is not None:
+        _check_tensors(q.device, torch.float32, lse=lse)
+        assert lse.shape == (T, Hq) and lse.stride(-1) == 1
+
+
+def gqa_prompt(q, k, v, cu_seqlens, scale: float, out, lse=None, stream=None) -> None:
+    """Causal attention over whole prompts: packed ``q [T, Hq, D]``, ``k``, ``v [T, Hkv, D]`` (D 64 or 128; any strides
+    that are multiples of 8) of the sequences ``cu_seqlens [B + 1]`` -> ``out [T, Hq, D]`` (+ ``lse [T, Hq]``). Query
+    head h reads KV head ``h // (Hq // Hkv)``."""
+    import torch
+
+    _check_gqa(q, k, v, 1, out, lse)
+    assert k.shape[0] == q.shape[0], "as many keys as queries"
+    _check_tensors(q.device, torch.int32, cu_seqlens=cu_seqlens)
+    assert cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1 and cu_seqlens.is_contiguous()
+    T, Hq, D = q.shape
+    rc = _on_device(q, lambda: load_library().mla_gqa_prompt_bf16(
+        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+        v.stride(1), cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, T, Hq, k.shape[1], D, float(scale), out.data_ptr(),
+        out.stride(0), out.stride(1), _ptr(lse), 0 if lse is None else lse.stride(0), _stream(stream)))
+    if rc != 0:
+        check(rc, "mla_gqa_prompt_bf16")
+
+
+@functools.lru_cache(maxsize=None)
+def gqa_workspace_bytes(max_seqlen_q: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of the workspace that ``gqa_chunk`` (``gqa_decode``: ``max_seqlen_q`` 1) needs, at any batch and length."""
+    out = _i64(0)
+    check(load_library().mla_gqa_workspace_bytes(max_seqlen_q, q_heads, kv_heads, head_dim, ctypes.byref(out)),
+          "mla_gqa_workspace_bytes")
+    return int(out.value)
+
+
+def gqa_workspace(max_seqlen_q: int, q_heads: int, kv_heads: int, head_dim: int, device):
+    """A workspace for ``gqa_chunk`` / ``gqa_decode`` calls that do not overlap in time."""
+    import torch
+
+    return torch.empty((gqa_workspace_bytes(max_seqlen_q, q_heads, kv_heads, head_dim),), dtype=torch.uint8, device=device)
+
+
+def _check_paged(q, k_pool, v_pool, page_table, seq_lens, out, lse) -> None:
+    import torch
+
+    _check_gqa(q, k_pool, v_pool, 2, out, lse)
+    for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
+        assert t.stride(0) == t.shape[1] * t.stride(1), f"{name}'s pages must follow one another"
+    _check_tensors(q.device, torch.int32, page_table=page_table, seq_lens=seq_lens)
+    assert seq_lens.dim() == 1 and seq_lens.is_contiguous()
+    assert page_table.dim() == 2 and page_table.shape[0] >= seq_lens.shape[0] and page_table.stride(1) == 1
+
+
+def _workspace(workspace, nbytes: int, q, stream):
+    import torch
+
+    if workspace is None:  # from torch's allocator, for this call
+        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
+        if stream is not None:
+            workspace.record_stream(stream)
+    assert workspace.device == q.device and workspace.is_contiguous()
+    return workspace
+
+
+def gqa_chunk(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q: int, scale: float, out, lse=None,
+              workspace=None, stream=None) -> None:
+    """Attention of each request's new tokens over its pages of a K/V cache, causal over prefix and chunk:
+    ``q [T, Hq, D]`` packed by ``cu_seqlens_q [B + 1]``, ``k_pool``, ``v_pool [pages, ps, Hkv, D]`` (any power-of-two
+    ``ps``), ``page_table [B, cols]``, ``seq_lens_k [B]`` (prefix and chunk) -> ``out [T, Hq, D]`` (+ ``lse [T, Hq]``).
+    ``max_seqlen_q``: at least every request's new tokens. ``workspace``: of ``gqa_workspace``, or None to take one from
+    torch's allocator."""
+    import torch
+
+    _check_paged(q, k_pool, v_pool, page_table, seq_lens_k, out, lse)
+    _check_tensors(q.device, torch.int32, cu_seqlens_q=cu_seqlens_q)
+    B = seq_lens_k.shape[0]
+    assert cu_seqlens_q.shape == (B + 1,) and cu_seqlens_q.is_contiguous()
+    T, Hq, D = q.shape
+    Hkv = k_pool.shape[2]
+    ws = _workspace(workspace, gqa_workspace_bytes(min(max_seqlen_q, T), Hq, Hkv, D), q, stream)
+    rc = _on_device(q, lambda: load_library().mla_gqa_chunk_bf16(
+        q.data_ptr(), q.stride(0), q.stride(1), k_pool.data_ptr(), k_pool.stride(1), k_pool.stride(2), v_pool.data_ptr(),
+        v_pool.stride(1), v_pool.stride(2), k_pool.shape[0], k_pool.shape[1], page_table.data_ptr(), page_table.shape[1],
+        page_table.stride(0), cu_seqlens_q.data_ptr(), seq_lens_k.data_ptr(), B, T, max_seqlen_q, Hq, Hkv, D,
+        float(scale), ws.data_ptr(), ws.numel() * ws.element_size(), out.data_ptr(), out.stride(0), out.stride(1),
+        _ptr(lse), 0 if lse is None else lse.stride(0), _stream(stream)))
+    if rc != 0:
+        check(rc, "mla_gqa_chunk_bf16")
+
+
+def gqa_decode(q, k_pool, v_pool, page_table, seq_lens, scale: float, out, lse=None, workspace=None, stream=None) -> None:
+    """``gqa_chunk`` with one new token a request: ``q [B, Hq, D]`` -> ``out [B, Hq, D]`` (+ ``lse [B, Hq]``)."""
+    _check_paged(q, k_pool, v_pool, page_table, seq_lens, out, lse)
+    B, Hq, D = q.shape
+    assert seq_lens.shape[0] == B
+    Hkv = k_pool.shape[2]
+    ws = _workspace(workspace, gqa_workspace_bytes(1, Hq, Hkv, D), q, stream)
+    rc = _on_device(q, lambda: load_library().mla_gqa_decode_bf16(
+        q.data_ptr(), q.stride(0), q.stride(1), k_pool.data_ptr(), k_pool.stride(1), k_pool.stride(2), v_pool.data_ptr(),
+        v_pool.stride(1), v_pool.stride(2), k_pool.shape[0], k_pool.shape[1], page_table.data_ptr(), page_table.shape[1],
+        page_table.stride(0), seq_lens.data_ptr(), B, Hq, Hkv, D, float(scale), ws.data_ptr(),
+        ws.numel() * ws.element_size(), out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse),
+        0 if lse is None else lse.stride(0), _stream(stream)))
+    if rc != 0:
+        check(rc, "mla_gqa_decode_bf16")
+
+
+class PageTables(NamedTuple):
+    """A step's tables on the device (``page_tables_from_lengths``)."""
+
+    page_table: "torch.Tensor"  # int32 [B, ceil(max_device_len / ps)] page ids, 0 past a request's pages
+    out_loc: "torch.Tensor"  # int32 [T] token locations of the new tokens, in batch order
+    positions: "torch.Tensor"  # int32 [T] their positions
+    cu_seqlens_q: "torch.Tensor"  # int32 [B + 1]
+    pages_taken: "torch.Tensor"  # int32 [1] free slots used; more than there are: nothing but this and cu_seqlens_q is written
+
+
+def page_tables_from_lengths(token_table, table_idx, cached_lens, device_lens, free_slots, page_size: int,
+                             max_device_len: int, max_extend: int, total_new: int, alloc_reqs: int | None = None,
+                             stream=None) -> PageTables:
+    """The tables of a step whose requests grow from ``cached_lens`` to ``device_lens`` tokens (int32 ``[B]`` on the
+    device, like ``table_idx``, their rows of ``token_table [rows, cols]``): the first ``alloc_reqs`` requests (default
+    all) take the pages that their new tokens start, in batch order, from ``free_slots`` (page-aligned token locations),
+    which fills their token table rows; then every request's page table, and the new tokens' locations and positions.
+    ``max_device_len``, ``max_extend`` and ``total_new`` are the host's: the longest request, the most new tokens of one,
+    and of all. Rows of requests that take pages must be distinct. One launch; nothing is read back."""
+    import torch
+
+    _check_tensors(token_table.device, torch.int32, token_table=token_table, table_idx=table_idx, cached_lens=cached_lens,
+                   device_lens=device_lens, free_slots=free_slots)
+    B = table_idx.shape[0]
+    assert token_table.dim() == 2 and token_table.stride(1) == 1
+    assert table_idx.shape == cached_lens.shape == device_lens.shape == (B,) and free_slots.dim() == 1
+    for t in (table_idx, cached_lens, device_lens, free_slots):
+        assert t.is_contiguous()
+    cols = -(-max_device_len // page_size)
+    i32 = dict(dtype=torch.int32, device=token_table.device)
+    pt = torch.empty((B, cols), **i32)
+    loc_pos = torch.empty((2, total_new), **i32)
+    cu_taken = torch.empty((B + 2,), **i32)
+    tables = PageTables(pt, loc_pos[0], loc_pos[1], cu_taken[: B + 1], cu_taken[B + 1 :])
+    if stream is not None:
+        for t in (pt, loc_pos, cu_taken):
+            t.record_stream(stream)
+    rc = _on_device(token_table, lambda: load_library().mla_page_tables_from_lengths(
+        token_table.data_ptr(), token_table.shape[0], token_table.shape[1], token_table.stride(0), table_idx.data_ptr(),
+        cached_lens.data_ptr(), device_lens.data_ptr(), B, B if alloc_reqs is None else alloc_reqs, free_slots.data_ptr(),
+        free_slots.shape[0], page_size, max_extend, pt.data_ptr(), cols, cols, tables.out_loc.data_ptr(),
+        tables.positions.data_ptr(), total_new, tables.cu_seqlens_q.data_ptr(), tables.pages_taken.data_ptr(),
+        _stream(stream)))
+    if rc != 0:
+        check(rc, "mla_page_tables_from_lengths")
+    return tables

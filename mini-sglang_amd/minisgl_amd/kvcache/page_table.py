@@ -19,6 +19,8 @@ from typing import Iterable, List, Tuple
 
 import torch
 
+from ..kernel.lib import PageTables, page_tables_from_lengths
+
 
 class PagedTokenTable:
     def __init__(self, num_pages: int, page_size: int, page_table: torch.Tensor) -> None:
@@ -70,3 +72,24 @@ class PagedTokenTable:
         """Return the pages holding tokens ``[0, length)`` of a row (a finished request)."""
         if length > 0:
             self.free_slots = torch.cat((self.free_slots, self.page_table[table_idx, :length : self.page_size]))
+
+    def allocate_step(self, reqs: Iterable, padding: Iterable = ()) -> PageTables:
+        """``allocate_paged``, the batch's page table, ``out_loc``, positions and query offsets in one launch, from the
+        requests' lengths (one host-to-device copy of three integers a request). Requests of ``padding`` (a padded
+        batch's dummy) follow and take no pages. The rows of ``reqs`` must be distinct."""
+        reqs, ps = list(reqs), self.page_size
+        batch = reqs + list(padding)
+        assert len({r.table_idx for r in reqs}) == len(reqs), "requests that take pages have rows of their own"
+        needed = sum(-(-r.device_len // ps) - -(-r.cached_len // ps) for r in reqs)
+        if needed > self.free_pages:
+            raise RuntimeError(f"out of KV pages: {needed} needed, {self.free_pages} free")
+        width = self.page_table.shape[1]
+        assert all(r.device_len <= width for r in batch), f"a token table row holds {width} tokens"
+        host = torch.tensor([[r.table_idx for r in batch], [r.cached_len for r in batch], [r.device_len for r in batch]],
+                            dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        rows, cached, device = host.to(self.device, non_blocking=True)
+        tables = page_tables_from_lengths(
+            self.page_table, rows, cached, device, self.free_slots, ps, max(r.device_len for r in batch),
+            max(r.extend_len for r in batch), sum(r.extend_len for r in batch), len(reqs))
+        self.free_slots = self.free_slots[needed:]
+        return tables
