@@ -39,6 +39,7 @@ struct GqaParams {
   float* ws_o;    // [slots, rows, D] partial outputs of split requests, normalised
   float* ws_lse;  // [slots, rows] their log2-domain LSEs
   int32_t target;  // items that a batch's keys are split into, about (0: no splitting)
+  int32_t fit;     // at most `target`, where that can be
 };
 
 // A request as the kernels see it; every read is bounded by what the host knows, whatever the device arrays hold.
@@ -60,68 +61,85 @@ __device__ __forceinline__ GqaRequest gqa_request(const GqaParams& p, int b) {
   return r;
 }
 
-__device__ __forceinline__ int wave_isum(int v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+// Inclusive scan over the wave (lane 63 holds the whole): DPP row shifts, then row broadcasts; a ds_bpermute step
+// would wait out the LDS latency each time.
+template <typename T, typename F>
+__device__ __forceinline__ T wave_scan(T v, F&& f) {
+  static_assert(sizeof(T) == 4, "one register");
+  auto step = [&](auto ctrl, auto rows) {
+    const int w = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    v = f(v, __builtin_bit_cast(T, w));  // lanes without a source add the bits of 0
+  };
+  step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr:1
+  step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15 to rows 1 and 3
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31 to rows 2 and 3
   return v;
 }
-__device__ __forceinline__ int64_t wave_isum64(int64_t v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+__device__ __forceinline__ int wave_iscan(int v) {
+  return wave_scan(v, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ float wave_fsum_all(float v) {
+  v = wave_scan(v, [](float a, float b) { return a + b; });
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// Keys of a split: the batch's keys, weighted with the row blocks that read them, over `target` items, in whole tiles
-// of 64 and at least kMin. Requests of more keys are cut into ceil(L / C) pieces. Every kernel of a call computes the
-// same C from the same lengths, so no plan is made on the host and a captured launch follows its lengths.
-// Sum over split requests of their pieces: ceil(L / C) <= 2 L / C, so 2 target slots hold them all.
-constexpr int kGqaMinSplit = 256;
+// Keys of a piece, C: the batch's keys, weighted with the row blocks that read them, over `target` items, in whole tiles
+// of 64 and at least kGqaMinSplit; with `fit`, enlarged until the pieces are at most `target` (the CTAs that run at once:
+// one more piece would be a round of its own). Requests of more keys are cut into ceil(L / C) pieces. Every kernel of a
+// call computes the same C from the same lengths, so no plan is made on the host and a captured launch follows its
+// lengths. C is above cost / target (the sum's rounding included), so a batch has fewer than `target` pieces more than
+// blocks; a request in pieces has L > C, so ceil(L / C) <= 2 L / C, and 2 target slots hold every piece.
+constexpr int kGqaMinSplit = 128;  // a tile for each wave of the stream kernel
 template <int kRows>
-__device__ __forceinline__ int gqa_split_keys(const GqaParams& p) {
+__device__ __forceinline__ int gqa_blocks(const GqaParams& p, const GqaRequest& r) {
+  return (r.E * p.group + kRows - 1) / kRows;
+}
+__device__ __forceinline__ int gqa_pieces(int L, int C) { return L > C ? (L - 1) / C + 1 : 1; }
+// r: request `lane` (batches of more than 64 requests read the others here)
+template <int kRows>
+__device__ __forceinline__ int gqa_piece_keys(const GqaParams& p, const GqaRequest& r) {
   if (p.target <= 0) return 0x7fffffff;
   const int lane = threadIdx.x & 63;
-  int64_t cost = 0;
-  for (int c0 = 0; c0 < p.batch; c0 += 64) {
-    const int b = c0 + lane;
-    if (b < p.batch) {
-      const GqaRequest r = gqa_request(p, b);
-      cost += (int64_t)((r.E * p.group + kRows - 1) / kRows) * r.L;
+  auto cost_of = [&](const GqaRequest& x) { return (float)gqa_blocks<kRows>(p, x) * (float)x.L; };
+  float cost = lane < p.batch ? cost_of(r) : 0.f;
+  for (int b = 64 + lane; b < p.batch; b += 64) cost += cost_of(gqa_request(p, b));
+  const float c = wave_fsum_all(cost) * (float)p.kv_heads / (float)p.target * 1.0001f + 64.f;
+  int C = max(c < 2e9f ? (int)c & ~63 : 0x7fffffc0, kGqaMinSplit);
+  if (p.fit && p.batch <= 64) {
+    for (int i = 0; i < 4 && C < (1 << 24); ++i) {
+      const int n = lane < p.batch ? gqa_blocks<kRows>(p, r) * gqa_pieces(r.L, C) * p.kv_heads : 0;
+      const int items = __builtin_amdgcn_readlane(wave_iscan(n), 63);
+      if (items <= p.target) break;
+      C = ((int)((float)C * (float)items / (float)p.target) + 64) & ~63;
     }
   }
-  cost = wave_isum64(cost) * p.kv_heads;
-  const int64_t c = (cost / p.target + 64) / 64 * 64;  // above cost / target
-  return (int)min(max(c, (int64_t)kGqaMinSplit), (int64_t)0x7fffffc0);
+  return __builtin_amdgcn_readfirstlane(C);
 }
 
 // Item `item` of the batch: request, block of kRows rows, KV head, piece of the keys. Items of a request are
 // ((block, piece), head), heads fastest. slot: of the item's partial result, < 0 for a request in one piece.
 struct GqaItem {
-  int b, block, head, piece, pieces, slot;
+  int b, block, head, piece, pieces, C, slot;
   GqaRequest r;
 };
 template <int kRows>
-__device__ __forceinline__ bool gqa_find(const GqaParams& p, int C, int item, GqaItem& it) {
+__device__ __forceinline__ bool gqa_find(const GqaParams& p, int item, GqaItem& it) {
   const int lane = threadIdx.x & 63;
+  GqaRequest r{0, 0, 0, 0};
+  if (lane < p.batch) r = gqa_request(p, lane);
+  it.C = gqa_piece_keys<kRows>(p, r);
   int acc = 0, slots = 0;
   for (int c0 = 0; c0 < p.batch; c0 += 64) {
-    const int b = c0 + lane;
-    GqaRequest r{0, 0, 0, 0};
-    int n = 0, ns = 0, pieces = 1;
-    if (b < p.batch) {
-      r = gqa_request(p, b);
-      pieces = r.L > C ? (r.L + C - 1) / C : 1;
-      n = (r.E * p.group + kRows - 1) / kRows * pieces * p.kv_heads;
-      ns = pieces > 1 ? n : 0;
+    if (c0 > 0) {
+      r = GqaRequest{0, 0, 0, 0};
+      if (c0 + lane < p.batch) r = gqa_request(p, c0 + lane);
     }
-    int incl = n, sincl = ns;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(incl, o), w = __shfl_up(sincl, o);
-      if (lane >= o) {
-        incl += u;
-        sincl += w;
-      }
-    }
+    const int pieces = gqa_pieces(r.L, it.C);
+    const int n = gqa_blocks<kRows>(p, r) * pieces * p.kv_heads, ns = pieces > 1 ? n : 0;
+    const int incl = wave_iscan(n), sincl = wave_iscan(ns);
     const uint64_t hit = __ballot(item >= acc + incl - n && item < acc + incl);
     if (hit != 0) {
       const int fl = __builtin_ctzll(hit);
@@ -138,17 +156,18 @@ __device__ __forceinline__ bool gqa_find(const GqaParams& p, int C, int item, Gq
       it.r.P = __builtin_amdgcn_readlane(r.P, fl);
       return true;
     }
-    acc += __shfl(incl, 63);
-    slots += __shfl(sincl, 63);
+    acc += __builtin_amdgcn_readlane(incl, 63);
+    slots += __builtin_amdgcn_readlane(sincl, 63);
   }
   return false;
 }
 
-// Token row of key j of request b (packed prompts: q0 + j); page ids are clamped into the pool.
-__device__ __forceinline__ int64_t gqa_row(const GqaParams& p, int b, int q0, int j) {
+// Token row of key j of request b (packed prompts: q0 + j); page ids are clamped into the pool. The host keeps pools
+// below 2^31 rows.
+__device__ __forceinline__ int gqa_row(const GqaParams& p, int b, int q0, int j) {
   if (p.page_table == nullptr) return q0 + j;
   const int pid = min(max(p.page_table[(int64_t)b * p.pt_stride + (j >> p.log2_ps)], 0), p.num_pages - 1);
-  return ((int64_t)pid << p.log2_ps) + (j & ((1 << p.log2_ps) - 1));
+  return (pid << p.log2_ps) + (j & ((1 << p.log2_ps) - 1));
 }
 
 hipError_t launch_gqa_rows(const GqaParams& p, int dim, hipStream_t stream);    // many rows a request

@@ -17,8 +17,11 @@ bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
 // Requests of up to this many rows (tokens times group) are streamed: their attention is bound by reading K and V.
 constexpr int kStreamRows = 64;
-// Items that a batch is cut into (mla_gqa.h), about: of a streamed batch, and of one in blocks of 128 rows.
-constexpr int kStreamTarget = 1024;
+// Items that a batch is cut into (mla_gqa.h): of a streamed batch, kStreamFit (the CTAs that run at once, two a compute
+// unit) where it has at most half as many (block, head) pairs, else about kStreamTarget, so that pieces of different
+// length even out; of one in blocks of 128 rows, about kRowsTarget.
+constexpr int kStreamFit = 512;
+constexpr int kStreamTarget = 2048;
 constexpr int kRowsTarget = 512;
 // A chunk batch of at least this many blocks fills the chip without cutting keys.
 constexpr int kRowsEnough = 1024;
@@ -101,6 +104,8 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
   if (!is_pow2(page_size)) return api_error(MLA_ERR_UNSUPPORTED, "%s: page_size %d must be a power of two", who, page_size);
   if (num_pages < 1 || pt_cols < 1 || (batch > 1 && pt_stride < pt_cols))
     return api_error(MLA_ERR_INVALID_ARG, "%s: num_pages %d, pt_cols %d, pt_stride %lld", who, num_pages, pt_cols, (long long)pt_stride);
+  if ((int64_t)num_pages * page_size > 0x7fffffff)
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: a pool of %d pages of %d passes 2^31 rows", who, num_pages, page_size);
   GqaParams p = {};
   if (int rc = attention_params(who, p, q, q_stride_t, q_stride_h, k_pool, k_row_stride, k_head_stride, v_pool,
                                 v_row_stride, v_head_stride, batch, total_q, q_heads, kv_heads, dim, scale, out,
@@ -122,7 +127,12 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
   p.max_q = max_q;
   const bool stream_kernel = most <= kStreamRows;
   const int64_t blocks = ((int64_t)total_q * p.group + kRowsBlock - 1) / kRowsBlock * kv_heads;
-  p.target = stream_kernel ? kStreamTarget : blocks >= kRowsEnough ? 0 : kRowsTarget;
+  if (stream_kernel) {
+    p.fit = 2 * ((int64_t)batch * kv_heads) <= kStreamFit;
+    p.target = p.fit ? kStreamFit : kStreamTarget;
+  } else {
+    p.target = blocks >= kRowsEnough ? 0 : kRowsTarget;
+  }
   p.ws_o = static_cast<float*>(workspace);
   p.ws_lse = p.ws_o + workspace_floats(most, dim) / (dim + 1) * dim;
   return done(stream_kernel ? launch_gqa_stream(p, dim, (hipStream_t)stream) : launch_gqa_rows(p, dim, (hipStream_t)stream), who);

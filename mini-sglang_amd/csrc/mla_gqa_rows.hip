@@ -33,9 +33,9 @@ __global__ __launch_bounds__(256, 2) void gqa_rows_kernel(const GqaParams p) {
   __shared__ __attribute__((aligned(16))) char s_v[kStage * kRowB];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int C = gqa_split_keys<kRows>(p);
   GqaItem it;
-  if (!gqa_find<kRows>(p, C, blockIdx.x, it)) return;
+  if (!gqa_find<kRows>(p, blockIdx.x, it)) return;
+  const int C = it.C;
   const int E = it.r.E, L = it.r.L, P = it.r.P, G = p.group;
   const int c32 = lane & 31, g32 = lane >> 5;
   const int r = it.block * kRows + 32 * wave + c32;  // this lane's row
@@ -63,9 +63,9 @@ __global__ __launch_bounds__(256, 2) void gqa_rows_kernel(const GqaParams p) {
     __syncthreads();
     for (int i = threadIdx.x; i < kStage * kChunks; i += 256) {
       const int t = i / kChunks, c = i % kChunks;
-      const int64_t row = gqa_row(p, it.b, it.r.q0, min(t0 + t, L - 1));  // keys past the last repeat it
-      *reinterpret_cast<u32x4*>(s_k + t * kRowB + kchunk<D>(c, t) * 16) = *reinterpret_cast<const u32x4*>(kh + row * p.k_row_stride + c * 8);
-      *reinterpret_cast<u32x4*>(s_v + t * kRowB + vchunk<D>(c, t) * 16) = *reinterpret_cast<const u32x4*>(vh + row * p.v_row_stride + c * 8);
+      const int row = gqa_row(p, it.b, it.r.q0, min(t0 + t, L - 1));  // keys past the last repeat it
+      *reinterpret_cast<u32x4*>(s_k + t * kRowB + kchunk<D>(c, t) * 16) = *reinterpret_cast<const u32x4*>(kh + (int64_t)row * p.k_row_stride + c * 8);
+      *reinterpret_cast<u32x4*>(s_v + t * kRowB + vchunk<D>(c, t) * 16) = *reinterpret_cast<const u32x4*>(vh + (int64_t)row * p.v_row_stride + c * 8);
     }
     __syncthreads();
     f32x16_t s = f32x16_t{};

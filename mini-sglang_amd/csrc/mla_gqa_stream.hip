@@ -15,16 +15,16 @@ constexpr float kLowest = -3.4028234663852886e38f;
 
 // NB blocks of 16 rows
 template <int D, int NB>
-__global__ __launch_bounds__(256, 2) void gqa_stream_kernel(const GqaParams p) {
+__global__ __launch_bounds__(256, NB == 4 && D == 128 ? 1 : 2) void gqa_stream_kernel(const GqaParams p) {
   constexpr int kRows = 16 * NB, kRowB = D * 2, kChunks = D / 8, kKs = D / 32, kDb = D / 16;
-  constexpr int kVLoads = kTileKeys * kChunks / 64;  // 16-byte loads of a lane per V tile
-  __shared__ __attribute__((aligned(16))) char s_v[4][kTileKeys * kRowB];
+  constexpr int kLoads = kTileKeys * kChunks / 64;  // 16-byte loads of a lane per K or V tile
+  __shared__ __attribute__((aligned(16))) char s_k[4][kTileKeys * kRowB], s_v[4][kTileKeys * kRowB];
   __shared__ float s_m[4][16], s_l[4][16];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int C = gqa_split_keys<kRows>(p);
   GqaItem it;
-  if (!gqa_find<kRows>(p, C, blockIdx.x, it)) return;
+  if (!gqa_find<kRows>(p, blockIdx.x, it)) return;
+  const int C = it.C;
   const int E = it.r.E, L = it.r.L, P = it.r.P, G = p.group;
   const int a16 = lane & 15, g = lane >> 4;
   int limit[NB];
@@ -53,51 +53,58 @@ __global__ __launch_bounds__(256, 2) void gqa_stream_kernel(const GqaParams p) {
 #pragma unroll
     for (int db = 0; db < kDb; ++db) O[nb][db] = f32x4{};
   }
-  u32x4 kr[2][kKs], vr[kVLoads];
-  auto load = [&](int t0) __attribute__((always_inline)) {
-    // token t < 32 of the tile: its row is in lane t (keys past the last repeat it)
-    const int64_t row = gqa_row(p, it.b, it.r.q0, min(t0 + (lane & 31), L - 1));
-    const int lo = (int)row, hi = (int)(row >> 32);
-    auto row_of = [&](int t) { return (int64_t)(uint32_t)__shfl(lo, t) | (int64_t)__shfl(hi, t) << 32; };
+  // A tile is loaded row by row, 16 lanes (D 64: 8) to a row, and goes through the wave's own LDS tiles into the operand
+  // layouts: with loads straight into the K operand's (a 16-byte chunk of 16 rows each), 64 requests of 1k to 8k tokens, 8
+  // KV heads, took 263 us where this takes 231. Non-temporal, since a row is read once (257 us without). row: of token
+  // t < 32 of the tile in lane t.
+  u32x4 kr[kLoads], vr[kLoads];
+  auto rows = [&](int t0) __attribute__((always_inline)) { return gqa_row(p, it.b, it.r.q0, min(t0 + (lane & 31), L - 1)); };
+  auto load = [&](int row) __attribute__((always_inline)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const __bf16* src = kh + row_of(16 * h + a16) * p.k_row_stride + 8 * g;
-#pragma unroll
-      for (int ks = 0; ks < kKs; ++ks) kr[h][ks] = *reinterpret_cast<const u32x4*>(src + 32 * ks);
-    }
-#pragma unroll
-    for (int u = 0; u < kVLoads; ++u) {
-      const int i = u * 64 + lane;
-      vr[u] = *reinterpret_cast<const u32x4*>(vh + row_of(i / kChunks) * p.v_row_stride + i % kChunks * 8);
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t rw = __shfl(row, (u * 64 + lane) / kChunks);
+      const int c = lane % kChunks * 8;
+      kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + rw * p.k_row_stride + c));
+      vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + rw * p.v_row_stride + c));
     }
   };
-  // V chunk c (16 bytes) of token t: pairs of chunks permuted, so that the 8 tokens of a transposing read differ
-  auto vpos = [&](int t, int c) { return t * kRowB + (D == 128 ? c ^ (2 * (t & 7)) : c ^ (2 * ((t >> 1) & 3))) * 16; };
+  // 16-byte chunk c of token t: pairs of chunks permuted, so that neither the K reads (16 rows' chunks c and c + 1) nor
+  // the transposing V reads (8 rows' chunk pairs) meet in a bank
+  auto pos = [&](int t, int c) __attribute__((always_inline)) { return t * kRowB + (D == 128 ? c ^ (2 * (t & 7)) : c ^ (2 * ((t >> 1) & 3))) * 16; };
 
-  int t0 = k0 + kTileKeys * wave;
-  if (t0 < k1) load(t0);
-  for (; t0 < k1; t0 += 4 * kTileKeys) {
-    bf16x8 kc[2][kKs];
+  constexpr int kStep = 4 * kTileKeys;
+  int t0 = k0 + kTileKeys * wave, row_next = 0;
+  if (t0 < k1) {
+    const int row = rows(t0);
+    row_next = rows(t0 + kStep);
+    load(row);
+  }
+  for (; t0 < k1; t0 += kStep) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int ks = 0; ks < kKs; ++ks) kc[h][ks] = __builtin_bit_cast(bf16x8, kr[h][ks]);
-#pragma unroll
-    for (int u = 0; u < kVLoads; ++u) {
-      const int i = u * 64 + lane;
-      *reinterpret_cast<u32x4*>(s_v[wave] + vpos(i / kChunks, i % kChunks)) = vr[u];
+    for (int u = 0; u < kLoads; ++u) {
+      const int at = pos((u * 64 + lane) / kChunks, lane % kChunks);
+      *reinterpret_cast<u32x4*>(s_k[wave] + at) = kr[u];
+      *reinterpret_cast<u32x4*>(s_v[wave] + at) = vr[u];
     }
-    if (t0 + 4 * kTileKeys < k1) load(t0 + 4 * kTileKeys);
+    if (t0 + kStep < k1) load(row_next);
+    if (t0 + 2 * kStep < k1) row_next = rows(t0 + 2 * kStep);
+    f32x4 sc[NB][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bf16x8 kc[kKs];
+#pragma unroll
+      for (int ks = 0; ks < kKs; ++ks) kc[ks] = *reinterpret_cast<const bf16x8*>(s_k[wave] + pos(16 * h + a16, 4 * ks + g));
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        sc[nb][h] = f32x4{};
+#pragma unroll
+        for (int ks = 0; ks < kKs; ++ks) sc[nb][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc[ks], qf[nb][ks], sc[nb][h], 0, 0, 0);
+      }
+    }
     u32x4 pb[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      f32x4 s[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[h] = f32x4{};
-#pragma unroll
-        for (int ks = 0; ks < kKs; ++ks) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc[h][ks], qf[nb][ks], s[h], 0, 0, 0);
-      }
+      f32x4(&s)[2] = sc[nb];
       // score (h, i) of a lane: row a16, key t0 + 16 h + 4 g + i
       float top = kLowest;
       const bool masked = t0 + kTileKeys - 1 > first_limit || t0 + kTileKeys > k1;
@@ -134,7 +141,7 @@ __global__ __launch_bounds__(256, 2) void gqa_stream_kernel(const GqaParams p) {
     for (int db = 0; db < kDb; ++db) {
       // tokens 4 g + 0..3 and 16 + 4 g + 0..3 of dim 16 db + a16, as the numerators lie
       const int t = 4 * g + (a16 >> 2), c = 2 * db + ((a16 & 3) >> 1);
-      auto at = [&](int tt) { return (MLA_LDS bf16x4*)(s_v[wave] + vpos(tt, c) + (a16 & 1) * 8); };
+      auto at = [&](int tt) { return (MLA_LDS bf16x4*)(s_v[wave] + pos(tt, c) + (a16 & 1) * 8); };
       const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at(t));
       const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at(t + 16));
       const bf16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -195,76 +202,81 @@ __global__ __launch_bounds__(256, 2) void gqa_stream_kernel(const GqaParams p) {
   }
 }
 
-// Partial results of split requests joined: one wave per 16 rows... of (request, block, head), a row at a time:
-//   lse = log2 sum_i 2^lse_i, out = sum_i 2^(lse_i - lse) o_i.
-// A CTA takes (block of kRows rows, head) number blockIdx.x of the batch, counted as the attention kernels count their
-// items with every request in one piece.
-template <int D, int kRows>
-__global__ __launch_bounds__(256) void gqa_merge_kernel(const GqaParams p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int C = gqa_split_keys<kRows>(p);
-  // the request of this (block, head), and the slots before it
-  int acc = 0, slots = 0, b = -1, local = 0, pieces = 1;
+// Partial results of requests in pieces, joined: lse = log2 sum_i 2^lse_i, out = sum_i 2^(lse_i - lse) o_i.
+// One CTA per (query, query head): its waves take every fourth piece (kWaves 4), or a wave per row (kWaves 1).
+template <int D, int kRows, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = p.kv_heads * p.group, t = blockIdx.x / heads, h = blockIdx.x % heads;
   GqaRequest r{0, 0, 0, 0};
-  for (int c0 = 0; c0 < p.batch && b < 0; c0 += 64) {
-    const int i = c0 + lane;
-    GqaRequest ri{0, 0, 0, 0};
-    int n = 0, ns = 0, pi = 1;
-    if (i < p.batch) {
-      ri = gqa_request(p, i);
-      pi = ri.L > C ? (ri.L + C - 1) / C : 1;
-      n = (ri.E * p.group + kRows - 1) / kRows * p.kv_heads;
-      ns = pi > 1 ? n * pi : 0;
+  if (lane < p.batch) r = gqa_request(p, lane);
+  const int C = gqa_piece_keys<kRows>(p, r);
+  int slots = 0, tok = -1, pieces = 1;
+  for (int c0 = 0; c0 < p.batch && tok < 0; c0 += 64) {
+    if (c0 > 0) {
+      r = GqaRequest{0, 0, 0, 0};
+      if (c0 + lane < p.batch) r = gqa_request(p, c0 + lane);
     }
-    int incl = n, sincl = ns;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(incl, o), w = __shfl_up(sincl, o);
-      if (lane >= o) {
-        incl += u;
-        sincl += w;
-      }
-    }
-    const int item = blockIdx.x;
-    const uint64_t hit = __ballot(item >= acc + incl - n && item < acc + incl);
+    const int pi = gqa_pieces(r.L, C);
+    const int ns = pi > 1 ? gqa_blocks<kRows>(p, r) * pi * p.kv_heads : 0, sincl = wave_iscan(ns);
+    const uint64_t hit = __ballot(t >= r.q0 && t < r.q0 + r.E);
     if (hit != 0) {
       const int fl = __builtin_ctzll(hit);
-      b = c0 + fl;
-      local = item - acc - __builtin_amdgcn_readlane(incl - n, fl);
-      slots += __builtin_amdgcn_readlane(sincl - ns, fl);
+      tok = t - __builtin_amdgcn_readlane(r.q0, fl);
       pieces = __builtin_amdgcn_readlane(pi, fl);
-      r.q0 = __builtin_amdgcn_readlane(ri.q0, fl);
-      r.E = __builtin_amdgcn_readlane(ri.E, fl);
-      r.L = __builtin_amdgcn_readlane(ri.L, fl);
+      slots += __builtin_amdgcn_readlane(sincl - ns, fl);
     } else {
-      acc += __shfl(incl, 63);
-      slots += __shfl(sincl, 63);
+      slots += __builtin_amdgcn_readlane(sincl, 63);
     }
   }
-  if (b < 0 || pieces == 1) return;
-  const int head = local % p.kv_heads, block = local / p.kv_heads;
-  const int64_t slot0 = slots + (int64_t)block * pieces * p.kv_heads + head;  // piece i: + i kv_heads
-  for (int row = wave; row < kRows; row += 4) {
-    const int rr = block * kRows + row, tok = rr / p.group, h = head * p.group + rr % p.group;
-    if (tok >= r.E) break;
-    float mt = kLowest;
-    for (int i = lane; i < pieces; i += 64) mt = fmaxf(mt, p.ws_lse[(slot0 + (int64_t)i * p.kv_heads) * kRows + row]);
-    mt = wave_max64(mt);
-    float lt = 0.f, o[D / 64] = {};
-    for (int i = 0; i < pieces; ++i) {
-      const int64_t at = (slot0 + (int64_t)i * p.kv_heads) * kRows + row;
-      const float f = __builtin_amdgcn_exp2f(p.ws_lse[at] - mt);
-      lt += f;
+  if (tok < 0 || pieces == 1) return;
+  const int rr = tok * p.group + h % p.group, row = rr % kRows;
+  // piece i of the row's block and head: slot0 + i kv_heads
+  const int64_t slot0 = slots + (int64_t)(rr / kRows) * pieces * p.kv_heads + h / p.group;
+  const float* lse = p.ws_lse + slot0 * kRows + row;
+  const float* part = p.ws_o + (slot0 * kRows + row) * D + (D / 64) * lane;
+  const int64_t ls = (int64_t)p.kv_heads * kRows, os = ls * D;
+  typedef float part_t __attribute__((ext_vector_type(D / 64)));
+  // parts wave, wave + kWaves, ... eight in flight; the first eight are requested before the LSEs are waited for
+  part_t x[8];
+  auto load = [&](int i) {
 #pragma unroll
-      for (int d = 0; d < D / 64; ++d) o[d] += f * p.ws_o[at * D + (D / 64) * lane + d];
+    for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const part_t*>(part + min(i + u * kWaves, pieces - 1) * os);
+  };
+  load(wave);
+  float mt = kLowest;
+  for (int i = lane; i < pieces; i += 64) mt = fmaxf(mt, lse[i * ls]);
+  mt = wave_max64(mt);
+  float lt = 0.f;
+  part_t o = {};
+  for (int i0 = 0; i0 < pieces; i0 += 64) {  // 64 pieces at a time: their weights in the lanes
+    const float f = i0 + lane < pieces ? __builtin_amdgcn_exp2f(lse[(i0 + lane) * ls] - mt) : 0.f;
+    lt += wave_sum64(f);
+    const int n = min(64, pieces - i0);
+    for (int i = wave; i < n; i += 8 * kWaves) {
+      if (i0 + i > wave) load(i0 + i);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int j = i + u * kWaves;
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(j, 63)));
+        if (j < n) o += x[u] * w;
+      }
     }
-    const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
-    __bf16* out = p.out + (int64_t)(r.q0 + tok) * p.out_stride_t + (int64_t)h * p.out_stride_h + (D / 64) * lane;
-    if constexpr (D == 128) *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(o[0] * inv, o[1] * inv);
-    else *out = (__bf16)(o[0] * inv);
-    if (lane == 0 && p.lse != nullptr)
-      p.lse[(int64_t)(r.q0 + tok) * p.lse_stride_t + h] = lt > 0.f || lt != lt ? (mt + log2f(lt)) * 0.69314718055994531f : -INFINITY;
   }
+  if constexpr (kWaves > 1) {
+    __shared__ part_t s_o[kWaves][64];
+    s_o[wave][lane] = o;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) o += s_o[w][lane];
+  }
+  const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
+  __bf16* out = p.out + (int64_t)t * p.out_stride_t + (int64_t)h * p.out_stride_h + (D / 64) * lane;
+  if constexpr (D == 128) *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(o[0] * inv, o[1] * inv);
+  else *out = (__bf16)(o[0] * inv);
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[(int64_t)t * p.lse_stride_t + h] = lt > 0.f || lt != lt ? (mt + log2f(lt)) * 0.69314718055994531f : -INFINITY;
 }
 
 template <int D, int NB>
@@ -275,18 +287,21 @@ void launch_stream(const GqaParams& p, int64_t grid, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_gqa_merge(const GqaParams& p, int dim, int rows, hipStream_t stream) {
-  const int64_t blocks = ((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch;
-  const dim3 grid((unsigned)(blocks * p.kv_heads)), cta(256);
-#define MLA_MERGE(D, R) \
-  if (dim == D && rows == R) hipLaunchKernelGGL((gqa_merge_kernel<D, R>), grid, cta, 0, stream, p)
-  MLA_MERGE(64, 16);
-  MLA_MERGE(64, 32);
-  MLA_MERGE(64, 64);
-  MLA_MERGE(64, 128);
-  MLA_MERGE(128, 16);
-  MLA_MERGE(128, 32);
-  MLA_MERGE(128, 64);
-  MLA_MERGE(128, 128);
+  const int64_t grid = (int64_t)p.total_q * p.kv_heads * p.group;
+  // few rows are cut into many pieces
+#define MLA_MERGE(D, R)                                                                                            \
+  if (dim == D && rows == R) {                                                                                     \
+    if (grid <= 2048) hipLaunchKernelGGL((gqa_merge_kernel<D, R, 4>), dim3((unsigned)grid), dim3(256), 0, stream, p); \
+    else hipLaunchKernelGGL((gqa_merge_kernel<D, R, 1>), dim3((unsigned)grid), dim3(64), 0, stream, p);             \
+  }
+  MLA_MERGE(64, 16)
+  MLA_MERGE(64, 32)
+  MLA_MERGE(64, 64)
+  MLA_MERGE(64, 128)
+  MLA_MERGE(128, 16)
+  MLA_MERGE(128, 32)
+  MLA_MERGE(128, 64)
+  MLA_MERGE(128, 128)
 #undef MLA_MERGE
   return hipGetLastError();
 }

@@ -517,54 +517,66 @@ def qkv_a_rows(qkv, q_rank: int, q_norm_weight, kv_norm_weight, positions, cos_s
     return out
 
 
-def _on_device(t, call):
-    """``call()`` with the device of tensor ``t`` current (launches and the current stream go by it)."""
+# The calls below are short on the GPU (a decode step's tables take 4 us), so each tensor is looked at once, and what
+# they share is not in helpers that pass tuples on (decode 20 -> 15 us on the host).
+
+
+def _launch(fn, name: str, device: int, stream, args) -> None:
+    """``fn(*args, stream)`` (default: the current stream of GPU ``device``) with that GPU current: launches go by it,
+    and the tensors may be on another than the caller's."""
     import torch
 
-    if t.device.index == torch.cuda.current_device():
-        return call()
-    with torch.cuda.device(t.device):
-        return call()
+    if torch._C._cuda_getDevice() == device:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
+    if rc != 0:
+        check(rc, name)
 
 
-def _check_tensors(device, dtype, **tensors) -> None:
-    for name, t in tensors.items():
-        assert t.device == device and t.is_cuda, f"{name} must be on {device}, the other tensors' GPU"
-        assert t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}"
-
-
-def _check_gqa(q, k, v, heads_dim: int, out, lse) -> None:
+def _check_gqa(device: int, shape, ks, q, k, v, out, lse) -> None:
+    """What the attention calls share; ``shape`` and ``ks`` are the shapes of q and k."""
     import torch
 
-    assert q.dim() == 3 and k.dim() == v.dim() == heads_dim + 2, "q is [T, Hq, D]; k and v end in [Hkv, D]"
-    T, Hq, D = q.shape
-    Hkv = k.shape[-2]
-    assert k.shape == v.shape and k.shape[-1] == D and Hkv > 0 and Hq % Hkv == 0, "k, v: D as q's, heads that divide q's"
-    _check_tensors(q.device, torch.bfloat16, q=q, k=k, v=v, out=out)
-    assert q.stride(-1) == 1 and k.stride(-1) == 1 and v.stride(-1) == 1 and out.stride(-1) == 1, "rows must be contiguous"
-    assert out.shape == q.shape
-    if lse is not None:
-        _check_tensors(q.device, torch.float32, lse=lse)
-        assert lse.shape == (T, Hq) and lse.stride(-1) == 1
+    bf16 = torch.bfloat16
+    assert len(shape) == 3 and ks[-1] == shape[2] and ks[-2] > 0 and shape[1] % ks[-2] == 0 and v.shape == ks, (
+        "q is [T, Hq, D]; k and v end in [Hkv, D] with q's D and heads that divide q's")
+    assert device >= 0 and k.get_device() == device and v.get_device() == device and out.get_device() == device and (
+        lse is None or lse.get_device() == device), "all tensors must be on one GPU"
+    assert q.dtype is bf16 and k.dtype is bf16 and v.dtype is bf16 and out.dtype is bf16 and out.shape == shape, (
+        "q, k, v and out are bf16, out of q's shape")
+    assert lse is None or lse.dtype is torch.float32 and lse.shape == shape[:2], "lse is fp32 [T, Hq]"
+
+
+def _check_index(t, n: int, device: int, name: str) -> int:
+    """Pointer of an int32 array of ``n`` entries."""
+    import torch
+
+    assert t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous() and t.get_device() == device, (
+        f"{name} must be int32 [{n}], contiguous, on the other tensors' GPU")
+    return t.data_ptr()
+
+
+def _check_strides(sq, sk, sv, so, sl) -> None:
+    assert sq[2] == 1 and sk[-1] == 1 and sv[-1] == 1 and so[2] == 1 and sl[1] == 1, "rows must be contiguous"
 
 
 def gqa_prompt(q, k, v, cu_seqlens, scale: float, out, lse=None, stream=None) -> None:
     """Causal attention over whole prompts: packed ``q [T, Hq, D]``, ``k``, ``v [T, Hkv, D]`` (D 64 or 128; any strides
     that are multiples of 8) of the sequences ``cu_seqlens [B + 1]`` -> ``out [T, Hq, D]`` (+ ``lse [T, Hq]``). Query
     head h reads KV head ``h // (Hq // Hkv)``."""
-    import torch
-
-    _check_gqa(q, k, v, 1, out, lse)
-    assert k.shape[0] == q.shape[0], "as many keys as queries"
-    _check_tensors(q.device, torch.int32, cu_seqlens=cu_seqlens)
-    assert cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1 and cu_seqlens.is_contiguous()
-    T, Hq, D = q.shape
-    rc = _on_device(q, lambda: load_library().mla_gqa_prompt_bf16(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-        v.stride(1), cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, T, Hq, k.shape[1], D, float(scale), out.data_ptr(),
-        out.stride(0), out.stride(1), _ptr(lse), 0 if lse is None else lse.stride(0), _stream(stream)))
-    if rc != 0:
-        check(rc, "mla_gqa_prompt_bf16")
+    device, shape, ks = q.get_device(), q.shape, k.shape
+    _check_gqa(device, shape, ks, q, k, v, out, lse)
+    T, Hq, D = shape
+    assert len(ks) == 3 and ks[0] == T, "as many keys as queries"
+    sq, sk, sv, so, sl = q.stride(), k.stride(), v.stride(), out.stride(), (Hq, 1) if lse is None else lse.stride()
+    _check_strides(sq, sk, sv, so, sl)
+    n = cu_seqlens.shape[0]
+    _launch(load_library().mla_gqa_prompt_bf16, "mla_gqa_prompt_bf16", device, stream, (
+        q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1],
+        _check_index(cu_seqlens, n, device, "cu_seqlens"), n - 1, T, Hq, ks[1], D, scale, out.data_ptr(), so[0], so[1],
+        None if lse is None else lse.data_ptr(), sl[0]))
 
 
 @functools.lru_cache(maxsize=None)
@@ -583,26 +595,17 @@ def gqa_workspace(max_seqlen_q: int, q_heads: int, kv_heads: int, head_dim: int,
     return torch.empty((gqa_workspace_bytes(max_seqlen_q, q_heads, kv_heads, head_dim),), dtype=torch.uint8, device=device)
 
 
-def _check_paged(q, k_pool, v_pool, page_table, seq_lens, out, lse) -> None:
+def _workspace(workspace, nbytes: int, q, device: int, stream):
+    """``(workspace, bytes)``: the caller's, or one from torch's allocator for this call."""
     import torch
 
-    _check_gqa(q, k_pool, v_pool, 2, out, lse)
-    for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
-        assert t.stride(0) == t.shape[1] * t.stride(1), f"{name}'s pages must follow one another"
-    _check_tensors(q.device, torch.int32, page_table=page_table, seq_lens=seq_lens)
-    assert seq_lens.dim() == 1 and seq_lens.is_contiguous()
-    assert page_table.dim() == 2 and page_table.shape[0] >= seq_lens.shape[0] and page_table.stride(1) == 1
-
-
-def _workspace(workspace, nbytes: int, q, stream):
-    import torch
-
-    if workspace is None:  # from torch's allocator, for this call
-        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=q.device)
-        if stream is not None:
-            workspace.record_stream(stream)
-    assert workspace.device == q.device and workspace.is_contiguous()
-    return workspace
+    if workspace is not None:
+        assert workspace.get_device() == device and workspace.is_contiguous(), "the workspace is one block on q's GPU"
+        return workspace, workspace.numel() * workspace.element_size()
+    workspace = q.new_empty((nbytes >> 1,))
+    if stream is not None and stream.cuda_stream != torch._C._cuda_getCurrentRawStream(device):
+        workspace.record_stream(stream)
+    return workspace, nbytes
 
 
 def gqa_chunk(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q: int, scale: float, out, lse=None,
@@ -611,41 +614,43 @@ def gqa_chunk(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqle
     ``q [T, Hq, D]`` packed by ``cu_seqlens_q [B + 1]``, ``k_pool``, ``v_pool [pages, ps, Hkv, D]`` (any power-of-two
     ``ps``), ``page_table [B, cols]``, ``seq_lens_k [B]`` (prefix and chunk) -> ``out [T, Hq, D]`` (+ ``lse [T, Hq]``).
     ``max_seqlen_q``: at least every request's new tokens. ``workspace``: of ``gqa_workspace``, or None to take one from
-    torch's allocator."""
-    import torch
-
-    _check_paged(q, k_pool, v_pool, page_table, seq_lens_k, out, lse)
-    _check_tensors(q.device, torch.int32, cu_seqlens_q=cu_seqlens_q)
-    B = seq_lens_k.shape[0]
-    assert cu_seqlens_q.shape == (B + 1,) and cu_seqlens_q.is_contiguous()
-    T, Hq, D = q.shape
-    Hkv = k_pool.shape[2]
-    ws = _workspace(workspace, gqa_workspace_bytes(min(max_seqlen_q, T), Hq, Hkv, D), q, stream)
-    rc = _on_device(q, lambda: load_library().mla_gqa_chunk_bf16(
-        q.data_ptr(), q.stride(0), q.stride(1), k_pool.data_ptr(), k_pool.stride(1), k_pool.stride(2), v_pool.data_ptr(),
-        v_pool.stride(1), v_pool.stride(2), k_pool.shape[0], k_pool.shape[1], page_table.data_ptr(), page_table.shape[1],
-        page_table.stride(0), cu_seqlens_q.data_ptr(), seq_lens_k.data_ptr(), B, T, max_seqlen_q, Hq, Hkv, D,
-        float(scale), ws.data_ptr(), ws.numel() * ws.element_size(), out.data_ptr(), out.stride(0), out.stride(1),
-        _ptr(lse), 0 if lse is None else lse.stride(0), _stream(stream)))
-    if rc != 0:
-        check(rc, "mla_gqa_chunk_bf16")
+    torch's allocator for this call."""
+    _gqa_paged(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q, scale, out, lse, workspace, stream)
 
 
 def gqa_decode(q, k_pool, v_pool, page_table, seq_lens, scale: float, out, lse=None, workspace=None, stream=None) -> None:
     """``gqa_chunk`` with one new token a request: ``q [B, Hq, D]`` -> ``out [B, Hq, D]`` (+ ``lse [B, Hq]``)."""
-    _check_paged(q, k_pool, v_pool, page_table, seq_lens, out, lse)
-    B, Hq, D = q.shape
-    assert seq_lens.shape[0] == B
-    Hkv = k_pool.shape[2]
-    ws = _workspace(workspace, gqa_workspace_bytes(1, Hq, Hkv, D), q, stream)
-    rc = _on_device(q, lambda: load_library().mla_gqa_decode_bf16(
-        q.data_ptr(), q.stride(0), q.stride(1), k_pool.data_ptr(), k_pool.stride(1), k_pool.stride(2), v_pool.data_ptr(),
-        v_pool.stride(1), v_pool.stride(2), k_pool.shape[0], k_pool.shape[1], page_table.data_ptr(), page_table.shape[1],
-        page_table.stride(0), seq_lens.data_ptr(), B, Hq, Hkv, D, float(scale), ws.data_ptr(),
-        ws.numel() * ws.element_size(), out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse),
-        0 if lse is None else lse.stride(0), _stream(stream)))
-    if rc != 0:
-        check(rc, "mla_gqa_decode_bf16")
+    _gqa_paged(q, k_pool, v_pool, page_table, None, seq_lens, 1, scale, out, lse, workspace, stream)
+
+
+def _gqa_paged(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens, max_q: int, scale: float, out, lse, workspace,
+               stream) -> None:
+    import torch
+
+    device, shape, ks, ps = q.get_device(), q.shape, k_pool.shape, page_table.shape
+    _check_gqa(device, shape, ks, q, k_pool, v_pool, out, lse)
+    T, Hq, D = shape
+    sq, sk, sv, so, sp, sl = (q.stride(), k_pool.stride(), v_pool.stride(), out.stride(), page_table.stride(),
+                              (Hq, 1) if lse is None else lse.stride())
+    _check_strides(sq, sk, sv, so, sl)
+    B = seq_lens.shape[0]
+    assert len(ks) == 4 and sk[0] == ks[1] * sk[1] and sv[0] == ks[1] * sv[1], "pools are [pages, ps, Hkv, D], pages one after another"
+    assert page_table.dtype is torch.int32 and len(ps) == 2 and ps[0] >= B and sp[1] == 1 and page_table.get_device() == device, (
+        "page_table is int32 [B, cols], on q's GPU")
+    Hkv = ks[2]
+    ws, nbytes = _workspace(workspace, gqa_workspace_bytes(min(max_q, T), Hq, Hkv, D), q, device, stream)
+    lens = _check_index(seq_lens, B, device, "seq_lens")
+    lse_ptr = None if lse is None else lse.data_ptr()
+    cache = (q.data_ptr(), sq[0], sq[1], k_pool.data_ptr(), sk[1], sk[2], v_pool.data_ptr(), sv[1], sv[2], ks[0], ks[1],
+             page_table.data_ptr(), ps[1], sp[0])
+    if cu_seqlens_q is None:
+        assert T == B, "one token a request"
+        _launch(load_library().mla_gqa_decode_bf16, "mla_gqa_decode_bf16", device, stream, (
+            *cache, lens, B, Hq, Hkv, D, scale, ws.data_ptr(), nbytes, out.data_ptr(), so[0], so[1], lse_ptr, sl[0]))
+    else:
+        cu = _check_index(cu_seqlens_q, B + 1, device, "cu_seqlens_q")
+        _launch(load_library().mla_gqa_chunk_bf16, "mla_gqa_chunk_bf16", device, stream, (
+            *cache, cu, lens, B, T, max_q, Hq, Hkv, D, scale, ws.data_ptr(), nbytes, out.data_ptr(), so[0], so[1], lse_ptr, sl[0]))
 
 
 class PageTables(NamedTuple):
@@ -669,28 +674,23 @@ def page_tables_from_lengths(token_table, table_idx, cached_lens, device_lens, f
     and of all. Rows of requests that take pages must be distinct. One launch; nothing is read back."""
     import torch
 
-    _check_tensors(token_table.device, torch.int32, token_table=token_table, table_idx=table_idx, cached_lens=cached_lens,
-                   device_lens=device_lens, free_slots=free_slots)
-    B = table_idx.shape[0]
-    assert token_table.dim() == 2 and token_table.stride(1) == 1
-    assert table_idx.shape == cached_lens.shape == device_lens.shape == (B,) and free_slots.dim() == 1
-    for t in (table_idx, cached_lens, device_lens, free_slots):
-        assert t.is_contiguous()
+    device, shape, st = token_table.get_device(), token_table.shape, token_table.stride()
+    assert device >= 0 and token_table.dtype is torch.int32 and len(shape) == 2 and st[1] == 1, "token_table: int32 [rows, cols] on the GPU"
+    B, F = table_idx.shape[0], free_slots.shape[0]
     cols = -(-max_device_len // page_size)
-    i32 = dict(dtype=torch.int32, device=token_table.device)
-    pt = torch.empty((B, cols), **i32)
-    loc_pos = torch.empty((2, total_new), **i32)
-    cu_taken = torch.empty((B + 2,), **i32)
-    tables = PageTables(pt, loc_pos[0], loc_pos[1], cu_taken[: B + 1], cu_taken[B + 1 :])
-    if stream is not None:
-        for t in (pt, loc_pos, cu_taken):
-            t.record_stream(stream)
-    rc = _on_device(token_table, lambda: load_library().mla_page_tables_from_lengths(
-        token_table.data_ptr(), token_table.shape[0], token_table.shape[1], token_table.stride(0), table_idx.data_ptr(),
-        cached_lens.data_ptr(), device_lens.data_ptr(), B, B if alloc_reqs is None else alloc_reqs, free_slots.data_ptr(),
-        free_slots.shape[0], page_size, max_extend, pt.data_ptr(), cols, cols, tables.out_loc.data_ptr(),
-        tables.positions.data_ptr(), total_new, tables.cu_seqlens_q.data_ptr(), tables.pages_taken.data_ptr(),
-        _stream(stream)))
-    if rc != 0:
-        check(rc, "mla_page_tables_from_lengths")
-    return tables
+    # one allocation, which the tables are cut from
+    cells = B * cols
+    made = token_table.new_empty((cells + 2 * total_new + B + 2,))
+    if stream is not None and stream.cuda_stream != torch._C._cuda_getCurrentRawStream(device):
+        made.record_stream(stream)
+    base = made.data_ptr()
+    loc = base + 4 * cells
+    pos = loc + 4 * total_new
+    cu = pos + 4 * total_new
+    _launch(load_library().mla_page_tables_from_lengths, "mla_page_tables_from_lengths", device, stream, (
+        token_table.data_ptr(), shape[0], shape[1], st[0], _check_index(table_idx, B, device, "table_idx"),
+        _check_index(cached_lens, B, device, "cached_lens"), _check_index(device_lens, B, device, "device_lens"), B,
+        B if alloc_reqs is None else alloc_reqs, _check_index(free_slots, F, device, "free_slots"), F, page_size, max_extend,
+        base, cols, cols, loc, pos, total_new, cu, cu + 4 * (B + 1)))
+    pt, loc, pos, cu, taken = made.split_with_sizes((cells, total_new, total_new, B + 1, 1))
+    return PageTables(pt.view(B, cols), loc, pos, cu, taken)
