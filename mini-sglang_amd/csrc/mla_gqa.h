@@ -40,6 +40,7 @@ struct GqaParams {
   float* ws_lse;  // [slots, rows] their log2-domain LSEs
   int32_t target;  // items that a batch's keys are split into, about (0: no splitting)
   int32_t fit;     // at most `target`, where that can be
+  int32_t wide;    // blocks of 256 rows (not split) instead of 128
 };
 
 // A request as the kernels see it; every read is bounded by what the host knows, whatever the device arrays hold.
@@ -120,12 +121,13 @@ __device__ __forceinline__ int gqa_piece_keys(const GqaParams& p, const GqaReque
 }
 
 // Item `item` of the batch: request, block of kRows rows, KV head, piece of the keys. Items of a request are
-// ((block, piece), head), heads fastest. slot: of the item's partial result, < 0 for a request in one piece.
+// ((block, piece), head), heads fastest. kLong: a request's last blocks, which see the most keys, come first, and of up
+// to 64 requests the longest, so that no long item runs alone at the end. slot: of the item's partial result, < 0 for a request in one piece.
 struct GqaItem {
   int b, block, head, piece, pieces, C, slot;
   GqaRequest r;
 };
-template <int kRows>
+template <int kRows, bool kLong>
 __device__ __forceinline__ bool gqa_find(const GqaParams& p, int item, GqaItem& it) {
   const int lane = threadIdx.x & 63;
   GqaRequest r{0, 0, 0, 0};
@@ -140,16 +142,28 @@ __device__ __forceinline__ bool gqa_find(const GqaParams& p, int item, GqaItem& 
     const int pieces = gqa_pieces(r.L, it.C);
     const int n = gqa_blocks<kRows>(p, r) * pieces * p.kv_heads, ns = pieces > 1 ? n : 0;
     const int incl = wave_iscan(n), sincl = wave_iscan(ns);
-    const uint64_t hit = __ballot(item >= acc + incl - n && item < acc + incl);
+    int first = acc + incl - n;  // the request's first item
+    if constexpr (kLong) {
+      if (p.batch <= 64) {  // after those of longer requests, and of as long ones before it
+        first = 0;
+        for (int i = 0; i < p.batch; ++i) {
+          const int ni = __builtin_amdgcn_readlane(n, i), li = __builtin_amdgcn_readlane(r.L, i);
+          if (li > r.L || (li == r.L && i < lane)) first += ni;
+        }
+      }
+    }
+    const uint64_t hit = __ballot(item >= first && item < first + n);
     if (hit != 0) {
       const int fl = __builtin_ctzll(hit);
-      const int local = item - acc - __builtin_amdgcn_readlane(incl - n, fl);
+      const int local = item - __builtin_amdgcn_readlane(first, fl);
       it.b = c0 + fl;
       it.pieces = __builtin_amdgcn_readlane(pieces, fl);
       it.head = local % p.kv_heads;
       it.piece = local / p.kv_heads % it.pieces;
       it.block = local / p.kv_heads / it.pieces;
-      it.slot = it.pieces > 1 ? slots + __builtin_amdgcn_readlane(sincl - ns, fl) + local : -1;
+      if constexpr (kLong) it.block = __builtin_amdgcn_readlane(n, fl) / (it.pieces * p.kv_heads) - 1 - it.block;
+      it.slot = it.pieces > 1 ? slots + __builtin_amdgcn_readlane(sincl - ns, fl) +
+                                    (it.block * it.pieces + it.piece) * p.kv_heads + it.head : -1;
       it.r.q0 = __builtin_amdgcn_readlane(r.q0, fl);
       it.r.E = __builtin_amdgcn_readlane(r.E, fl);
       it.r.L = __builtin_amdgcn_readlane(r.L, fl);

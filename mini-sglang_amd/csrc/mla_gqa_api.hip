@@ -51,6 +51,8 @@ int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_str
     return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8))
     return api_error(MLA_ERR_INVALID_ARG, "%s: q, k and v must be 16-byte and out 8-byte aligned", who);
+  if (k_row_stride > 0x7fffffff || v_row_stride > 0x7fffffff)
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: k and v rows lie more than 4 GiB apart", who);
   if (q_stride_t % 8 || q_stride_h % 8 || q_stride_t < 0 || q_stride_h < 0)
     return api_error(MLA_ERR_INVALID_ARG, "%s: q strides (%lld, %lld) must be non-negative multiples of 8", who,
                      (long long)q_stride_t, (long long)q_stride_h);
@@ -132,6 +134,7 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
     p.target = p.fit ? kStreamFit : kStreamTarget;
   } else {
     p.target = blocks >= kRowsEnough ? 0 : kRowsTarget;
+    p.wide = blocks >= kRowsEnough;
   }
   p.ws_o = static_cast<float*>(workspace);
   p.ws_lse = p.ws_o + workspace_floats(most, dim) / (dim + 1) * dim;
@@ -169,6 +172,7 @@ int mla_gqa_prompt_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   p.max_keys = total_q;
   p.cu_seqlens_q = cu_seqlens;
   p.max_q = total_q;
+  p.wide = ((int64_t)total_q * p.group + mla::kRowsBlock - 1) / mla::kRowsBlock * kv_heads >= mla::kRowsEnough;
   return mla::done(mla::launch_gqa_rows(p, head_dim, (hipStream_t)stream), who);
 }
 

@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256, NB == 4 && D == 128 ? 1 : 2) void gqa_stream_k
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GqaItem it;
-  if (!gqa_find<kRows>(p, blockIdx.x, it)) return;
+  if (!gqa_find<kRows, false>(p, blockIdx.x, it)) return;
   const int C = it.C;
   const int E = it.r.E, L = it.r.L, P = it.r.P, G = p.group;
   const int a16 = lane & 15, g = lane >> 4;

@@ -142,6 +142,18 @@ def test_prompt_strided():
     assert out[:, T:].isnan().all() and out[..., d:].isnan().all() and lse[T:].isnan().all() and lse[:, hq:].isnan().all()
 
 
+@pytest.mark.parametrize("dim,heads", [(64, (64, 64)), (128, (48, 48)), (128, (96, 32))])
+def test_many_blocks(dim, heads):
+    """Enough rows to fill the chip with blocks of 256: as a prompt, and as chunks whose pages end inside a stage."""
+    gen = torch.Generator().manual_seed(dim)
+    lens = [1500, 1, 290, 33, 1100]
+    q, k, v = randn(gen, sum(lens), heads[0], dim), randn(gen, sum(lens), heads[1], dim), randn(gen, sum(lens), heads[1], dim)
+    out, lse = run_prompt(q, k, v, lens, dim ** -0.5)
+    check(out, lse, R.prompt(q, k, v, lens, dim ** -0.5))
+    c = Paged(lens, [300, 5000, 0, 77, 64], *heads, dim, 16, seed=dim)
+    check(*c.run(), c.ref())
+
+
 @pytest.mark.parametrize("page_size", [1, 2, 16, 32, 64, 256])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_chunk_pages(page_size, dim):
