@@ -40,7 +40,8 @@ struct GqaParams {
   float* ws_lse;  // [slots, rows] their log2-domain LSEs
   int32_t target;  // items that a batch's keys are split into, about (0: no splitting)
   int32_t fit;     // at most `target`, where that can be
-  int32_t wide;    // blocks of 256 rows (not split) instead of 128
+  int32_t wide;    // blocks of 256 rows (of requests in one piece) instead of 128
+  int32_t out_16b;  // rows of out start 16-byte aligned
 };
 
 // A request as the kernels see it; every read is bounded by what the host knows, whatever the device arrays hold.
@@ -88,12 +89,16 @@ __device__ __forceinline__ float wave_fsum_all(float v) {
 }
 
 // Keys of a piece, C: the batch's keys, weighted with the row blocks that read them, over `target` items, in whole tiles
-// of 64 and at least kGqaMinSplit; with `fit`, enlarged until the pieces are at most `target` (the CTAs that run at once:
+// of 64 and at least gqa_min_split; with `fit`, enlarged until the pieces are at most `target` (the CTAs that run at once:
 // one more piece would be a round of its own). Requests of more keys are cut into ceil(L / C) pieces. Every kernel of a
 // call computes the same C from the same lengths, so no plan is made on the host and a captured launch follows its
 // lengths. C is above cost / target (the sum's rounding included), so a batch has fewer than `target` pieces more than
 // blocks; a request in pieces has L > C, so ceil(L / C) <= 2 L / C, and 2 target slots hold every piece.
-constexpr int kGqaMinSplit = 128;  // a tile for each wave of the stream kernel
+// Least keys of a piece: a tile for each wave of the stream kernel; 16 stages of the blocks (their joining takes 6 us).
+template <int kRows>
+constexpr int gqa_min_split() {
+  return kRows <= 64 ? 128 : 512;
+}
 template <int kRows>
 __device__ __forceinline__ int gqa_blocks(const GqaParams& p, const GqaRequest& r) {
   return (r.E * p.group + kRows - 1) / kRows;
@@ -108,7 +113,12 @@ __device__ __forceinline__ int gqa_piece_keys(const GqaParams& p, const GqaReque
   float cost = lane < p.batch ? cost_of(r) : 0.f;
   for (int b = 64 + lane; b < p.batch; b += 64) cost += cost_of(gqa_request(p, b));
   const float c = wave_fsum_all(cost) * (float)p.kv_heads / (float)p.target * 1.0001f + 64.f;
-  int C = max(c < 2e9f ? (int)c & ~63 : 0x7fffffc0, kGqaMinSplit);
+  int C = c < 2e9f ? (int)c & ~63 : 0x7fffffc0;
+  // blocks: `target` items are two CTAs a compute unit; short pieces, half as many. One against two, 64 query and 8 KV
+  // heads unless said: 8 chunks of 100 tokens on 2000 (32 heads) 53 / 64 us, 4 of 256 on 4000 (32) 96 / 106; one of 512 on
+  // 8000 190 / 182, one of 4096 on 28,000 (8 and 1) 585 / 535
+  if (kRows >= 128 && C < 2560) C *= 2;
+  C = max(C, gqa_min_split<kRows>());
   if (p.fit && p.batch <= 64) {
     for (int i = 0; i < 4 && C < (1 << 24); ++i) {
       const int n = lane < p.batch ? gqa_blocks<kRows>(p, r) * gqa_pieces(r.L, C) * p.kv_heads : 0;
@@ -145,11 +155,21 @@ __device__ __forceinline__ bool gqa_find(const GqaParams& p, int item, GqaItem& 
     int first = acc + incl - n;  // the request's first item
     if constexpr (kLong) {
       if (p.batch <= 64) {  // after those of longer requests, and of as long ones before it
+        // (keys of 2^25 and more count as alike: the order is any). Constant lanes, 16 at a time: a readlane of a
+        // loop's counter took 60 ns.
+        const int key = min(r.L, (1 << 25) - 1) * 64 + 63 - lane;
         first = 0;
-        for (int i = 0; i < p.batch; ++i) {
-          const int ni = __builtin_amdgcn_readlane(n, i), li = __builtin_amdgcn_readlane(r.L, i);
-          if (li > r.L || (li == r.L && i < lane)) first += ni;
-        }
+        auto group = [&](auto g0) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int ni = __builtin_amdgcn_readlane(n, decltype(g0)::value + i);
+            first += __builtin_amdgcn_readlane(key, decltype(g0)::value + i) > key ? ni : 0;
+          }
+        };
+        group(std::integral_constant<int, 0>{});
+        if (p.batch > 16) group(std::integral_constant<int, 16>{});
+        if (p.batch > 32) group(std::integral_constant<int, 32>{});
+        if (p.batch > 48) group(std::integral_constant<int, 48>{});
       }
     }
     const uint64_t hit = __ballot(item >= first && item < first + n);
@@ -168,6 +188,7 @@ __device__ __forceinline__ bool gqa_find(const GqaParams& p, int item, GqaItem& 
       it.r.E = __builtin_amdgcn_readlane(r.E, fl);
       it.r.L = __builtin_amdgcn_readlane(r.L, fl);
       it.r.P = __builtin_amdgcn_readlane(r.P, fl);
+      it.C = ((it.r.L + it.pieces - 1) / it.pieces + 63) & ~63;  // of the request: pieces alike
       return true;
     }
     acc += __builtin_amdgcn_readlane(incl, 63);

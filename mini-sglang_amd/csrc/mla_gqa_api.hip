@@ -26,6 +26,17 @@ constexpr int kRowsTarget = 512;
 // A chunk batch of at least this many blocks fills the chip without cutting keys.
 constexpr int kRowsEnough = 1024;
 constexpr int kRowsBlock = 128;
+// Keys (at most, by the page table's width) up to which cutting them gains nothing over joining the pieces.
+constexpr int kRowsOnePiece = 1024;
+
+// Blocks of 256 rows (head_dim 128): they read keys once for twice the rows, but start and end alone on their compute
+// unit. 256 / 128 rows: prompts of 8k tokens, 64 and 8 heads 1797 / 1894 us; one of 4096, 32 heads 149 / 156; four of 2048
+// 330 / 325; six of 250 to 1900, 32 heads 85 / 82; 64 of 100 55 / 46; four chunks of 2048 on up to 8k tokens 1190 / 1264;
+// one prompt of 8192, 8 and 1 heads (256 wide blocks) 191 / 173. avg: tokens of an average request; keys: of the longest,
+// by what the host knows.
+bool wide_blocks(int dim, int64_t blocks, int64_t avg, int64_t keys) {
+  return dim == 128 && blocks >= kRowsEnough && avg >= 1024 && keys >= 2560;
+}
 
 int stream_rows(int64_t most) { return most <= 16 ? 16 : most <= 32 ? 32 : 64; }
 
@@ -37,6 +48,7 @@ int64_t workspace_floats(int64_t most, int dim) {
 int check_heads(const char* who, int32_t q_heads, int32_t kv_heads, int32_t dim) {
   if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0)
     return api_error(MLA_ERR_INVALID_ARG, "%s: %d query heads are no multiple of %d KV heads", who, q_heads, kv_heads);
+  if (q_heads > 4096) return api_error(MLA_ERR_UNSUPPORTED, "%s: at most 4096 query heads, got %d", who, q_heads);
   if (dim != 64 && dim != 128) return api_error(MLA_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128, got %d", who, dim);
   return MLA_OK;
 }
@@ -86,6 +98,7 @@ int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_str
   p.out = static_cast<__bf16*>(out);
   p.out_stride_t = out_stride_t;
   p.out_stride_h = out_stride_h;
+  p.out_16b = aligned(out, 16) && out_stride_t % 8 == 0 && out_stride_h % 8 == 0;
   p.lse = lse;
   p.lse_stride_t = lse_stride_t;
   return MLA_OK;
@@ -133,8 +146,8 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
     p.fit = 2 * ((int64_t)batch * kv_heads) <= kStreamFit;
     p.target = p.fit ? kStreamFit : kStreamTarget;
   } else {
-    p.target = blocks >= kRowsEnough ? 0 : kRowsTarget;
-    p.wide = blocks >= kRowsEnough;
+    p.target = blocks >= kRowsEnough || p.max_keys <= kRowsOnePiece ? 0 : kRowsTarget;
+    p.wide = p.target == 0 && wide_blocks(dim, blocks, total_q / batch, p.max_keys);
   }
   p.ws_o = static_cast<float*>(workspace);
   p.ws_lse = p.ws_o + workspace_floats(most, dim) / (dim + 1) * dim;
@@ -172,7 +185,8 @@ int mla_gqa_prompt_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   p.max_keys = total_q;
   p.cu_seqlens_q = cu_seqlens;
   p.max_q = total_q;
-  p.wide = ((int64_t)total_q * p.group + mla::kRowsBlock - 1) / mla::kRowsBlock * kv_heads >= mla::kRowsEnough;
+  p.wide = mla::wide_blocks(head_dim, ((int64_t)total_q * p.group + mla::kRowsBlock - 1) / mla::kRowsBlock * kv_heads,
+                            total_q / batch, total_q / batch);
   return mla::done(mla::launch_gqa_rows(p, head_dim, (hipStream_t)stream), who);
 }
 

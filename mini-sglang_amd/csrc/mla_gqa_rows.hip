@@ -1,17 +1,16 @@
 // Grouped-head attention for many rows: whole prompts, and chunks of more than 64 rows (tokens times group) over a
 // paged cache. See mla_gqa.h for the mathematics.
 //
-// One CTA per (request, 128 NB rows, KV head, piece of the keys): four waves x 32 NB rows, one wave per SIMD (NB 2) or
-// two CTAs on a compute unit (NB 1).
+// One CTA per (request, 32 NW rows, KV head, piece of the keys), NW waves x 32 rows, two waves per SIMD: NW 4 (two CTAs
+// on a compute unit) or 8 (one).
 //  * Keys stream in stages of 32 through a K ring and a V ring in LDS, filled by 16-byte DMA loads whose sources are
 //    per token, so that a page may end anywhere (rows of a paged cache are looked up a window at a time into LDS).
 //    Keys past the last repeat it. 16-byte chunks are permuted within a row (kchunk, vchunk), so that neither the K
 //    reads (16 rows at a time) nor the transposing V reads meet in a bank.
 //  * S^T[32 keys x 32 rows] = K . Q^T and O^T[D dims x 32 rows] += V^T . P^T on 32x32x16 bf16 MFMA; queries and O stay
-//    in registers. With NB 2 each K and V operand read from LDS feeds two MFMAs: with one, reading 16 KB of operands a
-//    wave and stage takes as long as its MFMAs.
-//  * Software pipeline: step j issues the value MFMAs of stage j - 1 and the score MFMAs of stage j + 1 while the vector
-//    ALU runs the softmax of stage j, spread over the MFMAs.
+//    in registers.
+//  * Software pipeline: step j issues the score MFMAs of stage j + 1 and then the value MFMAs of stage j - 1 while the
+//    vector ALU runs the softmax of stage j, spread over the MFMAs.
 //  * Online softmax in the log2 domain against a lazy row reference: the maximum of the wave's first stage, moved (with O
 //    and l rescaled, and the stage redone) only when a stage's numerators sum past 2^32: fp32 keeps its relative
 //    precision at any scale.
@@ -39,27 +38,27 @@ __device__ __forceinline__ void static_for(F&& f) {
   static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-// Rings: group n is K stage n and V stage n - 1 (its values are needed two steps after K's scores). Step j issues group
-// j + kDist, scores stage j + 1, adds the values of stage j - 1 and reads ahead into V stage j. Every kSync steps a
-// barrier makes the groups up to j + kSync visible. A K slot is refilled kRing - kDist steps after its stage was read,
-// which must pass a barrier (kRing >= kDist + kSync - 1), V likewise (kRing >= kDist + kSync).
-template <int NB>
+// Rings: group n is K stage n and V stage n - 2. Step j issues group j + kDist, scores stage j + 1, adds the values of
+// stage j - 1 and reads ahead into K stage j + 2. Every kSync steps a barrier makes the groups up to j + kSync + 1
+// visible, those of the steps up to the next barrier. A slot is refilled kRing - kDist + 1 steps after its stage's last
+// read (K stage s in step s - 1, V stage s in step s + 1), which must pass a barrier: kRing >= kDist + kSync - 1.
+template <int NW>
 struct Rings;
 template <>
-struct Rings<1> {
-  static constexpr int kSync = 1, kDist = 3, kRing = 4, kWindow = 2048;
+struct Rings<4> {
+  static constexpr int kSync = 1, kDist = 4, kRing = 4, kWindow = 2048;
 };
 template <>
-struct Rings<2> {
-  static constexpr int kSync = 2, kDist = 6, kRing = 8, kWindow = 4096;
+struct Rings<8> {
+  static constexpr int kSync = 2, kDist = 7, kRing = 8, kWindow = 4096;
 };
-template <int NB>
+template <int NW>
 constexpr bool rings_ok() {
-  using S = Rings<NB>;
-  return S::kRing >= S::kDist + S::kSync && S::kDist > S::kSync && S::kRing % 2 == 0 && S::kRing % S::kSync == 0 &&
-         S::kWindow >= (2 * S::kRing + S::kDist) * kStage && S::kWindow % 256 == 0;
+  using S = Rings<NW>;
+  return S::kRing >= S::kDist + S::kSync - 1 && S::kDist >= S::kSync + 2 && S::kRing % 2 == 0 && S::kRing % S::kSync == 0 &&
+         S::kWindow >= (2 * S::kRing + S::kDist) * kStage;
 }
-static_assert(rings_ok<1>() && rings_ok<2>(), "ring lengths");
+static_assert(rings_ok<4>() && rings_ok<8>(), "ring lengths");
 
 // Position of 16-byte chunk c of token t in a K / V row of an LDS tile.
 template <int D>
@@ -83,35 +82,31 @@ __device__ __forceinline__ float sum_halves(float v) {
 // Pins a value to its slot of the instruction stream (volatile statements keep their order).
 __device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ void pin(uint32_t& x) { asm volatile("" : "+v"(x)); }
-template <int NB>
-__device__ __forceinline__ void pin_o(f32x16_t& o) {
-  if constexpr (NB == 2) asm volatile("" : "+a"(o));
-  else asm volatile("" : "+v"(o));
-}
+__device__ __forceinline__ void pin(f32x16_t& x) { asm volatile("" : "+v"(x)); }
 
-// The softmax of a stage as 24 micro-operations a block of rows: for u = 3 k + r (pair k of a lane's 16 scores), r < 2 is
-// the exponential of score 2 k + r, r == 2 adds the pair to the row sum and packs it. Spread over a step's MFMA slots in
-// proportion to their cost.
+// The softmax of a stage as 24 micro-operations: for u = 3 k + r (pair k of a lane's 16 scores), r < 2 is the exponential
+// of score 2 k + r, r == 2 adds the pair to the row sum and packs it. Spread over a step's MFMA slots in proportion to
+// their cost.
 constexpr int kUops = 24;
-constexpr int uop_weight(int u) { return u % 3 < 2 ? 5 : 6; }
 constexpr int uop_total(int n) {
   int t = 0;
-  for (int u = 0; u < n; ++u) t += uop_weight(u);
+  for (int u = 0; u < n; ++u) t += u % 3 < 2 ? 5 : 6;
   return t;
 }
-constexpr int uop_slot(int u, int nb, int slots) { return uop_total(u) * slots / uop_total(kUops * nb); }
+constexpr int uop_slot(int u, int slots) { return uop_total(u) * slots / uop_total(kUops); }
 
-template <int D, int NB, bool kPaged>
-__global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const GqaParams p) {
-  using S = Rings<NB>;
-  constexpr int kRows = 128 * NB, kRowB = D * 2, kTileB = kStage * kRowB;
+template <int D, int NW, bool kPaged>
+__global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p) {
+  using S = Rings<NW>;
+  constexpr int kRows = 32 * NW, kRowB = D * 2, kTileB = kStage * kRowB;
   constexpr int kKs = D / 16, kDb = D / 32, kVs = 2 * kDb;  // K operands, 32-dim blocks, V operands of a stage
-  constexpr int kOps = kVs + kKs, kSlots = NB * kOps;
-  constexpr int kLd = D / 64;                   // a wave's K (V) loads of a stage, 1 KB each
-  constexpr int kPerLoad = 1024 / kRowB;        // tokens of a load
+  constexpr int kSlots = kVs + kKs;                         // MFMAs of a step
+  constexpr int kLd = kTileB / 1024 / NW;                   // a wave's K (V) loads of a stage, 1 KB each
+  static_assert(kLd >= 1, "every wave loads K and V");
+  constexpr int kPerLoad = 1024 / kRowB;  // tokens of a load
   constexpr int kRingB = S::kRing * kTileB;
-  constexpr int kAK = NB == 2 ? 3 : D == 128 ? 4 : 3, kAV = NB == 2 ? 2 : 3;  // operands read ahead
-  static_assert(kAK <= kVs && kAV <= kVs, "read ahead within a step");
+  constexpr int kAK = D == 128 ? 4 : 3, kAV = 3;  // operands read ahead
+  static_assert(kAK <= kVs && kAV <= kKs, "read ahead by less than a step");
   __shared__ __attribute__((aligned(1024))) char smem[2 * kRingB];
   __shared__ int s_row[kPaged ? S::kWindow : 1];
 
@@ -121,42 +116,36 @@ __global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const Gq
   if (!gqa_find<kRows, true>(p, blockIdx.x, it)) return;
   const int E = it.r.E, L = it.r.L, P = it.r.P, G = p.group;
   const int c32 = lane & 31, g32 = lane >> 5;
-  const int row0 = it.block * kRows + 32 * NB * wave;  // the wave's first row
+  const int row0 = it.block * kRows + 32 * wave;  // the wave's first row
+  const int tok0 = row0 / G, rem0 = row0 - tok0 * G;
+  const float inv_g = 1.f / (float)G;
+  // token and head of the wave's row i (rem0 + i < G + 32: exact)
+  auto tok_of = [&](int i) __attribute__((always_inline)) { return tok0 + (int)(((float)(rem0 + i) + 0.5f) * inv_g); };
+  auto head_of = [&](int i, int tok) __attribute__((always_inline)) { return it.head * G + rem0 + i - (tok - tok0) * G; };
   const int last_tok = min(E - 1, (it.block * kRows + kRows - 1) / G);
   const int k0 = it.piece * it.C, k1 = min(it.pieces > 1 ? k0 + it.C : L, P + last_tok + 1);
   const int nst = __builtin_amdgcn_readfirstlane(k1 > k0 ? (k1 - k0 + kStage - 1) / kStage : 0);
   int W = 0;  // stages that the wave needs
-  if (row0 / G < E) W = (min(k1, P + min(E - 1, (row0 + 32 * NB - 1) / G) + 1) - k0 + kStage - 1) / kStage;
+  if (tok0 < E) W = (min(k1, P + min(E - 1, (row0 + 31) / G) + 1) - k0 + kStage - 1) / kStage;
   W = __builtin_amdgcn_readfirstlane(max(W, 0));
   // the first stage with a key that some row of the wave does not see
-  const int j_diag = __builtin_amdgcn_readfirstlane(max(min(P + row0 / G + 1, k1) - k0, 0) >> 5);
+  const int j_diag = __builtin_amdgcn_readfirstlane(max(min(P + tok0 + 1, k1) - k0, 0) >> 5);
 
-  const int head0 = it.head * G;
-  int limit[NB];  // last key of the lane's row, from k0
-  bf16x8 qf[NB][kKs];
+  const int tok = tok_of(c32), head = head_of(c32, tok);
+  const bool live = tok < E;
+  // last key of the lane's row, from k0; rows past the last query repeat the request's first (and are not written)
+  const int limit = min(live ? P + tok : k1 - 1, k1 - 1) - k0;
+  bf16x8 qf[kKs];
+  {
+    const __bf16* q = p.q + (int64_t)(it.r.q0 + (live ? tok : 0)) * p.q_stride_t + (int64_t)(live ? head : it.head * G) * p.q_stride_h + 8 * g32;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int r = row0 + 32 * nb + c32, tok = r / G;
-    const bool live = tok < E;
-    // rows past the last query repeat the request's first (their results are not written)
-    limit[nb] = min(live ? P + tok : k1 - 1, k1 - 1) - k0;
-    const __bf16* q = p.q + (int64_t)(it.r.q0 + (live ? tok : 0)) * p.q_stride_t + (int64_t)(head0 + (live ? r - tok * G : 0)) * p.q_stride_h + 8 * g32;
-#pragma unroll
-    for (int ks = 0; ks < kKs; ++ks) qf[nb][ks] = *reinterpret_cast<const bf16x8*>(q + 16 * ks);
+    for (int ks = 0; ks < kKs; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(q + 16 * ks);
   }
 
-  f32x16_t O[NB][kDb];
+  f32x16_t O[kDb];
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int db = 0; db < kDb; ++db) O[nb][db] = f32x16_t{};
-  float m_ref[NB], negm[NB], l_run[NB];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    m_ref[nb] = kLowest;
-    negm[nb] = -kLowest;
-    l_run[nb] = 0.f;
-  }
+  for (int db = 0; db < kDb; ++db) O[db] = f32x16_t{};
+  float m_ref = kLowest, negm = -kLowest, l_run = 0.f;
 
   if (nst > 0) {
     // ---- sources: token t of the piece
@@ -165,40 +154,41 @@ __global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const Gq
     auto fill = [&]() __attribute__((always_inline)) {
       if constexpr (kPaged) {
         const int need = min(S::kWindow, (nst + S::kDist + S::kRing) * kStage - w0);
-        int r[S::kWindow / 256];
+        for (int t0 = 0; t0 < need; t0 += 4 * 64 * NW) {
+          int r[4];
 #pragma unroll
-        for (int u = 0; u < S::kWindow / 256; ++u) {
-          const int t = threadIdx.x + 256 * u;
-          if (t < need) r[u] = gqa_row(p, it.b, it.r.q0, k0 + min(w0 + t, last));
-        }
+          for (int u = 0; u < 4; ++u) {
+            const int t = t0 + threadIdx.x + 64 * NW * u;
+            if (t < need) r[u] = gqa_row(p, it.b, it.r.q0, k0 + min(w0 + t, last));
+          }
 #pragma unroll
-        for (int u = 0; u < S::kWindow / 256; ++u) {
-          const int t = threadIdx.x + 256 * u;
-          if (t < need) s_row[t] = r[u];
+          for (int u = 0; u < 4; ++u) {
+            const int t = t0 + threadIdx.x + 64 * NW * u;
+            if (t < need) s_row[t] = r[u];
+          }
         }
       }
     };
     fill();
     // load i of a wave covers kPerLoad tokens of the stage, lane's token tk[i], 16-byte chunk position lane % (D / 8)
     const char* kb[kLd];
-    const char* vb_[kLd];
+    const char* vb[kLd];
     int tk[kLd];
 #pragma unroll
     for (int i = 0; i < kLd; ++i) {
       tk[i] = (wave * kLd + i) * kPerLoad + lane / (D / 8);
       const int c = lane % (D / 8);
       kb[i] = reinterpret_cast<const char*>(p.k + (int64_t)it.head * p.k_head_stride) + kchunk<D>(c, tk[i]) * 16;
-      vb_[i] = reinterpret_cast<const char*>(p.v + (int64_t)it.head * p.v_head_stride) + vchunk<D>(c, tk[i]) * 16;
+      vb[i] = reinterpret_cast<const char*>(p.v + (int64_t)it.head * p.v_head_stride) + vchunk<D>(c, tk[i]) * 16;
     }
     const uint32_t ks_b = (uint32_t)(p.k_row_stride * 2), vs_b = (uint32_t)(p.v_row_stride * 2);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(MLA_LDS char*)smem + wave * kLd * 1024;
-    int row[kLd], row_v[kLd];  // of group n's K stage and V stage
-#pragma unroll
-    for (int i = 0; i < kLd; ++i) row[i] = row_v[i] = 0;
+    int row[kLd], row_1[kLd], row_v[kLd];  // of group n's K stage, the one before, and V stage n - 2
     auto rows_of = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kLd; ++i) {
-        row_v[i] = row[i];
+        row_v[i] = row_1[i];
+        row_1[i] = row[i];
         if constexpr (kPaged) row[i] = s_row[n * kStage - w0 + tk[i]];
         else row[i] = it.r.q0 + k0 + min(n * kStage + tk[i], last);
       }
@@ -206,16 +196,12 @@ __global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const Gq
     auto dma = [&](int part, uint32_t kslot, uint32_t vslot) __attribute__((always_inline)) {
       const int i = part % kLd;
       if (part < kLd) dma16_vaddr(kb[i] + (uint64_t)(uint32_t)row[i] * ks_b, lds0 + kslot * kTileB + i * 1024);
-      else dma16_vaddr(vb_[i] + (uint64_t)(uint32_t)row_v[i] * vs_b, lds0 + kRingB + vslot * kTileB + i * 1024);
+      else dma16_vaddr(vb[i] + (uint64_t)(uint32_t)row_v[i] * vs_b, lds0 + kRingB + vslot * kTileB + i * 1024);
     };
-    // group n at once; group 0 loads V stage 0's slot with rows of no meaning (row_v is row 0 of the pool... of stage 0)
     auto group_now = [&](int n) __attribute__((always_inline)) {
       rows_of(n);
-      if (n == 0)
 #pragma unroll
-        for (int i = 0; i < kLd; ++i) row_v[i] = row[i];
-#pragma unroll
-      for (int part = 0; part < 2 * kLd; ++part) dma(part, n % S::kRing, (n + S::kRing - 1) % S::kRing);
+      for (int part = 0; part < 2 * kLd; ++part) dma(part, n % S::kRing, (n + S::kRing - 2) % S::kRing);
     };
     auto sync_groups = [&](auto ng) __attribute__((always_inline)) {
       wait_vmcnt<2 * kLd * decltype(ng)::value>();
@@ -223,14 +209,15 @@ __global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const Gq
     };
 
     barrier_lds();  // s_row is written
+    rows_of(0);     // groups 0 and 1 fill V slots of no stage with V stage 0
+#pragma unroll
+    for (int i = 0; i < kLd; ++i) row_1[i] = row[i];
     for (int n = 0; n < S::kDist - 1; ++n) group_now(n);
     // the queries stay in registers and have landed here, with the first groups issued behind them; the wait is
     // explicit, since the compiler does not count the DMA loads
     wait_vmcnt<0>();
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int ks = 0; ks < kKs; ++ks) asm volatile("" : "+v"(qf[nb][ks]));
+    for (int ks = 0; ks < kKs; ++ks) asm volatile("" : "+v"(qf[ks]));
 
     // ---- operand reads
     int k_off[kKs], v_off[kDb];
@@ -250,11 +237,11 @@ __global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const Gq
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
-    f32x16_t sc[2][NB];   // [parity]: scores of the stage being softmaxed / being computed
-    u32x4 pb[2][NB][2];   // [parity]: bf16 numerators P^T
+    f32x16_t sc[2];  // [parity]: scores of the stage being softmaxed / being computed
+    u32x4 pb[2][2];  // [parity]: bf16 numerators P^T
     bf16x8 vop[kAV + 1], kop[kAK + 1];
-    auto mask = [&](f32x16_t& s, int nb, int j, bool all) __attribute__((always_inline)) {
-      const int lim = all ? -1 : limit[nb] - j * kStage - 4 * g32;  // score i: key 8 (i / 4) + 4 g32 + i % 4
+    auto mask = [&](f32x16_t& s, int j, bool all) __attribute__((always_inline)) {
+      const int lim = all ? -1 : limit - j * kStage - 4 * g32;  // score i: key 8 (i / 4) + 4 g32 + i % 4
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (8 * (i >> 2) + (i & 3) > lim) s[i] = -INFINITY;
@@ -265,24 +252,24 @@ __global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const Gq
       for (int i = 1; i < 16; ++i) m = fmaxf(m, s[i]);
       return fmaxf(max_halves(m) * p.scale_log2, kLowest);  // (a stage of -inf alone: its numerators are 0)
     };
-    auto redo = [&](const f32x16_t& s, int nb, u32x4 (&dst)[2], float& l_step) __attribute__((always_inline)) {
-      const float m_new = fmaxf(top_of(s), m_ref[nb]), fr = __builtin_amdgcn_exp2f(m_ref[nb] - m_new);
-      m_ref[nb] = m_new;
-      negm[nb] = -m_new;
-      l_run[nb] *= fr;
+    auto redo = [&](const f32x16_t& s, u32x4 (&dst)[2], float& l_step) __attribute__((always_inline)) {
+      const float m_new = fmaxf(top_of(s), m_ref), fr = __builtin_amdgcn_exp2f(m_ref - m_new);
+      m_ref = m_new;
+      negm = -m_new;
+      l_run *= fr;
       float l = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[2 * k], p.scale_log2, negm[nb]));
-        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[2 * k + 1], p.scale_log2, negm[nb]));
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[2 * k], p.scale_log2, negm));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[2 * k + 1], p.scale_log2, negm));
         l += e0 + e1;
         dst[k >> 2][k & 3] = pack_bf16x2(e0, e1);
       }
       l_step = l;
 #pragma unroll
       for (int db = 0; db < kDb; ++db) {
-        O[nb][db] *= fr;
-        pin_o<NB>(O[nb][db]);
+        O[db] *= fr;
+        pin(O[db]);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -290,96 +277,78 @@ __global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const Gq
     // ---- pipelined step; U: its number modulo the rings
     auto step_fast = [&](auto u_c) __attribute__((always_inline)) {
       constexpr int U = decltype(u_c)::value, par = U & 1;
-      constexpr int v_prev = (U + S::kRing - 1) % S::kRing, v_cur = U % S::kRing, k_next = (U + 1) % S::kRing;
-      constexpr int kslot = (U + S::kDist) % S::kRing, vslot = (U + S::kDist - 1) % S::kRing;
+      constexpr int v_prev = (U + S::kRing - 1) % S::kRing, k_next = (U + 1) % S::kRing, k_next2 = (U + 2) % S::kRing;
+      constexpr int kslot = (U + S::kDist) % S::kRing, vslot = (U + S::kDist + S::kRing - 2) % S::kRing;
       constexpr int kDmaEvery = kSlots / (2 * kLd);
-      float l_step[NB], ev[2];
+      float l_step, ev[2];
       static_for<kSlots>([&](auto s_c) __attribute__((always_inline)) {
-        constexpr int s = decltype(s_c)::value, o = s / NB, nb = s % NB;
-        if constexpr (o < kVs) {
-          O[nb][o >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[o % (kAV + 1)], __builtin_bit_cast(bf16x8, pb[par ^ 1][nb][o & 1]), O[nb][o >> 1], 0, 0, 0);
-          pin_o<NB>(O[nb][o >> 1]);
+        constexpr int s = decltype(s_c)::value;
+        if constexpr (s < kKs) {
+          if constexpr (s == 0) sc[par ^ 1] = f32x16_t{};
+          sc[par ^ 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[s % (kAK + 1)], qf[s], sc[par ^ 1], 0, 0, 0);
         } else {
-          constexpr int ks = o - kVs;
-          if constexpr (ks == 0) sc[par ^ 1][nb] = f32x16_t{};
-          sc[par ^ 1][nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kop[ks % (kAK + 1)], qf[nb][ks], sc[par ^ 1][nb], 0, 0, 0);
+          constexpr int st = s - kKs;
+          O[st >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[st % (kAV + 1)], __builtin_bit_cast(bf16x8, pb[par ^ 1][st & 1]), O[st >> 1], 0, 0, 0);
+          pin(O[st >> 1]);
         }
         if constexpr (s % kDmaEvery == kDmaEvery - 1) dma(s / kDmaEvery, kslot, vslot);
-        if constexpr (nb == NB - 1) {  // operand reads
-          constexpr int st = o + kAV, stn = o + kAV - kOps, ks = o - kVs + kAK;
-          if constexpr (st < kVs) vop[st % (kAV + 1)] = vread(v_prev, st);
-          if constexpr (stn >= 0 && stn < kAV) vop[stn % (kAV + 1)] = vread(v_cur, stn);
-          if constexpr (ks >= 0 && ks < kKs) kop[ks % (kAK + 1)] = kread(k_next, ks);
+        {  // operand reads
+          constexpr int ks = s + kAK, ksn = s + kAK - kSlots, st = s - kKs + kAV;
+          if constexpr (ks < kKs) kop[ks % (kAK + 1)] = kread(k_next, ks);
+          if constexpr (ksn >= 0 && ksn < kAK) kop[ksn % (kAK + 1)] = kread(k_next2, ksn);
+          if constexpr (st >= 0 && st < kVs) vop[st % (kAV + 1)] = vread(v_prev, st);
         }
-        static_for<kUops * NB>([&](auto w_c) __attribute__((always_inline)) {
-          constexpr int w = decltype(w_c)::value;
-          if constexpr (uop_slot(w, NB, kSlots) == s) {
-            constexpr int b = w / kUops, u = w % kUops, k = u / 3, r = u % 3;
+        static_for<kUops>([&](auto w_c) __attribute__((always_inline)) {
+          constexpr int u = decltype(w_c)::value, k = u / 3, r = u % 3;
+          if constexpr (uop_slot(u, kSlots) == s) {
             if constexpr (r < 2) {
-              ev[r] = __builtin_amdgcn_exp2f(fmaf(sc[par][b][2 * k + r], p.scale_log2, negm[b]));
+              ev[r] = __builtin_amdgcn_exp2f(fmaf(sc[par][2 * k + r], p.scale_log2, negm));
               pin(ev[r]);
             } else {
-              l_step[b] = k == 0 ? ev[0] + ev[1] : l_step[b] + ev[0] + ev[1];
+              l_step = k == 0 ? ev[0] + ev[1] : l_step + ev[0] + ev[1];
               uint32_t x = pack_bf16x2(ev[0], ev[1]);
-              pin(l_step[b]);
+              pin(l_step);
               pin(x);
-              pb[par][b][k >> 2][k & 3] = x;
+              pb[par][k >> 2][k & 3] = x;
             }
           }
         });
         __builtin_amdgcn_sched_barrier(0);
       });
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        if (__ballot(l_step[nb] >= kLazyMax) != 0) redo(sc[par][nb], nb, pb[par][nb], l_step[nb]);
-        l_run[nb] += l_step[nb];
-      }
+      if (__ballot(l_step >= kLazyMax) != 0) redo(sc[par], pb[par], l_step);
+      l_run += l_step;
     };
     auto step = [&](auto u_c, int j) __attribute__((always_inline)) {
       constexpr int U = decltype(u_c)::value, par = U & 1;
       if (j > nst) return;
-      if constexpr (U % S::kSync == 0) sync_groups(ic<S::kDist - 1 - S::kSync>{});
+      if constexpr (U % S::kSync == 0) sync_groups(ic<S::kDist - 2 - S::kSync>{});
       if (__builtin_expect(j <= W && W > 0, 1)) {
         rows_of(j + S::kDist);
-        if (__builtin_expect(j >= j_diag || j == W, 0))
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mask(sc[par][nb], nb, j, j == W);
-        if constexpr (U == 0) if (__builtin_expect(j == 0, 0))
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            m_ref[nb] = top_of(sc[par][nb]);
-            negm[nb] = -m_ref[nb];
-          }
+        if (__builtin_expect(j >= j_diag || j == W, 0)) mask(sc[par], j, j == W);
+        if constexpr (U == 0) if (__builtin_expect(j == 0, 0)) {
+          m_ref = top_of(sc[par]);
+          negm = -m_ref;
+        }
         step_fast(u_c);
         if constexpr (U == 0) if (__builtin_expect(j == 0, 0))
           // step 0 has no stage before it: its value pass multiplied zeros with what the V ring's last slot held
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int db = 0; db < kDb; ++db) O[nb][db] = f32x16_t{};
+          for (int db = 0; db < kDb; ++db) O[db] = f32x16_t{};
       } else {
         group_now(j + S::kDist);
       }
     };
 
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) pb[1][nb][0] = pb[1][nb][1] = u32x4{};
+    pb[1][0] = pb[1][1] = u32x4{};
     // step -1: the scores of stage 0
     __builtin_amdgcn_s_barrier();
     group_now(S::kDist - 1);
     if (W > 0) {
+      sc[0] = f32x16_t{};
 #pragma unroll
-      for (int ks = 0; ks < kKs; ++ks) {
-        const bf16x8 a = kread(0, ks);
+      for (int ks = 0; ks < kKs; ++ks) sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kread(0, ks), qf[ks], sc[0], 0, 0, 0);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          if (ks == 0) sc[0][nb] = f32x16_t{};
-          sc[0][nb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[nb][ks], sc[0][nb], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int st = 0; st < kAV; ++st) vop[st] = vread(S::kRing - 1, st);
-      // first K operands of step 0 (stage 1) are read inside the step: kAK <= kVs
+      for (int ks = 0; ks < kAK; ++ks) kop[ks] = kread(1, ks);
     }
     for (int j0 = 0; j0 <= nst; j0 += S::kRing) {
       if constexpr (kPaged) {
@@ -396,45 +365,60 @@ __global__ __launch_bounds__(256, NB == 2 ? 1 : 2) void gqa_rows_kernel(const Gq
     wait_vmcnt<0>();  // the last groups have landed before the CTA ends
   }
 
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int r = row0 + 32 * nb + c32, tok = r / G, head = head0 + r - tok * G;
-    const float l = sum_halves(l_run[nb]);
-    if (tok >= E) continue;
-    const bool some = l > 0.f || l != l;
-    const float inv = some ? 1.f / l : 0.f, lse2 = some ? m_ref[nb] + log2f(l) : -INFINITY;
-    if (it.slot >= 0) {
-      const int64_t at = (int64_t)it.slot * kRows + 32 * NB * wave + 32 * nb + c32;
-#pragma unroll
-      for (int db = 0; db < kDb; ++db)
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          f32x4 v;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = O[nb][db][4 * i4 + i] * inv;
-          *reinterpret_cast<f32x4*>(p.ws_o + at * D + 32 * db + 8 * i4 + 4 * g32) = v;
-        }
-      if (g32 == 0) p.ws_lse[at] = lse2;
-      continue;
-    }
-    __bf16* o = p.out + (int64_t)(it.r.q0 + tok) * p.out_stride_t + (int64_t)head * p.out_stride_h;
+  // ---- results: a lane holds row c32, dims 32 db + 8 i4 + 4 g32 + 0..3
+  const float l = sum_halves(l_run);
+  const bool some = l > 0.f || l != l;
+  const float inv = some ? 1.f / l : 0.f, lse2 = some ? m_ref + log2f(l) : -INFINITY;
+  if (it.slot >= 0) {
+    if (!live) return;
+    const int64_t at = (int64_t)it.slot * kRows + 32 * wave + c32;
 #pragma unroll
     for (int db = 0; db < kDb; ++db)
 #pragma unroll
       for (int i4 = 0; i4 < 4; ++i4) {
-        u32x2 v;
-        v[0] = pack_bf16x2(O[nb][db][4 * i4] * inv, O[nb][db][4 * i4 + 1] * inv);
-        v[1] = pack_bf16x2(O[nb][db][4 * i4 + 2] * inv, O[nb][db][4 * i4 + 3] * inv);
-        *reinterpret_cast<u32x2*>(o + 32 * db + 8 * i4 + 4 * g32) = v;
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = O[db][4 * i4 + i] * inv;
+        *reinterpret_cast<f32x4*>(p.ws_o + at * D + 32 * db + 8 * i4 + 4 * g32) = v;
       }
-    if (p.lse != nullptr && g32 == 0) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2 * 0.69314718055994531f;
+    if (g32 == 0) p.ws_lse[at] = lse2;
+    return;
   }
+  if (p.lse != nullptr && g32 == 0 && live) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2 * 0.69314718055994531f;
+  auto packed = [&](int db, int i4) __attribute__((always_inline)) {
+    return u32x2{pack_bf16x2(O[db][4 * i4] * inv, O[db][4 * i4 + 1] * inv), pack_bf16x2(O[db][4 * i4 + 2] * inv, O[db][4 * i4 + 3] * inv)};
+  };
+  auto out_row = [&](int t, int h) __attribute__((always_inline)) { return p.out + (int64_t)(it.r.q0 + t) * p.out_stride_t + (int64_t)h * p.out_stride_h; };
+  if (p.out_16b) {
+    // whole rows at a time, through the wave's part of the rings
+    barrier_lds();  // every wave is done with them
+    MLA_LDS char* mine = (MLA_LDS char*)smem + wave * 32 * kRowB;
+    constexpr int kCh = D / 8;
+#pragma unroll
+    for (int db = 0; db < kDb; ++db)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4)
+        *reinterpret_cast<MLA_LDS u32x2*>(mine + c32 * kRowB + ((4 * db + i4) ^ (c32 % kCh)) * 16 + 8 * g32) = packed(db, i4);
+#pragma unroll
+    for (int i = 0; i < 32 * kCh / 64; ++i) {
+      const int r = i * (64 / kCh) + lane / kCh, c = lane % kCh;
+      const u32x4 v = *reinterpret_cast<const MLA_LDS u32x4*>(mine + r * kRowB + (c ^ (r % kCh)) * 16);
+      const int t = tok_of(r);
+      if (t < E) *reinterpret_cast<u32x4*>(out_row(t, head_of(r, t)) + 8 * c) = v;
+    }
+    return;
+  }
+  if (!live) return;
+#pragma unroll
+  for (int db = 0; db < kDb; ++db)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4) *reinterpret_cast<u32x2*>(out_row(tok, head) + 32 * db + 8 * i4 + 4 * g32) = packed(db, i4);
 }
 
-template <int D, int NB>
+template <int D, int NW>
 void launch_rows(const GqaParams& p, unsigned grid, hipStream_t stream) {
-  if (p.page_table != nullptr) hipLaunchKernelGGL((gqa_rows_kernel<D, NB, true>), dim3(grid), dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((gqa_rows_kernel<D, NB, false>), dim3(grid), dim3(256), 0, stream, p);
+  if (p.page_table != nullptr) hipLaunchKernelGGL((gqa_rows_kernel<D, NW, true>), dim3(grid), dim3(64 * NW), 0, stream, p);
+  else hipLaunchKernelGGL((gqa_rows_kernel<D, NW, false>), dim3(grid), dim3(64 * NW), 0, stream, p);
 }
 
 }  // namespace
@@ -442,13 +426,16 @@ void launch_rows(const GqaParams& p, unsigned grid, hipStream_t stream) {
 hipError_t launch_gqa_merge(const GqaParams& p, int dim, int rows, hipStream_t stream);
 
 hipError_t launch_gqa_rows(const GqaParams& p, int dim, hipStream_t stream) {
+  // the workspace holds pieces of 128 rows
+  if (p.wide && (p.target > 0 || dim != 128)) return hipErrorInvalidValue;
   const int rows = p.wide ? 256 : 128;
   // sum over requests of ceil(E group / rows), then of ceil(L / C) pieces each
   const int64_t blocks = ((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch;
   const int64_t grid = blocks * p.kv_heads + p.target;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  if (dim == 128) p.wide ? launch_rows<128, 2>(p, (unsigned)grid, stream) : launch_rows<128, 1>(p, (unsigned)grid, stream);
-  else p.wide ? launch_rows<64, 2>(p, (unsigned)grid, stream) : launch_rows<64, 1>(p, (unsigned)grid, stream);
+  if (p.wide) launch_rows<128, 8>(p, (unsigned)grid, stream);
+  else if (dim == 128) launch_rows<128, 4>(p, (unsigned)grid, stream);
+  else launch_rows<64, 4>(p, (unsigned)grid, stream);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.target > 0) e = launch_gqa_merge(p, dim, rows, stream);
   return e;

@@ -134,23 +134,37 @@ def test_prompt_strided():
     views = lambda x: (x[:, : hq * d].unflatten(1, (hq, d)), x[:, hq * d : (hq + hk) * d].unflatten(1, (hk, d)),  # noqa: E731
                        x[:, (hq + hk) * d : (hq + 2 * hk) * d].unflatten(1, (hk, d)))
     q, k, v = views(dev)
-    out = torch.full((hq, T + spare, d + 4), NAN, dtype=torch.bfloat16, device=DEV)
-    lse = torch.full((T + spare, hq + 3), NAN, device=DEV)
-    lib.gqa_prompt(q, k, v, i32(cumulative(lens)), d ** -0.5, out[..., :d].transpose(0, 1), lse[:, :hq])
-    torch.cuda.synchronize()
-    check(out[:, :T, :d].transpose(0, 1), lse[:T, :hq], R.prompt(*views(qkv), lens, d ** -0.5))
-    assert out[:, T:].isnan().all() and out[..., d:].isnan().all() and lse[T:].isnan().all() and lse[:, hq:].isnan().all()
+    ref = R.prompt(*views(qkv), lens, d ** -0.5)
+    for more in (4, 8):  # rows of out 8- and 16-byte aligned
+        out = torch.full((hq, T + spare, d + more), NAN, dtype=torch.bfloat16, device=DEV)
+        lse = torch.full((T + spare, hq + 3), NAN, device=DEV)
+        lib.gqa_prompt(q, k, v, i32(cumulative(lens)), d ** -0.5, out[..., :d].transpose(0, 1), lse[:, :hq])
+        torch.cuda.synchronize()
+        check(out[:, :T, :d].transpose(0, 1), lse[:T, :hq], ref)
+        assert out[:, T:].isnan().all() and out[..., d:].isnan().all() and lse[T:].isnan().all() and lse[:, hq:].isnan().all()
 
 
 @pytest.mark.parametrize("dim,heads", [(64, (64, 64)), (128, (48, 48)), (128, (96, 32))])
 def test_many_blocks(dim, heads):
-    """Enough rows to fill the chip with blocks of 256: as a prompt, and as chunks whose pages end inside a stage."""
+    """More blocks than the chip holds at once: as a prompt, and as chunks whose pages end inside a stage."""
     gen = torch.Generator().manual_seed(dim)
     lens = [1500, 1, 290, 33, 1100]
     q, k, v = randn(gen, sum(lens), heads[0], dim), randn(gen, sum(lens), heads[1], dim), randn(gen, sum(lens), heads[1], dim)
     out, lse = run_prompt(q, k, v, lens, dim ** -0.5)
     check(out, lse, R.prompt(q, k, v, lens, dim ** -0.5))
     c = Paged(lens, [300, 5000, 0, 77, 64], *heads, dim, 16, seed=dim)
+    check(*c.run(), c.ref())
+
+
+@pytest.mark.parametrize("heads,page_size", [((72, 24), 1), ((60, 60), 64)])
+def test_blocks_of_256_rows(heads, page_size):
+    """Long requests that fill the chip with wide blocks; the largest prefix passes the looked-up window of rows."""
+    gen = torch.Generator().manual_seed(heads[0])
+    lens = [2700]
+    q, k, v = randn(gen, sum(lens), heads[0], 128), randn(gen, sum(lens), heads[1], 128), randn(gen, sum(lens), heads[1], 128)
+    out, lse = run_prompt(q, k, v, lens, 0.1)
+    check(out, lse, R.prompt(q, k, v, lens, 0.1))
+    c = Paged([1100, 1000], [6000, 40], *heads, 128, page_size, seed=heads[0])
     check(*c.run(), c.ref())
 
 
