@@ -40,7 +40,8 @@ struct GqaParams {
   float* ws_lse;  // [slots, rows] their log2-domain LSEs
   int32_t target;  // items that a batch's keys are split into, about (0: no splitting)
   int32_t fit;     // at most `target`, where that can be
-  int32_t wide;    // blocks of 256 rows (of requests in one piece) instead of 128
+  int32_t wide;    // of requests in one piece: blocks of 256 rows instead of 128; eight waves a CTA of the stream kernel
+                   // instead of four
   int32_t out_16b;  // rows of out start 16-byte aligned
 };
 

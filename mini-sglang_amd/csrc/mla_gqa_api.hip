@@ -22,6 +22,11 @@ constexpr int kStreamRows = 64;
 // length even out; of one in blocks of 128 rows, about kRowsTarget.
 constexpr int kStreamFit = 512;
 constexpr int kStreamTarget = 2048;
+// Keys (at most, by the page table's width) up to which a request is one piece and nothing is joined: with few pairs, a
+// CTA of eight waves each (a request of 500 keys, 8 KV heads 8.6 us, 10.3 in pieces; of 1000 12.5, 10.4: one compute unit
+// loads 64 bytes a cycle), and with many (64 requests of up to 1000 34.5 us, 43.8 in pieces; 200 of them 82, 103).
+constexpr int kStreamOnePieceFew = 512;
+constexpr int kStreamOnePiece = 1024;
 constexpr int kRowsTarget = 512;
 // A chunk batch of at least this many blocks fills the chip without cutting keys.
 constexpr int kRowsEnough = 1024;
@@ -143,8 +148,11 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
   const bool stream_kernel = most <= kStreamRows;
   const int64_t blocks = ((int64_t)total_q * p.group + kRowsBlock - 1) / kRowsBlock * kv_heads;
   if (stream_kernel) {
-    p.fit = 2 * ((int64_t)batch * kv_heads) <= kStreamFit;
-    p.target = p.fit ? kStreamFit : kStreamTarget;
+    const int64_t pairs = (int64_t)batch * kv_heads;
+    p.fit = 2 * pairs <= kStreamFit;
+    const bool short_keys = p.max_keys <= (p.fit ? kStreamOnePieceFew : kStreamOnePiece);
+    p.target = short_keys ? 0 : p.fit ? kStreamFit : kStreamTarget;
+    p.wide = short_keys && p.fit;
   } else {
     p.target = blocks >= kRowsEnough || p.max_keys <= kRowsOnePiece ? 0 : kRowsTarget;
     p.wide = p.target == 0 && wide_blocks(dim, blocks, total_q / batch, p.max_keys);

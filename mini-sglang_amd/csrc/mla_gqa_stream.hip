@@ -1,7 +1,7 @@
 // Grouped-head attention for few rows: single tokens and chunks of up to 64 rows (tokens times group) over a paged
 // cache, with the keys of a batch split over the chip and joined by an fp32 log-sum-exp merge. See mla_gqa.h.
 //
-// One CTA per (request, rows, KV head, piece of the keys). Its four waves take tiles of 32 keys in turn and share
+// One CTA per (request, rows, KV head, piece of the keys). Its NW waves take tiles of 32 keys in turn and share
 // nothing until the end, so there is no barrier in the stream: a wave loads a tile's K straight into the operand layout
 // of the score MFMA and its V through a private LDS tile that transposes it, and requests the next tile before it
 // computes the present one. Bound: HBM (each K and V row is read once).
@@ -13,13 +13,13 @@ namespace {
 constexpr int kTileKeys = 32;
 constexpr float kLowest = -3.4028234663852886e38f;
 
-// NB blocks of 16 rows
-template <int D, int NB>
-__global__ __launch_bounds__(256, NB == 4 && D == 128 ? 1 : 2) void gqa_stream_kernel(const GqaParams p) {
+// NB blocks of 16 rows, NW waves
+template <int D, int NB, int NW>
+__global__ __launch_bounds__(64 * NW, NB == 4 && D == 128 ? 1 : 2) void gqa_stream_kernel(const GqaParams p) {
   constexpr int kRows = 16 * NB, kRowB = D * 2, kChunks = D / 8, kKs = D / 32, kDb = D / 16;
   constexpr int kLoads = kTileKeys * kChunks / 64;  // 16-byte loads of a lane per K or V tile
-  __shared__ __attribute__((aligned(16))) char s_k[4][kTileKeys * kRowB], s_v[4][kTileKeys * kRowB];
-  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ __attribute__((aligned(16))) char s_k[NW][kTileKeys * kRowB], s_v[NW][kTileKeys * kRowB];
+  __shared__ float s_m[NW][16], s_l[NW][16];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GqaItem it;
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256, NB == 4 && D == 128 ? 1 : 2) void gqa_stream_k
   // the transposing V reads (8 rows' chunk pairs) meet in a bank
   auto pos = [&](int t, int c) __attribute__((always_inline)) { return t * kRowB + (D == 128 ? c ^ (2 * (t & 7)) : c ^ (2 * ((t >> 1) & 3))) * 16; };
 
-  constexpr int kStep = 4 * kTileKeys;
+  constexpr int kStep = NW * kTileKeys;
   int t0 = k0 + kTileKeys * wave, row_next = 0;
   if (t0 < k1) {
     const int row = rows(t0);
@@ -166,14 +166,15 @@ __global__ __launch_bounds__(256, NB == 4 && D == 128 ? 1 : 2) void gqa_stream_k
       s_l[wave][a16] = lw;
     }
     __syncthreads();
-    // thread: row threadIdx / 16, dims in steps of 64 from 4 (threadIdx % 16)
-    const int row = threadIdx.x >> 4, x = threadIdx.x & 15;
+    // kTpr threads a row, 4 dims each at a time
+    constexpr int kTpr = 4 * NW;
+    const int row = threadIdx.x / kTpr, x = threadIdx.x % kTpr;
     float mt = s_m[0][row];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) mt = fmaxf(mt, s_m[w][row]);
-    float f[4], lt = 0.f;
+    for (int w = 1; w < NW; ++w) mt = fmaxf(mt, s_m[w][row]);
+    float f[NW], lt = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       f[w] = __builtin_amdgcn_exp2f(s_m[w][row] - mt);
       lt += f[w] * s_l[w][row];
     }
@@ -182,11 +183,10 @@ __global__ __launch_bounds__(256, NB == 4 && D == 128 ? 1 : 2) void gqa_stream_k
     const int r = it.block * kRows + 16 * nb + row, tok = r / G, head = it.head * G + r % G;
     if (tok >= E) continue;
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) {
-      const int c = 16 * d + x;
+    for (int c = x; c < D / 4; c += kTpr) {
       f32x4 o = f32x4{};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) o += *reinterpret_cast<const f32x4*>(s_v[w] + row * (D * 4) + ((c + row) % (D / 4)) * 16) * f[w];
+      for (int w = 0; w < NW; ++w) o += *reinterpret_cast<const f32x4*>(s_v[w] + row * (D * 4) + ((c + row) % (D / 4)) * 16) * f[w];
       o *= inv;
       if (it.slot >= 0) {
         *reinterpret_cast<f32x4*>(p.ws_o + ((int64_t)it.slot * kRows + 16 * nb + row) * D + 4 * c) = o;
@@ -281,7 +281,13 @@ __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams 
 
 template <int D, int NB>
 void launch_stream(const GqaParams& p, int64_t grid, hipStream_t stream) {
-  hipLaunchKernelGGL((gqa_stream_kernel<D, NB>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+  if constexpr (NB < 4) {
+    if (p.wide) {
+      hipLaunchKernelGGL((gqa_stream_kernel<D, NB, 8>), dim3((unsigned)grid), dim3(512), 0, stream, p);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((gqa_stream_kernel<D, NB, 4>), dim3((unsigned)grid), dim3(256), 0, stream, p);
 }
 
 }  // namespace

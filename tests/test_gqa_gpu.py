@@ -156,15 +156,15 @@ def test_many_blocks(dim, heads):
     check(*c.run(), c.ref())
 
 
-@pytest.mark.parametrize("heads,page_size", [((72, 24), 1), ((60, 60), 64)])
+@pytest.mark.parametrize("heads,page_size", [((51, 17), 1)])
 def test_blocks_of_256_rows(heads, page_size):
     """Long requests that fill the chip with wide blocks; the largest prefix passes the looked-up window of rows."""
     gen = torch.Generator().manual_seed(heads[0])
-    lens = [2700]
+    lens = [2600]
     q, k, v = randn(gen, sum(lens), heads[0], 128), randn(gen, sum(lens), heads[1], 128), randn(gen, sum(lens), heads[1], 128)
     out, lse = run_prompt(q, k, v, lens, 0.1)
     check(out, lse, R.prompt(q, k, v, lens, 0.1))
-    c = Paged([1100, 1000], [6000, 40], *heads, 128, page_size, seed=heads[0])
+    c = Paged([1600, 1000], [3500, 40], *heads, 128, page_size, seed=heads[0])
     check(*c.run(), c.ref())
 
 
@@ -185,7 +185,7 @@ def test_chunk_groups(heads, extends):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("lens", [[1], [2, 31, 32, 33, 127, 128, 129], [5000], [1, 9000, 300], [257] * 70])
+@pytest.mark.parametrize("lens", [[1], [2, 31, 32, 33, 127, 128, 129], [5000], [1, 9000, 300], [257] * 70, [300, 1, 512], [700] * 70 + [1024, 3] * 40])
 def test_decode_lengths(dim, lens):
     c = Paged([1] * len(lens), [n - 1 for n in lens], 8, 2, dim, 16, seed=len(lens) + lens[0])
     ref = c.ref()
