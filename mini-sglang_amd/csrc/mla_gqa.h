@@ -206,6 +206,41 @@ __device__ __forceinline__ int gqa_row(const GqaParams& p, int b, int q0, int j)
   return (pid << p.log2_ps) + (j & ((1 << p.log2_ps) - 1));
 }
 
+// A row's values that are not finite, although its sum is: V held an infinity or a NaN at some key, and if the row does
+// not attend that key, the matrix product (weight zero times it) put it there all the same. The row by itself, over the
+// keys of the item that it attends, by the whole wave: as slow as it is rare. m: its reference (log2 domain); at: its
+// row of the workspace.
+template <int D>
+__device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem& it, int r, int k0, int k1, float m, int64_t at) {
+  typedef __bf16 dims_t __attribute__((ext_vector_type(D / 64)));
+  typedef float part_t __attribute__((ext_vector_type(D / 64)));
+  const int d0 = (threadIdx.x & 63) * (D / 64), tok = r / p.group, head = it.head * p.group + r % p.group;
+  const int end = min(k1, it.r.P + tok + 1);
+  auto load = [&](const __bf16* x) { return __builtin_convertvector(*reinterpret_cast<const dims_t*>(x + d0), part_t); };
+  const part_t q = load(p.q + (int64_t)(it.r.q0 + tok) * p.q_stride_t + (int64_t)head * p.q_stride_h);
+  part_t o = {};
+  float l = 0.f;
+  for (int j = k0; j < end; ++j) {
+    const int64_t row = gqa_row(p, it.b, it.r.q0, j);
+    const part_t x = q * load(p.k + row * p.k_row_stride + (int64_t)it.head * p.k_head_stride);
+    float s = x[0];
+    if constexpr (D == 128) s += x[1];
+    const float e = __builtin_amdgcn_exp2f(fmaf(wave_sum64(s), p.scale_log2, -m));
+    l += e;
+    o += e * load(p.v + row * p.v_row_stride + (int64_t)it.head * p.v_head_stride);
+  }
+  o *= l > 0.f ? 1.f / l : 0.f;
+  wait_vmcnt<0>();  // after the row's first stores
+  if (it.slot >= 0) {
+    *reinterpret_cast<part_t*>(p.ws_o + at * D + d0) = o;
+  } else {
+    *reinterpret_cast<dims_t*>(p.out + (int64_t)(it.r.q0 + tok) * p.out_stride_t + (int64_t)head * p.out_stride_h + d0) = __builtin_convertvector(o, dims_t);
+  }
+}
+
+// A launch holds fewer than 2^32 threads.
+inline bool gqa_grid_ok(int64_t ctas, int threads) { return ctas <= 0x7fffffff && ctas * threads <= (int64_t)UINT32_MAX; }
+
 hipError_t launch_gqa_rows(const GqaParams& p, int dim, hipStream_t stream);    // many rows a request
 hipError_t launch_gqa_stream(const GqaParams& p, int dim, hipStream_t stream);  // up to 64 rows a request
 

@@ -85,6 +85,7 @@ int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_str
   if (lse != nullptr && total_q > 1 && lse_stride_t < q_heads)
     return api_error(MLA_ERR_INVALID_ARG, "%s: lse_stride_t %lld < %d heads", who, (long long)lse_stride_t, q_heads);
   if (!(scale > 0.f) || !isfinite(scale)) return api_error(MLA_ERR_INVALID_ARG, "%s: bad scale", who);
+  if (batch > 65535) return api_error(MLA_ERR_UNSUPPORTED, "%s: at most 65535 requests, got %d", who, batch);
   if ((int64_t)total_q * q_heads > 0x7fffffff) return api_error(MLA_ERR_UNSUPPORTED, "%s: total_q * q_heads passes 2^31", who);
   p.q = static_cast<const __bf16*>(q);
   p.q_stride_t = q_stride_t;

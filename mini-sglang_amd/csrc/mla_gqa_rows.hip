@@ -60,11 +60,11 @@ constexpr bool rings_ok() {
 }
 static_assert(rings_ok<4>() && rings_ok<8>(), "ring lengths");
 
-// Position of 16-byte chunk c of token t in a K / V row of an LDS tile.
+// Position of 16-byte chunk c of token t in a K / V row of an LDS tile. A 16-byte read serves 16 lanes at a time, of each
+// 32 lanes 0-3, 12-15 and 20-27, then the others: their tokens' chunks lie in different banks.
 template <int D>
 __device__ __forceinline__ int kchunk(int c, int t) {
-  const int hi = ((t >> 3) ^ (t >> 4)) & 1;
-  return D == 128 ? c ^ ((t & 7) | (hi << 3)) : c ^ (((t >> 1) & 3) | (hi << 2));
+  return D == 128 ? c ^ (t & 15) : c ^ ((t >> 1) & 7);
 }
 template <int D>
 __device__ __forceinline__ int vchunk(int c, int t) {
@@ -369,50 +369,65 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
   const float l = sum_halves(l_run);
   const bool some = l > 0.f || l != l;
   const float inv = some ? 1.f / l : 0.f, lse2 = some ? m_ref + log2f(l) : -INFINITY;
+  const int64_t at = (int64_t)it.slot * kRows + 32 * wave + c32;
   if (it.slot >= 0) {
-    if (!live) return;
-    const int64_t at = (int64_t)it.slot * kRows + 32 * wave + c32;
+    if (live) {
 #pragma unroll
-    for (int db = 0; db < kDb; ++db)
+      for (int db = 0; db < kDb; ++db)
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        f32x4 v;
+        for (int i4 = 0; i4 < 4; ++i4) {
+          f32x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = O[db][4 * i4 + i] * inv;
-        *reinterpret_cast<f32x4*>(p.ws_o + at * D + 32 * db + 8 * i4 + 4 * g32) = v;
-      }
-    if (g32 == 0) p.ws_lse[at] = lse2;
-    return;
-  }
-  if (p.lse != nullptr && g32 == 0 && live) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2 * 0.69314718055994531f;
-  auto packed = [&](int db, int i4) __attribute__((always_inline)) {
-    return u32x2{pack_bf16x2(O[db][4 * i4] * inv, O[db][4 * i4 + 1] * inv), pack_bf16x2(O[db][4 * i4 + 2] * inv, O[db][4 * i4 + 3] * inv)};
-  };
-  auto out_row = [&](int t, int h) __attribute__((always_inline)) { return p.out + (int64_t)(it.r.q0 + t) * p.out_stride_t + (int64_t)h * p.out_stride_h; };
-  if (p.out_16b) {
-    // whole rows at a time, through the wave's part of the rings
-    barrier_lds();  // every wave is done with them
-    MLA_LDS char* mine = (MLA_LDS char*)smem + wave * 32 * kRowB;
-    constexpr int kCh = D / 8;
-#pragma unroll
-    for (int db = 0; db < kDb; ++db)
-#pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4)
-        *reinterpret_cast<MLA_LDS u32x2*>(mine + c32 * kRowB + ((4 * db + i4) ^ (c32 % kCh)) * 16 + 8 * g32) = packed(db, i4);
-#pragma unroll
-    for (int i = 0; i < 32 * kCh / 64; ++i) {
-      const int r = i * (64 / kCh) + lane / kCh, c = lane % kCh;
-      const u32x4 v = *reinterpret_cast<const MLA_LDS u32x4*>(mine + r * kRowB + (c ^ (r % kCh)) * 16);
-      const int t = tok_of(r);
-      if (t < E) *reinterpret_cast<u32x4*>(out_row(t, head_of(r, t)) + 8 * c) = v;
+          for (int i = 0; i < 4; ++i) v[i] = O[db][4 * i4 + i] * inv;
+          *reinterpret_cast<f32x4*>(p.ws_o + at * D + 32 * db + 8 * i4 + 4 * g32) = v;
+        }
+      if (g32 == 0) p.ws_lse[at] = lse2;
     }
-    return;
+  } else {
+    if (p.lse != nullptr && g32 == 0 && live) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2 * 0.69314718055994531f;
+    auto packed = [&](int db, int i4) __attribute__((always_inline)) {
+      return u32x2{pack_bf16x2(O[db][4 * i4] * inv, O[db][4 * i4 + 1] * inv), pack_bf16x2(O[db][4 * i4 + 2] * inv, O[db][4 * i4 + 3] * inv)};
+    };
+    auto out_row = [&](int t, int h) __attribute__((always_inline)) { return p.out + (int64_t)(it.r.q0 + t) * p.out_stride_t + (int64_t)h * p.out_stride_h; };
+    if (p.out_16b) {
+      // whole rows at a time, through the wave's part of the rings
+      barrier_lds();  // every wave is done with them
+      MLA_LDS char* mine = (MLA_LDS char*)smem + wave * 32 * kRowB;
+      constexpr int kCh = D / 8;
+#pragma unroll
+      for (int db = 0; db < kDb; ++db)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+          *reinterpret_cast<MLA_LDS u32x2*>(mine + c32 * kRowB + ((4 * db + i4) ^ (c32 % kCh)) * 16 + 8 * g32) = packed(db, i4);
+#pragma unroll
+      for (int i = 0; i < 32 * kCh / 64; ++i) {
+        const int r = i * (64 / kCh) + lane / kCh, c = lane % kCh;
+        const u32x4 v = *reinterpret_cast<const MLA_LDS u32x4*>(mine + r * kRowB + (c ^ (r % kCh)) * 16);
+        const int t = tok_of(r);
+        if (t < E) *reinterpret_cast<u32x4*>(out_row(t, head_of(r, t)) + 8 * c) = v;
+      }
+    } else if (live) {
+#pragma unroll
+      for (int db = 0; db < kDb; ++db)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) *reinterpret_cast<u32x2*>(out_row(tok, head) + 32 * db + 8 * i4 + 4 * g32) = packed(db, i4);
+    }
   }
-  if (!live) return;
+  // finite sums times 0 are 0
+  float zero = 0.f;
 #pragma unroll
   for (int db = 0; db < kDb; ++db)
 #pragma unroll
-    for (int i4 = 0; i4 < 4; ++i4) *reinterpret_cast<u32x2*>(out_row(tok, head) + 32 * db + 8 * i4 + 4 * g32) = packed(db, i4);
+    for (int i = 0; i < 16; ++i) zero = fmaf(O[db][i], 0.f, zero);
+  uint64_t bad = __ballot(live && zero != 0.f && l < INFINITY);
+  if (__builtin_expect(bad != 0, 0)) {
+    bad = (bad | bad >> 32) & 0xffffffff;
+    for (; bad != 0; bad &= bad - 1) {
+      const int i = __builtin_ctzll(bad);
+      const float m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, m_ref), i));
+      gqa_row_again<D>(p, it, row0 + i, k0, k1, m, (int64_t)it.slot * kRows + 32 * wave + i);
+    }
+  }
 }
 
 template <int D, int NW>
@@ -432,7 +447,7 @@ hipError_t launch_gqa_rows(const GqaParams& p, int dim, hipStream_t stream) {
   // sum over requests of ceil(E group / rows), then of ceil(L / C) pieces each
   const int64_t blocks = ((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch;
   const int64_t grid = blocks * p.kv_heads + p.target;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  if (!gqa_grid_ok(grid, 2 * rows)) return hipErrorInvalidValue;
   if (p.wide) launch_rows<128, 8>(p, (unsigned)grid, stream);
   else if (dim == 128) launch_rows<128, 4>(p, (unsigned)grid, stream);
   else launch_rows<64, 4>(p, (unsigned)grid, stream);

@@ -181,12 +181,14 @@ __global__ __launch_bounds__(64 * NW, NB == 4 && D == 128 ? 1 : 2) void gqa_stre
     const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
     const float lse2 = lt > 0.f || lt != lt ? mt + log2f(lt) : -INFINITY;
     const int r = it.block * kRows + 16 * nb + row, tok = r / G, head = it.head * G + r % G;
-    if (tok >= E) continue;
+    float zero = 0.f;
 #pragma unroll
-    for (int c = x; c < D / 4; c += kTpr) {
+    for (int c = tok < E ? x : D; c < D / 4; c += kTpr) {
       f32x4 o = f32x4{};
 #pragma unroll
       for (int w = 0; w < NW; ++w) o += *reinterpret_cast<const f32x4*>(s_v[w] + row * (D * 4) + ((c + row) % (D / 4)) * 16) * f[w];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zero = fmaf(o[i], 0.f, zero);
       o *= inv;
       if (it.slot >= 0) {
         *reinterpret_cast<f32x4*>(p.ws_o + ((int64_t)it.slot * kRows + 16 * nb + row) * D + 4 * c) = o;
@@ -195,9 +197,19 @@ __global__ __launch_bounds__(64 * NW, NB == 4 && D == 128 ? 1 : 2) void gqa_stre
         *reinterpret_cast<u32x2*>(p.out + (int64_t)(it.r.q0 + tok) * p.out_stride_t + (int64_t)head * p.out_stride_h + 4 * c) = v;
       }
     }
-    if (x == 0) {
+    if (x == 0 && tok < E) {
       if (it.slot >= 0) p.ws_lse[(int64_t)it.slot * kRows + 16 * nb + row] = lse2;
       else if (p.lse != nullptr) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2 * 0.69314718055994531f;
+    }
+    uint64_t bad = __ballot(zero != 0.f && lt < INFINITY);  // finite sums times 0 are 0
+    if (__builtin_expect(bad != 0, 0)) {
+      while (bad != 0) {
+        const int first = __builtin_ctzll(bad) / kTpr * kTpr;  // the row's first lane
+        const int i = (64 * wave + first) / kTpr;
+        const float m_row = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mt), first));
+        gqa_row_again<D>(p, it, it.block * kRows + 16 * nb + i, k0, k1, m_row, (int64_t)it.slot * kRows + 16 * nb + i);
+        bad &= ~(((1ull << kTpr) - 1) << first);
+      }
     }
   }
 }
@@ -294,6 +306,7 @@ void launch_stream(const GqaParams& p, int64_t grid, hipStream_t stream) {
 
 hipError_t launch_gqa_merge(const GqaParams& p, int dim, int rows, hipStream_t stream) {
   const int64_t grid = (int64_t)p.total_q * p.kv_heads * p.group;
+  if (!gqa_grid_ok(grid, 64)) return hipErrorInvalidValue;
   // few rows are cut into many pieces
 #define MLA_MERGE(D, R)                                                                                            \
   if (dim == D && rows == R) {                                                                                     \
@@ -317,7 +330,7 @@ hipError_t launch_gqa_stream(const GqaParams& p, int dim, hipStream_t stream) {
   const int rows = most <= 16 ? 16 : most <= 32 ? 32 : 64;
   const int64_t blocks = ((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch;
   const int64_t grid = blocks * p.kv_heads + p.target;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  if (!gqa_grid_ok(grid, 512)) return hipErrorInvalidValue;
   if (dim == 128) rows == 16 ? launch_stream<128, 1>(p, grid, stream) : rows == 32 ? launch_stream<128, 2>(p, grid, stream) : launch_stream<128, 4>(p, grid, stream);
   else rows == 16 ? launch_stream<64, 1>(p, grid, stream) : rows == 32 ? launch_stream<64, 2>(p, grid, stream) : launch_stream<64, 4>(p, grid, stream);
   hipError_t e = hipGetLastError();

@@ -637,8 +637,8 @@ def _gqa_paged(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens, max_q: int
     assert len(ks) == 4 and sk[0] == ks[1] * sk[1] and sv[0] == ks[1] * sv[1], "pools are [pages, ps, Hkv, D], pages one after another"
     assert page_table.dtype is torch.int32 and len(ps) == 2 and ps[0] >= B and sp[1] == 1 and page_table.get_device() == device, (
         "page_table is int32 [B, cols], on q's GPU")
-    Hkv = ks[2]
-    ws, nbytes = _workspace(workspace, gqa_workspace_bytes(min(max_q, T), Hq, Hkv, D), q, device, stream)
+    Hkv, max_q = ks[2], min(max_q, T)
+    ws, nbytes = _workspace(workspace, gqa_workspace_bytes(max_q, Hq, Hkv, D), q, device, stream)
     lens = _check_index(seq_lens, B, device, "seq_lens")
     lse_ptr = None if lse is None else lse.data_ptr()
     cache = (q.data_ptr(), sq[0], sq[1], k_pool.data_ptr(), sk[1], sk[2], v_pool.data_ptr(), sv[1], sv[2], ks[0], ks[1],

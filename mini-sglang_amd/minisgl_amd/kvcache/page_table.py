@@ -79,6 +79,7 @@ class PagedTokenTable:
         batch's dummy) follow and take no pages. The rows of ``reqs`` must be distinct."""
         reqs, ps = list(reqs), self.page_size
         batch = reqs + list(padding)
+        assert batch, "a step has requests"
         assert len({r.table_idx for r in reqs}) == len(reqs), "requests that take pages have rows of their own"
         needed = sum(-(-r.device_len // ps) - -(-r.cached_len // ps) for r in reqs)
         if needed > self.free_pages:

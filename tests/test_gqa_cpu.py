@@ -56,14 +56,14 @@ ATTENTION = [
     (dict(q=None), INVALID, "null"), (dict(k=None), INVALID, "null"), (dict(v=None), INVALID, "null"), (dict(out=None), INVALID, "null"),
     (dict(q=P + 8), INVALID, "aligned"), (dict(k=P + 2), INVALID, "aligned"), (dict(v=P + 8), INVALID, "aligned"), (dict(out=P + 4), INVALID, "aligned"),
     (dict(qt=1028), INVALID, "q strides"), (dict(qh=-128), INVALID, "q strides"),
-    (dict(kr=260), INVALID, "k and v strides"), (dict(kh=4), INVALID, "k and v strides"), (dict(vr=-256), INVALID, "k and v strides"),
+    (dict(kr=1 << 32), UNSUPPORTED, "4 GiB"), (dict(kr=260), INVALID, "k and v strides"), (dict(kh=4), INVALID, "k and v strides"), (dict(vr=-256), INVALID, "k and v strides"),
     (dict(oh=124), INVALID, "out strides"), (dict(ot=1022), INVALID, "out strides"), (dict(ot=1020), INVALID, "out strides"),
-    (dict(lt=7), INVALID, "lse_stride"), (dict(scale=0.0), INVALID, "scale"), (dict(scale=float("nan")), INVALID, "scale"),
+    (dict(hq=8192, hk=1), UNSUPPORTED, "query heads"), (dict(lt=7), INVALID, "lse_stride"), (dict(scale=0.0), INVALID, "scale"), (dict(scale=float("nan")), INVALID, "scale"),
     (dict(scale=float("inf")), INVALID, "scale"),
 ]
 PAGED = [
     (dict(ps=24), UNSUPPORTED, "page_size"), (dict(ps=0), UNSUPPORTED, "page_size"), (dict(pages=0), INVALID, "num_pages"),
-    (dict(cols=0), INVALID, "pt_cols"), (dict(pts=3), INVALID, "pt_stride"), (dict(pt=None), INVALID, "null"), (dict(lens=None), INVALID, "null"),
+    (dict(pages=1 << 20, ps=1 << 12), UNSUPPORTED, "2^31 rows"), (dict(batch=70000), UNSUPPORTED, "65535"), (dict(cols=0), INVALID, "pt_cols"), (dict(pts=3), INVALID, "pt_stride"), (dict(pt=None), INVALID, "null"), (dict(lens=None), INVALID, "null"),
     (dict(ws=None), INVALID, "null"), (dict(ws=P + 8), INVALID, "workspace"), (dict(ws_bytes=1000), INVALID, "workspace"),
 ]
 
@@ -123,6 +123,8 @@ def test_step_refuses_shared_rows_and_missing_pages():
         table.allocate_step([Req(table_idx=1, cached_len=0, device_len=1), Req(table_idx=1, cached_len=0, device_len=1)])
     with pytest.raises(RuntimeError, match="out of KV pages: 5 needed, 4 free"):
         table.allocate_step([Req(table_idx=0, cached_len=0, device_len=17), Req(table_idx=1, cached_len=0, device_len=33)])
+    with pytest.raises(AssertionError, match="has requests"):
+        table.allocate_step([])
     with pytest.raises(AssertionError, match="holds 64 tokens"):
         table.allocate_step([Req(table_idx=0, cached_len=65, device_len=66)])
     assert table.free_pages == 4

@@ -276,6 +276,33 @@ def test_values_that_are_nan_stay_in_their_request():
         assert (x.double().cpu() - y).abs().max() < 0.05
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [NAN, float("inf"), -float("inf")])
+def test_later_tokens_that_are_not_finite_reach_no_earlier_row(dim, value):
+    """The last tokens' K and V are NaN or infinite: the queries before them are as without them, in one piece and in
+    several (a piece that no early query reaches included); those that attend them are not finite."""
+    gen = torch.Generator().manual_seed(23)
+    lens = [200, 70]
+    q, k, v = (randn(gen, sum(lens), h, dim) for h in (6, 2, 2))
+    ref = R.prompt(q, k, v, lens, 0.1)
+    last = [198, 199, 269]
+    keep = [i for i in range(270) if i not in last]
+    for t in (k, v):
+        t[last] = value
+    out, lse = run_prompt(q, k, v, lens, 0.1)
+    check(out[keep], lse[keep], R.Attention(*(x[keep] for x in ref)))
+    assert not out[last].isfinite().any(-1).all(-1).any()
+    for extends, prefixes, heads in (([4, 2], [40, 2000], (6, 2)), ([4, 2], [300, 100], (6, 2)), ([90, 2], [3000, 40], (6, 2)), ([20], [1300], (4, 1)), ([20], [900], (8, 2))):
+        c = Paged(extends, prefixes, *heads, dim, 16, seed=24)
+        ref = c.ref()
+        at = int(c.pt[0, (c.lens[0] - 1) // 16]) * 16 + (c.lens[0] - 1) % 16
+        c.v.view(-1, heads[1], dim)[at] = value
+        out, lse = c.run()
+        keep = [i for i in range(c.T) if i != extends[0] - 1]
+        check(out[keep], lse[keep], R.Attention(*(x[keep] for x in ref)), f"{extends} on {prefixes}")
+        assert not out[extends[0] - 1].isfinite().any()
+
+
 @pytest.mark.parametrize("extends", [[1, 1], [160, 20]])
 def test_pool_past_32_bits(extends):
     """K and V rows past 2^31 bytes and 2^31 elements from the pool's start."""
