@@ -338,7 +338,7 @@ int mla_q_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, int32
  *        Rows of q behind the last request are not read, and those of out and lse stay as they are.
  * A key or value that a query does not attend does not reach its row, whatever it holds: cache rows past a length are
  * not read, and a row that an infinity or a NaN in a later token's value came near (weight zero times it, in the matrix
- * product) is computed again by itself, which is slow (1.5 us per row and 1000 keys).
+ * product) is computed again by itself, which is slow (0.13 ms per 1000 keys).
  *
  * mla_gqa_prompt_bf16: whole prompts; k and v are packed like q (row cu_seqlens[b] + j), as many keys as queries.
  */

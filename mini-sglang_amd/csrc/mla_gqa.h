@@ -206,28 +206,59 @@ __device__ __forceinline__ int gqa_row(const GqaParams& p, int b, int q0, int j)
   return (pid << p.log2_ps) + (j & ((1 << p.log2_ps) - 1));
 }
 
-// A row's values that are not finite, although its sum is: V held an infinity or a NaN at some key, and if the row does
-// not attend that key, the matrix product (weight zero times it) put it there all the same. The row by itself, over the
-// keys of the item that it attends, by the whole wave: as slow as it is rare. m: its reference (log2 domain); at: its
-// row of the workspace.
+// For a row whose values are not finite although its sum is: V held an infinity or a NaN at some key. If one of the
+// item's keys that the row does not attend holds one, the matrix product (weight zero times it) may have put it there,
+// and the row is computed by itself over the keys that it attends, by the whole wave, until it is NaN throughout: slow
+// (0.13 ms per 1000 keys) and rare. m: the row's reference (log2 domain); at: its row of the workspace.
 template <int D>
 __device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem& it, int r, int k0, int k1, float m, int64_t at) {
   typedef __bf16 dims_t __attribute__((ext_vector_type(D / 64)));
   typedef float part_t __attribute__((ext_vector_type(D / 64)));
+  constexpr int kU = 8;  // keys in flight
   const int d0 = (threadIdx.x & 63) * (D / 64), tok = r / p.group, head = it.head * p.group + r % p.group;
-  const int end = min(k1, it.r.P + tok + 1);
+  const int end = min(k1, it.r.P + tok + 1), hi = min(it.r.L, k0 + ((k1 - k0 + 31) & ~31));
   auto load = [&](const __bf16* x) { return __builtin_convertvector(*reinterpret_cast<const dims_t*>(x + d0), part_t); };
+  auto value = [&](int64_t row) { return load(p.v + row * p.v_row_stride + (int64_t)it.head * p.v_head_stride); };
+  auto finite = [](part_t x) {
+    float zero = x[0] * 0.f;
+    if constexpr (D == 128) zero = fmaf(x[1], 0.f, zero);
+    return zero == 0.f;
+  };
+  bool near = false;
+  for (int j = max(end, k0); j < hi && !near; j += kU) {
+    part_t v[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) v[u] = value(gqa_row(p, it.b, it.r.q0, min(j + u, hi - 1)));
+    bool all = true;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) all = all && finite(v[u]);
+    near = __ballot(!all) != 0;
+  }
+  if (!near) return;
   const part_t q = load(p.q + (int64_t)(it.r.q0 + tok) * p.q_stride_t + (int64_t)head * p.q_stride_h);
   part_t o = {};
   float l = 0.f;
-  for (int j = k0; j < end; ++j) {
-    const int64_t row = gqa_row(p, it.b, it.r.q0, j);
-    const part_t x = q * load(p.k + row * p.k_row_stride + (int64_t)it.head * p.k_head_stride);
-    float s = x[0];
-    if constexpr (D == 128) s += x[1];
-    const float e = __builtin_amdgcn_exp2f(fmaf(wave_sum64(s), p.scale_log2, -m));
-    l += e;
-    o += e * load(p.v + row * p.v_row_stride + (int64_t)it.head * p.v_head_stride);
+  for (int j = k0; j < end; j += kU) {
+    part_t x[kU], v[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int64_t row = gqa_row(p, it.b, it.r.q0, min(j + u, end - 1));
+      x[u] = q * load(p.k + row * p.k_row_stride + (int64_t)it.head * p.k_head_stride);
+      v[u] = value(row);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      float s = x[u][0];
+      if constexpr (D == 128) s += x[u][1];
+      const float e = __builtin_amdgcn_exp2f(fmaf(wave_sum64(s), p.scale_log2, -m));
+      if (j + u < end) {
+        l += e;
+        o += e * v[u];
+      }
+    }
+    bool done = o[0] != o[0];
+    if constexpr (D == 128) done = done && o[1] != o[1];
+    if (__ballot(!done) == 0) break;
   }
   o *= l > 0.f ? 1.f / l : 0.f;
   wait_vmcnt<0>();  // after the row's first stores
