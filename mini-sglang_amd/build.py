@@ -1,8 +1,9 @@
-"""Build libmla_amd.so (gfx950) from csrc/*.hip with hipcc, in-tree.
+"""Build libmla_amd.so (gfx950) from csrc/*.hip with hipcc, in-tree, and the Python calls of its short launches
+(csrc/binding, a CPython module over torch's C++ tensors) with g++.
 
 Usage: python mini-sglang_amd/build.py [--jobs N]
-The library lands in minisgl_amd/kernel/libmla_amd.so, where
-minisgl_amd.kernel.lib loads it. Every call recompiles, and
+The library lands in minisgl_amd/kernel/libmla_amd.so and the module beside it, where
+minisgl_amd.kernel.lib loads them. Every call recompiles, and
 fails if the device assembly breaks a wait-state rule (asm_check.py).
 """
 
@@ -26,6 +27,9 @@ OUT = os.path.join(HERE, "minisgl_amd", "kernel", "libmla_amd.so")
 # measured-peak kernels of the benchmark: a separate library, not part of libmla_amd's ABI
 PEAKS_SRC = os.path.join(CSRC, "peaks", "mla_peaks.hip")
 PEAKS_OUT = os.path.join(HERE, "minisgl_amd", "benchmark", "libmla_peaks.so")
+# Python calls of the entry points with short launches
+BINDING_SRC = os.path.join(CSRC, "binding", "mla_torch.cpp")
+BINDING_OUT = os.path.join(HERE, "minisgl_amd", "kernel", "_mla_torch.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 # packed-fp32 VALU forms are disabled for all device code built here.
@@ -78,16 +82,36 @@ def _link(objs, out: str) -> None:
     os.replace(tmp, out)
 
 
+def _build_binding() -> None:
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    include = os.path.join(root, "include")
+    tmp = BINDING_OUT + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-std=c++17", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{include}",
+           f"-I{os.path.join(include, 'torch', 'csrc', 'api', 'include')}", f"-I{sysconfig.get_paths()['include']}",
+           BINDING_SRC, "-o", tmp, f"-L{os.path.join(root, 'lib')}", "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{res.stderr}")
+    os.replace(tmp, BINDING_OUT)
+
+
 def build(jobs: int | None = None, verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
     sources = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     jobs = jobs or min(8, len(sources) + 1)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        binding = ex.submit(_build_binding)
         objs = list(ex.map(_compile, sources + [PEAKS_SRC]))
+        binding.result()
     _link(objs[:-1], OUT)
     _link(objs[-1:], PEAKS_OUT)
     if verbose:
-        print(f"built {OUT} from {len(sources)} sources, and {PEAKS_OUT}")
+        print(f"built {OUT} from {len(sources)} sources, {BINDING_OUT} and {PEAKS_OUT}")
     return OUT
 
 

@@ -517,66 +517,51 @@ def qkv_a_rows(qkv, q_rank: int, q_norm_weight, kv_norm_weight, positions, cos_s
     return out
 
 
-# The calls below are short on the GPU (a decode step's tables take 4 us), so each tensor is looked at once, and what
-# they share is not in helpers that pass tuples on (decode 20 -> 15 us on the host).
+# The calls below are short on the GPU (a decode step's tables take 4 us), so their tensors are checked and read in C++
+# (csrc/binding/mla_torch.cpp: a decode call 13.4 -> 8.2 us on the host, 6 of them its two launches; a step's tables 11.2 ->
+# 5.2) where the calls above do it here and in ctypes.
 
 
-def _launch(fn, name: str, device: int, stream, args) -> None:
-    """``fn(*args, stream)`` (default: the current stream of GPU ``device``) with that GPU current: launches go by it,
-    and the tensors may be on another than the caller's."""
+@functools.lru_cache(maxsize=None)
+def load_binding():
+    import torch  # loads the libraries that the module needs
+
+    lib = load_library()
+    try:
+        from . import _mla_torch as binding
+    except ImportError as e:
+        raise MLAKernelError(f"minisgl_amd.kernel._mla_torch does not load ({e}): build it with "
+                             "`python mini-sglang_amd/build.py`") from e
+    entry_points = (lib.mla_gqa_prompt_bf16, lib.mla_gqa_workspace_bytes, lib.mla_gqa_chunk_bf16, lib.mla_gqa_decode_bf16,
+                    lib.mla_page_tables_from_lengths)
+    binding.bind(*(ctypes.cast(f, _vp).value for f in entry_points), torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+    return binding
+
+
+_OTHER_DEVICE = -1
+
+
+def _again(device, call, name: str, *args):
+    """The rest of a call that did not go through at once: with the tensors' GPU current, or its error."""
     import torch
 
-    if torch._C._cuda_getDevice() == device:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream)
-    if rc != 0:
+    with torch.cuda.device(device):
+        rc = call(*args)
+    if isinstance(rc, int) and rc != 0:
         check(rc, name)
-
-
-def _check_gqa(device: int, shape, ks, q, k, v, out, lse) -> None:
-    """What the attention calls share; ``shape`` and ``ks`` are the shapes of q and k."""
-    import torch
-
-    bf16 = torch.bfloat16
-    assert len(shape) == 3 and ks[-1] == shape[2] and ks[-2] > 0 and shape[1] % ks[-2] == 0 and v.shape == ks, (
-        "q is [T, Hq, D]; k and v end in [Hkv, D] with q's D and heads that divide q's")
-    assert device >= 0 and k.get_device() == device and v.get_device() == device and out.get_device() == device and (
-        lse is None or lse.get_device() == device), "all tensors must be on one GPU"
-    assert q.dtype is bf16 and k.dtype is bf16 and v.dtype is bf16 and out.dtype is bf16 and out.shape == shape, (
-        "q, k, v and out are bf16, out of q's shape")
-    assert lse is None or lse.dtype is torch.float32 and lse.shape == shape[:2], "lse is fp32 [T, Hq]"
-
-
-def _check_index(t, n: int, device: int, name: str) -> int:
-    """Pointer of an int32 array of ``n`` entries."""
-    import torch
-
-    assert t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous() and t.get_device() == device, (
-        f"{name} must be int32 [{n}], contiguous, on the other tensors' GPU")
-    return t.data_ptr()
-
-
-def _check_strides(sq, sk, sv, so, sl) -> None:
-    assert sq[2] == 1 and sk[-1] == 1 and sv[-1] == 1 and so[2] == 1 and sl[1] == 1, "rows must be contiguous"
+    return rc
 
 
 def gqa_prompt(q, k, v, cu_seqlens, scale: float, out, lse=None, stream=None) -> None:
     """Causal attention over whole prompts: packed ``q [T, Hq, D]``, ``k``, ``v [T, Hkv, D]`` (D 64 or 128; any strides
     that are multiples of 8) of the sequences ``cu_seqlens [B + 1]`` -> ``out [T, Hq, D]`` (+ ``lse [T, Hq]``). Query
     head h reads KV head ``h // (Hq // Hkv)``."""
-    device, shape, ks = q.get_device(), q.shape, k.shape
-    _check_gqa(device, shape, ks, q, k, v, out, lse)
-    T, Hq, D = shape
-    assert len(ks) == 3 and ks[0] == T, "as many keys as queries"
-    sq, sk, sv, so, sl = q.stride(), k.stride(), v.stride(), out.stride(), (Hq, 1) if lse is None else lse.stride()
-    _check_strides(sq, sk, sv, so, sl)
-    n = cu_seqlens.shape[0]
-    _launch(load_library().mla_gqa_prompt_bf16, "mla_gqa_prompt_bf16", device, stream, (
-        q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1],
-        _check_index(cu_seqlens, n, device, "cu_seqlens"), n - 1, T, Hq, ks[1], D, scale, out.data_ptr(), so[0], so[1],
-        None if lse is None else lse.data_ptr(), sl[0]))
+    call = load_binding().gqa_prompt
+    rc = call(q, k, v, cu_seqlens, scale, out, lse, stream)
+    if rc == _OTHER_DEVICE:
+        _again(q.device, call, "mla_gqa_prompt_bf16", q, k, v, cu_seqlens, scale, out, lse, stream)
+    elif rc != 0:
+        check(rc, "mla_gqa_prompt_bf16")
 
 
 @functools.lru_cache(maxsize=None)
@@ -595,19 +580,6 @@ def gqa_workspace(max_seqlen_q: int, q_heads: int, kv_heads: int, head_dim: int,
     return torch.empty((gqa_workspace_bytes(max_seqlen_q, q_heads, kv_heads, head_dim),), dtype=torch.uint8, device=device)
 
 
-def _workspace(workspace, nbytes: int, q, device: int, stream):
-    """``(workspace, bytes)``: the caller's, or one from torch's allocator for this call."""
-    import torch
-
-    if workspace is not None:
-        assert workspace.get_device() == device and workspace.is_contiguous(), "the workspace is one block on q's GPU"
-        return workspace, workspace.numel() * workspace.element_size()
-    workspace = q.new_empty((nbytes >> 1,))
-    if stream is not None and stream.cuda_stream != torch._C._cuda_getCurrentRawStream(device):
-        workspace.record_stream(stream)
-    return workspace, nbytes
-
-
 def gqa_chunk(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q: int, scale: float, out, lse=None,
               workspace=None, stream=None) -> None:
     """Attention of each request's new tokens over its pages of a K/V cache, causal over prefix and chunk:
@@ -615,42 +587,25 @@ def gqa_chunk(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqle
     ``ps``), ``page_table [B, cols]``, ``seq_lens_k [B]`` (prefix and chunk) -> ``out [T, Hq, D]`` (+ ``lse [T, Hq]``).
     ``max_seqlen_q``: at least every request's new tokens. ``workspace``: of ``gqa_workspace``, or None to take one from
     torch's allocator for this call."""
-    _gqa_paged(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q, scale, out, lse, workspace, stream)
+    assert cu_seqlens_q is not None, "cu_seqlens_q is [B + 1]"
+    call = load_binding().gqa_paged
+    rc = call(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q, scale, out, lse, workspace, stream)
+    if rc == _OTHER_DEVICE:
+        _again(q.device, call, "mla_gqa_chunk_bf16", q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q,
+               scale, out, lse, workspace, stream)
+    elif rc != 0:
+        check(rc, "mla_gqa_chunk_bf16")
 
 
 def gqa_decode(q, k_pool, v_pool, page_table, seq_lens, scale: float, out, lse=None, workspace=None, stream=None) -> None:
     """``gqa_chunk`` with one new token a request: ``q [B, Hq, D]`` -> ``out [B, Hq, D]`` (+ ``lse [B, Hq]``)."""
-    _gqa_paged(q, k_pool, v_pool, page_table, None, seq_lens, 1, scale, out, lse, workspace, stream)
-
-
-def _gqa_paged(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens, max_q: int, scale: float, out, lse, workspace,
-               stream) -> None:
-    import torch
-
-    device, shape, ks, ps = q.get_device(), q.shape, k_pool.shape, page_table.shape
-    _check_gqa(device, shape, ks, q, k_pool, v_pool, out, lse)
-    T, Hq, D = shape
-    sq, sk, sv, so, sp, sl = (q.stride(), k_pool.stride(), v_pool.stride(), out.stride(), page_table.stride(),
-                              (Hq, 1) if lse is None else lse.stride())
-    _check_strides(sq, sk, sv, so, sl)
-    B = seq_lens.shape[0]
-    assert len(ks) == 4 and sk[0] == ks[1] * sk[1] and sv[0] == ks[1] * sv[1], "pools are [pages, ps, Hkv, D], pages one after another"
-    assert page_table.dtype is torch.int32 and len(ps) == 2 and ps[0] >= B and sp[1] == 1 and page_table.get_device() == device, (
-        "page_table is int32 [B, cols], on q's GPU")
-    Hkv, max_q = ks[2], min(max_q, T)
-    ws, nbytes = _workspace(workspace, gqa_workspace_bytes(max_q, Hq, Hkv, D), q, device, stream)
-    lens = _check_index(seq_lens, B, device, "seq_lens")
-    lse_ptr = None if lse is None else lse.data_ptr()
-    cache = (q.data_ptr(), sq[0], sq[1], k_pool.data_ptr(), sk[1], sk[2], v_pool.data_ptr(), sv[1], sv[2], ks[0], ks[1],
-             page_table.data_ptr(), ps[1], sp[0])
-    if cu_seqlens_q is None:
-        assert T == B, "one token a request"
-        _launch(load_library().mla_gqa_decode_bf16, "mla_gqa_decode_bf16", device, stream, (
-            *cache, lens, B, Hq, Hkv, D, scale, ws.data_ptr(), nbytes, out.data_ptr(), so[0], so[1], lse_ptr, sl[0]))
-    else:
-        cu = _check_index(cu_seqlens_q, B + 1, device, "cu_seqlens_q")
-        _launch(load_library().mla_gqa_chunk_bf16, "mla_gqa_chunk_bf16", device, stream, (
-            *cache, cu, lens, B, T, max_q, Hq, Hkv, D, scale, ws.data_ptr(), nbytes, out.data_ptr(), so[0], so[1], lse_ptr, sl[0]))
+    call = load_binding().gqa_paged
+    rc = call(q, k_pool, v_pool, page_table, None, seq_lens, 1, scale, out, lse, workspace, stream)
+    if rc == _OTHER_DEVICE:
+        _again(q.device, call, "mla_gqa_decode_bf16", q, k_pool, v_pool, page_table, None, seq_lens, 1, scale, out, lse,
+               workspace, stream)
+    elif rc != 0:
+        check(rc, "mla_gqa_decode_bf16")
 
 
 class PageTables(NamedTuple):
@@ -672,25 +627,12 @@ def page_tables_from_lengths(token_table, table_idx, cached_lens, device_lens, f
     which fills their token table rows; then every request's page table, and the new tokens' locations and positions.
     ``max_device_len``, ``max_extend`` and ``total_new`` are the host's: the longest request, the most new tokens of one,
     and of all. Rows of requests that take pages must be distinct. One launch; nothing is read back."""
-    import torch
-
-    device, shape, st = token_table.get_device(), token_table.shape, token_table.stride()
-    assert device >= 0 and token_table.dtype is torch.int32 and len(shape) == 2 and st[1] == 1, "token_table: int32 [rows, cols] on the GPU"
-    B, F = table_idx.shape[0], free_slots.shape[0]
-    cols = -(-max_device_len // page_size)
-    # one allocation, which the tables are cut from
-    cells = B * cols
-    made = token_table.new_empty((cells + 2 * total_new + B + 2,))
-    if stream is not None and stream.cuda_stream != torch._C._cuda_getCurrentRawStream(device):
-        made.record_stream(stream)
-    base = made.data_ptr()
-    loc = base + 4 * cells
-    pos = loc + 4 * total_new
-    cu = pos + 4 * total_new
-    _launch(load_library().mla_page_tables_from_lengths, "mla_page_tables_from_lengths", device, stream, (
-        token_table.data_ptr(), shape[0], shape[1], st[0], _check_index(table_idx, B, device, "table_idx"),
-        _check_index(cached_lens, B, device, "cached_lens"), _check_index(device_lens, B, device, "device_lens"), B,
-        B if alloc_reqs is None else alloc_reqs, _check_index(free_slots, F, device, "free_slots"), F, page_size, max_extend,
-        base, cols, cols, loc, pos, total_new, cu, cu + 4 * (B + 1)))
-    pt, loc, pos, cu, taken = made.split_with_sizes((cells, total_new, total_new, B + 1, 1))
-    return PageTables(pt.view(B, cols), loc, pos, cu, taken)
+    call = load_binding().page_tables
+    got = call(token_table, table_idx, cached_lens, device_lens, free_slots, page_size, max_device_len, max_extend, total_new,
+               alloc_reqs, stream)
+    if got == _OTHER_DEVICE:
+        got = _again(token_table.device, call, "mla_page_tables_from_lengths", token_table, table_idx, cached_lens, device_lens,
+                     free_slots, page_size, max_device_len, max_extend, total_new, alloc_reqs, stream)
+    elif isinstance(got, int):
+        check(got, "mla_page_tables_from_lengths")
+    return PageTables(*got)

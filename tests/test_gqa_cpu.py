@@ -113,6 +113,12 @@ def test_bindings_refuse_host_tensors_and_wrong_types():
         lib.gqa_decode(q[:1], pool, pool, pt, cu[:1], 0.1, torch.empty_like(q[:1]))
     with pytest.raises(AssertionError, match="GPU"):
         lib.page_tables_from_lengths(pt, cu[:1], cu[:1], cu[:1], cu, 16, 4, 4, 4)
+    with pytest.raises(AssertionError, match="cu_seqlens_q"):
+        lib.gqa_chunk(q[:1], pool, pool, pt, None, cu[:1], 1, 0.1, torch.empty_like(q[:1]))
+    with pytest.raises(TypeError, match="k must be a tensor"):
+        lib.gqa_prompt(q, None, k, cu, 0.1, torch.empty_like(q))
+    with pytest.raises(AssertionError, match=r"\[T, Hkv, D\]"):
+        lib.gqa_prompt(q, pool, pool, cu, 0.1, torch.empty_like(q))
     with pytest.raises(AssertionError, match="heads that divide"):
         lib.gqa_prompt(q, torch.zeros((4, 3, 64), dtype=torch.bfloat16), torch.zeros((4, 3, 64), dtype=torch.bfloat16), cu, 0.1, torch.empty_like(q))
 
