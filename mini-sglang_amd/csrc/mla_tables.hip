@@ -33,33 +33,36 @@ __global__ __launch_bounds__(256) void page_tables_kernel(const PageTablesParams
   int c, d;
   lens(b, c, d);
   int32_t* row = p.token_table + (int64_t)min(max(p.table_idx[b], 0), p.tt_rows - 1) * p.tt_stride;
-  int sum[3] = {0, 0, 0};  // pages of the requests before b, of all; new tokens before b
+  // pages of the requests before b, of all; new tokens before b. Sums stop at 2^31 - 1: a wrapped one would pass for few
+  // pages, or for an offset in front of out_loc.
+  int sum[3] = {0, 0, 0};
+  auto add = [](int x, int y) { return __builtin_elementwise_add_sat(x, y); };
   for (int i = threadIdx.x; i < p.batch; i += 256) {
     int ci, di;
     lens(i, ci, di);
     const int n = i < p.alloc_reqs ? page(di + ps - 1) - page(ci + ps - 1) : 0;
-    sum[1] += n;
+    sum[1] = add(sum[1], n);
     if (i < b) {
-      sum[0] += n;
-      sum[2] += di - ci;
+      sum[0] = add(sum[0], n);
+      sum[2] = add(sum[2], di - ci);
     }
   }
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum[k] += __shfl_xor(sum[k], o);
+    for (int o = 32; o >= 1; o >>= 1) sum[k] = add(sum[k], __shfl_xor(sum[k], o));
     if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6][k] = sum[k];
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 3; ++k) sum[k] = s_sum[0][k] + s_sum[1][k] + s_sum[2][k] + s_sum[3][k];
+  for (int k = 0; k < 3; ++k) sum[k] = add(add(s_sum[0][k], s_sum[1][k]), add(s_sum[2][k], s_sum[3][k]));
   const int before = sum[0], all = sum[1], fresh_before = sum[2];
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     p.cu_seqlens_q[b] = fresh_before;
-    if (b == p.batch - 1) p.cu_seqlens_q[p.batch] = fresh_before + d - c;
+    if (b == p.batch - 1) p.cu_seqlens_q[p.batch] = add(fresh_before, d - c);
     if (b == 0) *p.pages_taken = all;
   }
-  if (all > p.num_free) return;  // out of pages: no table is touched
+  if (all > min(p.num_free, 0x7ffffffe)) return;  // out of pages: no table is touched
   const int first = page(c + ps - 1), last = page(d + ps - 1);
   const bool takes = b < p.alloc_reqs;
   const int32_t* free_slots = p.free_slots + before - first;  // page j of the row: free_slots[j]
@@ -91,7 +94,8 @@ __global__ __launch_bounds__(256) void page_tables_kernel(const PageTablesParams
 }  // namespace
 
 hipError_t launch_page_tables(const PageTablesParams& p, int32_t max_extend, hipStream_t stream) {
-  const int64_t tokens = (int64_t)max_extend + p.page_size - 1;  // of a request, to the end of its last page
+  // tokens of a request, to the end of its last page; within the table, so that a thread's index stays below 2^31
+  const int64_t tokens = (int64_t)(max_extend < p.tt_cols ? max_extend : p.tt_cols) + p.page_size - 1;
   const int64_t most = tokens > p.pt_cols ? tokens : p.pt_cols;
   const dim3 grid((unsigned)((most + kChunk - 1) / kChunk > 0 ? (most + kChunk - 1) / kChunk : 1), (unsigned)p.batch);
   if (p.log2_ps >= 0) hipLaunchKernelGGL(page_tables_kernel<true>, grid, dim3(256), 0, stream, p);

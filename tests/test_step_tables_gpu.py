@@ -104,6 +104,25 @@ def test_out_of_pages_writes_no_table():
     assert t.cu_seqlens_q.tolist() == [0, 1, 401]
 
 
+def test_sums_past_32_bits():
+    """Lengths whose sums pass 2^31: the sums stop there and nothing is written outside the tables; pages that pass it are
+    more than the free slots."""
+    n, cols = 3000, 1 << 20
+    table = torch.arange(cols, dtype=torch.int32, device=DEV).view(1, cols)
+    same, zero, long = i32([0] * n), i32([0] * n), i32([cols] * n)
+    t = lib.page_tables_from_lengths(table, same, zero, long, i32([]), 1, 100, 100, 1000, 0)
+    cu = [min(i * cols, 2**31 - 1) for i in range(n + 1)]
+    assert t.cu_seqlens_q.tolist() == cu and int(t.pages_taken) == 0
+    assert t.out_loc[:100].tolist() == list(range(100)) and t.positions[:100].tolist() == list(range(100))
+    assert torch.equal(t.page_table, torch.arange(100, dtype=torch.int32, device=DEV).expand(n, 100))
+    t = lib.page_tables_from_lengths(table, same, zero, long, i32([7] * 100), 1, 100, 100, 1000)
+    assert int(t.pages_taken) == 2**31 - 1 and t.cu_seqlens_q.tolist() == cu
+    assert torch.equal(table[0], torch.arange(cols, dtype=torch.int32, device=DEV))
+    # more new tokens than a table holds
+    t = lib.page_tables_from_lengths(table, i32([0]), i32([0]), i32([cols]), i32([]), 1, 100, 2**31 - 1, 1000, 0)
+    assert t.out_loc.tolist() == list(range(1000)) and t.cu_seqlens_q.tolist() == [0, cols]
+
+
 def test_capture_and_replay():
     cached, device = [20, 3, 90], [21, 4, 91]
     table, idx, free = make(cached, device, 16, 128, seed=7, spare=10)
