@@ -334,8 +334,9 @@ int mla_q_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, int32
  *   out  [total_q, q_heads, head_dim] strides (out_stride_t, out_stride_h), 8-byte aligned, multiples of 4, either order
  *   lse  [total_q, q_heads] fp32 (row stride lse_stride_t) or NULL
  *   cu_seqlens_q [batch + 1], seq_lens_k [batch] int32 device arrays; offsets past total_q, lengths past the page
- *        table's pt_cols * page_size tokens and page ids outside [0, num_pages) are cut or clamped, never followed.
+ *        table's pt_cols * page_size tokens (and 2^31 - 2^20) and page ids outside [0, num_pages) are cut or clamped, never followed.
  *        Rows of q behind the last request are not read, and those of out and lse stay as they are.
+ * out and lse overlap none of the inputs.
  * A key or value that a query does not attend does not reach its row, whatever it holds: cache rows past a length are
  * not read, and a row that an infinity or a NaN in a later token's value came near (weight zero times it, in the matrix
  * product) is computed again by itself, which is slow (0.13 ms per 1000 keys).
@@ -352,7 +353,8 @@ int mla_gqa_prompt_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, c
  * mla_gqa_chunk_bf16: each request's last E tokens (E from cu_seqlens_q, at most max_q; queries past max_q are left
  * out) over its seq_lens_k[b] keys in a paged cache, any power-of-two page_size; row of key j: page_table[b, j /
  * page_size] * page_size + j % page_size, for row strides that hold for the whole pool. Keys are split over the chip
- * where there are few rows: `workspace` (16-byte aligned) holds the partial results, mla_gqa_workspace_bytes of it.
+ * where there are few rows: `workspace` (16-byte aligned) holds the partial results, mla_gqa_workspace_bytes of it (which
+ * is enough for every call with at most max_q queries a request, at any batch and length).
  * Calls that overlap in time need workspaces of their own; nothing in one has to be kept or cleared between calls.
  *
  * mla_gqa_decode_bf16: the same with one token a request (query b is request b's last token).
@@ -387,7 +389,7 @@ int mla_gqa_decode_bf16(const void *q, int64_t q_stride_b, int64_t q_stride_h, c
  *   out_loc[cu_seqlens_q[b] + i] = token_table[row, c + i], positions[...] = c + i, for i < d - c (entries at and past
  *                      total_new are not written)
  *   *pages_taken = the free slots needed; if they are more than num_free, only this and cu_seqlens_q are written.
- * max_extend bounds d - c (tokens past it may be left out), pt_cols * page_size should hold the longest d. Any
+ * Sums stop at 2^31 - 1. max_extend bounds d - c (tokens past it may be left out), pt_cols * page_size should hold the longest d. Any
  * page_size. Replaces CacheManager.allocate_paged and the scheduler's slot and position gathers
  * (python/minisgl/scheduler/cache.py:42-53,119-161, scheduler/scheduler.py:198-214) with the page table of
  * python/minisgl/attention/fa.py:84-97.

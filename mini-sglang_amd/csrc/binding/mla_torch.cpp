@@ -200,7 +200,7 @@ PyObject* gqa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t* cu = nullptr;
     if (decode) require(x.T == B, "one token a request");
     else cu = index(a[4], "cu_seqlens_q", B + 1, x.device);
-    const int32_t max_q = (int32_t)std::min<int64_t>(integer(a[6]), x.T);
+    const int32_t max_q = (int32_t)std::max<int64_t>(std::min<int64_t>(integer(a[6]), x.T), -1);
     const float scale = number(a[7]);
     if (!is_current(x.device)) return PyLong_FromLong(kOtherDevice);
     void* stream = stream_of(a[11], x.device);

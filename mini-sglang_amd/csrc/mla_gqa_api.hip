@@ -2,6 +2,8 @@
 // argument checks, the choice of kernel, and launches.
 #include <math.h>
 
+#include <algorithm>
+
 #include "mla_gqa.h"
 
 namespace mla {
@@ -142,7 +144,8 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
   p.page_table = page_table;
   p.pt_stride = pt_stride;
   const int64_t keys = (int64_t)pt_cols * page_size;
-  p.max_keys = (int32_t)(keys < 0x7fff0000 ? keys : 0x7fff0000);
+  // a piece's end, its length rounded up to 64 keys in each of the pieces before it, stays below 2^31
+  p.max_keys = (int32_t)(keys < 0x7ff00000 ? keys : 0x7ff00000);
   p.cu_seqlens_q = cu_seqlens_q;
   p.seq_lens_k = seq_lens_k;
   p.max_q = max_q;
@@ -172,7 +175,9 @@ int mla_gqa_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads, in
   const char* who = "mla_gqa_workspace_bytes";
   if (bytes == nullptr || max_q < 0) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: bytes is null or max_q %d < 0", who, max_q);
   if (int rc = mla::check_heads(who, q_heads, kv_heads, head_dim)) return rc;
-  *bytes = 4 * mla::workspace_floats((int64_t)max_q * (q_heads / kv_heads), head_dim);
+  const int64_t most = (int64_t)max_q * (q_heads / kv_heads);
+  // fewer queries may take the stream kernel, whose batches are cut into more pieces
+  *bytes = 4 * std::max(mla::workspace_floats(most, head_dim), mla::workspace_floats(std::min<int64_t>(most, mla::kStreamRows), head_dim));
   return mla::done(hipSuccess, who);
 }
 

@@ -14,6 +14,11 @@
 //  * Online softmax in the log2 domain against a lazy row reference: the maximum of the wave's first stage, moved (with O
 //    and l rescaled, and the stage redone) only when a stage's numerators sum past 2^32: fp32 keeps its relative
 //    precision at any scale.
+// Bound: the MFMAs, and under them power: prompts of 7.8k and 8.1k tokens with 64 and 8 heads of 128 take 1.76 ms, 1164
+// TFLOP/s, with the MFMAs busy for 62 % of the cycles at 1.83 GHz (alone, on random operands, they run at 1829 TFLOP/s
+// and 1.74 GHz); four chunks of 2048 on up to 8192, pages of 64, 1.17 ms, 1170 TFLOP/s. Short calls are bound by their
+// CTA's chain: 1.2 us to find the request, 2 to the first stage, 0.45 a stage for a lone CTA, 1 to 1.8 for the results.
+// Waves of 64 rows (one per SIMD; each K and V operand read once for two MFMAs) took 1098 TFLOP/s where these took 1170.
 #include <type_traits>
 
 #include "mla_gqa.h"

@@ -2,9 +2,12 @@
 // cache, with the keys of a batch split over the chip and joined by an fp32 log-sum-exp merge. See mla_gqa.h.
 //
 // One CTA per (request, rows, KV head, piece of the keys). Its NW waves take tiles of 32 keys in turn and share
-// nothing until the end, so there is no barrier in the stream: a wave loads a tile's K straight into the operand layout
-// of the score MFMA and its V through a private LDS tile that transposes it, and requests the next tile before it
-// computes the present one. Bound: HBM (each K and V row is read once).
+// nothing until the end, so there is no barrier in the stream: a wave brings a tile's K and V into the MFMAs' operand
+// layouts through private LDS tiles, and requests the next tile before it computes the present one.
+// Bound: HBM (each K and V row is read once), and below some 20 MB the chain of dependent loads (lengths, page, tile) and
+// the merge's launch. Measured with the merge: 64 requests of 1k to 8k tokens, 64 and 8 heads of 128, 226 us (5.7 TB/s);
+// 8 of 32k to 128k, 8 heads and 1, 60 us (5.4 TB/s); 16 chunks of 1 to 8 on 1k to 16k, 32 and 8 heads, pages of one
+// token, 112 us (5.1 TB/s); one request of 1500, 32 and 8 heads, 9.6 us.
 #include "mla_gqa.h"
 
 namespace mla {
@@ -216,6 +219,7 @@ __global__ __launch_bounds__(64 * NW, NB == 4 && D == 128 ? 1 : 2) void gqa_stre
 
 // Partial results of requests in pieces, joined: lse = log2 sum_i 2^lse_i, out = sum_i 2^(lse_i - lse) o_i.
 // One CTA per (query, query head): its waves take every fourth piece (kWaves 4), or a wave per row (kWaves 1).
+// Bound: dependent loads (lengths, the pieces' lse, their rows). 3.8 us for 32 rows, 6 for 4096 rows of 64 requests.
 template <int D, int kRows, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -104,6 +104,11 @@ def test_workspace_bytes():
     assert lib.load_library().mla_gqa_workspace_bytes(-1, 8, 1, 128, ctypes.byref(n)) == INVALID
 
 
+def test_workspace_of_many_queries_is_enough_for_fewer():
+    sizes = [lib.gqa_workspace_bytes(n, 8, 1, 128) for n in (0, 1, 2, 3, 4, 5, 8, 9, 16, 17, 300, 4096)]
+    assert sizes == sorted(sizes)
+
+
 def test_bindings_refuse_host_tensors_and_wrong_types():
     q, k = torch.zeros((4, 8, 64), dtype=torch.bfloat16), torch.zeros((4, 2, 64), dtype=torch.bfloat16)
     cu, pool, pt = torch.zeros(2, dtype=torch.int32), torch.zeros((3, 16, 2, 64), dtype=torch.bfloat16), torch.zeros((1, 2), dtype=torch.int32)

@@ -368,6 +368,13 @@ def test_capture_and_replay_with_other_lengths(extends, prefixes):
         assert torch.equal(got[0], out) and torch.equal(got[1], lse), "replay and eager call differ"
 
 
+@pytest.mark.parametrize("extends", [[1, 1], [5, 8], [16, 3], [300, 1]])
+def test_one_workspace_for_steps_of_all_sizes(extends):
+    c = Paged(extends, [4000, 2500], 8, 1, 128, 16, seed=sum(extends))
+    out, lse = c.run(workspace=lib.gqa_workspace(300, 8, 1, 128, DEV))
+    check(out, lse, c.ref())
+
+
 def test_two_streams_with_workspaces_of_their_own():
     a, b = (Paged([2, 1], [4000, 900], 8, 2, 128, 16, seed=s) for s in (19, 20))
     streams = [torch.cuda.Stream() for _ in range(2)]
