@@ -193,6 +193,17 @@ def test_decode_lengths(dim, lens):
     check(*c.run(), ref, "as a chunk")
 
 
+@pytest.mark.parametrize("extends, prefixes", [
+    ([1] * 100, [2999, 4] * 50),  # pieces that fit the CTAs running at once
+    ([1] * 301, [1499, 1] * 150 + [8999]),  # many pairs
+    ([3, 2, 0] * 30, [2000, 7, 40] * 30),
+    ([20, 1] * 40, [1500, 90] * 40),  # blocks
+])
+def test_split_keys_of_more_requests_than_a_wave_has_lanes(extends, prefixes):
+    c = Paged(extends, prefixes, 8, 2, 64, 16, seed=len(extends))
+    check(*c.run(), c.ref())
+
+
 @pytest.mark.parametrize("heads", [(16, 2), (64, 4)])
 def test_chunk_long_prefix(heads):
     """Few rows on long prefixes: keys are split and joined, in both kernels, a piece that ends inside a chunk's
