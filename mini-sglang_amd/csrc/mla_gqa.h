@@ -98,7 +98,7 @@ __device__ __forceinline__ float wave_fsum_all(float v) {
 // Least keys of a piece: a tile for each wave of the stream kernel; 16 stages of the blocks (their joining takes 6 us).
 template <int kRows>
 constexpr int gqa_min_split() {
-  return kRows <= 64 ? 128 : 512;
+  return kRows <= 32 ? 128 : 512;
 }
 template <int kRows>
 __device__ __forceinline__ int gqa_blocks(const GqaParams& p, const GqaRequest& r) {
@@ -273,6 +273,6 @@ __device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem&
 inline bool gqa_grid_ok(int64_t ctas, int threads) { return ctas <= 0x7fffffff && ctas * threads <= (int64_t)UINT32_MAX; }
 
 hipError_t launch_gqa_rows(const GqaParams& p, int dim, hipStream_t stream);    // many rows a request
-hipError_t launch_gqa_stream(const GqaParams& p, int dim, hipStream_t stream);  // up to 64 rows a request
+hipError_t launch_gqa_stream(const GqaParams& p, int dim, int rows, hipStream_t stream);  // CTAs of 16 or 32 rows
 
 }  // namespace mla

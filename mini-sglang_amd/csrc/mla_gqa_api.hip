@@ -17,24 +17,25 @@ int done(hipError_t e, const char* who) {
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
-// Requests of up to this many rows (tokens times group) are streamed: their attention is bound by reading K and V.
-constexpr int kStreamRows = 64;
-// Items that a batch is cut into (mla_gqa.h): of a streamed batch, kStreamFit (the CTAs that run at once, two a compute
-// unit) where it has at most half as many (block, head) pairs, else about kStreamTarget, so that pieces of different
-// length even out; of one in blocks of 128 rows, about kRowsTarget.
-constexpr int kStreamFit = 512;
-constexpr int kStreamTarget = 2048;
-// Keys (at most, by the page table's width) up to which a request is one piece and nothing is joined: with few pairs, a
-// CTA of eight waves each (a request of 500 keys, 8 KV heads 8.6 us, 10.3 in pieces; of 1000 12.5, 10.4: one compute unit
-// loads 64 bytes a cycle), and with many (64 requests of up to 1000 34.5 us, 43.8 in pieces; 200 of them 82, 103).
-constexpr int kStreamOnePieceFew = 512;
-constexpr int kStreamOnePiece = 1024;
-constexpr int kRowsTarget = 512;
-// A chunk batch of at least this many blocks fills the chip without cutting keys.
-constexpr int kRowsEnough = 1024;
-constexpr int kRowsBlock = 128;
-// Keys (at most, by the page table's width) up to which cutting them gains nothing over joining the pieces.
-constexpr int kRowsOnePiece = 1024;
+// A launch's kernel: CTAs of 16 or 32 rows that stream keys, or (rows 128) blocks; how many items a paged batch is cut
+// into (target, fit: mla_gqa.h; 0: requests in one piece), and whether its CTAs are the wide ones.
+struct Choice {
+  int rows, target;
+  bool fit, wide;
+};
+
+// CTAs that run at once, two a compute unit, and about how many pieces of different length even out.
+constexpr int kFit = 512;
+constexpr int kTarget = 2048;
+constexpr int kBlocksTarget = 512;
+constexpr int kBlock = 128;
+// A paged batch of at least this many blocks fills the chip without cutting keys; up to this many keys (by the page
+// table's width) cutting them gains nothing over joining the pieces: in blocks, and streamed by more CTAs than run at once.
+constexpr int kBlocksEnough = 1024;
+constexpr int kOnePieceBlocks = 1024;
+constexpr int kOnePieceMany = 1600;
+// Requests of more than 16 rows are streamed in pieces up to this many CTAs of 16 rows times keys.
+constexpr int64_t kFewWork = 1 << 18;
 
 // Blocks of 256 rows (head_dim 128): they read keys once for twice the rows, but start and end alone on their compute
 // unit. 256 / 128 rows: prompts of 8k tokens, 64 and 8 heads 1797 / 1894 us; one of 4096, 32 heads 149 / 156; four of 2048
@@ -42,14 +43,46 @@ constexpr int kRowsOnePiece = 1024;
 // one prompt of 8192, 8 and 1 heads (256 wide blocks) 191 / 173. avg: tokens of an average request; keys: of the longest,
 // by what the host knows.
 bool wide_blocks(int dim, int64_t blocks, int64_t avg, int64_t keys) {
-  return dim == 128 && blocks >= kRowsEnough && avg >= 1024 && keys >= 2560;
+  return dim == 128 && blocks >= kBlocksEnough && avg >= 1024 && keys >= 2560;
 }
 
-int stream_rows(int64_t most) { return most <= 16 ? 16 : most <= 32 ? 32 : 64; }
+// batch, total_q, most: requests, their queries, the most rows (queries times group) of one; keys: the most keys of one
+// (paged), or 0: packed prompts.
+//
+// Where 16- or 32-row CTAs of eight waves are no more than the compute units, each takes a request's keys in one piece:
+// their waves share the keys, so that a lone CTA's chain is short. 16 / 32 rows / blocks, us, head_dim 128 unless said:
+// prompts of 2000, 2 and 2 heads 20 / 25 / 36; 4000, 2 and 1 51 / 43 / 63; four of 300, 8 and 2 (304 CTAs of 32 rows) 16 /
+// 17 / 12; four chunks of 64 on 900, 8 heads and 1 15 / 19 / 23, on 2000 24 / 29 / 25, 32 and 8 heads 27 / 19 / 24. Against
+// cut keys: 8 CTAs on 600 keys 10 / 11, on 1000 13 / 11; 128 on 1000 19 / 19; 256 on 1000 25 / 31, on 3000 67 / 73; at
+// head_dim 64 8 on 1000 9.1 / 9.4, 128 on 2000 21 / 20. With more CTAs, one token a request, 8 KV heads: 40 requests of up
+// to 1600 45 / 46, 64 56 / 63, 256 186 / 202; 40 of up to 3000 75 / 67, 256 327 / 333.
+// Few rows on longer keys are cut in CTAs of 16 rows: a chunk of 100 on 2000, 8 heads and 1, 17 in blocks 21; on 4000 20,
+// 22; on 8000 26, 24. Else up to 32 rows are streamed, bound by reading K and V: 64 chunks of 8 on 1k to 8k, 32 and 8
+// heads, 256, in blocks 277; with 64 and 8 heads (64 rows) 432, 297.
+Choice choose(int dim, int32_t batch, int64_t total_q, int32_t group, int32_t kv_heads, int64_t most, int64_t keys) {
+  auto ctas = [&](int rows) { return std::max<int64_t>((total_q * group + rows - 1) / rows, batch) * kv_heads; };
+  auto one_piece = [&](int64_t n) { return 2 * n <= kFit && (keys == 0 || keys * dim <= (512 + 4 * n) * 128); };
+  for (int rows : {16, 32}) {
+    if (one_piece(ctas(rows))) return {rows, 0, false, true};
+    if (most <= rows) break;
+  }
+  const int64_t blocks = (total_q * group + kBlock - 1) / kBlock * kv_heads;
+  if (keys == 0) return {kBlock, 0, false, wide_blocks(dim, blocks, total_q / batch, total_q / batch)};
+  if (most > 16 && 2 * ctas(16) <= kFit && ctas(16) * keys <= kFewWork) return {16, kFit, true, false};
+  if (most <= 32) {
+    const int rows = most <= 16 ? 16 : 32;
+    if (2 * ctas(rows) <= kFit) return {rows, kFit, true, false};
+    return {rows, keys <= kOnePieceMany ? 0 : kTarget, false, false};
+  }
+  if (blocks >= kBlocksEnough || keys <= kOnePieceBlocks) return {kBlock, 0, false, wide_blocks(dim, blocks, total_q / batch, keys)};
+  return {kBlock, kBlocksTarget, false, false};
+}
 
-int64_t workspace_floats(int64_t most, int dim) {
-  const bool stream = most <= kStreamRows;
-  return 2 * (int64_t)(stream ? kStreamTarget : kRowsTarget) * (stream ? stream_rows(most) : kRowsBlock) * (dim + 1);
+// Rows of partial results: 2 target pieces of any choice for requests of up to `most` rows.
+int64_t workspace_rows(int64_t most) {
+  static_assert(2 * kTarget * 32 >= 2 * kBlocksTarget * kBlock && 2 * kTarget * 32 >= 2 * kFit * 16, "32 rows streamed need the most");
+  static_assert(2 * kTarget * 16 >= 2 * kFit * 16, "and 16 rows");
+  return 2 * (int64_t)kTarget * (most <= 16 ? 16 : 32);
 }
 
 int check_heads(const char* who, int32_t q_heads, int32_t kv_heads, int32_t dim) {
@@ -112,6 +145,13 @@ int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_str
   return MLA_OK;
 }
 
+int launch(const char* who, GqaParams& p, const Choice& c, int dim, void* stream) {
+  p.target = c.target;
+  p.fit = c.fit;
+  p.wide = c.wide;
+  return done(c.rows == kBlock ? launch_gqa_rows(p, dim, (hipStream_t)stream) : launch_gqa_stream(p, dim, c.rows, (hipStream_t)stream), who);
+}
+
 int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
           int64_t k_row_stride, int64_t k_head_stride, const void* v_pool, int64_t v_row_stride, int64_t v_head_stride,
           int32_t num_pages, int32_t page_size, const int32_t* page_table, int32_t pt_cols, int64_t pt_stride,
@@ -135,7 +175,7 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
                                 out_stride_t, out_stride_h, lse, lse_stride_t))
     return rc;
   const int64_t most = (int64_t)max_q * p.group;  // rows of a request and KV head
-  const int64_t need = 4 * workspace_floats(most, dim);
+  const int64_t need = 4 * workspace_rows(most) * (dim + 1);
   if (!aligned(workspace, 16) || workspace_bytes < need)
     return api_error(MLA_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
                      (long long)need, (long long)workspace_bytes);
@@ -149,21 +189,9 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
   p.cu_seqlens_q = cu_seqlens_q;
   p.seq_lens_k = seq_lens_k;
   p.max_q = max_q;
-  const bool stream_kernel = most <= kStreamRows;
-  const int64_t blocks = ((int64_t)total_q * p.group + kRowsBlock - 1) / kRowsBlock * kv_heads;
-  if (stream_kernel) {
-    const int64_t pairs = (int64_t)batch * kv_heads;
-    p.fit = 2 * pairs <= kStreamFit;
-    const bool short_keys = p.max_keys <= (p.fit ? kStreamOnePieceFew : kStreamOnePiece);
-    p.target = short_keys ? 0 : p.fit ? kStreamFit : kStreamTarget;
-    p.wide = short_keys && p.fit;
-  } else {
-    p.target = blocks >= kRowsEnough || p.max_keys <= kRowsOnePiece ? 0 : kRowsTarget;
-    p.wide = p.target == 0 && wide_blocks(dim, blocks, total_q / batch, p.max_keys);
-  }
   p.ws_o = static_cast<float*>(workspace);
-  p.ws_lse = p.ws_o + workspace_floats(most, dim) / (dim + 1) * dim;
-  return done(stream_kernel ? launch_gqa_stream(p, dim, (hipStream_t)stream) : launch_gqa_rows(p, dim, (hipStream_t)stream), who);
+  p.ws_lse = p.ws_o + workspace_rows(most) * dim;
+  return launch(who, p, choose(dim, batch, total_q, p.group, kv_heads, most, p.max_keys), dim, stream);
 }
 
 }  // namespace
@@ -175,9 +203,7 @@ int mla_gqa_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads, in
   const char* who = "mla_gqa_workspace_bytes";
   if (bytes == nullptr || max_q < 0) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: bytes is null or max_q %d < 0", who, max_q);
   if (int rc = mla::check_heads(who, q_heads, kv_heads, head_dim)) return rc;
-  const int64_t most = (int64_t)max_q * (q_heads / kv_heads);
-  // fewer queries may take the stream kernel, whose batches are cut into more pieces
-  *bytes = 4 * std::max(mla::workspace_floats(most, head_dim), mla::workspace_floats(std::min<int64_t>(most, mla::kStreamRows), head_dim));
+  *bytes = 4 * mla::workspace_rows((int64_t)max_q * (q_heads / kv_heads)) * (head_dim + 1);
   return mla::done(hipSuccess, who);
 }
 
@@ -199,9 +225,7 @@ int mla_gqa_prompt_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h, c
   p.max_keys = total_q;
   p.cu_seqlens_q = cu_seqlens;
   p.max_q = total_q;
-  p.wide = mla::wide_blocks(head_dim, ((int64_t)total_q * p.group + mla::kRowsBlock - 1) / mla::kRowsBlock * kv_heads,
-                            total_q / batch, total_q / batch);
-  return mla::done(mla::launch_gqa_rows(p, head_dim, (hipStream_t)stream), who);
+  return mla::launch(who, p, mla::choose(head_dim, batch, total_q, p.group, kv_heads, (int64_t)total_q * p.group, 0), head_dim, stream);
 }
 
 int mla_gqa_chunk_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool, int64_t k_row_stride,

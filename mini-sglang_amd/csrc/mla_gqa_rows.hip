@@ -1,5 +1,5 @@
-// Grouped-head attention for many rows: whole prompts, and chunks of more than 64 rows (tokens times group) over a
-// paged cache. See mla_gqa.h for the mathematics.
+// Grouped-head attention for many rows (tokens times group): whole prompts, and chunks over a paged cache. See mla_gqa.h for
+// the mathematics.
 //
 // One CTA per (request, 32 NW rows, KV head, piece of the keys), NW waves x 32 rows, two waves per SIMD: NW 4 (two CTAs
 // on a compute unit) or 8 (one).

@@ -1,5 +1,6 @@
-// Grouped-head attention for few rows: single tokens and chunks of up to 64 rows (tokens times group) over a paged
-// cache, with the keys of a batch split over the chip and joined by an fp32 log-sum-exp merge. See mla_gqa.h.
+// Grouped-head attention for few rows (tokens times group): single tokens, chunks of up to 32 rows over a paged cache, with
+// the keys of a batch split over the chip and joined by an fp32 log-sum-exp merge, and chunks and prompts of which few
+// CTAs come. See mla_gqa.h.
 //
 // One CTA per (request, rows, KV head, piece of the keys). Its NW waves take tiles of 32 keys in turn and share
 // nothing until the end, so there is no barrier in the stream: a wave brings a tile's K and V into the MFMAs' operand
@@ -18,7 +19,7 @@ constexpr float kLowest = -3.4028234663852886e38f;
 
 // NB blocks of 16 rows, NW waves
 template <int D, int NB, int NW>
-__global__ __launch_bounds__(64 * NW, NB == 4 && D == 128 ? 1 : 2) void gqa_stream_kernel(const GqaParams p) {
+__global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams p) {
   constexpr int kRows = 16 * NB, kRowB = D * 2, kChunks = D / 8, kKs = D / 32, kDb = D / 16;
   constexpr int kLoads = kTileKeys * kChunks / 64;  // 16-byte loads of a lane per K or V tile
   __shared__ __attribute__((aligned(16))) char s_k[NW][kTileKeys * kRowB], s_v[NW][kTileKeys * kRowB];
@@ -297,13 +298,8 @@ __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams 
 
 template <int D, int NB>
 void launch_stream(const GqaParams& p, int64_t grid, hipStream_t stream) {
-  if constexpr (NB < 4) {
-    if (p.wide) {
-      hipLaunchKernelGGL((gqa_stream_kernel<D, NB, 8>), dim3((unsigned)grid), dim3(512), 0, stream, p);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((gqa_stream_kernel<D, NB, 4>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+  if (p.wide) hipLaunchKernelGGL((gqa_stream_kernel<D, NB, 8>), dim3((unsigned)grid), dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL((gqa_stream_kernel<D, NB, 4>), dim3((unsigned)grid), dim3(256), 0, stream, p);
 }
 
 }  // namespace
@@ -319,24 +315,20 @@ hipError_t launch_gqa_merge(const GqaParams& p, int dim, int rows, hipStream_t s
   }
   MLA_MERGE(64, 16)
   MLA_MERGE(64, 32)
-  MLA_MERGE(64, 64)
   MLA_MERGE(64, 128)
   MLA_MERGE(128, 16)
   MLA_MERGE(128, 32)
-  MLA_MERGE(128, 64)
   MLA_MERGE(128, 128)
 #undef MLA_MERGE
   return hipGetLastError();
 }
 
-hipError_t launch_gqa_stream(const GqaParams& p, int dim, hipStream_t stream) {
-  const int64_t most = (int64_t)p.max_q * p.group;
-  const int rows = most <= 16 ? 16 : most <= 32 ? 32 : 64;
+hipError_t launch_gqa_stream(const GqaParams& p, int dim, int rows, hipStream_t stream) {
   const int64_t blocks = ((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch;
   const int64_t grid = blocks * p.kv_heads + p.target;
   if (!gqa_grid_ok(grid, 512)) return hipErrorInvalidValue;
-  if (dim == 128) rows == 16 ? launch_stream<128, 1>(p, grid, stream) : rows == 32 ? launch_stream<128, 2>(p, grid, stream) : launch_stream<128, 4>(p, grid, stream);
-  else rows == 16 ? launch_stream<64, 1>(p, grid, stream) : rows == 32 ? launch_stream<64, 2>(p, grid, stream) : launch_stream<64, 4>(p, grid, stream);
+  if (dim == 128) rows == 16 ? launch_stream<128, 1>(p, grid, stream) : launch_stream<128, 2>(p, grid, stream);
+  else rows == 16 ? launch_stream<64, 1>(p, grid, stream) : launch_stream<64, 2>(p, grid, stream);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.target > 0) e = launch_gqa_merge(p, dim, rows, stream);
   return e;

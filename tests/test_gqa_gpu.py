@@ -314,9 +314,9 @@ def test_later_tokens_that_are_not_finite_reach_no_earlier_row(dim, value):
         assert not out[extends[0] - 1].isfinite().any()
 
 
-@pytest.mark.parametrize("extends", [[1, 1], [160, 20]])
-def test_pool_past_32_bits(extends):
-    """K and V rows past 2^31 bytes and 2^31 elements from the pool's start."""
+@pytest.mark.parametrize("extends,pad", [([1, 1], 0), ([160, 20], 0), ([160, 20], 8192 // 16 + 64)])
+def test_pool_past_32_bits(extends, pad):
+    """K and V rows past 2^31 bytes and 2^31 elements from the pool's start; with rows behind the requests, in blocks."""
     pages, ps, hk, d = 17000, 64, 8, 128  # 1.1 G elements a pool, 2.2 GB
     gen = torch.Generator(device=DEV).manual_seed(0)
     k = torch.empty((2 * pages, ps, hk, d), dtype=torch.bfloat16, device=DEV)
@@ -327,13 +327,13 @@ def test_pool_past_32_bits(extends):
         v[p] = torch.randn(k[p].shape, generator=gen, device=DEV).to(torch.bfloat16)
     pt = torch.tensor([used[:4], used[4:]], dtype=torch.int32)
     lens, T = [250, 256], sum(extends)
-    q = torch.randn((T, 16, d), generator=gen, device=DEV).to(torch.bfloat16)
-    out, lse = torch.empty_like(q), torch.empty((T, 16), device=DEV)
-    lib.gqa_chunk(q, k, v, pt.to(DEV), i32(cumulative(extends)), i32(lens), max(extends), d ** -0.5, out, lse)
+    q = torch.randn((T + pad, 16, d), generator=gen, device=DEV).to(torch.bfloat16)
+    out, lse = torch.empty_like(q), torch.empty((T + pad, 16), device=DEV)
+    lib.gqa_chunk(q, k, v, pt.to(DEV), i32(cumulative(extends)), i32(lens), max(extends) + pad, d ** -0.5, out, lse)
     torch.cuda.synchronize()
     index = torch.tensor(used, device=DEV)
     small = torch.tensor([[0, 1, 2, 3], [4, 5, 6, 7]], dtype=torch.int32)
-    check(out, lse, R.chunk(q.cpu(), k[index].cpu(), v[index].cpu(), small, extends, lens, d ** -0.5))
+    check(out[:T], lse[:T], R.chunk(q[:T].cpu(), k[index].cpu(), v[index].cpu(), small, extends, lens, d ** -0.5))
 
 
 def test_device_lengths_and_page_ids_out_of_range_are_cut():
@@ -383,6 +383,111 @@ def test_capture_and_replay_with_other_lengths(extends, prefixes):
 def test_one_workspace_for_steps_of_all_sizes(extends):
     c = Paged(extends, [4000, 2500], 8, 1, 128, 16, seed=sum(extends))
     out, lse = c.run(workspace=lib.gqa_workspace(300, 8, 1, 128, DEV))
+    check(out, lse, c.ref())
+
+
+def padding(q_heads):
+    """Rows behind the last request that make a batch one of more 32-row CTAs than compute units: its kernel is the blocks'."""
+    return 8192 // q_heads + 64
+
+
+class InBlocks(Paged):
+    """A small batch that takes the kernel of the large ones."""
+
+    def __init__(self, extends, prefixes, q_heads, *args, **kw):
+        super().__init__(extends, prefixes, q_heads, *args, spare_rows=padding(q_heads), **kw)
+
+    def run(self, workspace=None):
+        out, lse = super().run(self.q.shape[0], workspace)
+        assert out[self.T :].isnan().all() and lse[self.T :].isnan().all()
+        return out[: self.T], lse[: self.T]
+
+
+def prompt_in_blocks(q, k, v, lens, scale):
+    T, pad = q.shape[0], padding(q.shape[1])
+    out, lse = run_prompt(*(torch.cat((x, torch.full((pad, *x.shape[1:]), NAN, dtype=x.dtype))) for x in (q, k, v)), lens, scale)
+    assert out[T:].isnan().all() and lse[T:].isnan().all()
+    return out[:T], lse[:T]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads", [(1, 1), (8, 1), (4, 4), (6, 2), (14, 2), (20, 4), (48, 3)])
+def test_prompt_heads_in_blocks(dim, heads):
+    gen = torch.Generator().manual_seed(heads[0] * dim)
+    lens = [33, 1, 0, 129, 64]
+    q, k, v = randn(gen, sum(lens), heads[0], dim), randn(gen, sum(lens), heads[1], dim), randn(gen, sum(lens), heads[1], dim)
+    check(*prompt_in_blocks(q, k, v, lens, dim ** -0.5), R.prompt(q, k, v, lens, dim ** -0.5))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens", [[1], [31, 32, 33], [127, 128, 129], [255, 257], [1500, 3, 700], [2, 17, 1, 0, 40] * 30])
+def test_prompt_lengths_in_blocks(dim, lens):
+    gen = torch.Generator().manual_seed(sum(lens))
+    q, k, v = randn(gen, sum(lens), 4, dim), randn(gen, sum(lens), 2, dim), randn(gen, sum(lens), 2, dim)
+    check(*prompt_in_blocks(q, k, v, lens, dim ** -0.5), R.prompt(q, k, v, lens, dim ** -0.5))
+
+
+@pytest.mark.parametrize("page_size", [1, 2, 16, 32, 256])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_chunk_pages_in_blocks(page_size, dim):
+    for prefixes in ([0, 33, 500, 1030], [0, 33, 500, 30]):  # keys split, and in one piece
+        c = InBlocks([1, 40, 128, 77], prefixes, 8, 2, dim, page_size, seed=page_size + dim)
+        check(*c.run(), c.ref())
+
+
+@pytest.mark.parametrize("heads", [(1, 1), (8, 8), (12, 3), (14, 2), (28, 4), (64, 1)])
+@pytest.mark.parametrize("extends", [[1, 1, 1], [9, 4, 16], [70, 1, 33]])
+def test_chunk_groups_in_blocks(heads, extends):
+    c = InBlocks(extends, [700, 15, 64], *heads, 128, 16, seed=heads[0] + extends[0])
+    check(*c.run(), c.ref())
+
+
+def test_no_keys_and_far_scores_in_blocks():
+    c = InBlocks([0, 5, 0, 2, 0], [30, 8, 0, 0, 7], 4, 2, 128, 16, seed=6)
+    check(*c.run(), c.ref())
+    c = InBlocks([200, 3], [40, 3], 4, 1, 64, 16, seed=7)
+    c.lens = [197, 2]
+    out, lse = c.run()
+    check(out, lse, c.ref())
+    assert (out[:3] == 0).all() and (lse[:3] == -float("inf")).all()
+    c = InBlocks([140], [200], 8, 2, 128, 16, seed=13, scale=3.0)
+    rows = c.pt[0].long()[torch.arange(340) // 16] * 16 + torch.arange(340) % 16
+    k = c.k.view(-1, 2, 128)
+    k[rows] = (k[rows].float() * torch.linspace(0.01, 2.0, 340)[:, None, None]).to(torch.bfloat16)
+    check(*c.run(), c.ref())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [NAN, float("inf"), -float("inf")])
+def test_later_tokens_that_are_not_finite_in_blocks(dim, value):
+    gen = torch.Generator().manual_seed(23)
+    lens, last = [200, 70], [198, 199, 269]
+    q, k, v = (randn(gen, sum(lens), h, dim) for h in (6, 2, 2))
+    ref = R.prompt(q, k, v, lens, 0.1)
+    keep = [i for i in range(270) if i not in last]
+    for t in (k, v):
+        t[last] = value
+    out, lse = prompt_in_blocks(q, k, v, lens, 0.1)
+    check(out[keep], lse[keep], R.Attention(*(x[keep] for x in ref)))
+    assert not out[last].isfinite().any(-1).all(-1).any()
+    for extends, prefixes in (([90, 2], [3000, 40]), ([20, 40], [300, 2])):
+        c = InBlocks(extends, prefixes, 6, 2, dim, 16, seed=24)
+        ref = c.ref()
+        at = int(c.pt[0, (c.lens[0] - 1) // 16]) * 16 + (c.lens[0] - 1) % 16
+        c.v.view(-1, 2, dim)[at] = value
+        out, lse = c.run()
+        keep = [i for i in range(c.T) if i != extends[0] - 1]
+        check(out[keep], lse[keep], R.Attention(*(x[keep] for x in ref)))
+
+
+def test_device_lengths_and_page_ids_out_of_range_are_cut_in_blocks():
+    c = InBlocks([1, 130], [40, 100], 4, 2, 64, 16, seed=16)
+    c.k.nan_to_num_(0.5), c.v.nan_to_num_(0.5)
+    c.pt[0, 0], c.pt[1, 1] = 10 ** 6, -5
+    c.lens = [41, 10 ** 9]
+    out, lse = c.run()
+    c.pt.clamp_(0, c.k.shape[0] - 1)
+    c.lens = [41, c.pt.shape[1] * 16]
     check(out, lse, c.ref())
 
 
