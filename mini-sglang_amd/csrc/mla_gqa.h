@@ -40,8 +40,7 @@ struct GqaParams {
   float* ws_lse;  // [slots, rows] their log2-domain LSEs
   int32_t target;  // items that a batch's keys are split into, about (0: no splitting)
   int32_t fit;     // at most `target`, where that can be
-  int32_t wide;    // of requests in one piece: blocks of 256 rows instead of 128; eight waves a CTA of the stream kernel
-                   // instead of four
+  int32_t wide;    // eight waves a CTA instead of four, sharing an item's keys
   int32_t out_16b;  // rows of out start 16-byte aligned
 };
 
@@ -272,7 +271,7 @@ __device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem&
 // A launch holds fewer than 2^32 threads.
 inline bool gqa_grid_ok(int64_t ctas, int threads) { return ctas <= 0x7fffffff && ctas * threads <= (int64_t)UINT32_MAX; }
 
-hipError_t launch_gqa_rows(const GqaParams& p, int dim, hipStream_t stream);    // many rows a request
+hipError_t launch_gqa_rows(const GqaParams& p, int dim, int rows, hipStream_t stream);    // blocks of 128 or 256 rows
 hipError_t launch_gqa_stream(const GqaParams& p, int dim, int rows, hipStream_t stream);  // CTAs of 16 or 32 rows
 
 }  // namespace mla

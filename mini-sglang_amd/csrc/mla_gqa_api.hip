@@ -34,6 +34,10 @@ constexpr int kBlock = 128;
 constexpr int kBlocksEnough = 1024;
 constexpr int kOnePieceBlocks = 1024;
 constexpr int kOnePieceMany = 1600;
+// Prompts of at least this many tokens on average (head_dim 128), in blocks alone on their compute units: two halves of a
+// block's keys side by side. With / without, us: 3000, 8 heads and 1 46 / 51; 4000, 4 and 1 57 / 65, at head_dim 64 42 / 52;
+// 1000, 16 and 2 23 / 23, at head_dim 64 17 / 18; four of 300, 8 and 2 15 / 12.
+constexpr int64_t kAloneTokens = 2048;
 // Requests of more than 16 rows are streamed in pieces up to this many CTAs of 16 rows times keys.
 constexpr int64_t kFewWork = 1 << 18;
 
@@ -67,14 +71,18 @@ Choice choose(int dim, int32_t batch, int64_t total_q, int32_t group, int32_t kv
     if (most <= rows) break;
   }
   const int64_t blocks = (total_q * group + kBlock - 1) / kBlock * kv_heads;
-  if (keys == 0) return {kBlock, 0, false, wide_blocks(dim, blocks, total_q / batch, total_q / batch)};
+  const int64_t avg = total_q / batch;
+  if (keys == 0) {
+    if (wide_blocks(dim, blocks, avg, avg)) return {2 * kBlock, 0, false, false};
+    return {kBlock, 0, false, 2 * ctas(kBlock) <= kFit && avg * 128 >= kAloneTokens * dim};
+  }
   if (most > 16 && 2 * ctas(16) <= kFit && ctas(16) * keys <= kFewWork) return {16, kFit, true, false};
   if (most <= 32) {
     const int rows = most <= 16 ? 16 : 32;
     if (2 * ctas(rows) <= kFit) return {rows, kFit, true, false};
     return {rows, keys <= kOnePieceMany ? 0 : kTarget, false, false};
   }
-  if (blocks >= kBlocksEnough || keys <= kOnePieceBlocks) return {kBlock, 0, false, wide_blocks(dim, blocks, total_q / batch, keys)};
+  if (blocks >= kBlocksEnough || keys <= kOnePieceBlocks) return {wide_blocks(dim, blocks, avg, keys) ? 2 * kBlock : kBlock, 0, false, false};
   return {kBlock, kBlocksTarget, false, false};
 }
 
@@ -149,7 +157,7 @@ int launch(const char* who, GqaParams& p, const Choice& c, int dim, void* stream
   p.target = c.target;
   p.fit = c.fit;
   p.wide = c.wide;
-  return done(c.rows == kBlock ? launch_gqa_rows(p, dim, (hipStream_t)stream) : launch_gqa_stream(p, dim, c.rows, (hipStream_t)stream), who);
+  return done(c.rows >= kBlock ? launch_gqa_rows(p, dim, c.rows, (hipStream_t)stream) : launch_gqa_stream(p, dim, c.rows, (hipStream_t)stream), who);
 }
 
 int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,

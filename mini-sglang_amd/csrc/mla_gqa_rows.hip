@@ -2,7 +2,7 @@
 // the mathematics.
 //
 // One CTA per (request, 32 NW rows, KV head, piece of the keys), NW waves x 32 rows, two waves per SIMD: NW 4 (two CTAs
-// on a compute unit) or 8 (one).
+// on a compute unit) or 8 (one). With KS 2 a CTA has two of four waves, each for half of the keys, joined at the end.
 //  * Keys stream in stages of 32 through a K ring and a V ring in LDS, filled by 16-byte DMA loads whose sources are
 //    per token, so that a page may end anywhere (rows of a paged cache are looked up a window at a time into LDS).
 //    Keys past the last repeat it. 16-byte chunks are permuted within a row (kchunk, vchunk), so that neither the K
@@ -100,8 +100,8 @@ constexpr int uop_total(int n) {
 }
 constexpr int uop_slot(int u, int slots) { return uop_total(u) * slots / uop_total(kUops); }
 
-template <int D, int NW, bool kPaged>
-__global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p) {
+template <int D, int NW, int KS, bool kPaged>
+__global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaParams p) {
   using S = Rings<NW>;
   constexpr int kRows = 32 * NW, kRowB = D * 2, kTileB = kStage * kRowB;
   constexpr int kKs = D / 16, kDb = D / 32, kVs = 2 * kDb;  // K operands, 32-dim blocks, V operands of a stage
@@ -112,11 +112,13 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
   constexpr int kRingB = S::kRing * kTileB;
   constexpr int kAK = D == 128 ? 4 : 3, kAV = 3;  // operands read ahead
   static_assert(kAK <= kVs && kAV <= kKs, "read ahead by less than a step");
-  __shared__ __attribute__((aligned(1024))) char smem[2 * kRingB];
+  __shared__ __attribute__((aligned(1024))) char smem[KS * 2 * kRingB];
+  static_assert(KS == 1 || !kPaged, "one window of rows");
   __shared__ int s_row[kPaged ? S::kWindow : 1];
 
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wave_all % NW, part = wave_all / NW;  // part: of the keys
   GqaItem it;
   if (!gqa_find<kRows, true>(p, blockIdx.x, it)) return;
   const int E = it.r.E, L = it.r.L, P = it.r.P, G = p.group;
@@ -128,8 +130,10 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
   auto tok_of = [&](int i) __attribute__((always_inline)) { return tok0 + (int)(((float)(rem0 + i) + 0.5f) * inv_g); };
   auto head_of = [&](int i, int tok) __attribute__((always_inline)) { return it.head * G + rem0 + i - (tok - tok0) * G; };
   const int last_tok = min(E - 1, (it.block * kRows + kRows - 1) / G);
-  const int k0 = it.piece * it.C, k1 = min(it.pieces > 1 ? k0 + it.C : L, P + last_tok + 1);
-  const int nst = __builtin_amdgcn_readfirstlane(k1 > k0 ? (k1 - k0 + kStage - 1) / kStage : 0);
+  const int k0_all = it.piece * it.C, k1_all = min(it.pieces > 1 ? k0_all + it.C : L, P + last_tok + 1);
+  // stages, of each part alike (the last part's may lie past its keys)
+  const int nst = __builtin_amdgcn_readfirstlane(k1_all > k0_all ? ((k1_all - k0_all + kStage - 1) / kStage + KS - 1) / KS : 0);
+  const int k0 = k0_all + part * nst * kStage, k1 = part + 1 < KS ? min(k0 + nst * kStage, k1_all) : k1_all;
   int W = 0;  // stages that the wave needs
   if (tok0 < E) W = (min(k1, P + min(E - 1, (row0 + 31) / G) + 1) - k0 + kStage - 1) / kStage;
   W = __builtin_amdgcn_readfirstlane(max(W, 0));
@@ -187,7 +191,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
       vb[i] = reinterpret_cast<const char*>(p.v + (int64_t)it.head * p.v_head_stride) + vchunk<D>(c, tk[i]) * 16;
     }
     const uint32_t ks_b = (uint32_t)(p.k_row_stride * 2), vs_b = (uint32_t)(p.v_row_stride * 2);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(MLA_LDS char*)smem + wave * kLd * 1024;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(MLA_LDS char*)smem + part * 2 * kRingB + wave * kLd * 1024;
     int row[kLd], row_1[kLd], row_v[kLd];  // of group n's K stage, the one before, and V stage n - 2
     auto rows_of = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
@@ -198,15 +202,15 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
         else row[i] = it.r.q0 + k0 + min(n * kStage + tk[i], last);
       }
     };
-    auto dma = [&](int part, uint32_t kslot, uint32_t vslot) __attribute__((always_inline)) {
-      const int i = part % kLd;
-      if (part < kLd) dma16_vaddr(kb[i] + (uint64_t)(uint32_t)row[i] * ks_b, lds0 + kslot * kTileB + i * 1024);
+    auto dma = [&](int n, uint32_t kslot, uint32_t vslot) __attribute__((always_inline)) {
+      const int i = n % kLd;
+      if (n < kLd) dma16_vaddr(kb[i] + (uint64_t)(uint32_t)row[i] * ks_b, lds0 + kslot * kTileB + i * 1024);
       else dma16_vaddr(vb[i] + (uint64_t)(uint32_t)row_v[i] * vs_b, lds0 + kRingB + vslot * kTileB + i * 1024);
     };
     auto group_now = [&](int n) __attribute__((always_inline)) {
       rows_of(n);
 #pragma unroll
-      for (int part = 0; part < 2 * kLd; ++part) dma(part, n % S::kRing, (n + S::kRing - 2) % S::kRing);
+      for (int l = 0; l < 2 * kLd; ++l) dma(l, n % S::kRing, (n + S::kRing - 2) % S::kRing);
     };
     auto sync_groups = [&](auto ng) __attribute__((always_inline)) {
       wait_vmcnt<2 * kLd * decltype(ng)::value>();
@@ -227,11 +231,11 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
     // ---- operand reads
     int k_off[kKs], v_off[kDb];
 #pragma unroll
-    for (int ks = 0; ks < kKs; ++ks) k_off[ks] = c32 * kRowB + kchunk<D>(2 * ks + g32, c32) * 16;
+    for (int ks = 0; ks < kKs; ++ks) k_off[ks] = part * 2 * kRingB + c32 * kRowB + kchunk<D>(2 * ks + g32, c32) * 16;
     // V^T operand: keys 16 ksp + 8 e + 4 g32 + 0..3 (e = 0, 1) of dims 32 db + 16 (gq & 1) + ..., as the numerators lie
     const int gq = lane >> 4, a16 = lane & 15, vt = 4 * (gq >> 1) + (a16 >> 2);
 #pragma unroll
-    for (int db = 0; db < kDb; ++db) v_off[db] = kRingB + vt * kRowB + vchunk<D>(4 * db + 2 * (gq & 1) + ((a16 & 3) >> 1), vt) * 16 + (a16 & 1) * 8;
+    for (int db = 0; db < kDb; ++db) v_off[db] = part * 2 * kRingB + kRingB + vt * kRowB + vchunk<D>(4 * db + 2 * (gq & 1) + ((a16 & 3) >> 1), vt) * 16 + (a16 & 1) * 8;
     auto kread = [&](int slot, int ks) __attribute__((always_inline)) {
       return *reinterpret_cast<const MLA_LDS bf16x8*>((const MLA_LDS char*)smem + slot * kTileB + k_off[ks]);
     };
@@ -370,6 +374,32 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
     wait_vmcnt<0>();  // the last groups have landed before the CTA ends
   }
 
+  if constexpr (KS == 2) {
+    // the second part's O to the first's waves, lane by lane, through its own rings, its sums through the first's V ring;
+    // the first's K ring serves the output
+    static_assert(NW * 64 * kDb * 16 * 4 <= 2 * kRingB && NW * 64 * 2 * 4 <= kRingB && NW * 32 * kRowB <= kRingB, "they fit");
+    MLA_LDS float* s = (MLA_LDS float*)((MLA_LDS char*)smem + 2 * kRingB) + wave * 64 * kDb * 16 + lane;
+    MLA_LDS float* s_ml = (MLA_LDS float*)((MLA_LDS char*)smem + kRingB) + wave * 128 + lane;
+    __syncthreads();  // both are done with their rings
+    if (part == 1) {
+#pragma unroll
+      for (int db = 0; db < kDb; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[64 * (16 * db + i)] = O[db][i];
+      s_ml[0] = m_ref;
+      s_ml[64] = l_run;
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const float m1 = s_ml[0], l1 = s_ml[64], m = fmaxf(m_ref, m1);
+    const float f0 = __builtin_amdgcn_exp2f(m_ref - m), f1 = __builtin_amdgcn_exp2f(m1 - m);
+    m_ref = m;
+    l_run = l_run * f0 + l1 * f1;
+#pragma unroll
+    for (int db = 0; db < kDb; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) O[db][i] = O[db][i] * f0 + s[64 * (16 * db + i)] * f1;
+  }
   // ---- results: a lane holds row c32, dims 32 db + 8 i4 + 4 g32 + 0..3
   const float l = sum_halves(l_run);
   const bool some = l > 0.f || l != l;
@@ -396,7 +426,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
     auto out_row = [&](int t, int h) __attribute__((always_inline)) { return p.out + (int64_t)(it.r.q0 + t) * p.out_stride_t + (int64_t)h * p.out_stride_h; };
     if (p.out_16b) {
       // whole rows at a time, through the wave's part of the rings
-      barrier_lds();  // every wave is done with them
+      if constexpr (KS == 1) barrier_lds();  // every wave is done with them
       MLA_LDS char* mine = (MLA_LDS char*)smem + wave * 32 * kRowB;
       constexpr int kCh = D / 8;
 #pragma unroll
@@ -430,30 +460,33 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_rows_kernel(const GqaParams p)
     for (; bad != 0; bad &= bad - 1) {
       const int i = __builtin_ctzll(bad);
       const float m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, m_ref), i));
-      gqa_row_again<D>(p, it, row0 + i, k0, k1, m, (int64_t)it.slot * kRows + 32 * wave + i);
+      gqa_row_again<D>(p, it, row0 + i, k0_all, k1_all, m, (int64_t)it.slot * kRows + 32 * wave + i);
     }
   }
 }
 
 template <int D, int NW>
 void launch_rows(const GqaParams& p, unsigned grid, hipStream_t stream) {
-  if (p.page_table != nullptr) hipLaunchKernelGGL((gqa_rows_kernel<D, NW, true>), dim3(grid), dim3(64 * NW), 0, stream, p);
-  else hipLaunchKernelGGL((gqa_rows_kernel<D, NW, false>), dim3(grid), dim3(64 * NW), 0, stream, p);
+  if (p.page_table != nullptr) hipLaunchKernelGGL((gqa_rows_kernel<D, NW, 1, true>), dim3(grid), dim3(64 * NW), 0, stream, p);
+  else hipLaunchKernelGGL((gqa_rows_kernel<D, NW, 1, false>), dim3(grid), dim3(64 * NW), 0, stream, p);
 }
 
 }  // namespace
 
 hipError_t launch_gqa_merge(const GqaParams& p, int dim, int rows, hipStream_t stream);
 
-hipError_t launch_gqa_rows(const GqaParams& p, int dim, hipStream_t stream) {
+hipError_t launch_gqa_rows(const GqaParams& p, int dim, int rows, hipStream_t stream) {
   // the workspace holds pieces of 128 rows
-  if (p.wide && (p.target > 0 || dim != 128)) return hipErrorInvalidValue;
-  const int rows = p.wide ? 256 : 128;
+  if (rows == 256 && (p.target > 0 || dim != 128)) return hipErrorInvalidValue;
+  if (p.wide && (rows == 256 || p.page_table != nullptr)) return hipErrorInvalidValue;
   // sum over requests of ceil(E group / rows), then of ceil(L / C) pieces each
   const int64_t blocks = ((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch;
   const int64_t grid = blocks * p.kv_heads + p.target;
-  if (!gqa_grid_ok(grid, 2 * rows)) return hipErrorInvalidValue;
-  if (p.wide) launch_rows<128, 8>(p, (unsigned)grid, stream);
+  if (!gqa_grid_ok(grid, 512)) return hipErrorInvalidValue;
+  if (p.wide) {
+    if (dim == 128) hipLaunchKernelGGL((gqa_rows_kernel<128, 4, 2, false>), dim3((unsigned)grid), dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((gqa_rows_kernel<64, 4, 2, false>), dim3((unsigned)grid), dim3(512), 0, stream, p);
+  } else if (rows == 256) launch_rows<128, 8>(p, (unsigned)grid, stream);
   else if (dim == 128) launch_rows<128, 4>(p, (unsigned)grid, stream);
   else launch_rows<64, 4>(p, (unsigned)grid, stream);
   hipError_t e = hipGetLastError();

@@ -6,9 +6,10 @@
 // nothing until the end, so there is no barrier in the stream: a wave brings a tile's K and V into the MFMAs' operand
 // layouts through private LDS tiles, and requests the next tile before it computes the present one.
 // Bound: HBM (each K and V row is read once), and below some 20 MB the chain of dependent loads (lengths, page, tile) and
-// the merge's launch. Measured with the merge: 64 requests of 1k to 8k tokens, 64 and 8 heads of 128, 226 us (5.7 TB/s);
+// the merge's launch. Measured with the merge: 64 requests of 1k to 8k tokens, 64 and 8 heads of 128, 223 us (5.8 TB/s);
 // 8 of 32k to 128k, 8 heads and 1, 60 us (5.4 TB/s); 16 chunks of 1 to 8 on 1k to 16k, 32 and 8 heads, pages of one
-// token, 112 us (5.1 TB/s); one request of 1500, 32 and 8 heads, 9.6 us.
+// token, 112 us (5.1 TB/s); one request of 1500, 32 and 8 heads, 9.6 us; in one piece, eight waves: three chunks of 5 to
+// 60 on up to 500, 28 and 4 heads, 8.6 us.
 #include "mla_gqa.h"
 
 namespace mla {
@@ -59,8 +60,9 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
   }
   // A tile is loaded row by row, 16 lanes (D 64: 8) to a row, and goes through the wave's own LDS tiles into the operand
   // layouts: with loads straight into the K operand's (a 16-byte chunk of 16 rows each), 64 requests of 1k to 8k tokens, 8
-  // KV heads, took 263 us where this takes 231. Non-temporal, since a row is read once (257 us without). row: of token
-  // t < 32 of the tile in lane t.
+  // KV heads, took 263 us where this takes 231. Non-temporal, since a row is read once (257 us without). Two tiles in
+  // flight a wave gained nothing (229 us / 235; four chunks of 64 on 900 keys 15.5 / 16.6). row: of token t < 32 of the tile
+  // in lane t.
   u32x4 kr[kLoads], vr[kLoads];
   auto rows = [&](int t0) __attribute__((always_inline)) { return gqa_row(p, it.b, it.r.q0, min(t0 + (lane & 31), L - 1)); };
   auto load = [&](int row) __attribute__((always_inline)) {

@@ -427,6 +427,25 @@ def test_prompt_lengths_in_blocks(dim, lens):
     check(*prompt_in_blocks(q, k, v, lens, dim ** -0.5), R.prompt(q, k, v, lens, dim ** -0.5))
 
 
+@pytest.mark.parametrize("dim,lens,heads", [(64, [2100], (6, 2)), (64, [1300], (12, 2)), (64, [3001, 70], (4, 4)), (128, [2049], (10, 5)), (128, [4100], (4, 1))])
+@pytest.mark.parametrize("value", [None, NAN, float("inf")])
+def test_long_prompts_on_few_heads(dim, lens, heads, value):
+    """Blocks alone on their compute units, the first of them without keys in the second half; later tokens that are not
+    finite."""
+    gen = torch.Generator().manual_seed(lens[0])
+    q, k, v = randn(gen, sum(lens), heads[0], dim), randn(gen, sum(lens), heads[1], dim), randn(gen, sum(lens), heads[1], dim)
+    ref = R.prompt(q, k, v, lens, 0.1)
+    keep = list(range(sum(lens)))
+    if value is not None:
+        last = [lens[0] - 1, lens[0] - 40]
+        v[last] = value
+        keep = [i for i in keep if not lens[0] - 40 <= i < lens[0]]
+    out, lse = run_prompt(q, k, v, lens, 0.1)
+    check(out[keep], lse[keep], R.Attention(*(x[keep] for x in ref)))
+    if value is not None:
+        assert not out[lens[0] - 40 : lens[0]].isfinite().any()
+
+
 @pytest.mark.parametrize("page_size", [1, 2, 16, 32, 256])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_chunk_pages_in_blocks(page_size, dim):
