@@ -10,6 +10,8 @@
 // 8 of 32k to 128k, 8 heads and 1, 60 us (5.4 TB/s); 16 chunks of 1 to 8 on 1k to 16k, 32 and 8 heads, pages of one
 // token, 112 us (5.1 TB/s); one request of 1500, 32 and 8 heads, 9.6 us; in one piece, eight waves: three chunks of 5 to
 // 60 on up to 500, 28 and 4 heads, 8.6 us.
+#include <type_traits>
+
 #include "mla_gqa.h"
 
 namespace mla {
@@ -46,8 +48,13 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
   const int last_tok = min(E - 1, (it.block * kRows + kRows - 1) / G);
   const int first_limit = P + it.block * kRows / G;  // of the item's first row: no key up to it is masked
   const int k0 = it.piece * C, k1 = min(it.pieces > 1 ? k0 + C : L, P + last_tok + 1);
-  const __bf16* kh = p.k + (int64_t)it.head * p.k_head_stride;
-  const __bf16* vh = p.v + (int64_t)it.head * p.v_head_stride;
+  // of the lane's 16-byte chunk; row strides in bytes, below 2^32 by the host. As 32 bits an address is one multiply-add,
+  // which eight waves on their own gain by (a prompt of 8000, one head 76 -> 70 us; chunks of 64 on 900 13.8 -> 13.2); streams
+  // at HBM's rate lose (16 chunks of 1 to 8 on 1k to 16k 107 -> 109, decode of 32k to 128k 59.4 -> 60.3).
+  using stride_t = std::conditional_t<NW == 8, uint32_t, int64_t>;
+  const char* kh = reinterpret_cast<const char*>(p.k + (int64_t)it.head * p.k_head_stride + lane % kChunks * 8);
+  const char* vh = reinterpret_cast<const char*>(p.v + (int64_t)it.head * p.v_head_stride + lane % kChunks * 8);
+  const stride_t ks_b = (stride_t)(p.k_row_stride * 2), vs_b = (stride_t)(p.v_row_stride * 2);
 
   f32x4 O[NB][kDb];
   float m[NB], l[NB];
@@ -68,10 +75,9 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
   auto load = [&](int row) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      const int64_t rw = __shfl(row, (u * 64 + lane) / kChunks);
-      const int c = lane % kChunks * 8;
-      kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + rw * p.k_row_stride + c));
-      vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + rw * p.v_row_stride + c));
+      const std::conditional_t<NW == 8, uint64_t, int64_t> rw = (stride_t)__shfl(row, (u * 64 + lane) / kChunks);
+      kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + rw * ks_b));
+      vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + rw * vs_b));
     }
   };
   // 16-byte chunk c of token t: pairs of chunks permuted, so that neither the K reads (16 rows' chunks c and c + 1) nor
