@@ -38,6 +38,14 @@ constexpr int kOnePieceMany = 1600;
 // block's keys side by side. With / without, us: 3000, 8 heads and 1 46 / 51; 4000, 4 and 1 57 / 65, at head_dim 64 42 / 52;
 // 1000, 16 and 2 23 / 23, at head_dim 64 17 / 18; four of 300, 8 and 2 15 / 12.
 constexpr int64_t kAloneTokens = 2048;
+// CTAs of 16 rows, four waves each, that run at once (head_dim 64: as many as its registers allow; 128: two a compute unit, and
+// some more of ragged requests): up to here their chains are shorter than a block's. Against blocks, us, head_dim 64: seven
+// prompts of 1 to 300, 8 and 2 heads 6.4 / 9.1; four of 300 8.0 / 10.0; one of 1000, 16 and 2 (1000 CTAs) 16 / 18; eight of
+// 300, 8 and 2 (1200) 11 / 10; 128: nine of 1 to 300, 8 and 2 (550) 10 / 12; 600, 16 and 4 (600) 15 / 16; sixteen of 100
+// (800) 10.1 / 9.4. Paged, up to 512 keys: sixteen chunks of 20 on 400, 32 and 8 heads of 64, 11.1 / 12.6; twenty of 30 and
+// 10 on 200 9.4 / 10.9, on 900 21 / 20.
+constexpr int64_t kAtOnce64 = 1024;
+constexpr int64_t kAtOnce128 = 600;
 // Requests of more than 16 rows are streamed in pieces up to this many CTAs of 16 rows times keys.
 constexpr int64_t kFewWork = 1 << 18;
 
@@ -72,10 +80,13 @@ Choice choose(int dim, int32_t batch, int64_t total_q, int32_t group, int32_t kv
   }
   const int64_t blocks = (total_q * group + kBlock - 1) / kBlock * kv_heads;
   const int64_t avg = total_q / batch;
+  const bool at_once = ctas(16) <= (dim == 64 ? kAtOnce64 : kAtOnce128);
   if (keys == 0) {
     if (wide_blocks(dim, blocks, avg, avg)) return {2 * kBlock, 0, false, false};
-    return {kBlock, 0, false, 2 * ctas(kBlock) <= kFit && avg * 128 >= kAloneTokens * dim};
+    const bool halves = 2 * ctas(kBlock) <= kFit && avg * 128 >= kAloneTokens * dim;
+    return at_once && !halves ? Choice{16, 0, false, false} : Choice{kBlock, 0, false, halves};
   }
+  if (most > 32 && keys <= 512 && at_once) return {16, 0, false, false};
   if (most > 16 && 2 * ctas(16) <= kFit && ctas(16) * keys <= kFewWork) return {16, kFit, true, false};
   if (most <= 32) {
     const int rows = most <= 16 ? 16 : 32;

@@ -314,7 +314,7 @@ def test_later_tokens_that_are_not_finite_reach_no_earlier_row(dim, value):
         assert not out[extends[0] - 1].isfinite().any()
 
 
-@pytest.mark.parametrize("extends,pad", [([1, 1], 0), ([160, 20], 0), ([160, 20], 8192 // 16 + 64)])
+@pytest.mark.parametrize("extends,pad", [([1, 1], 0), ([160, 20], 0), ([160, 20], 16384 // 16 + 128)])
 def test_pool_past_32_bits(extends, pad):
     """K and V rows past 2^31 bytes and 2^31 elements from the pool's start; with rows behind the requests, in blocks."""
     pages, ps, hk, d = 17000, 64, 8, 128  # 1.1 G elements a pool, 2.2 GB
@@ -387,8 +387,8 @@ def test_one_workspace_for_steps_of_all_sizes(extends):
 
 
 def padding(q_heads):
-    """Rows behind the last request that make a batch one of more 32-row CTAs than compute units: its kernel is the blocks'."""
-    return 8192 // q_heads + 64
+    """Rows behind the last request that make a batch one of more 16-row CTAs than run at once: its kernel is the blocks'."""
+    return 16384 // q_heads + 128
 
 
 class InBlocks(Paged):
@@ -425,6 +425,18 @@ def test_prompt_lengths_in_blocks(dim, lens):
     gen = torch.Generator().manual_seed(sum(lens))
     q, k, v = randn(gen, sum(lens), 4, dim), randn(gen, sum(lens), 2, dim), randn(gen, sum(lens), 2, dim)
     check(*prompt_in_blocks(q, k, v, lens, dim ** -0.5), R.prompt(q, k, v, lens, dim ** -0.5))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,heads", [([150, 30, 300, 1, 200, 90, 20, 0, 250, 50], (8, 2)), ([60] * 9, (16, 4)), ([550], (17, 17)), ([1] * 40, (30, 15))])
+def test_prompts_between_few_ctas_and_blocks(dim, lens, heads):
+    """16-row CTAs that run at once, four waves each."""
+    gen = torch.Generator().manual_seed(len(lens))
+    q, k, v = randn(gen, sum(lens), heads[0], dim), randn(gen, sum(lens), heads[1], dim), randn(gen, sum(lens), heads[1], dim)
+    out, lse = run_prompt(q, k, v, lens, dim ** -0.5)
+    check(out, lse, R.prompt(q, k, v, lens, dim ** -0.5))
+    c = Paged([n % 61 for n in lens], [n // 2 for n in lens], *heads, dim, 16, seed=len(lens))
+    check(*c.run(), c.ref())
 
 
 @pytest.mark.parametrize("dim,lens,heads", [(64, [2100], (6, 2)), (64, [1300], (12, 2)), (64, [3001, 70], (4, 4)), (128, [2049], (10, 5)), (128, [4100], (4, 1))])
