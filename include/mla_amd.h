@@ -354,7 +354,8 @@ int mla_gqa_prompt_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, c
  * out) over its seq_lens_k[b] keys in a paged cache, any power-of-two page_size; row of key j: page_table[b, j /
  * page_size] * page_size + j % page_size, for row strides that hold for the whole pool. Keys are split over the chip
  * where there are few rows: `workspace` (16-byte aligned) holds the partial results, mla_gqa_workspace_bytes of it (which
- * is enough for every call with at most max_q queries a request, at any batch and length).
+ * is enough for every call with at most max_q queries a request, at any batch and length). NULL with 0 bytes will do where
+ * they are not: a call that splits them then returns MLA_ERR_INVALID_ARG before it launches anything.
  * Calls that overlap in time need workspaces of their own; nothing in one has to be kept or cleared between calls.
  *
  * mla_gqa_decode_bf16: the same with one token a request (query b is request b's last token).

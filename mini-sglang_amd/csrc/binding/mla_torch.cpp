@@ -204,32 +204,35 @@ PyObject* gqa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const float scale = number(a[7]);
     if (!is_current(x.device)) return PyLong_FromLong(kOtherDevice);
     void* stream = stream_of(a[11], x.device);
-    int64_t bytes = 0;
-    at::Tensor made;
-    void* ws;
-    if (a[10] == Py_None) {  // from torch's allocator, for this call
-      if (const int rc = g.workspace_bytes(max_q, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, &bytes)) return PyLong_FromLong(rc);
-      made = at::empty({bytes}, x.q.options().dtype(at::kByte));
-      used_on(a[11], stream, x.device, made);
-      ws = made.data_ptr();
-    } else {
+    const int32_t* pt_ptr = static_cast<const int32_t*>(pt.data_ptr());
+    auto call = [&](void* ws, int64_t bytes) {
+      return launched([&] {
+        if (decode)
+          return g.decode(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), x.k.data_ptr(), x.k.stride(1), x.k.stride(2), x.v.data_ptr(),
+                          x.v.stride(1), x.v.stride(2), (int32_t)x.k.size(0), (int32_t)ps, pt_ptr, (int32_t)pt.size(1), pt.stride(0),
+                          lens_ptr, (int32_t)B, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale, ws, bytes, x.out.data_ptr(),
+                          x.out.stride(0), x.out.stride(1), x.lse_ptr(), x.lse_stride(), stream);
+        return g.chunk(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), x.k.data_ptr(), x.k.stride(1), x.k.stride(2), x.v.data_ptr(),
+                       x.v.stride(1), x.v.stride(2), (int32_t)x.k.size(0), (int32_t)ps, pt_ptr, (int32_t)pt.size(1), pt.stride(0), cu,
+                       lens_ptr, (int32_t)B, (int32_t)x.T, max_q, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale, ws, bytes,
+                       x.out.data_ptr(), x.out.stride(0), x.out.stride(1), x.lse_ptr(), x.lse_stride(), stream);
+      });
+    };
+    if (a[10] != Py_None) {
       const at::Tensor& w = tensor(a[10], "workspace");
       require(gpu_of(w) == x.device && w.is_contiguous(), "the workspace is one block on q's GPU");
-      bytes = (int64_t)w.nbytes();
-      ws = w.data_ptr();
+      return PyLong_FromLong(call(w.data_ptr(), (int64_t)w.nbytes()));
     }
-    const int32_t *pt_ptr = static_cast<const int32_t*>(pt.data_ptr());
-    return PyLong_FromLong(launched([&] {
-      if (decode)
-        return g.decode(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), x.k.data_ptr(), x.k.stride(1), x.k.stride(2), x.v.data_ptr(),
-                        x.v.stride(1), x.v.stride(2), (int32_t)x.k.size(0), (int32_t)ps, pt_ptr, (int32_t)pt.size(1), pt.stride(0),
-                        lens_ptr, (int32_t)B, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale, ws, bytes, x.out.data_ptr(),
-                        x.out.stride(0), x.out.stride(1), x.lse_ptr(), x.lse_stride(), stream);
-      return g.chunk(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), x.k.data_ptr(), x.k.stride(1), x.k.stride(2), x.v.data_ptr(),
-                     x.v.stride(1), x.v.stride(2), (int32_t)x.k.size(0), (int32_t)ps, pt_ptr, (int32_t)pt.size(1), pt.stride(0), cu,
-                     lens_ptr, (int32_t)B, (int32_t)x.T, max_q, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale, ws, bytes,
-                     x.out.data_ptr(), x.out.stride(0), x.out.stride(1), x.lse_ptr(), x.lse_stride(), stream);
-    }));
+    // without one first; where keys are split, one from torch's allocator, for this call (2 us)
+    long rc = call(nullptr, 0);
+    if (rc == MLA_ERR_INVALID_ARG) {
+      int64_t bytes = 0;
+      if ((rc = g.workspace_bytes(max_q, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, &bytes))) return PyLong_FromLong(rc);
+      const at::Tensor made = at::empty({bytes}, x.q.options().dtype(at::kByte));
+      used_on(a[11], stream, x.device, made);
+      rc = call(made.data_ptr(), bytes);
+    }
+    return PyLong_FromLong(rc);
   });
 }
 

@@ -181,7 +181,7 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
     return api_error(MLA_ERR_INVALID_ARG, "%s: batch %d, total_q %d, max_q %d", who, batch, total_q, max_q);
   if (int rc = check_heads(who, q_heads, kv_heads, dim)) return rc;
   if (batch == 0 || total_q == 0 || max_q == 0) return done(hipSuccess, who);
-  if (page_table == nullptr || seq_lens_k == nullptr || workspace == nullptr)
+  if (page_table == nullptr || seq_lens_k == nullptr || (workspace == nullptr && workspace_bytes != 0))
     return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
   if (!is_pow2(page_size)) return api_error(MLA_ERR_UNSUPPORTED, "%s: page_size %d must be a power of two", who, page_size);
   if (num_pages < 1 || pt_cols < 1 || (batch > 1 && pt_stride < pt_cols))
@@ -195,22 +195,25 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
     return rc;
   const int64_t most = (int64_t)max_q * p.group;  // rows of a request and KV head
   const int64_t need = 4 * workspace_rows(most) * (dim + 1);
-  if (!aligned(workspace, 16) || workspace_bytes < need)
+  const int64_t keys = (int64_t)pt_cols * page_size;
+  // a piece's end, its length rounded up to 64 keys in each of the pieces before it, stays below 2^31
+  p.max_keys = (int32_t)(keys < 0x7ff00000 ? keys : 0x7ff00000);
+  const Choice choice = choose(dim, batch, total_q, p.group, kv_heads, most, p.max_keys);
+  if (!aligned(workspace, 16) || (workspace_bytes < need && (workspace != nullptr || choice.target > 0)))
     return api_error(MLA_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
                      (long long)need, (long long)workspace_bytes);
   p.num_pages = num_pages;
   for (p.log2_ps = 0; (1 << p.log2_ps) < page_size;) ++p.log2_ps;
   p.page_table = page_table;
   p.pt_stride = pt_stride;
-  const int64_t keys = (int64_t)pt_cols * page_size;
-  // a piece's end, its length rounded up to 64 keys in each of the pieces before it, stays below 2^31
-  p.max_keys = (int32_t)(keys < 0x7ff00000 ? keys : 0x7ff00000);
   p.cu_seqlens_q = cu_seqlens_q;
   p.seq_lens_k = seq_lens_k;
   p.max_q = max_q;
-  p.ws_o = static_cast<float*>(workspace);
-  p.ws_lse = p.ws_o + workspace_rows(most) * dim;
-  return launch(who, p, choose(dim, batch, total_q, p.group, kv_heads, most, p.max_keys), dim, stream);
+  if (workspace != nullptr) {
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_lse = p.ws_o + workspace_rows(most) * dim;
+  }
+  return launch(who, p, choice, dim, stream);
 }
 
 }  // namespace

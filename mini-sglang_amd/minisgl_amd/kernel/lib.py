@@ -586,7 +586,7 @@ def gqa_chunk(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqle
     ``q [T, Hq, D]`` packed by ``cu_seqlens_q [B + 1]``, ``k_pool``, ``v_pool [pages, ps, Hkv, D]`` (any power-of-two
     ``ps``), ``page_table [B, cols]``, ``seq_lens_k [B]`` (prefix and chunk) -> ``out [T, Hq, D]`` (+ ``lse [T, Hq]``).
     ``max_seqlen_q``: at least every request's new tokens. ``workspace``: of ``gqa_workspace``, or None to take one from
-    torch's allocator for this call."""
+    torch's allocator for this call, where its keys are split."""
     assert cu_seqlens_q is not None, "cu_seqlens_q is [B + 1]"
     call = load_binding().gqa_paged
     rc = call(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q, scale, out, lse, workspace, stream)

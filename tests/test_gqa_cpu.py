@@ -109,6 +109,11 @@ def test_workspace_of_many_queries_is_enough_for_fewer():
     assert sizes == sorted(sizes)
 
 
+def test_no_workspace_where_keys_are_split():
+    for rc in (chunk(cols=1000, pts=1000, ws=None, ws_bytes=0), decode(cols=1000, pts=1000, ws=None, ws_bytes=0)):
+        assert rc == INVALID and "workspace" in lib.load_library().mla_last_error().decode()
+
+
 def test_bindings_refuse_host_tensors_and_wrong_types():
     q, k = torch.zeros((4, 8, 64), dtype=torch.bfloat16), torch.zeros((4, 2, 64), dtype=torch.bfloat16)
     cu, pool, pt = torch.zeros(2, dtype=torch.int32), torch.zeros((3, 16, 2, 64), dtype=torch.bfloat16), torch.zeros((1, 2), dtype=torch.int32)
