@@ -386,6 +386,32 @@ def test_one_workspace_for_steps_of_all_sizes(extends):
     check(out, lse, c.ref())
 
 
+def test_captured_calls_without_a_workspace():
+    """Two graphs whose split keys use memory of their own pools, replayed in turn with eager calls and allocations between."""
+    made = []
+    for seed, extends, prefixes in ((31, [1, 1, 1], [3000, 40, 5000]), (32, [200, 3], [4000, 10])):
+        c = Paged(extends, prefixes, 8, 2, 128, 16, seed=seed)
+        cu, lens = i32(cumulative(extends)), i32(c.lens)
+        dev = [x.to(DEV) for x in (c.q, c.k, c.v, c.pt)]
+        out, lse = torch.empty_like(dev[0]), torch.empty(c.q.shape[:2], device=DEV)
+        call = lambda dev=dev, cu=cu, lens=lens, n=max(extends), s=c.scale, out=out, lse=lse: lib.gqa_chunk(*dev, cu, lens, n, s, out, lse)  # noqa: E731
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        made.append((graph, out, lse, c.ref(), call))  # which holds the inputs
+    for _ in range(3):
+        for graph, out, lse, ref, _ in made:
+            out.fill_(NAN), lse.fill_(NAN)
+            graph.replay()
+            junk = torch.full((1 << 25,), NAN, device=DEV)
+            other = Paged([1, 7], [3000, 60], 8, 2, 128, 16, seed=33)
+            check(*other.run(), other.ref(), "eager, between replays")
+            check(out, lse, ref)
+            del junk
+
+
 def padding(q_heads):
     """Rows behind the last request that make a batch one of more 16-row CTAs than run at once: its kernel is the blocks'."""
     return 16384 // q_heads + 128
