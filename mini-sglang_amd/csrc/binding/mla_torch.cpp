@@ -2,8 +2,9 @@
 // the tensors, the entry point with their pointers and strides on a stream), with the tensors read in C++. A call of 28
 // arguments took 6 us in Python and 2 in ctypes, more than most of these kernels run.
 //
-// Every function returns the entry point's code, or kOtherDevice where the tensors' GPU is not the current one (the
-// caller makes it current and calls again). A tensor that does not fit raises AssertionError, as in lib.py.
+// Every function returns the entry point's code, kOtherDevice where the tensors' GPU is not the current one, or kOtherStream
+// where it takes memory from torch's allocator for a stream that is not the current one (the caller makes the GPU or the
+// stream current and calls again). A tensor that does not fit raises AssertionError, as in lib.py.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -17,7 +18,7 @@
 
 namespace {
 
-constexpr long kOtherDevice = -1;
+constexpr long kOtherDevice = -1, kOtherStream = -2;
 
 // set by bind(): the entry points of the loaded library, and torch's current device and raw stream
 struct {
@@ -91,15 +92,9 @@ void* current_stream(long device) {
 void* stream_of(PyObject* stream, long device) {
   return stream == Py_None ? current_stream(device) : as_pointer(PyObject_GetAttrString(stream, "cuda_stream"));
 }
-// memory from torch's allocator belongs to the current stream; a call on another one has to say so
-void used_on(PyObject* stream, void* raw, long device, const at::Tensor& t) {
-  if (stream == Py_None || raw == current_stream(device)) return;
-  PyObject* o = THPVariable_Wrap(t);
-  PyObject* r = o == nullptr ? nullptr : PyObject_CallMethod(o, "record_stream", "O", stream);
-  Py_XDECREF(o);
-  if (r == nullptr) throw Refused();
-  Py_DECREF(r);
-}
+// Memory from torch's allocator belongs to the current stream: work that is queued there may still use the block's last
+// content, and nothing orders another stream's launch behind it.
+bool allocates_for(PyObject* stream, void* raw, long device) { return stream == Py_None || raw == current_stream(device); }
 
 const int32_t* index(PyObject* o, const char* name, int64_t n, long device) {
   const at::Tensor& t = tensor(o, name);
@@ -228,8 +223,8 @@ PyObject* gqa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (rc == MLA_ERR_INVALID_ARG) {
       int64_t bytes = 0;
       if ((rc = g.workspace_bytes(max_q, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, &bytes))) return PyLong_FromLong(rc);
+      if (!allocates_for(a[11], stream, x.device)) return PyLong_FromLong(kOtherStream);
       const at::Tensor made = at::empty({bytes}, x.q.options().dtype(at::kByte));
-      used_on(a[11], stream, x.device, made);
       rc = call(made.data_ptr(), bytes);
     }
     return PyLong_FromLong(rc);
@@ -256,11 +251,11 @@ PyObject* page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     require(ps > 0 && max_len >= 0 && total >= 0, "page_size is positive, max_device_len and total_new are not negative");
     if (!is_current(device)) return PyLong_FromLong(kOtherDevice);
     void* stream = stream_of(a[10], device);
+    if (!allocates_for(a[10], stream, device)) return PyLong_FromLong(kOtherStream);
     const int64_t cols = ((int64_t)max_len + ps - 1) / ps, cells = B * cols;
     at::AutoDispatchBelowADInplaceOrView below;
     // one allocation, which the tables are cut from
     at::Tensor made = at::empty({cells + 2 * (int64_t)total + B + 2}, tt.options());
-    used_on(a[10], stream, device, made);
     int32_t* base = static_cast<int32_t*>(made.data_ptr());
     int32_t *loc = base + cells, *pos = loc + total, *cu = pos + total;
     const long rc = launched([&] {

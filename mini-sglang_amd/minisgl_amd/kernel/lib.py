@@ -538,15 +538,25 @@ def load_binding():
     return binding
 
 
-_OTHER_DEVICE = -1
+_OTHER_DEVICE, _OTHER_STREAM = -1, -2
 
 
-def _again(device, call, name: str, *args):
-    """The rest of a call that did not go through at once: with the tensors' GPU current, or its error."""
+def _again(rc: int, device, call, name: str, *args):
+    """The rest of a call (its last argument the stream) that did not go through at once: with the tensors' GPU current, with
+    the stream current that memory is allocated for (only there is a block's last use ordered before the launch), or its
+    error. Results of such an allocation are marked as used on the caller's stream, for when they are freed."""
     import torch
 
     with torch.cuda.device(device):
-        rc = call(*args)
+        if rc == _OTHER_DEVICE:
+            rc = call(*args)
+        if rc == _OTHER_STREAM:
+            stream, callers = args[-1], torch.cuda.current_stream()
+            assert stream.device == device, "the stream is another GPU's"
+            with torch.cuda.stream(stream):
+                rc = call(*args)
+            if isinstance(rc, tuple):
+                rc[0].record_stream(callers)  # of the block that all of them lie in
     if isinstance(rc, int) and rc != 0:
         check(rc, name)
     return rc
@@ -558,10 +568,8 @@ def gqa_prompt(q, k, v, cu_seqlens, scale: float, out, lse=None, stream=None) ->
     head h reads KV head ``h // (Hq // Hkv)``."""
     call = load_binding().gqa_prompt
     rc = call(q, k, v, cu_seqlens, scale, out, lse, stream)
-    if rc == _OTHER_DEVICE:
-        _again(q.device, call, "mla_gqa_prompt_bf16", q, k, v, cu_seqlens, scale, out, lse, stream)
-    elif rc != 0:
-        check(rc, "mla_gqa_prompt_bf16")
+    if rc != 0:
+        _again(rc, q.device, call, "mla_gqa_prompt_bf16", q, k, v, cu_seqlens, scale, out, lse, stream)
 
 
 @functools.lru_cache(maxsize=None)
@@ -586,26 +594,22 @@ def gqa_chunk(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqle
     ``q [T, Hq, D]`` packed by ``cu_seqlens_q [B + 1]``, ``k_pool``, ``v_pool [pages, ps, Hkv, D]`` (any power-of-two
     ``ps``), ``page_table [B, cols]``, ``seq_lens_k [B]`` (prefix and chunk) -> ``out [T, Hq, D]`` (+ ``lse [T, Hq]``).
     ``max_seqlen_q``: at least every request's new tokens. ``workspace``: of ``gqa_workspace``, or None to take one from
-    torch's allocator for this call, where its keys are split."""
+    torch's allocator for this call (on ``stream``), where its keys are split."""
     assert cu_seqlens_q is not None, "cu_seqlens_q is [B + 1]"
     call = load_binding().gqa_paged
     rc = call(q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q, scale, out, lse, workspace, stream)
-    if rc == _OTHER_DEVICE:
-        _again(q.device, call, "mla_gqa_chunk_bf16", q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q,
+    if rc != 0:
+        _again(rc, q.device, call, "mla_gqa_chunk_bf16", q, k_pool, v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q,
                scale, out, lse, workspace, stream)
-    elif rc != 0:
-        check(rc, "mla_gqa_chunk_bf16")
 
 
 def gqa_decode(q, k_pool, v_pool, page_table, seq_lens, scale: float, out, lse=None, workspace=None, stream=None) -> None:
     """``gqa_chunk`` with one new token a request: ``q [B, Hq, D]`` -> ``out [B, Hq, D]`` (+ ``lse [B, Hq]``)."""
     call = load_binding().gqa_paged
     rc = call(q, k_pool, v_pool, page_table, None, seq_lens, 1, scale, out, lse, workspace, stream)
-    if rc == _OTHER_DEVICE:
-        _again(q.device, call, "mla_gqa_decode_bf16", q, k_pool, v_pool, page_table, None, seq_lens, 1, scale, out, lse,
+    if rc != 0:
+        _again(rc, q.device, call, "mla_gqa_decode_bf16", q, k_pool, v_pool, page_table, None, seq_lens, 1, scale, out, lse,
                workspace, stream)
-    elif rc != 0:
-        check(rc, "mla_gqa_decode_bf16")
 
 
 class PageTables(NamedTuple):
@@ -626,13 +630,12 @@ def page_tables_from_lengths(token_table, table_idx, cached_lens, device_lens, f
     all) take the pages that their new tokens start, in batch order, from ``free_slots`` (page-aligned token locations),
     which fills their token table rows; then every request's page table, and the new tokens' locations and positions.
     ``max_device_len``, ``max_extend`` and ``total_new`` are the host's: the longest request, the most new tokens of one,
-    and of all. Rows of requests that take pages must be distinct. One launch; nothing is read back."""
+    and of all. Rows of requests that take pages must be distinct. One launch; nothing is read back. The tables are
+    allocated on ``stream`` (default the current one)."""
     call = load_binding().page_tables
     got = call(token_table, table_idx, cached_lens, device_lens, free_slots, page_size, max_device_len, max_extend, total_new,
                alloc_reqs, stream)
-    if got == _OTHER_DEVICE:
-        got = _again(token_table.device, call, "mla_page_tables_from_lengths", token_table, table_idx, cached_lens, device_lens,
+    if isinstance(got, int):
+        got = _again(got, token_table.device, call, "mla_page_tables_from_lengths", token_table, table_idx, cached_lens, device_lens,
                      free_slots, page_size, max_device_len, max_extend, total_new, alloc_reqs, stream)
-    elif isinstance(got, int):
-        check(got, "mla_page_tables_from_lengths")
     return PageTables(*got)
