@@ -165,6 +165,20 @@ def _stream(stream) -> int | None:
     return stream.cuda_stream
 
 
+def _made(stream, make):
+    """``make()``, a tensor that a launch on ``stream`` reads or writes: made on that stream, since nothing orders the launch
+    behind what the current stream still does with a block that it gave back."""
+    import torch
+
+    if stream is None:
+        return make()
+    callers = torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        t = make()
+    t.record_stream(callers)  # which uses the result, when it is freed
+    return t
+
+
 def device_cu_count(device: int = 0) -> int:
     out = ctypes.c_int32(0)
     check(load_library().mla_device_cu_count(device, ctypes.byref(out)), "mla_device_cu_count")
@@ -181,7 +195,7 @@ def store_rows(cache, indices, x, stream=None) -> None:
     row_bytes = x[0].numel() * x.element_size() if n else cache[0].numel() * cache.element_size()
     assert cache[0].numel() * cache.element_size() == row_bytes, "row widths differ"
     assert indices.dim() == 1 and indices.shape[0] == n and indices.dtype in (torch.int32, torch.int64)
-    x2 = x.reshape(n, -1) if n else x
+    x2 = _made(stream, lambda: x.reshape(n, -1)) if n else x
     c2 = cache.view(cache.shape[0], -1)
     assert x2.stride(-1) == 1 and c2.stride(-1) == 1, "rows must be contiguous"
     check(
@@ -203,7 +217,7 @@ def page_table_from_tokens(token_table, table_idx, max_seqlen_k: int, page_size:
     B = table_idx.shape[0]
     cols = -(-max_seqlen_k // page_size)
     if out is None:
-        out = torch.empty((B, cols), dtype=torch.int32, device=token_table.device)
+        out = _made(stream, lambda: torch.empty((B, cols), dtype=torch.int32, device=token_table.device))
     check(
         load_library().mla_page_table_from_tokens(
             _ptr(token_table), token_table.shape[0], token_table.shape[1], token_table.stride(0),
@@ -434,7 +448,7 @@ def rmsnorm(x, weight, eps: float, out=None, stream=None):
     rows, n = x.shape
     assert weight.shape == (n,) and weight.dtype == torch.bfloat16 and weight.is_contiguous()
     if out is None:
-        out = torch.empty_like(x)
+        out = _made(stream, lambda: torch.empty_like(x))
     assert out.shape == x.shape and out.dtype == torch.bfloat16 and out.stride(1) == 1
     check(
         load_library().mla_rmsnorm_bf16(_ptr(x), x.stride(0), _ptr(weight), rows, n, float(eps), _ptr(out),
@@ -455,7 +469,7 @@ def latent_rows(kv, norm_weight, positions, cos_sin, eps: float, interleaved: bo
     assert positions.shape == (T,) and positions.dtype == torch.int32 and positions.is_contiguous()
     assert cos_sin.dim() == 2 and cos_sin.shape[1] == 64 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous()
     if out is None:
-        out = torch.empty((T, 576), dtype=torch.bfloat16, device=kv.device)
+        out = _made(stream, lambda: torch.empty((T, 576), dtype=torch.bfloat16, device=kv.device))
     assert out.shape == (T, 576) and out.dtype == torch.bfloat16 and out.stride(1) == 1
     check(
         load_library().mla_latent_rows_bf16(
@@ -504,7 +518,7 @@ def qkv_a_rows(qkv, q_rank: int, q_norm_weight, kv_norm_weight, positions, cos_s
     assert positions.shape == (T,) and positions.dtype == torch.int32 and positions.is_contiguous()
     assert cos_sin.dim() == 2 and cos_sin.shape[1] == 64 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous()
     if out is None:
-        out = torch.empty((T, 576), dtype=torch.bfloat16, device=qkv.device)
+        out = _made(stream, lambda: torch.empty((T, 576), dtype=torch.bfloat16, device=qkv.device))
     assert out.shape == (T, 576) and out.dtype == torch.bfloat16 and out.stride(1) == 1
     check(
         load_library().mla_qkv_a_rows_bf16(

@@ -135,3 +135,38 @@ def test_capture_on_a_forked_stream():
         assert torch.equal(out, other) and torch.equal(lse, other_lse)
         assert ((out.double().cpu() - ref.out).abs() <= ref.out_bound).all()
         del junk
+
+
+def test_other_results_on_another_stream():
+    """The calls that make their result, where none is given, and rows that are copied to be stored."""
+    gen = torch.Generator().manual_seed(4)
+    T, side = 3001, torch.cuda.Stream()
+    qkv = torch.randn((T, 512 + 576), generator=gen).to(torch.bfloat16).to(DEV)
+    w512, w576 = torch.ones(512, dtype=torch.bfloat16, device=DEV), torch.ones(576, dtype=torch.bfloat16, device=DEV)
+    pos, cos_sin = i32(list(range(T))), torch.randn((T, 64), generator=gen).to(DEV)
+    table, rows = i32(list(range(64 * 4096))).view(64, 4096), i32(list(range(64)))
+    wide, slots = qkv.view(T, 2, 544).transpose(0, 1).contiguous().transpose(0, 1), i32(list(range(T)))
+
+    def store(stream=None):
+        cache = torch.zeros((T, 1088), dtype=torch.bfloat16, device=DEV)
+        torch.cuda.synchronize()
+        freed_while_written(T * 1088 * 2)
+        lib.store_rows(cache, slots, wide, stream=stream)
+        return cache
+
+    calls = [
+        (T * 576 * 2, lambda **kw: lib.rmsnorm(qkv[:, :576], w576, 1e-6, **kw)),
+        (T * 576 * 2, lambda **kw: lib.latent_rows(qkv[:, 512:], w512, pos, cos_sin, 1e-6, False, **kw)),
+        (T * 576 * 2, lambda **kw: lib.qkv_a_rows(qkv.clone() if not kw else copy, 512, w512, w512, pos, cos_sin, 1e-6, False, **kw)),
+        (64 * 256 * 4, lambda **kw: lib.page_table_from_tokens(table, rows, 4096, 16, **kw)),
+        (T * 1088 * 2, store),
+    ]
+    for nbytes, call in calls:
+        copy = qkv.clone()
+        want = call()
+        torch.cuda.synchronize()
+        at = freed_while_written(nbytes)
+        got = call(stream=side)
+        assert call is store or got.untyped_storage().data_ptr() != at
+        torch.cuda.synchronize()
+        assert owned_by(side, nbytes) and torch.equal(got, want)
