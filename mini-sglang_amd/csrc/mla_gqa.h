@@ -208,9 +208,10 @@ __device__ __forceinline__ int gqa_row(const GqaParams& p, int b, int q0, int j)
 // For a row whose values are not finite although its sum is: V held an infinity or a NaN at some key. If one of the
 // item's keys that the row does not attend holds one, the matrix product (weight zero times it) may have put it there,
 // and the row is computed by itself over the keys that it attends, by the whole wave, until it is NaN throughout: slow
-// (0.13 ms per 1000 keys) and rare. m: the row's reference (log2 domain); at: its row of the workspace.
+// (0.13 ms per 1000 keys) and rare. Its reference is its own running maximum, not the products': the scores here are sums in
+// another order. at: the row's row of the workspace.
 template <int D>
-__device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem& it, int r, int k0, int k1, float m, int64_t at) {
+__device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem& it, int r, int k0, int k1, int64_t at) {
   typedef __bf16 dims_t __attribute__((ext_vector_type(D / 64)));
   typedef float part_t __attribute__((ext_vector_type(D / 64)));
   constexpr int kU = 8;  // keys in flight
@@ -236,7 +237,7 @@ __device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem&
   if (!near) return;
   const part_t q = load(p.q + (int64_t)(it.r.q0 + tok) * p.q_stride_t + (int64_t)head * p.q_stride_h);
   part_t o = {};
-  float l = 0.f;
+  float l = 0.f, m = -3.4028234663852886e38f;
   for (int j = k0; j < end; j += kU) {
     part_t x[kU], v[kU];
 #pragma unroll
@@ -245,11 +246,23 @@ __device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem&
       x[u] = q * load(p.k + row * p.k_row_stride + (int64_t)it.head * p.k_head_stride);
       v[u] = value(row);
     }
+    float s[kU], top = m;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      float s = x[u][0];
-      if constexpr (D == 128) s += x[u][1];
-      const float e = __builtin_amdgcn_exp2f(fmaf(wave_sum64(s), p.scale_log2, -m));
+      float part = x[u][0];
+      if constexpr (D == 128) part += x[u][1];
+      s[u] = wave_sum64(part);
+      if (j + u >= end) s[u] = -INFINITY;
+      top = fmaxf(top, s[u]);
+    }
+    // unscaled differences: exact next to the maximum, at any size of the scores
+    const float f = __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
+    m = top;
+    l *= f;
+    o *= f;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const float e = __builtin_amdgcn_exp2f((s[u] - m) * p.scale_log2);
       if (j + u < end) {
         l += e;
         o += e * v[u];

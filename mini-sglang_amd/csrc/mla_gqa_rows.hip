@@ -12,8 +12,10 @@
 //  * Software pipeline: step j issues the score MFMAs of stage j + 1 and then the value MFMAs of stage j - 1 while the
 //    vector ALU runs the softmax of stage j, spread over the MFMAs.
 //  * Online softmax in the log2 domain against a lazy row reference: the maximum of the wave's first stage, moved (with O
-//    and l rescaled, and the stage redone) only when a stage's numerators sum past 2^32: fp32 keeps its relative
-//    precision at any scale.
+//    and l rescaled, and the stage redone) only when a lane's numerators of a stage sum past 2^32. The reference is a
+//    rounded product m = round(max s * scale), the numerators are 2^(fma(s, scale, -m) - d): d = fma(max s, scale, -m), what
+//    the rounding left out, keeps the largest at 1. Below |m| = 2^24 it is at most half a bit and taken as 0, which keeps the
+//    subtraction out of the loop; a wave with a row past that redoes its stages.
 // Bound: the MFMAs, and under them power: prompts of 7.8k and 8.1k tokens with 64 and 8 heads of 128 take 1.76 ms, 1164
 // TFLOP/s, with the MFMAs busy for 62 % of the cycles at 1.83 GHz (alone, on random operands, they run at 1829 TFLOP/s
 // and 1.74 GHz); four chunks of 2048 on up to 8192, pages of 64, 1.17 ms, 1170 TFLOP/s. Short calls are bound by their
@@ -31,6 +33,7 @@ typedef float f32x16_t __attribute__((__vector_size__(64)));
 constexpr int kStage = 32;
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr float kLazyMax = 4294967296.0f;
+constexpr float kFar = 16777216.0f;  // references from here on have a rounding that counts
 
 template <int N>
 using ic = std::integral_constant<int, N>;
@@ -154,7 +157,8 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
   f32x16_t O[kDb];
 #pragma unroll
   for (int db = 0; db < kDb; ++db) O[db] = f32x16_t{};
-  float m_ref = kLowest, negm = -kLowest, l_run = 0.f;
+  float m_ref = kLowest, negm = -kLowest, d_ref = 0.f, l_run = 0.f;
+  uint64_t far = 0;  // lanes whose reference is past kFar
 
   if (nst > 0) {
     // ---- sources: token t of the piece
@@ -255,22 +259,33 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
       for (int i = 0; i < 16; ++i)
         if (8 * (i >> 2) + (i & 3) > lim) s[i] = -INFINITY;
     };
-    auto top_of = [&](const f32x16_t& s) __attribute__((always_inline)) {
-      float m = s[0];
+    // the reference of a stage by itself: m, and what its rounding left out
+    auto top_of = [&](const f32x16_t& s, float& m, float& d) __attribute__((always_inline)) {
+      float t = s[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) m = fmaxf(m, s[i]);
-      return fmaxf(max_halves(m) * p.scale_log2, kLowest);  // (a stage of -inf alone: its numerators are 0)
+      for (int i = 1; i < 16; ++i) t = fmaxf(t, s[i]);
+      t = max_halves(t);
+      m = fmaxf(t * p.scale_log2, kLowest);  // (a stage of -inf alone: its numerators are 0)
+      d = fabsf(m) >= kFar && m > kLowest ? fmaf(t, p.scale_log2, -m) : 0.f;
+    };
+    auto refer = [&](float m, float d) __attribute__((always_inline)) {
+      m_ref = m;
+      negm = -m;
+      d_ref = d;
+      far = __ballot(fabsf(m) >= kFar && m > kLowest);
     };
     auto redo = [&](const f32x16_t& s, u32x4 (&dst)[2], float& l_step) __attribute__((always_inline)) {
-      const float m_new = fmaxf(top_of(s), m_ref), fr = __builtin_amdgcn_exp2f(m_ref - m_new);
-      m_ref = m_new;
-      negm = -m_new;
+      float m, d;
+      top_of(s, m, d);
+      if (!(m > m_ref || (m == m_ref && d > d_ref))) m = m_ref, d = d_ref;
+      const float fr = __builtin_amdgcn_exp2f((m_ref - m) + (d_ref - d));
+      refer(m, d);
       l_run *= fr;
       float l = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[2 * k], p.scale_log2, negm));
-        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[2 * k + 1], p.scale_log2, negm));
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[2 * k], p.scale_log2, negm) - d_ref);
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[2 * k + 1], p.scale_log2, negm) - d_ref);
         l += e0 + e1;
         dst[k >> 2][k & 3] = pack_bf16x2(e0, e1);
       }
@@ -324,7 +339,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
         });
         __builtin_amdgcn_sched_barrier(0);
       });
-      if (__ballot(l_step >= kLazyMax) != 0) redo(sc[par], pb[par], l_step);
+      if ((__ballot(l_step >= kLazyMax) | far) != 0) redo(sc[par], pb[par], l_step);
       l_run += l_step;
     };
     auto step = [&](auto u_c, int j) __attribute__((always_inline)) {
@@ -335,8 +350,9 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
         rows_of(j + S::kDist);
         if (__builtin_expect(j >= j_diag || j == W, 0)) mask(sc[par], j, j == W);
         if constexpr (U == 0) if (__builtin_expect(j == 0, 0)) {
-          m_ref = top_of(sc[par]);
-          negm = -m_ref;
+          float m, d;
+          top_of(sc[par], m, d);
+          refer(m, d);
         }
         step_fast(u_c);
         if constexpr (U == 0) if (__builtin_expect(j == 0, 0))
@@ -377,9 +393,9 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
   if constexpr (KS == 2) {
     // the second part's O to the first's waves, lane by lane, through its own rings, its sums through the first's V ring;
     // the first's K ring serves the output
-    static_assert(NW * 64 * kDb * 16 * 4 <= 2 * kRingB && NW * 64 * 2 * 4 <= kRingB && NW * 32 * kRowB <= kRingB, "they fit");
+    static_assert(NW * 64 * kDb * 16 * 4 <= 2 * kRingB && NW * 64 * 3 * 4 <= kRingB && NW * 32 * kRowB <= kRingB, "they fit");
     MLA_LDS float* s = (MLA_LDS float*)((MLA_LDS char*)smem + 2 * kRingB) + wave * 64 * kDb * 16 + lane;
-    MLA_LDS float* s_ml = (MLA_LDS float*)((MLA_LDS char*)smem + kRingB) + wave * 128 + lane;
+    MLA_LDS float* s_ml = (MLA_LDS float*)((MLA_LDS char*)smem + kRingB) + wave * 192 + lane;
     __syncthreads();  // both are done with their rings
     if (part == 1) {
 #pragma unroll
@@ -388,12 +404,16 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
         for (int i = 0; i < 16; ++i) s[64 * (16 * db + i)] = O[db][i];
       s_ml[0] = m_ref;
       s_ml[64] = l_run;
+      s_ml[128] = d_ref;
     }
     __syncthreads();
     if (part == 1) return;
-    const float m1 = s_ml[0], l1 = s_ml[64], m = fmaxf(m_ref, m1);
-    const float f0 = __builtin_amdgcn_exp2f(m_ref - m), f1 = __builtin_amdgcn_exp2f(m1 - m);
+    const float m1 = s_ml[0], l1 = s_ml[64], d1 = s_ml[128];
+    const bool second = m1 > m_ref || (m1 == m_ref && d1 > d_ref);
+    const float m = second ? m1 : m_ref, d = second ? d1 : d_ref;
+    const float f0 = __builtin_amdgcn_exp2f((m_ref - m) + (d_ref - d)), f1 = __builtin_amdgcn_exp2f((m1 - m) + (d1 - d));
     m_ref = m;
+    d_ref = d;
     l_run = l_run * f0 + l1 * f1;
 #pragma unroll
     for (int db = 0; db < kDb; ++db)
@@ -403,7 +423,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
   // ---- results: a lane holds row c32, dims 32 db + 8 i4 + 4 g32 + 0..3
   const float l = sum_halves(l_run);
   const bool some = l > 0.f || l != l;
-  const float inv = some ? 1.f / l : 0.f, lse2 = some ? m_ref + log2f(l) : -INFINITY;
+  const float inv = some ? 1.f / l : 0.f, lse2 = some ? m_ref + (d_ref + log2f(l)) : -INFINITY;
   const int64_t at = (int64_t)it.slot * kRows + 32 * wave + c32;
   if (it.slot >= 0) {
     if (live) {
@@ -459,8 +479,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
     bad = (bad | bad >> 32) & 0xffffffff;
     for (; bad != 0; bad &= bad - 1) {
       const int i = __builtin_ctzll(bad);
-      const float m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, m_ref), i));
-      gqa_row_again<D>(p, it, row0 + i, k0_all, k1_all, m, (int64_t)it.slot * kRows + 32 * wave + i);
+      gqa_row_again<D>(p, it, row0 + i, k0_all, k1_all, (int64_t)it.slot * kRows + 32 * wave + i);
     }
   }
 }

@@ -116,6 +116,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
     u32x4 pb[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
+      // the scaled scores are rounded before their maximum is taken from them: the largest numerator is 1 at any size
+#pragma clang fp contract(off)
       f32x4(&s)[2] = sc[nb];
       // score (h, i) of a lane: row a16, key t0 + 16 h + 4 g + i
       float top = kLowest;
@@ -218,8 +220,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
       while (bad != 0) {
         const int first = __builtin_ctzll(bad) / kTpr * kTpr;  // the row's first lane
         const int i = (64 * wave + first) / kTpr;
-        const float m_row = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mt), first));
-        gqa_row_again<D>(p, it, it.block * kRows + 16 * nb + i, k0, k1, m_row, (int64_t)it.slot * kRows + 16 * nb + i);
+        gqa_row_again<D>(p, it, it.block * kRows + 16 * nb + i, k0, k1, (int64_t)it.slot * kRows + 16 * nb + i);
         bad &= ~(((1ull << kTpr) - 1) << first);
       }
     }

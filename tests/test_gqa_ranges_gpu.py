@@ -1,0 +1,133 @@
+"""Grouped-head attention at the ends of the numbers' range, in every kernel: scores far past 2^24, whose fp32 spacing is
+more than one, and values whose sums come near fp32's largest."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from minisgl_amd.kernel import lib
+from test_gqa_gpu import DEV, InBlocks, Paged, i32, padding, prompt_in_blocks, run_prompt
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+class Exact:
+    """Attention of one request in 64 bits: ``q [E, Hq, D]`` over ``k, v [L, Hkv, D]``, head by head."""
+
+    def __init__(self, q, k, v, scale):
+        E, Hq, _ = q.shape
+        L, Hkv, _ = k.shape
+        seen = (torch.arange(L) <= (L - E + torch.arange(E))[:, None]).to(DEV)
+        out, top, lse, size = [], [], [], []
+        for h in range(Hq):
+            kh, vh = k[:, h * Hkv // Hq].to(DEV).double(), v[:, h * Hkv // Hq].to(DEV).double()
+            s = torch.where(seen, q[:, h].to(DEV).double() @ kh.t() * scale, -float("inf"))
+            top.append(s.amax(-1)), lse.append(torch.logsumexp(s, -1))
+            p = torch.exp(s - lse[-1][:, None])
+            out.append(p @ vh), size.append(p @ vh.abs())
+        self.out, self.size = torch.stack(out, 1), torch.stack(size, 1)
+        self.top, self.lse, self.keys = torch.stack(top, 1), torch.stack(lse, 1), L
+
+    def check(self, out, lse, what=""):
+        """For scores that are one exact product each: the kernels round the scaled score (and their constant scale times
+        log2 e), 2^-22 of it at most. That moves a weight by as much while |top| is below 2^13; from there on the nearest
+        other bf16 key is 2^-8 |top| >= 32 away and weighs nothing, and keys that are alike have rounded alike. Numerators
+        and results are rounded to bf16, half a step each; sums have L roundings."""
+        out, lse = out.to(DEV).double(), lse.to(DEV).double()
+        moved = (2.0 ** -22 * (self.top.abs() + 200)).clamp_max(2.0 ** -9)
+        rel = 2.0 ** -8 + 2 * moved + 2 * (self.keys + 16) * 2.0 ** -24
+        bound = 1.02 * (rel[..., None] * self.size + 2.0 ** -8 * self.out.abs())
+        assert out.isfinite().all() and lse.isfinite().all(), what
+        over = (out - self.out).abs() - bound
+        assert over.max() <= 0, f"{what}: out is {float(over.max()):.3e} past its bound"
+        off = (lse - self.lse).abs() - (2.0 ** -21 * (self.lse.abs() + 200) + (self.keys + 16) * 2.0 ** -24)
+        assert off.max() <= 0, f"{what}: lse is {float(off.max()):.3e} past its bound"
+
+
+def far(gen, tokens, q_heads, keys, kv_heads, dim, rising=False):
+    """Queries and keys of one dimension: scores of exact products, from hundreds to 2^34, of either sign."""
+    q, k = torch.zeros((tokens, q_heads, dim)), torch.zeros((keys, kv_heads, dim))
+    at = int(torch.randint(0, dim, (1,), generator=gen))
+    sign = torch.randint(0, 2, (tokens, q_heads), generator=gen) * 2.0 - 1
+    q[..., at] = sign * 2.0 ** torch.randint(0, 22, (tokens, q_heads), generator=gen)
+    k[..., at] = torch.randn((keys, kv_heads), generator=gen) * 4096
+    if rising:
+        k[..., at] = (torch.arange(keys)[:, None] - keys / 3) * 16
+    return q.to(torch.bfloat16), k.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("lens,heads,dim,blocks", [
+    ([300, 1, 77], (8, 2), 128, False), ([300, 1, 77], (8, 2), 64, False),  # 16-row CTAs
+    ([300, 1, 77], (8, 2), 128, True), ([700, 33], (6, 2), 64, True),  # blocks of 128 rows
+    ([2100], (6, 2), 64, False), ([4100], (4, 1), 128, False),  # in two halves of the keys
+    ([2600], (51, 17), 128, False),  # blocks of 256 rows
+])
+def test_far_scores_of_prompts(lens, heads, dim, blocks, rising):
+    gen = torch.Generator().manual_seed(sum(lens))
+    q, k = far(gen, sum(lens), heads[0], sum(lens), heads[1], dim, rising)
+    v = torch.randn((sum(lens), heads[1], dim), generator=gen).to(torch.bfloat16)
+    out, lse = (prompt_in_blocks if blocks else run_prompt)(q, k, v, lens, 0.125)
+    at = 0
+    for n in lens:
+        one = slice(at, at + n)
+        Exact(q[one], k[one], v[one], 0.125).check(out[one], lse[one], f"{n} of {lens}")
+        at += n
+
+
+@pytest.mark.parametrize("kind,extends,prefixes,heads", [
+    (Paged, [1, 1], [3000, 40], (8, 2)), (Paged, [3, 2], [5000, 600], (16, 4)),  # streamed, split and joined
+    (InBlocks, [200, 3], [3000, 700], (8, 2)), (InBlocks, [90, 40], [300, 64], (6, 2)),  # blocks, split and in one piece
+])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_far_scores_over_pages(kind, extends, prefixes, heads, dim):
+    """Keys split over pieces: each piece's largest score is its own, and one key of the prefix wins for either sign."""
+    gen = torch.Generator().manual_seed(dim + len(extends))
+    c = kind(extends, prefixes, *heads, dim, 16, seed=dim, scale=0.125)
+    rows, keys, at = [], [], 0
+    for b, (e, n) in enumerate(zip(extends, c.lens)):
+        q, k = far(gen, e, heads[0], n, heads[1], dim)
+        one = k.abs().amax((0, 1)).argmax()
+        k[..., one] *= 0.25
+        k[prefixes[b] // 3, :, one], k[prefixes[b] // 2, :, one] = 24576.0, -24576.0
+        j = torch.arange(n)
+        rows.append(c.pt[b].long()[j // 16] * 16 + j % 16)
+        c.k.view(-1, heads[1], dim)[rows[-1]] = k
+        c.q[at : at + e] = q
+        keys.append(k)
+        at += e
+    out, lse = c.run()
+    at = 0
+    for e, k, r in zip(extends, keys, rows):
+        one = slice(at, at + e)
+        Exact(c.q[one], k, c.v.view(-1, heads[1], dim)[r], 0.125).check(out[one], lse[one])
+        at += e
+
+
+@pytest.mark.parametrize("blocks", [False, True])
+def test_far_scores_beside_a_later_token_that_is_not_finite(blocks):
+    """A row computed again by itself, its scores summed in another order than the product's."""
+    gen = torch.Generator().manual_seed(9)
+    n, hq, hk, dim = 150, 4, 2, 128
+    q, k = far(gen, n, hq, n, hk, dim)
+    v = torch.randn((n, hk, dim), generator=gen).to(torch.bfloat16)
+    want = Exact(q[:-1], k[:-1], v[:-1], 0.125)
+    v[-1] = NAN
+    out, lse = (prompt_in_blocks if blocks else run_prompt)(q, k, v, [n], 0.125)
+    want.check(out[:-1], lse[:-1])
+    assert not out[-1].isfinite().any()
+
+
+@pytest.mark.parametrize("extends", [[1, 2], [140]])
+@pytest.mark.parametrize("blocks", [False, True])
+def test_far_scores_of_full_rows(extends, blocks):
+    """Scores of about 1e10 that are sums over all dimensions: their fp32 sums differ by more than one, so a row's weights
+    are only known to be some average of its values; no sum may pass for no keys, or leave the range."""
+    c = (InBlocks if blocks else Paged)(extends, [300] * len(extends), 8, 2, 128, 16, seed=5, scale=1e10 * 128 ** -0.5)
+    c.v = c.v.abs() + 0.5
+    out, lse = c.run()
+    ref = c.ref()
+    assert out.isfinite().all() and lse.isfinite().all() and float(out.float().min()) >= 0.49
+    assert ((lse.double().cpu() - ref.lse).abs() <= ref.lse_bound).all()
