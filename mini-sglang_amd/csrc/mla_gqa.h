@@ -9,6 +9,8 @@
 // r % group, so a K or V row is read once for all of them, and one new token fills group rows of a tile.
 #pragma once
 
+#include <limits.h>
+
 #include "mla_common.h"
 #include "mla_device.h"
 
@@ -205,79 +207,116 @@ __device__ __forceinline__ int gqa_row(const GqaParams& p, int b, int q0, int j)
   return (pid << p.log2_ps) + (j & ((1 << p.log2_ps) - 1));
 }
 
-// For a row whose values are not finite although its sum is: V held an infinity or a NaN at some key. If one of the
-// item's keys that the row does not attend holds one, the matrix product (weight zero times it) may have put it there,
-// and the row is computed by itself over the keys that it attends, by the whole wave, until it is NaN throughout: slow
-// (0.13 ms per 1000 keys) and rare. Its reference is its own running maximum, not the products': the scores here are sums in
-// another order. at: the row's row of the workspace.
+// For rows (bits of `rows`, row0 + bit) whose values are not finite although their sums of numerators are. Either V holds an
+// infinity or a NaN at a key that such a row attends, and that is its result; or at a key that it does not attend, and the
+// matrix product (weight zero times it) put it there; or finite values added up past fp32's range before a maximum that
+// makes them small was seen (numerators are relative to a running or a lazy reference). The last two are computed again,
+// row by row by the whole wave, until NaN throughout: slow (0.13 ms per 1000 keys) and rare. One pass over the item's V tells
+// which: each lane notes for its dims the first key that is not finite, and compares with what the row came out as. (It skips
+// to the first row's last key once that explains all that came out.)
+// The reference is a running maximum of its own, not the products': the scores here are sums in another order. A second sum
+// of values times 2^-32 stays in range whatever they are (below 2^31 keys), and is the result where the first did not.
+// at: row0's row of the workspace.
 template <int D>
-__device__ __forceinline__ void gqa_row_again(const GqaParams& p, const GqaItem& it, int r, int k0, int k1, int64_t at) {
-  typedef __bf16 dims_t __attribute__((ext_vector_type(D / 64)));
-  typedef float part_t __attribute__((ext_vector_type(D / 64)));
-  constexpr int kU = 8;  // keys in flight
-  const int d0 = (threadIdx.x & 63) * (D / 64), tok = r / p.group, head = it.head * p.group + r % p.group;
-  const int end = min(k1, it.r.P + tok + 1), hi = min(it.r.L, k0 + ((k1 - k0 + 31) & ~31));
+__device__ __forceinline__ void gqa_rows_again(const GqaParams& p, const GqaItem& it, int row0, uint64_t rows, int k0, int k1, int64_t at) {
+  constexpr int kN = D / 64;  // dims of a lane
+  typedef __bf16 dims_t __attribute__((ext_vector_type(kN)));
+  typedef float part_t __attribute__((ext_vector_type(kN)));
+  constexpr int kU = 8, kScan = 16;  // keys in flight (32: no faster)
+  const int d0 = (threadIdx.x & 63) * kN, hi = min(it.r.L, k0 + ((k1 - k0 + 31) & ~31));
   auto load = [&](const __bf16* x) { return __builtin_convertvector(*reinterpret_cast<const dims_t*>(x + d0), part_t); };
   auto value = [&](int64_t row) { return load(p.v + row * p.v_row_stride + (int64_t)it.head * p.v_head_stride); };
-  auto finite = [](part_t x) {
-    float zero = x[0] * 0.f;
-    if constexpr (D == 128) zero = fmaf(x[1], 0.f, zero);
-    return zero == 0.f;
+  auto finite = [](float x) { return x * 0.f == 0.f; };
+  // the rows' stores, by other lanes of the wave, have landed
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  wait_vmcnt<0>();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  auto token = [&](int r) { return r / p.group; };
+  auto end_of = [&](int r) { return min(k1, it.r.P + token(r) + 1); };
+  auto partial = [&](int r) { return p.ws_o + (at + (r - row0)) * D + d0; };
+  auto out_row = [&](int r) {
+    return p.out + (int64_t)(it.r.q0 + token(r)) * p.out_stride_t + (int64_t)(it.head * p.group + r % p.group) * p.out_stride_h;
   };
-  bool near = false;
-  for (int j = max(end, k0); j < hi && !near; j += kU) {
-    part_t v[kU];
+  auto result = [&](int r) { return it.slot >= 0 ? *reinterpret_cast<const part_t*>(partial(r)) : load(out_row(r)); };
+  bool bad[kN] = {};  // dims of the lane in which some row is not finite
+  for (uint64_t left = rows; left != 0; left &= left - 1) {
+    const part_t was = result(row0 + __builtin_ctzll(left));
 #pragma unroll
-    for (int u = 0; u < kU; ++u) v[u] = value(gqa_row(p, it.b, it.r.q0, min(j + u, hi - 1)));
-    bool all = true;
-#pragma unroll
-    for (int u = 0; u < kU; ++u) all = all && finite(v[u]);
-    near = __ballot(!all) != 0;
+    for (int e = 0; e < kN; ++e) bad[e] = bad[e] || !finite(was[e]);
   }
-  if (!near) return;
-  const part_t q = load(p.q + (int64_t)(it.r.q0 + tok) * p.q_stride_t + (int64_t)head * p.q_stride_h);
-  part_t o = {};
-  float l = 0.f, m = -3.4028234663852886e38f;
-  for (int j = k0; j < end; j += kU) {
-    part_t x[kU], v[kU];
+  int first[kN], last = -1;  // keys of the lane's dims that are not finite
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int64_t row = gqa_row(p, it.b, it.r.q0, min(j + u, end - 1));
-      x[u] = q * load(p.k + row * p.k_row_stride + (int64_t)it.head * p.k_head_stride);
-      v[u] = value(row);
-    }
-    float s[kU], top = m;
+  for (int e = 0; e < kN; ++e) first[e] = INT_MAX;
+  const int end0 = end_of(row0 + __builtin_ctzll(rows));  // all of the rows attend the keys before it
+  for (int j = k0; j < hi;) {
+    part_t v[kScan];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      float part = x[u][0];
-      if constexpr (D == 128) part += x[u][1];
-      s[u] = wave_sum64(part);
-      if (j + u >= end) s[u] = -INFINITY;
-      top = fmaxf(top, s[u]);
-    }
-    // unscaled differences: exact next to the maximum, at any size of the scores
-    const float f = __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
-    m = top;
-    l *= f;
-    o *= f;
+    for (int u = 0; u < kScan; ++u) v[u] = value(gqa_row(p, it.b, it.r.q0, min(j + u, hi - 1)));
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const float e = __builtin_amdgcn_exp2f((s[u] - m) * p.scale_log2);
-      if (j + u < end) {
-        l += e;
-        o += e * v[u];
+    for (int u = 0; u < kScan; ++u)
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (!finite(v[u][e])) {
+          last = min(j + u, hi - 1);
+          first[e] = min(first[e], last);
+        }
+    j += kScan;
+    bool open = false;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) open = open || (bad[e] && first[e] >= end0);
+    if (__ballot(open) == 0) j = max(j, end0);
+  }
+  for (; rows != 0; rows &= rows - 1) {
+    const int r = row0 + __builtin_ctzll(rows), tok = token(r), head = it.head * p.group + r % p.group, end = end_of(r);
+    const part_t was = result(r);
+    bool again = last >= end;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) again = again || (!finite(was[e]) && first[e] >= end);
+    if (__ballot(again) == 0) continue;
+    const part_t q = load(p.q + (int64_t)(it.r.q0 + tok) * p.q_stride_t + (int64_t)head * p.q_stride_h);
+    part_t o = {}, small = {};
+    float l = 0.f, m = -3.4028234663852886e38f;
+    for (int j = k0; j < end; j += kU) {
+      part_t x[kU], v[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int64_t row = gqa_row(p, it.b, it.r.q0, min(j + u, end - 1));
+        x[u] = q * load(p.k + row * p.k_row_stride + (int64_t)it.head * p.k_head_stride);
+        v[u] = value(row);
       }
+      float s[kU], top = m;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        float sum = x[u][0];
+        if constexpr (kN == 2) sum += x[u][1];
+        s[u] = wave_sum64(sum);
+        if (j + u >= end) s[u] = -INFINITY;
+        top = fmaxf(top, s[u]);
+      }
+      // unscaled differences: exact next to the maximum, at any size of the scores
+      const float f = __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
+      m = top;
+      l *= f;
+      o *= f;
+      small *= f;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const float e = __builtin_amdgcn_exp2f((s[u] - m) * p.scale_log2);
+        if (j + u < end) {
+          l += e;
+          o += e * v[u];
+          small += e * (v[u] * 0x1p-32f);
+        }
+      }
+      bool done = small[0] != small[0];
+      if constexpr (kN == 2) done = done && small[1] != small[1];
+      if (__ballot(!done) == 0) break;
     }
-    bool done = o[0] != o[0];
-    if constexpr (D == 128) done = done && o[1] != o[1];
-    if (__ballot(!done) == 0) break;
-  }
-  o *= l > 0.f ? 1.f / l : 0.f;
-  wait_vmcnt<0>();  // after the row's first stores
-  if (it.slot >= 0) {
-    *reinterpret_cast<part_t*>(p.ws_o + at * D + d0) = o;
-  } else {
-    *reinterpret_cast<dims_t*>(p.out + (int64_t)(it.r.q0 + tok) * p.out_stride_t + (int64_t)head * p.out_stride_h + d0) = __builtin_convertvector(o, dims_t);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) o[e] = finite(o[e]) ? o[e] * inv : small[e] * inv * 0x1p32f;
+    if (it.slot >= 0) *reinterpret_cast<part_t*>(partial(r)) = o;
+    else *reinterpret_cast<dims_t*>(out_row(r) + d0) = __builtin_convertvector(o, dims_t);
   }
 }
 

@@ -476,11 +476,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
     for (int i = 0; i < 16; ++i) zero = fmaf(O[db][i], 0.f, zero);
   uint64_t bad = __ballot(live && zero != 0.f && l < INFINITY);
   if (__builtin_expect(bad != 0, 0)) {
-    bad = (bad | bad >> 32) & 0xffffffff;
-    for (; bad != 0; bad &= bad - 1) {
-      const int i = __builtin_ctzll(bad);
-      gqa_row_again<D>(p, it, row0 + i, k0_all, k1_all, (int64_t)it.slot * kRows + 32 * wave + i);
-    }
+    gqa_rows_again<D>(p, it, row0, (bad | bad >> 32) & 0xffffffff, k0_all, k1_all, (int64_t)it.slot * kRows + 32 * wave);
   }
 }
 

@@ -217,12 +217,13 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
     }
     uint64_t bad = __ballot(zero != 0.f && lt < INFINITY);  // finite sums times 0 are 0
     if (__builtin_expect(bad != 0, 0)) {
-      while (bad != 0) {
-        const int first = __builtin_ctzll(bad) / kTpr * kTpr;  // the row's first lane
-        const int i = (64 * wave + first) / kTpr;
-        gqa_row_again<D>(p, it, it.block * kRows + 16 * nb + i, k0, k1, (int64_t)it.slot * kRows + 16 * nb + i);
-        bad &= ~(((1ull << kTpr) - 1) << first);
-      }
+      constexpr int kWr = 64 / kTpr;  // rows of a wave
+      uint64_t rows = 0;
+#pragma unroll
+      for (int i = 0; i < kWr; ++i)
+        if ((bad >> (i * kTpr) & ((1ull << kTpr) - 1)) != 0) rows |= 1ull << i;
+      const int r0 = 16 * nb + kWr * wave;
+      gqa_rows_again<D>(p, it, it.block * kRows + r0, rows, k0, k1, (int64_t)it.slot * kRows + r0);
     }
   }
 }

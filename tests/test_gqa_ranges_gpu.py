@@ -131,3 +131,98 @@ def test_far_scores_of_full_rows(extends, blocks):
     ref = c.ref()
     assert out.isfinite().all() and lse.isfinite().all() and float(out.float().min()) >= 0.49
     assert ((lse.double().cpu() - ref.lse).abs() <= ref.lse_bound).all()
+
+
+def rising_scores(gen, tokens, q_heads, keys, kv_heads, dim, nats):
+    """Queries and keys of one dimension, scores (at scale 0.125) rising by ``nats`` over the keys."""
+    q, k = torch.zeros((tokens, q_heads, dim)), torch.zeros((keys, kv_heads, dim))
+    at = int(torch.randint(0, dim, (1,), generator=gen))
+    q[..., at] = 8.0
+    k[..., at] = torch.linspace(-nats / 2, nats / 2, keys)[:, None]
+    return q.to(torch.bfloat16), k.to(torch.bfloat16)
+
+
+def huge(gen, *shape, most):
+    """Values of either sign, from 1 to 2^most."""
+    size = 2.0 ** (torch.rand(shape, generator=gen) * most)
+    return (size * (torch.randint(0, 2, shape, generator=gen) * 2 - 1)).to(torch.bfloat16)
+
+
+PROMPTS = [([300, 1, 77], (8, 2), 128, False), ([300, 1, 77], (8, 2), 64, False), ([300, 1, 77], (8, 2), 128, True),
+           ([700, 33], (6, 2), 64, True), ([2100], (6, 2), 64, False), ([4100], (4, 1), 128, False), ([2600], (51, 17), 128, False)]
+
+
+@pytest.mark.parametrize("lens,heads,dim,blocks", PROMPTS)
+def test_values_near_the_largest_of_prompts(lens, heads, dim, blocks):
+    """Finite values whose weighted sums are finite, under scores whose largest comes last: no partial sum may pass
+    fp32's range for good."""
+    gen = torch.Generator().manual_seed(sum(lens))
+    for nats, most in ((20, 100), (60, 126)):
+        if most == 126 and max(lens) > 1000:
+            continue  # every row is computed again by itself
+        q, k, v = [], [], []
+        for n in lens:
+            for x, y in zip((q, k), rising_scores(gen, n, heads[0], n, heads[1], dim, nats)):
+                x.append(y)
+            v.append(huge(gen, n, heads[1], dim, most=most))
+        out, lse = (prompt_in_blocks if blocks else run_prompt)(torch.cat(q), torch.cat(k), torch.cat(v), lens, 0.125)
+        at = 0
+        for n, x, y, z in zip(lens, q, k, v):
+            one = slice(at, at + n)
+            Exact(x, y, z, 0.125).check(out[one], lse[one], f"{n} of {lens}, {nats} nats, up to 2^{most}")
+            at += n
+
+
+@pytest.mark.parametrize("kind,extends,prefixes,heads", [
+    (Paged, [1, 1], [3000, 40], (8, 2)), (Paged, [3, 2], [5000, 600], (16, 4)), (Paged, [20], [300], (8, 2)),
+    (InBlocks, [200, 3], [3000, 700], (8, 2)), (InBlocks, [90, 40], [300, 64], (6, 2)),
+])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_near_the_largest_over_pages(kind, extends, prefixes, heads, dim):
+    """Keys of low scores and values near the largest before keys of high scores and ordinary values, which are the
+    result; and a rise over all keys."""
+    gen = torch.Generator().manual_seed(dim + len(extends))
+    for low in (False, True):
+        c = kind(extends, prefixes, *heads, dim, 16, seed=dim, scale=0.125)
+        made, at = [], 0
+        for b, (e, n) in enumerate(zip(extends, c.lens)):
+            q, k = rising_scores(gen, e, heads[0], n, heads[1], dim, 60)
+            v = huge(gen, n, heads[1], dim, most=100)
+            if low:
+                half = prefixes[b] * 2 // 3
+                k[:half] = -k[:half].abs() - (k != 0)[:half] * 200.0
+                v[:half], v[half:] = 2.0 ** 127, torch.randn(v[half:].shape, generator=gen).to(torch.bfloat16)
+            j = torch.arange(n)
+            rows = c.pt[b].long()[j // 16] * 16 + j % 16
+            c.k.view(-1, heads[1], dim)[rows], c.v.view(-1, heads[1], dim)[rows] = k, v
+            c.q[at : at + e] = q
+            made.append((slice(at, at + e), q, k, v))
+            at += e
+        out, lse = c.run()
+        for one, q, k, v in made:
+            Exact(q, k, v, 0.125).check(out[one], lse[one], f"low {low}")
+
+
+@pytest.mark.parametrize("lens,heads,dim,blocks", PROMPTS[:6])
+def test_an_infinity_that_rows_attend_stays_what_it_is(lens, heads, dim, blocks):
+    """One dimension of one token is infinite: the rows from it on are so in that dimension alone, beside a later token
+    that is NaN too; a token of both signs' infinity gives NaN."""
+    gen = torch.Generator().manual_seed(dim)
+    randn = lambda h: torch.randn((sum(lens), h, dim), generator=gen).to(torch.bfloat16)  # noqa: E731
+    q, k, v = randn(heads[0]), randn(heads[1]), randn(heads[1])
+    n, x = lens[0], lens[0] // 3
+    want = Exact(q[:n], k[:n], v[:n], 0.125)
+    for later in (False, True):
+        w = v.clone()
+        w[x, :, 5], w[x + 7, :, 9], w[x + 8, :, 9] = -float("inf"), float("inf"), -float("inf")
+        if later:
+            w[n - 1] = NAN
+        out, lse = (prompt_in_blocks if blocks else run_prompt)(q, k, w, lens, 0.125)
+        out, lse, rows = out[:n], lse[:n], n - later
+        assert (out[x:rows, :, 5] == -float("inf")).all() and out[x + 8 : rows, :, 9].isnan().all() and (out[x + 7, :, 9] == float("inf")).all()
+        assert not later or out[n - 1].isnan().all()
+        fixed = out.clone()
+        fixed[x:, :, 5], fixed[x + 7 :, :, 9] = want.out[x:, :, 5].to(out), want.out[x + 7 :, :, 9].to(out)
+        if later:
+            fixed[n - 1] = want.out[n - 1].to(out)
+        want.check(fixed, lse)
