@@ -390,9 +390,12 @@ int mla_gqa_decode_bf16(const void *q, int64_t q_stride_b, int64_t q_stride_h, c
  *   page_table[b, j] = token_table[row, j * page_size] / page_size for j < ceil(d / page_size), 0 for further j < pt_cols
  *   cu_seqlens_q[b] = sum over requests before b of d - c, and their sum in cu_seqlens_q[batch]
  *   out_loc[cu_seqlens_q[b] + i] = token_table[row, c + i], positions[...] = c + i, for i < d - c (entries at and past
- *                      total_new are not written)
- *   *pages_taken = the free slots needed; if they are more than num_free, only this and cu_seqlens_q are written.
- * Sums stop at 2^31 - 1. max_extend bounds d - c (tokens past it may be left out), pt_cols * page_size should hold the longest d. Any
+ *                      total_new are not written); entries from the new tokens' number up to total_new (a captured
+ *                      launch whose lengths became fewer) are -1, which mla_store_rows stores nothing at, and 0
+ *   *pages_taken = the free slots needed; if they are more than num_free, the token table stays as it is, cu_seqlens_q is
+ *                      written, page_table is 0, out_loc -1 and positions 0 throughout.
+ * Sums stop at 2^31 - 1. max_extend, about the most new tokens of a request, sizes the launch (a request of more takes
+ * longer); pt_cols * page_size should hold the longest d. Any
  * page_size. Replaces CacheManager.allocate_paged and the scheduler's slot and position gathers
  * (python/minisgl/scheduler/cache.py:42-53,119-161, scheduler/scheduler.py:198-214) with the page table of
  * python/minisgl/attention/fa.py:84-97.

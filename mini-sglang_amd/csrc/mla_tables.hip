@@ -23,7 +23,7 @@ __device__ __forceinline__ int page_of(int t, int ps, int log2_ps) {
 template <bool kPow2>
 __global__ __launch_bounds__(256) void page_tables_kernel(const PageTablesParams p) {
   __shared__ int s_sum[4][3];
-  const int b = blockIdx.y, x0 = blockIdx.x * kChunk + threadIdx.x, ps = p.page_size;
+  const int b = blockIdx.y, ps = p.page_size;
   auto page = [&](int t) { return page_of<kPow2>(t, ps, p.log2_ps); };
   // lengths, cut to the table's width
   auto lens = [&](int i, int& c, int& d) {
@@ -62,31 +62,49 @@ __global__ __launch_bounds__(256) void page_tables_kernel(const PageTablesParams
     if (b == p.batch - 1) p.cu_seqlens_q[p.batch] = add(fresh_before, d - c);
     if (b == 0) *p.pages_taken = all;
   }
-  if (all > min(p.num_free, 0x7ffffffe)) return;  // out of pages: no table is touched
+  // slots and positions that no token has: -1, which no row is stored at, and 0
+  auto none = [&](int64_t n, int64_t stride) {
+    for (; n < p.total_new; n += stride) {
+      p.out_loc[n] = -1;
+      p.positions[n] = 0;
+    }
+  };
+  const int64_t ctas = gridDim.x, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (all > min(p.num_free, 0x7ffffffe)) {  // out of pages: the token table stays, the others hold nothing
+    none(b * ctas * 256 + id, ctas * p.batch * 256);
+    for (int64_t i = id; i < p.pt_cols; i += ctas * 256) p.page_table[b * p.pt_stride + i] = 0;
+    return;
+  }
+  if (b == p.batch - 1) none(add(fresh_before, d - c) + id, ctas * 256);
   const int first = page(c + ps - 1), last = page(d + ps - 1);
   const bool takes = b < p.alloc_reqs;
   const int32_t* free_slots = p.free_slots + before - first;  // page j of the row: free_slots[j]
   // tokens from c to the end of the last page taken
   const int span = (takes && last > first ? min(last * ps, p.tt_cols) : d) - c;
-  int loc[kPer], head[kPer];
+  // once, unless a request has more new tokens than the launch was made for
+  const unsigned need = max(span, p.pt_cols);
+  for (unsigned x = blockIdx.x * kChunk; x < need; x += gridDim.x * kChunk) {
+    const int x0 = x + threadIdx.x;
+    int loc[kPer], head[kPer];
 #pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    const int i = x0 + 256 * u, pos = c + i, j = page(pos);
-    if (i < span) loc[u] = takes && j >= first ? free_slots[j] + pos - j * ps : row[pos];
-    if (i < last) head[u] = takes && i >= first ? free_slots[i] : row[i * ps];
-  }
-#pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    const int i = x0 + 256 * u, pos = c + i;
-    const int64_t n = (int64_t)fresh_before + i;
-    if (i < span && takes && page(pos) >= first) row[pos] = loc[u];
-    if (i < span && pos < d && n < p.total_new) {
-      p.out_loc[n] = loc[u];
-      p.positions[n] = pos;
+    for (int u = 0; u < kPer; ++u) {
+      const int i = x0 + 256 * u, pos = c + i, j = page(pos);
+      if (i < span) loc[u] = takes && j >= first ? free_slots[j] + pos - j * ps : row[pos];
+      if (i < last) head[u] = takes && i >= first ? free_slots[i] : row[i * ps];
     }
-    if (i < p.pt_cols) {
-      const int v = i < last ? head[u] : 0;
-      p.page_table[b * p.pt_stride + i] = kPow2 ? v >> p.log2_ps : v / ps - (v % ps != 0 && v < 0);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int i = x0 + 256 * u, pos = c + i;
+      const int64_t n = (int64_t)fresh_before + i;
+      if (i < span && takes && page(pos) >= first) row[pos] = loc[u];
+      if (i < span && pos < d && n < p.total_new) {
+        p.out_loc[n] = loc[u];
+        p.positions[n] = pos;
+      }
+      if (i < p.pt_cols) {
+        const int v = i < last ? head[u] : 0;
+        p.page_table[b * p.pt_stride + i] = kPow2 ? v >> p.log2_ps : v / ps - (v % ps != 0 && v < 0);
+      }
     }
   }
 }

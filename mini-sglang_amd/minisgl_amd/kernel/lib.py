@@ -630,10 +630,11 @@ class PageTables(NamedTuple):
     """A step's tables on the device (``page_tables_from_lengths``)."""
 
     page_table: "torch.Tensor"  # int32 [B, ceil(max_device_len / ps)] page ids, 0 past a request's pages
-    out_loc: "torch.Tensor"  # int32 [T] token locations of the new tokens, in batch order
-    positions: "torch.Tensor"  # int32 [T] their positions
+    out_loc: "torch.Tensor"  # int32 [T] token locations of the new tokens, in batch order; -1 past them
+    positions: "torch.Tensor"  # int32 [T] their positions; 0 past them
     cu_seqlens_q: "torch.Tensor"  # int32 [B + 1]
-    pages_taken: "torch.Tensor"  # int32 [1] free slots used; more than there are: nothing but this and cu_seqlens_q is written
+    # int32 [1] free slots used; more than there are: the token table stays, page_table is 0, out_loc -1, positions 0
+    pages_taken: "torch.Tensor"
 
 
 def page_tables_from_lengths(token_table, table_idx, cached_lens, device_lens, free_slots, page_size: int,
@@ -643,8 +644,8 @@ def page_tables_from_lengths(token_table, table_idx, cached_lens, device_lens, f
     device, like ``table_idx``, their rows of ``token_table [rows, cols]``): the first ``alloc_reqs`` requests (default
     all) take the pages that their new tokens start, in batch order, from ``free_slots`` (page-aligned token locations),
     which fills their token table rows; then every request's page table, and the new tokens' locations and positions.
-    ``max_device_len``, ``max_extend`` and ``total_new`` are the host's: the longest request, the most new tokens of one,
-    and of all. Rows of requests that take pages must be distinct. One launch; nothing is read back. The tables are
+    ``max_device_len``, ``max_extend`` and ``total_new`` are the host's: the longest request, the most new tokens of one
+    (which sizes the launch), and of all; a captured call follows its lengths, fewer new tokens than ``total_new`` included. Rows of requests that take pages must be distinct. One launch; nothing is read back. The tables are
     allocated on ``stream`` (default the current one)."""
     call = load_binding().page_tables
     got = call(token_table, table_idx, cached_lens, device_lens, free_slots, page_size, max_device_len, max_extend, total_new,

@@ -202,3 +202,57 @@ def test_steps_of_an_engine(page_size):
             lib.gqa_prompt(qd, kd, vd, t.cu_seqlens_q, scale, packed, packed_lse)
             assert ((packed.double().cpu() - ref.out).abs() <= ref.out_bound).all()
             assert ((packed_lse.double().cpu() - ref.lse).abs() <= ref.lse_bound).all()
+
+
+def test_replays_with_fewer_and_more_new_tokens():
+    """A captured step of padded size: fewer new tokens leave no slot of an earlier replay behind (nothing is stored at
+    -1), none at all too; requests longer than the launch was made for, up to the tokens that the tables hold."""
+    table, idx, free = make([20, 3, 90], [320, 303, 390], 16, 512, seed=8, spare=10)
+    dev, rows, c, d, f = table.to(DEV), i32(idx), i32([0] * 3), i32([0] * 3), free.to(DEV)
+    total = 64
+    call = lambda: lib.page_tables_from_lengths(dev, rows, c, d, f, 16, 512, 4, total)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t = call()
+    rows_of_x = torch.ones((total, 8), dtype=torch.bfloat16, device=DEV)
+    for extends in ([4, 4, 4], [1, 0, 2], [0, 0, 0], [4, 1, 4], [40, 4, 20], [0, 0, 300], [0, 1, 0]):
+        now, then = [20, 3, 90], [20 + extends[0], 3 + extends[1], 90 + extends[2]]
+        dev.copy_(table), c.copy_(i32(now)), d.copy_(i32(then))
+        graph.replay()
+        cache = torch.zeros((16 * 100, 8), dtype=torch.bfloat16, device=DEV)
+        lib.store_rows(cache, t.out_loc, rows_of_x)
+        torch.cuda.synchronize()
+        ref = R.step_tables(table, idx, now, then, free, 16, 32, 3)
+        n = min(sum(extends), total)
+        assert torch.equal(dev.cpu(), ref.token_table) and torch.equal(t.page_table.cpu(), ref.page_table)
+        assert t.out_loc.tolist() == ref.out_loc[:n] + [-1] * (total - n) and t.positions.tolist() == ref.positions[:n] + [0] * (total - n)
+        assert t.cu_seqlens_q.tolist() == ref.cu_seqlens_q and int(t.pages_taken) == ref.pages_taken
+        assert sorted(ref.out_loc[:n]) == cache[:, 0].nonzero().flatten().tolist()
+
+
+@pytest.mark.parametrize("page_size", [1, 16, 24])
+def test_out_of_pages_leaves_nothing_to_be_followed(page_size):
+    """Kernels that are queued behind the tables find no slot and page 0, whatever the memory held."""
+    cached, device = [5, 0, 70], [6, 3000, 75]
+    table, idx, free = make(cached, device, page_size, 3000, seed=9)
+    total = 3100
+    for _ in range(3):
+        torch.full((3 * 3000 + 2 * total + 5,), 77, dtype=torch.int32, device=DEV)  # given back at once
+        dev = table.to(DEV)
+        t = lib.page_tables_from_lengths(dev, i32(idx), i32(cached), i32(device), free[:2].to(DEV), page_size, 3000, 3000, total)
+        torch.cuda.synchronize()
+        assert torch.equal(dev.cpu(), table) and int(t.pages_taken) > 2 and t.cu_seqlens_q.tolist() == [0, 1, 3001, 3006]
+        assert (t.page_table == 0).all() and (t.out_loc == -1).all() and (t.positions == 0).all()
+
+
+@pytest.mark.parametrize("hint", [0, 1, 5, 10 ** 6])
+def test_most_new_tokens_only_size_the_launch(hint):
+    cached, device = [0, 17, 4000, 3], [2500, 18, 4100, 3]
+    table, idx, free = make(cached, device, 16, 4500, seed=10)
+    dev = table.to(DEV)
+    t = lib.page_tables_from_lengths(dev, i32(idx), i32(cached), i32(device), free.to(DEV), 16, 4100, hint, 2601)
+    ref = R.step_tables(table, idx, cached, device, free, 16, 257, 4)
+    assert torch.equal(dev.cpu(), ref.token_table) and torch.equal(t.page_table.cpu(), ref.page_table)
+    assert t.out_loc.tolist() == ref.out_loc and t.positions.tolist() == ref.positions
