@@ -40,7 +40,8 @@ struct GqaParams {
   int64_t lse_stride_t;
   float* ws_o;    // [slots, rows, D] partial outputs of split requests, normalised
   float* ws_lse;  // [slots, rows] their log2-domain LSEs
-  int32_t target;  // items that a batch's keys are split into, about (0: no splitting)
+  int32_t target;  // items that a batch's keys are split into, about (0: no splitting), a power of two
+  int32_t log2_target;
   int32_t fit;     // at most `target`, where that can be
   int32_t wide;    // eight waves a CTA instead of four, sharing an item's keys
   int32_t out_16b;  // rows of out start 16-byte aligned
@@ -85,17 +86,19 @@ __device__ __forceinline__ T wave_scan(T v, F&& f) {
 __device__ __forceinline__ int wave_iscan(int v) {
   return wave_scan(v, [](int a, int b) { return a + b; });
 }
-__device__ __forceinline__ float wave_fsum_all(float v) {
-  v = wave_scan(v, [](float a, float b) { return a + b; });
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+__device__ __forceinline__ uint32_t wave_sum_sat(uint32_t v) {
+  v = wave_scan(v, [](uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); });
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Keys of a piece, C: the batch's keys, weighted with the row blocks that read them, over `target` items, in whole tiles
 // of 64 and at least gqa_min_split; with `fit`, enlarged until the pieces are at most `target` (the CTAs that run at once:
 // one more piece would be a round of its own). Requests of more keys are cut into ceil(L / C) pieces. Every kernel of a
 // call computes the same C from the same lengths, so no plan is made on the host and a captured launch follows its
-// lengths. C is above cost / target (the sum's rounding included), so a batch has fewer than `target` pieces more than
-// blocks; a request in pieces has L > C, so ceil(L / C) <= 2 L / C, and 2 target slots hold every piece.
+// lengths; in whole numbers, since the kernels find each other's partial results by it: a sum that one of them rounds
+// otherwise would join foreign ones. C is above cost / target, so a batch has fewer than `target` pieces more than
+// blocks; a request in pieces has L > C, so ceil(L / C) <= 2 L / C, and 2 target slots hold every piece. The cost counts
+// 16 keys as one and stops at 2^32 - 1, where requests stay in one piece.
 // Least keys of a piece: a tile for each wave of the stream kernel; 16 stages of the blocks (their joining takes 6 us).
 template <int kRows>
 constexpr int gqa_min_split() {
@@ -111,11 +114,16 @@ template <int kRows>
 __device__ __forceinline__ int gqa_piece_keys(const GqaParams& p, const GqaRequest& r) {
   if (p.target <= 0) return 0x7fffffff;
   const int lane = threadIdx.x & 63;
-  auto cost_of = [&](const GqaRequest& x) { return (float)gqa_blocks<kRows>(p, x) * (float)x.L; };
-  float cost = lane < p.batch ? cost_of(r) : 0.f;
-  for (int b = 64 + lane; b < p.batch; b += 64) cost += cost_of(gqa_request(p, b));
-  const float c = wave_fsum_all(cost) * (float)p.kv_heads / (float)p.target * 1.0001f + 64.f;
-  int C = c < 2e9f ? (int)c & ~63 : 0x7fffffc0;
+  auto cost_of = [&](const GqaRequest& x) {
+    const uint64_t c = (uint64_t)(uint32_t)gqa_blocks<kRows>(p, x) * (uint32_t)((x.L + 15) >> 4);
+    return c < UINT32_MAX ? (uint32_t)c : UINT32_MAX;
+  };
+  uint32_t cost = lane < p.batch ? cost_of(r) : 0;
+  for (int b = 64 + lane; b < p.batch; b += 64) cost = __builtin_elementwise_add_sat(cost, cost_of(gqa_request(p, b)));
+  cost = wave_sum_sat(cost);
+  if (cost == UINT32_MAX) return 0x7fffffc0;
+  const uint64_t c = ((uint64_t)cost * (uint32_t)(16 * p.kv_heads) >> p.log2_target) + 64;
+  int C = c < 0x7fffffc0 ? (int)c & ~63 : 0x7fffffc0;
   // blocks: `target` items are two CTAs a compute unit; short pieces, half as many. One against two, 64 query and 8 KV
   // heads unless said: 8 chunks of 100 tokens on 2000 (32 heads) 53 / 64 us, 4 of 256 on 4000 (32) 96 / 106; one of 512 on
   // 8000 190 / 182, one of 4096 on 28,000 (8 and 1) 585 / 535
@@ -126,7 +134,7 @@ __device__ __forceinline__ int gqa_piece_keys(const GqaParams& p, const GqaReque
       const int n = lane < p.batch ? gqa_blocks<kRows>(p, r) * gqa_pieces(r.L, C) * p.kv_heads : 0;
       const int items = __builtin_amdgcn_readlane(wave_iscan(n), 63);
       if (items <= p.target) break;
-      C = ((int)((float)C * (float)items / (float)p.target) + 64) & ~63;
+      C = (int)(((uint64_t)C * (uint32_t)items >> p.log2_target) + 64) & ~63;
     }
   }
   return __builtin_amdgcn_readfirstlane(C);

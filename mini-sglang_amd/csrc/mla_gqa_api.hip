@@ -28,6 +28,7 @@ struct Choice {
 constexpr int kFit = 512;
 constexpr int kTarget = 2048;
 constexpr int kBlocksTarget = 512;
+static_assert(!(kFit & (kFit - 1)) && !(kTarget & (kTarget - 1)) && !(kBlocksTarget & (kBlocksTarget - 1)), "powers of two");
 constexpr int kBlock = 128;
 // A paged batch of at least this many blocks fills the chip without cutting keys; up to this many keys (by the page
 // table's width) cutting them gains nothing over joining the pieces: in blocks, and streamed by more CTAs than run at once.
@@ -166,6 +167,7 @@ int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_str
 
 int launch(const char* who, GqaParams& p, const Choice& c, int dim, void* stream) {
   p.target = c.target;
+  for (p.log2_target = 0; (1 << p.log2_target) < c.target;) ++p.log2_target;
   p.fit = c.fit;
   p.wide = c.wide;
   return done(c.rows >= kBlock ? launch_gqa_rows(p, dim, c.rows, (hipStream_t)stream) : launch_gqa_stream(p, dim, c.rows, (hipStream_t)stream), who);

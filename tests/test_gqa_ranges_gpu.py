@@ -226,3 +226,43 @@ def test_an_infinity_that_rows_attend_stays_what_it_is(lens, heads, dim, blocks)
         if later:
             fixed[n - 1] = want.out[n - 1].to(out)
         want.check(fixed, lse)
+
+
+@pytest.mark.parametrize("n,heads,tokens,most", [(300, (8, 1), 1, 1 << 17), (64, (8, 2), 1, 1 << 19), (300, (8, 1), 3, 1 << 17), (40, (8, 1), 20, 1 << 20)])
+def test_split_keys_whose_sum_passes_24_bits(n, heads, tokens, most):
+    """Long requests on one shared prefix: the lengths' sum, by which both kernels of the call find the pieces, is past
+    what fp32 counts one by one. More requests than a wave has lanes, and few."""
+    gen = torch.Generator().manual_seed(n + tokens)
+    dim, ps, (hq, hk) = 64, 64, heads
+    on_gpu = torch.Generator(device=DEV).manual_seed(n)
+    k, v = (torch.randn((most // ps, ps, hk, dim), generator=on_gpu, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    pt = torch.randperm(most // ps, generator=gen).to(torch.int32)
+    lens = torch.randint(most // 4, most + 1, (n,), generator=gen).tolist()
+    lens[:3] = [most, tokens, most - 1]
+    assert sum(lens) > 1 << 24
+    q = torch.randn((n * tokens, hq, dim), generator=gen).to(torch.bfloat16).to(DEV)
+    out, lse = torch.full_like(q, NAN), torch.full((n * tokens, hq), NAN, device=DEV)
+    lib.gqa_chunk(q, k, v, pt.to(DEV).expand(n, -1).contiguous(), i32(list(range(0, n * tokens + 1, tokens))), i32(lens), tokens, 0.125, out, lse)
+    torch.cuda.synchronize()
+    rows = (pt.long()[:, None] * ps + torch.arange(ps)).flatten().to(DEV)
+    over = []
+    for h in range(hk):
+        k64, v64 = (x.view(-1, hk, dim)[rows, h].double() for x in (k, v))
+        size64 = v64.abs()
+        group = slice(h * hq // hk, (h + 1) * hq // hk)
+        for b, L in enumerate(lens):
+            one = slice(b * tokens, (b + 1) * tokens)
+            s = torch.matmul(k64[:L], q[one, group].double().flatten(0, 1).t().contiguous()).t().reshape(tokens, -1, L) * 0.125
+            for i in range(tokens - 1):
+                s[i, :, L - tokens + 1 + i :] = -float("inf")
+            z = torch.logsumexp(s, -1)
+            p = torch.exp(s - z[..., None]).flatten(0, 1)
+            cut = -(-L // 4096)
+            p = torch.nn.functional.pad(p, (0, cut * 4096 - L)).view(-1, cut, 4096).transpose(0, 1).contiguous()
+            ref, size = (torch.bmm(p, x[: cut * 4096].view(cut, 4096, dim)).sum(0).view(tokens, -1, dim) for x in (v64, size64))
+            # scores are sums of D products, sum |q k| scale <= 200 here: (D + 16) roundings of 2^-24
+            delta = (dim + 16) * 2.0 ** -24 * 200
+            rel = 2.0 ** -8 + 2 * delta + 2 * (L + 16) * 2.0 ** -24
+            over.append(((out[one, group].double() - ref).abs() - 1.02 * (rel * size + 2.0 ** -8 * ref.abs())).max())
+            over.append(((lse[one, group].double() - z).abs() - (delta + (L + 16) * 2.0 ** -24 + 2.0 ** -22 * z.abs())).max())
+    assert float(torch.stack(over).max()) <= 0
