@@ -1,10 +1,10 @@
 """Build libmla_amd.so (gfx950) from csrc/*.hip with hipcc, in-tree, and the Python calls of its short launches
-(csrc/binding, a CPython module over torch's C++ tensors) with g++.
+(csrc/binding, a CPython module over torch's C++ tensors) with the same compiler.
 
 Usage: python mini-sglang_amd/build.py [--jobs N]
 The library lands in minisgl_amd/kernel/libmla_amd.so and the module beside it, where
-minisgl_amd.kernel.lib loads them. Every call recompiles, and
-fails if the device assembly breaks a wait-state rule (asm_check.py).
+minisgl_amd.kernel.lib loads them. Every call recompiles; the library is built whether or not the module can be (its calls
+then raise), and the build fails if the device assembly breaks a wait-state rule (asm_check.py).
 """
 
 from __future__ import annotations
@@ -90,13 +90,14 @@ def _build_binding() -> None:
     root = os.path.dirname(torch.__file__)
     include = os.path.join(root, "include")
     tmp = BINDING_OUT + ".tmp"
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-std=c++17", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{include}",
-           f"-I{os.path.join(include, 'torch', 'csrc', 'api', 'include')}", f"-I{sysconfig.get_paths()['include']}",
+    built_for = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
+    cmd = [HIPCC, "-no-hip-rt", "-x", "c++", "-O2", "-fPIC", "-std=c++17", "-shared", "-Wno-unused-command-line-argument",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DMLA_BUILT_FOR="{built_for}"',
+           f"-I{include}", f"-I{os.path.join(include, 'torch', 'csrc', 'api', 'include')}", f"-I{sysconfig.get_paths()['include']}",
            BINDING_SRC, "-o", tmp, f"-L{os.path.join(root, 'lib')}", "-lc10", "-ltorch_cpu", "-ltorch_python"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{res.stderr}")
+        raise RuntimeError(f"hipcc failed for {BINDING_SRC}:\n{res.stderr}")
     os.replace(tmp, BINDING_OUT)
 
 
@@ -107,9 +108,9 @@ def build(jobs: int | None = None, verbose: bool = True) -> str:
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         binding = ex.submit(_build_binding)
         objs = list(ex.map(_compile, sources + [PEAKS_SRC]))
-        binding.result()
     _link(objs[:-1], OUT)
     _link(objs[-1:], PEAKS_OUT)
+    binding.result()
     if verbose:
         print(f"built {OUT} from {len(sources)} sources, {BINDING_OUT} and {PEAKS_OUT}")
     return OUT

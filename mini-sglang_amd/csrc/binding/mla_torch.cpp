@@ -311,4 +311,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mla_torch", nullptr, -1, methods}
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__mla_torch() { return PyModule_Create(&module); }
+// built_for: the torch and Python whose headers this was compiled with, "torch V, Python X.Y", by the build
+PyMODINIT_FUNC PyInit__mla_torch() {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", MLA_BUILT_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import sys
 from typing import NamedTuple, Tuple
 
 import numpy as np
@@ -546,6 +547,10 @@ def load_binding():
     except ImportError as e:
         raise MLAKernelError(f"minisgl_amd.kernel._mla_torch does not load ({e}): build it with "
                              "`python mini-sglang_amd/build.py`") from e
+    now = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
+    if binding.built_for != now:  # it reads tensors by the layout that it was compiled with
+        raise MLAKernelError(f"minisgl_amd.kernel._mla_torch was built for {binding.built_for}, this is {now}: build it with "
+                             "`python mini-sglang_amd/build.py`")
     entry_points = (lib.mla_gqa_prompt_bf16, lib.mla_gqa_workspace_bytes, lib.mla_gqa_chunk_bf16, lib.mla_gqa_decode_bf16,
                     lib.mla_page_tables_from_lengths)
     binding.bind(*(ctypes.cast(f, _vp).value for f in entry_points), torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
