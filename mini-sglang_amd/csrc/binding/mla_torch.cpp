@@ -105,6 +105,9 @@ const int32_t* index(PyObject* o, const char* name, int64_t n, long device) {
   return static_cast<const int32_t*>(t.data_ptr());
 }
 
+// A dimension of one element has no stride of its own: torch gives it any.
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
+
 // What the attention calls share.
 struct Attention {
   const at::Tensor &q, &k, &v, &out;
@@ -126,12 +129,12 @@ struct Attention {
             "q, k, v and out are bf16, out of q's shape");
     require(lse == nullptr || (lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == T && lse->size(1) == Hq),
             "lse is fp32 [T, Hq]");
-    require(q.stride(2) == 1 && k.stride(-1) == 1 && v.stride(-1) == 1 && out.stride(2) == 1 && (lse == nullptr || lse->stride(1) == 1),
+    require(q.stride(2) == 1 && k.stride(-1) == 1 && v.stride(-1) == 1 && out.stride(2) == 1 && (lse == nullptr || stride_of(*lse, 1) <= 1),
             "rows must be contiguous");
     require(T <= INT32_MAX && Hq <= INT32_MAX && Hkv <= INT32_MAX, "sizes past 32 bits");
   }
   float* lse_ptr() const { return lse == nullptr ? nullptr : static_cast<float*>(lse->data_ptr()); }
-  int64_t lse_stride() const { return lse == nullptr ? Hq : lse->stride(0); }
+  int64_t lse_stride() const { return lse == nullptr || T == 1 ? Hq : lse->stride(0); }
 };
 
 // A call's body: its value, or the Python error that it or torch has set.
@@ -170,9 +173,10 @@ PyObject* gqa_prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!is_current(x.device)) return PyLong_FromLong(kOtherDevice);
     void* stream = stream_of(a[7], x.device);
     return PyLong_FromLong(launched([&] {
-      return g.prompt(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), x.k.data_ptr(), x.k.stride(0), x.k.stride(1), x.v.data_ptr(),
-                      x.v.stride(0), x.v.stride(1), cu_ptr, (int32_t)(cu.size(0) - 1), (int32_t)x.T, (int32_t)x.Hq, (int32_t)x.Hkv,
-                      (int32_t)x.D, scale, x.out.data_ptr(), x.out.stride(0), x.out.stride(1), x.lse_ptr(), x.lse_stride(), stream);
+      return g.prompt(x.q.data_ptr(), stride_of(x.q, 0), stride_of(x.q, 1), x.k.data_ptr(), stride_of(x.k, 0), stride_of(x.k, 1),
+                      x.v.data_ptr(), stride_of(x.v, 0), stride_of(x.v, 1), cu_ptr, (int32_t)(cu.size(0) - 1), (int32_t)x.T,
+                      (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale, x.out.data_ptr(), stride_of(x.out, 0), stride_of(x.out, 1),
+                      x.lse_ptr(), x.lse_stride(), stream);
     }));
   });
 }
@@ -182,14 +186,20 @@ PyObject* gqa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 12, [&]() -> PyObject* {
     const Attention x(a[0], a[1], a[2], a[8], a[9], 4);
     const int64_t ps = x.k.size(1);
-    require(x.k.stride(0) == ps * x.k.stride(1) && x.v.stride(0) == ps * x.v.stride(1), "pages of the pools must follow one another");
+    // rows lie one stride apart over the whole pool: of its tokens, or of its pages where they hold one
+    auto row_stride = [&](const at::Tensor& t) {
+      require(t.size(0) == 1 || ps == 1 || t.stride(0) == ps * t.stride(1), "pages of the pools must follow one another");
+      return ps == 1 ? stride_of(t, 0) : t.stride(1);
+    };
+    const int64_t k_row = row_stride(x.k), v_row = row_stride(x.v);
     const at::Tensor& lens = tensor(a[5], "seq_lens");
     require(lens.dim() == 1, "seq_lens is [B]");
     const int64_t B = lens.size(0);
     const int32_t* lens_ptr = index(a[5], "seq_lens", B, x.device);
     const at::Tensor& pt = tensor(a[3], "page_table");
-    require(pt.scalar_type() == at::kInt && pt.dim() == 2 && pt.size(0) >= B && pt.stride(1) == 1 && gpu_of(pt) == x.device,
+    require(pt.scalar_type() == at::kInt && pt.dim() == 2 && pt.size(0) >= B && stride_of(pt, 1) <= 1 && gpu_of(pt) == x.device,
             "page_table is int32 [B, cols], on q's GPU");
+    const int64_t pt_row = pt.size(0) == 1 ? pt.size(1) : pt.stride(0);
     require(B <= INT32_MAX && pt.size(1) <= INT32_MAX && x.k.size(0) <= INT32_MAX && ps <= INT32_MAX, "sizes past 32 bits");
     const bool decode = a[4] == Py_None;
     const int32_t* cu = nullptr;
@@ -203,14 +213,14 @@ PyObject* gqa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto call = [&](void* ws, int64_t bytes) {
       return launched([&] {
         if (decode)
-          return g.decode(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), x.k.data_ptr(), x.k.stride(1), x.k.stride(2), x.v.data_ptr(),
-                          x.v.stride(1), x.v.stride(2), (int32_t)x.k.size(0), (int32_t)ps, pt_ptr, (int32_t)pt.size(1), pt.stride(0),
-                          lens_ptr, (int32_t)B, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale, ws, bytes, x.out.data_ptr(),
-                          x.out.stride(0), x.out.stride(1), x.lse_ptr(), x.lse_stride(), stream);
-        return g.chunk(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), x.k.data_ptr(), x.k.stride(1), x.k.stride(2), x.v.data_ptr(),
-                       x.v.stride(1), x.v.stride(2), (int32_t)x.k.size(0), (int32_t)ps, pt_ptr, (int32_t)pt.size(1), pt.stride(0), cu,
-                       lens_ptr, (int32_t)B, (int32_t)x.T, max_q, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale, ws, bytes,
-                       x.out.data_ptr(), x.out.stride(0), x.out.stride(1), x.lse_ptr(), x.lse_stride(), stream);
+          return g.decode(x.q.data_ptr(), stride_of(x.q, 0), stride_of(x.q, 1), x.k.data_ptr(), k_row, stride_of(x.k, 2),
+                          x.v.data_ptr(), v_row, stride_of(x.v, 2), (int32_t)x.k.size(0), (int32_t)ps, pt_ptr, (int32_t)pt.size(1),
+                          pt_row, lens_ptr, (int32_t)B, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale, ws, bytes,
+                          x.out.data_ptr(), stride_of(x.out, 0), stride_of(x.out, 1), x.lse_ptr(), x.lse_stride(), stream);
+        return g.chunk(x.q.data_ptr(), stride_of(x.q, 0), stride_of(x.q, 1), x.k.data_ptr(), k_row, stride_of(x.k, 2),
+                       x.v.data_ptr(), v_row, stride_of(x.v, 2), (int32_t)x.k.size(0), (int32_t)ps, pt_ptr, (int32_t)pt.size(1),
+                       pt_row, cu, lens_ptr, (int32_t)B, (int32_t)x.T, max_q, (int32_t)x.Hq, (int32_t)x.Hkv, (int32_t)x.D, scale,
+                       ws, bytes, x.out.data_ptr(), stride_of(x.out, 0), stride_of(x.out, 1), x.lse_ptr(), x.lse_stride(), stream);
       });
     };
     if (a[10] != Py_None) {
@@ -237,7 +247,7 @@ PyObject* page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 11, [&]() -> PyObject* {
     const at::Tensor& tt = tensor(a[0], "token_table");
     const long device = gpu_of(tt);
-    require(device >= 0 && tt.scalar_type() == at::kInt && tt.dim() == 2 && tt.stride(1) == 1, "token_table is int32 [rows, cols] on the GPU");
+    require(device >= 0 && tt.scalar_type() == at::kInt && tt.dim() == 2 && stride_of(tt, 1) <= 1, "token_table is int32 [rows, cols] on the GPU");
     const at::Tensor &idx = tensor(a[1], "table_idx"), &free = tensor(a[4], "free_slots");
     require(idx.dim() == 1 && free.dim() == 1, "table_idx and free_slots have one dimension");
     const int64_t B = idx.size(0), F = free.size(0);
@@ -259,7 +269,8 @@ PyObject* page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int32_t* base = static_cast<int32_t*>(made.data_ptr());
     int32_t *loc = base + cells, *pos = loc + total, *cu = pos + total;
     const long rc = launched([&] {
-      return g.tables(static_cast<int32_t*>(tt.data_ptr()), (int32_t)tt.size(0), (int32_t)tt.size(1), tt.stride(0), idx_ptr, cached,
+      return g.tables(static_cast<int32_t*>(tt.data_ptr()), (int32_t)tt.size(0), (int32_t)tt.size(1),
+                      tt.size(0) == 1 ? tt.size(1) : tt.stride(0), idx_ptr, cached,
                       lens, (int32_t)B, alloc, free_ptr, (int32_t)F, ps, max_extend, base, (int32_t)cols, cols, loc, pos, total, cu,
                       cu + B + 1, stream);
     });
