@@ -328,8 +328,15 @@ __device__ __forceinline__ void gqa_rows_again(const GqaParams& p, const GqaItem
   }
 }
 
-// A launch holds fewer than 2^32 threads.
-inline bool gqa_grid_ok(int64_t ctas, int threads) { return ctas <= 0x7fffffff && ctas * threads <= (int64_t)UINT32_MAX; }
+// CTAs of a launch of `rows` rows: sum over requests of ceil(E group / rows), then of ceil(L / C) pieces each.
+inline int64_t gqa_ctas(const GqaParams& p, int rows) {
+  return (((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch) * p.kv_heads + p.target;
+}
+// Whether a call's launches hold fewer than 2^32 threads each, the merge's too: looked at before the first of them.
+inline bool gqa_grids_ok(const GqaParams& p, int rows) {
+  auto ok = [](int64_t ctas, int threads) { return ctas <= 0x7fffffff && ctas * threads <= (int64_t)UINT32_MAX; };
+  return ok(gqa_ctas(p, rows), p.wide || rows == 256 ? 512 : 256) && (p.target == 0 || ok((int64_t)p.total_q * p.kv_heads * p.group, 64));
+}
 
 hipError_t launch_gqa_rows(const GqaParams& p, int dim, int rows, hipStream_t stream);    // blocks of 128 or 256 rows
 hipError_t launch_gqa_stream(const GqaParams& p, int dim, int rows, hipStream_t stream);  // CTAs of 16 or 32 rows

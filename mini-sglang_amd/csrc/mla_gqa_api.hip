@@ -170,6 +170,8 @@ int launch(const char* who, GqaParams& p, const Choice& c, int dim, void* stream
   for (p.log2_target = 0; (1 << p.log2_target) < c.target;) ++p.log2_target;
   p.fit = c.fit;
   p.wide = c.wide;
+  if (!gqa_grids_ok(p, c.rows))
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: %d rows of %d heads are more than a launch holds", who, p.total_q, p.kv_heads * p.group);
   return done(c.rows >= kBlock ? launch_gqa_rows(p, dim, c.rows, (hipStream_t)stream) : launch_gqa_stream(p, dim, c.rows, (hipStream_t)stream), who);
 }
 

@@ -494,10 +494,7 @@ hipError_t launch_gqa_rows(const GqaParams& p, int dim, int rows, hipStream_t st
   // the workspace holds pieces of 128 rows
   if (rows == 256 && (p.target > 0 || dim != 128)) return hipErrorInvalidValue;
   if (p.wide && (rows == 256 || p.page_table != nullptr)) return hipErrorInvalidValue;
-  // sum over requests of ceil(E group / rows), then of ceil(L / C) pieces each
-  const int64_t blocks = ((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch;
-  const int64_t grid = blocks * p.kv_heads + p.target;
-  if (!gqa_grid_ok(grid, 512)) return hipErrorInvalidValue;
+  const int64_t grid = gqa_ctas(p, rows);
   if (p.wide) {
     if (dim == 128) hipLaunchKernelGGL((gqa_rows_kernel<128, 4, 2, false>), dim3((unsigned)grid), dim3(512), 0, stream, p);
     else hipLaunchKernelGGL((gqa_rows_kernel<64, 4, 2, false>), dim3((unsigned)grid), dim3(512), 0, stream, p);

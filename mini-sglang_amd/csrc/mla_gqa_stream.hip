@@ -316,7 +316,6 @@ void launch_stream(const GqaParams& p, int64_t grid, hipStream_t stream) {
 
 hipError_t launch_gqa_merge(const GqaParams& p, int dim, int rows, hipStream_t stream) {
   const int64_t grid = (int64_t)p.total_q * p.kv_heads * p.group;
-  if (!gqa_grid_ok(grid, 64)) return hipErrorInvalidValue;
   // few rows are cut into many pieces
 #define MLA_MERGE(D, R)                                                                                            \
   if (dim == D && rows == R) {                                                                                     \
@@ -334,9 +333,7 @@ hipError_t launch_gqa_merge(const GqaParams& p, int dim, int rows, hipStream_t s
 }
 
 hipError_t launch_gqa_stream(const GqaParams& p, int dim, int rows, hipStream_t stream) {
-  const int64_t blocks = ((int64_t)p.total_q * p.group + rows - 1) / rows + p.batch;
-  const int64_t grid = blocks * p.kv_heads + p.target;
-  if (!gqa_grid_ok(grid, 512)) return hipErrorInvalidValue;
+  const int64_t grid = gqa_ctas(p, rows);
   if (dim == 128) rows == 16 ? launch_stream<128, 1>(p, grid, stream) : launch_stream<128, 2>(p, grid, stream);
   else rows == 16 ? launch_stream<64, 1>(p, grid, stream) : launch_stream<64, 2>(p, grid, stream);
   hipError_t e = hipGetLastError();

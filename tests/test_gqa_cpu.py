@@ -169,3 +169,15 @@ def test_oracle_tables_against_the_allocator():
     ref = R.step_tables(table, [2, 0], [0, 0], [19, 8], free, 8, 3, 2)
     assert torch.equal(ref.token_table, host.page_table) and ref.out_loc == host.out_loc(reqs).tolist()
     assert ref.pages_taken == 4 and ref.page_table.tolist() == [[0, 1, 2], [3, 0, 0]]
+
+
+def test_launches_past_2_to_32_threads_are_refused_before_the_first():
+    """The joining of split keys, a launch of its own, holds more threads here than the attention's; it was refused when
+    that was launched already."""
+    wide = dict(qt=2016 * 128, kr=63 * 128, vr=63 * 128, hq=2016, hk=63, ot=2016 * 128, lt=2016, cols=400, pts=400)
+    for rc in (decode(batch=65535, **wide), chunk(batch=65535, T=65535, max_q=1, **wide)):
+        assert rc == UNSUPPORTED and "more than a launch holds" in lib.load_library().mla_last_error().decode()
+    rc = prompt(T=1 << 19, hq=4096, hk=4096, qt=4096 * 128, kr=4096 * 128, vr=4096 * 128, ot=4096 * 128, lt=4096)
+    assert rc == UNSUPPORTED and "total_q * q_heads" in lib.load_library().mla_last_error().decode()
+    rc = prompt(T=(1 << 19) - 1, batch=65535, hq=4096, hk=4096, qt=4096 * 128, kr=4096 * 128, vr=4096 * 128, ot=4096 * 128, lt=4096)
+    assert rc == UNSUPPORTED and "more than a launch holds" in lib.load_library().mla_last_error().decode()
