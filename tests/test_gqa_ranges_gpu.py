@@ -266,3 +266,41 @@ def test_split_keys_whose_sum_passes_24_bits(n, heads, tokens, most):
             over.append(((out[one, group].double() - ref).abs() - 1.02 * (rel * size + 2.0 ** -8 * ref.abs())).max())
             over.append(((lse[one, group].double() - z).abs() - (delta + (L + 16) * 2.0 ** -24 + 2.0 ** -22 * z.abs())).max())
     assert float(torch.stack(over).max()) <= 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [NAN, float("inf"), -float("inf")])
+@pytest.mark.parametrize("blocks", [False, True])
+def test_every_head_of_a_token_whose_key_is_not_finite(dim, value, blocks):
+    """Queries of both signs make such a score NaN: no head and no dimension of the rows that attend it is finite, and
+    the rows before are as they were."""
+    gen = torch.Generator().manual_seed(31)
+    lens, last = [200, 70], [198, 199, 269]
+    q, k, v = (torch.randn((270, h, dim), generator=gen).to(torch.bfloat16) for h in (6, 2, 2))
+    call = prompt_in_blocks if blocks else run_prompt
+    clean, clean_lse = call(q, k, v, lens, 0.1)
+    for t in (k, v):
+        t[last] = value
+    out, lse = call(q, k, v, lens, 0.1)
+    assert not out[last].isfinite().any() and not lse[last].isfinite().any()
+    keep = [i for i in range(270) if i not in last]
+    assert out[keep].isfinite().all() and torch.equal(lse[keep], clean_lse[keep])
+    # computed again in fp32 or as before: numerators rounded to bf16 or not, results rounded twice
+    assert ((out[keep].double() - clean[keep].double()).abs() <= 2.0 ** -7 * 4 + 2.0 ** -7 * clean[keep].double().abs()).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens", [[2999, 4] * 32, [20000, 3] * 32, [30000] + [2100] * 40, [17000, 300, 1] * 20, [5000] * 40 + [64] * 24])
+def test_pieces_enlarged_until_they_run_at_once(dim, lens):
+    """At most 64 requests of few CTAs, cut into more pieces at first than run at once (512 of two KV heads)."""
+    first = max((2 * sum((n + 15) // 16 * 16 for n in lens) // 512 + 64) // 64 * 64, 128)  # keys of a piece
+    assert 2 * sum(-(-n // first) for n in lens) > 512
+    c = Paged([1] * len(lens), [n - 1 for n in lens], 8, 2, dim, 16, seed=len(lens))
+    for out, lse in (c.decode(), c.run()):
+        at = 0
+        for b, n in enumerate(lens):
+            rows = c.pt[b].long()[torch.arange(n) // 16] * 16 + torch.arange(n) % 16
+            ref = Exact(c.q[b : b + 1], c.k.view(-1, 2, dim)[rows], c.v.view(-1, 2, dim)[rows], c.scale)
+            rel = 2.0 ** -8 + 2 * (dim + 16) * 2.0 ** -24 * 200 + 2 * (n + 16) * 2.0 ** -24
+            assert ((out[b : b + 1].double() - ref.out).abs() <= 1.02 * (rel * ref.size + 2.0 ** -8 * ref.out.abs())).all(), (b, n)
+            assert ((lse[b : b + 1].double() - ref.lse).abs() <= (dim + 16) * 2.0 ** -24 * 200 + (n + 16) * 2.0 ** -24 + 2.0 ** -22 * ref.lse.abs()).all(), (b, n)
