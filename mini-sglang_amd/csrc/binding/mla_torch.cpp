@@ -228,7 +228,8 @@ PyObject* gqa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
       require(gpu_of(w) == x.device && w.is_contiguous(), "the workspace is one block on q's GPU");
       return PyLong_FromLong(call(w.data_ptr(), (int64_t)w.nbytes()));
     }
-    // without one first; where keys are split, one from torch's allocator, for this call (a call without it 3.8 us, with it 4.8)
+    // without one first; where keys are split, one from torch's allocator, for this call. On the host: a request of 100 keys, in
+    // one piece, 3.9 us with or without a workspace given; of 1500, two launches, 7.2 with, 7.2 to 8.0 without
     long rc = call(nullptr, 0);
     if (rc == MLA_ERR_INVALID_ARG) {
       int64_t bytes = 0;

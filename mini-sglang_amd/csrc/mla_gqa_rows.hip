@@ -17,9 +17,10 @@
 //    the rounding left out, keeps the largest at 1. Below |m| = 2^24 it is at most half a bit and taken as 0, which keeps the
 //    subtraction out of the loop; a wave with a row past that redoes its stages.
 // Bound: the MFMAs, and under them power: prompts of 7.8k and 8.1k tokens with 64 and 8 heads of 128 take 1.76 ms, 1164
-// TFLOP/s, with the MFMAs busy for 62 % of the cycles at 1.83 GHz (alone, on random operands, they run at 1829 TFLOP/s
-// and 1.74 GHz); four chunks of 2048 on up to 8192, pages of 64, 1.17 ms, 1170 TFLOP/s. Short calls are bound by their
-// CTA's chain: 1.2 us to find the request, 2 to the first stage, 0.45 a stage for a lone CTA, 1 to 1.8 for the results.
+// TFLOP/s, with the MFMAs busy for 62 % of the cycles at 1.4 to 1.8 GHz from dispatch to dispatch (alone, on random operands,
+// they run at 1829 TFLOP/s and 1.74 GHz); four chunks of 2048 on up to 8192, pages of 64, 1.17 ms, 1170 TFLOP/s. Short calls
+// are bound by their CTA's chain: 1.2 us to find the request, 2 to the first stage, 0.45 a stage for a lone CTA, 1 to 1.8 for
+// the results.
 // Waves of 64 rows (one per SIMD; each K and V operand read once for two MFMAs) took 1098 TFLOP/s where these took 1170.
 #include <type_traits>
 

@@ -230,7 +230,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
 
 // Partial results of requests in pieces, joined: lse = log2 sum_i 2^lse_i, out = sum_i 2^(lse_i - lse) o_i.
 // One CTA per (query, query head): its waves take every fourth piece (kWaves 4), or a wave per row (kWaves 1).
-// Bound: dependent loads (lengths, the pieces' lse, their rows). 3.8 us for 32 rows, 6 for 4096 rows of 64 requests.
+// Bound: dependent loads (lengths, the pieces' lse, their rows). 4.3 us for 32 rows, 7 for 4096 rows of 64 requests.
 template <int D, int kRows, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

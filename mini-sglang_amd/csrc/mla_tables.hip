@@ -18,8 +18,8 @@ __device__ __forceinline__ int page_of(int t, int ps, int log2_ps) {
 
 // CTA (x, b) takes the x-th kChunk tokens and columns of request b; it sums the lengths before b itself, in the one round
 // trip that its own lengths take. Bound: writes, and with few tokens the launch and three dependent loads (lengths, free
-// slot, store). 256 prompts of up to 8192 tokens at page size 1, 23 MB: 10.3 us, 11.9 with the tokens of a thread one after
-// the other, 10.4 with four neighbouring ones a thread and 16-byte stores; a decode step of 64 requests 4.7.
+// slot, store). 256 prompts of up to 8192 tokens at page size 1, 23 MB: 10.5 us, 1.6 more with the tokens of a thread one after
+// the other, 0.1 more with four neighbouring ones a thread and 16-byte stores; a decode step of 64 requests 4.2.
 template <bool kPow2>
 __global__ __launch_bounds__(256) void page_tables_kernel(const PageTablesParams p) {
   __shared__ int s_sum[4][3];

@@ -533,8 +533,8 @@ def qkv_a_rows(qkv, q_rank: int, q_norm_weight, kv_norm_weight, positions, cos_s
 
 
 # The calls below are short on the GPU (a decode step's tables take 4 us), so their tensors are checked and read in C++
-# (csrc/binding/mla_torch.cpp: a decode call 13.4 -> 8.2 us on the host, 6 of them its two launches; a step's tables 11.2 ->
-# 5.2) where the calls above do it here and in ctypes.
+# (csrc/binding/mla_torch.cpp: on the host, a decode call whose keys are split, of two launches, 13.4 -> 7.2 to 8.2 us; a
+# step's tables 11.2 -> 5.3) where the calls above do it here and in ctypes.
 
 
 @functools.lru_cache(maxsize=None)
