@@ -107,6 +107,8 @@ const int32_t* index(PyObject* o, const char* name, int64_t n, long device) {
 
 // A dimension of one element has no stride of its own: torch gives it any.
 int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
+// (an expanded dimension has stride 0, and more than one element)
+bool one_apart(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 || t.stride(dim) == 1; }
 
 // What the attention calls share.
 struct Attention {
@@ -129,7 +131,7 @@ struct Attention {
             "q, k, v and out are bf16, out of q's shape");
     require(lse == nullptr || (lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == T && lse->size(1) == Hq),
             "lse is fp32 [T, Hq]");
-    require(q.stride(2) == 1 && k.stride(-1) == 1 && v.stride(-1) == 1 && out.stride(2) == 1 && (lse == nullptr || stride_of(*lse, 1) <= 1),
+    require(q.stride(2) == 1 && k.stride(-1) == 1 && v.stride(-1) == 1 && out.stride(2) == 1 && (lse == nullptr || one_apart(*lse, 1)),
             "rows must be contiguous");
     require(T <= INT32_MAX && Hq <= INT32_MAX && Hkv <= INT32_MAX, "sizes past 32 bits");
   }
@@ -197,7 +199,7 @@ PyObject* gqa_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t B = lens.size(0);
     const int32_t* lens_ptr = index(a[5], "seq_lens", B, x.device);
     const at::Tensor& pt = tensor(a[3], "page_table");
-    require(pt.scalar_type() == at::kInt && pt.dim() == 2 && pt.size(0) >= B && stride_of(pt, 1) <= 1 && gpu_of(pt) == x.device,
+    require(pt.scalar_type() == at::kInt && pt.dim() == 2 && pt.size(0) >= B && one_apart(pt, 1) && gpu_of(pt) == x.device,
             "page_table is int32 [B, cols], on q's GPU");
     const int64_t pt_row = pt.size(0) == 1 ? pt.size(1) : pt.stride(0);
     require(B <= INT32_MAX && pt.size(1) <= INT32_MAX && x.k.size(0) <= INT32_MAX && ps <= INT32_MAX, "sizes past 32 bits");
@@ -248,7 +250,7 @@ PyObject* page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 11, [&]() -> PyObject* {
     const at::Tensor& tt = tensor(a[0], "token_table");
     const long device = gpu_of(tt);
-    require(device >= 0 && tt.scalar_type() == at::kInt && tt.dim() == 2 && stride_of(tt, 1) <= 1, "token_table is int32 [rows, cols] on the GPU");
+    require(device >= 0 && tt.scalar_type() == at::kInt && tt.dim() == 2 && one_apart(tt, 1), "token_table is int32 [rows, cols] on the GPU");
     const at::Tensor &idx = tensor(a[1], "table_idx"), &free = tensor(a[4], "free_slots");
     require(idx.dim() == 1 && free.dim() == 1, "table_idx and free_slots have one dimension");
     const int64_t B = idx.size(0), F = free.size(0);

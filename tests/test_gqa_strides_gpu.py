@@ -80,3 +80,30 @@ def test_pages_that_do_not_follow_one_another_are_refused():
     q, out = torch.zeros((1, 4, 64), dtype=torch.bfloat16, device=DEV), torch.zeros((1, 4, 64), dtype=torch.bfloat16, device=DEV)
     with pytest.raises(AssertionError, match="follow one another"):
         lib.gqa_decode(q, pool[:, 0], pool[:, 1], i32([[0, 1]]), i32([20]), 0.1, out)
+
+
+def test_expanded_tensors():
+    """Rows that lie on each other: read where only read (one query, one KV head for all), refused where an entry past
+    the memory would be, and where results would be written over each other."""
+    gen = torch.Generator().manual_seed(4)
+    T, hq, hk, d = 40, 4, 2, 64
+    q, k, v = randn(gen, 1, hq, d), randn(gen, T, 1, d), randn(gen, T, 1, d)
+    qd, kd, vd = q.to(DEV).expand(T, hq, d), k.to(DEV).expand(T, hk, d), v.to(DEV).expand(T, hk, d)
+    out, lse = torch.empty((T, hq, d), dtype=torch.bfloat16, device=DEV), torch.empty((T, hq), device=DEV)
+    lib.gqa_prompt(qd, kd, vd, i32([0, T]), 0.2, out, lse)
+    check(out, lse, R.prompt(q.expand(T, hq, d), k.expand(T, hk, d), v.expand(T, hk, d), [T], 0.2))
+    with pytest.raises(AssertionError, match="contiguous"):
+        lib.gqa_prompt(qd, kd, vd, i32([0, T]), 0.2, out, torch.empty((T, 1), device=DEV).expand(T, hq))
+    with pytest.raises(lib.MLAKernelError, match="lse_stride"):
+        lib.gqa_prompt(qd, kd, vd, i32([0, T]), 0.2, out, torch.empty((1, hq), device=DEV).expand(T, hq))
+    with pytest.raises(lib.MLAKernelError, match="out strides"):
+        lib.gqa_prompt(qd, kd, vd, i32([0, T]), 0.2, torch.empty_like(out[:1]).expand(T, hq, d))
+    pool, one = torch.zeros((6, 16, hk, d), dtype=torch.bfloat16, device=DEV), i32([[3], [3]])
+    with pytest.raises(AssertionError, match="page_table is int32"):
+        lib.gqa_decode(qd[:2], pool, pool, one.expand(2, 4), i32([20, 30]), 0.1, out[:2])
+    with pytest.raises(lib.MLAKernelError, match="pt_stride"):
+        lib.gqa_decode(qd[:2], pool, pool, i32([[0, 1, 2, 3]]).expand(2, 4), i32([20, 30]), 0.1, out[:2])
+    with pytest.raises(AssertionError, match="token_table is int32"):
+        lib.page_tables_from_lengths(one.expand(2, 64), i32([0, 1]), i32([0, 0]), i32([20, 20]), i32(list(range(0, 96, 16))), 16, 20, 20, 40)
+    with pytest.raises(lib.MLAKernelError, match="token table"):
+        lib.page_tables_from_lengths(i32([[0] * 64]).expand(2, 64), i32([0, 1]), i32([0, 0]), i32([20, 20]), i32(list(range(0, 96, 16))), 16, 20, 20, 40)
