@@ -196,7 +196,9 @@ def store_rows(cache, indices, x, stream=None) -> None:
     row_bytes = x[0].numel() * x.element_size() if n else cache[0].numel() * cache.element_size()
     assert cache[0].numel() * cache.element_size() == row_bytes, "row widths differ"
     assert indices.dim() == 1 and indices.shape[0] == n and indices.dtype in (torch.int32, torch.int64)
-    x2 = _made(stream, lambda: x.reshape(n, -1)) if n else x
+    x2 = x
+    if n:
+        x2 = x.view(n, -1) if x[0].is_contiguous() else _made(stream, lambda: x.reshape(n, -1))
     c2 = cache.view(cache.shape[0], -1)
     assert x2.stride(-1) == 1 and c2.stride(-1) == 1, "rows must be contiguous"
     check(

@@ -170,3 +170,26 @@ def test_other_results_on_another_stream():
         assert call is store or got.untyped_storage().data_ptr() != at
         torch.cuda.synchronize()
         assert owned_by(side, nbytes) and torch.equal(got, want)
+
+
+def test_tables_captured_on_a_forked_stream():
+    table, free = torch.zeros((4, 256), dtype=torch.int32, device=DEV), i32(list(range(0, 16 * 64, 16)))
+    rows, cached, lens, side = i32([0, 1, 2, 3]), i32([0] * 4), i32([100, 3, 17, 256]), torch.cuda.Stream()
+    call = lambda **kw: lib.page_tables_from_lengths(table, rows, cached, lens, free, 16, 256, 256, 400, **kw)  # noqa: E731
+    want = [x.clone() for x in call()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        now = torch.cuda.current_stream()
+        side.wait_stream(now)
+        t = call(stream=side)
+        now.wait_stream(side)
+        copy = t.out_loc + 0
+    for _ in range(4):
+        table.zero_()
+        graph.replay()
+        junk = torch.full((1 << 22,), -9, dtype=torch.int32, device=DEV)
+        eager = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(t, want, eager)) and torch.equal(copy, want[1])
+        del junk
