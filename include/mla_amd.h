@@ -382,11 +382,11 @@ int mla_gqa_decode_bf16(const void *q, int64_t q_stride_b, int64_t q_stride_h, c
 
 /*
  * The tables of a scheduler step from its requests' lengths, bit-exact, in one launch. Request b owns row table_idx[b]
- * of the token table ([rows, cols] int32, one token location per column) and grows from cached_lens[b] = c to
+ * (cut to the table) of the token table ([rows, cols] int32, one token location per column) and grows from cached_lens[b] = c to
  * device_lens[b] = d tokens (cut to 0 <= c <= d <= cols). The first alloc_reqs requests take, in batch order, one entry
  * of free_slots (page-aligned token locations) for each page first = ceil(c / page_size) .. ceil(d / page_size) - 1 of
  * their row; the others (padding, whose rows are filled already) take none. Rows of requests that take pages are
- * distinct. Written:
+ * distinct, and no other request's. Written:
  *   token_table[row, j * page_size + i] = slot + i of each page j taken (i < page_size, while inside cols)
  *   page_table[b, j] = token_table[row, j * page_size] / page_size for j < ceil(d / page_size), 0 for further j < pt_cols
  *   cu_seqlens_q[b] = sum over requests before b of d - c, and their sum in cu_seqlens_q[batch]

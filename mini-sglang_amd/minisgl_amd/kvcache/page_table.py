@@ -76,16 +76,18 @@ class PagedTokenTable:
     def allocate_step(self, reqs: Iterable, padding: Iterable = ()) -> PageTables:
         """``allocate_paged``, the batch's page table, ``out_loc``, positions and query offsets in one launch, from the
         requests' lengths (one host-to-device copy of three integers a request). Requests of ``padding`` (a padded
-        batch's dummy) follow and take no pages. The rows of ``reqs`` must be distinct."""
-        reqs, ps = list(reqs), self.page_size
-        batch = reqs + list(padding)
+        batch's dummy) follow and take no pages. The rows of ``reqs`` must be distinct, and none of them the padding's."""
+        reqs, padding, ps = list(reqs), list(padding), self.page_size
+        batch = reqs + padding
         assert batch, "a step has requests"
-        assert len({r.table_idx for r in reqs}) == len(reqs), "requests that take pages have rows of their own"
+        taken = {r.table_idx for r in reqs}
+        assert len(taken) == len(reqs) and taken.isdisjoint([r.table_idx for r in padding]), "requests that take pages have rows of their own"
+        height, width = self.page_table.shape
+        assert all(0 <= r.table_idx < height for r in batch), f"the token table has {height} rows"
+        assert all(r.device_len <= width for r in batch), f"a token table row holds {width} tokens"
         needed = sum(-(-r.device_len // ps) - -(-r.cached_len // ps) for r in reqs)
         if needed > self.free_pages:
             raise RuntimeError(f"out of KV pages: {needed} needed, {self.free_pages} free")
-        width = self.page_table.shape[1]
-        assert all(r.device_len <= width for r in batch), f"a token table row holds {width} tokens"
         host = torch.tensor([[r.table_idx for r in batch], [r.cached_len for r in batch], [r.device_len for r in batch]],
                             dtype=torch.int32, pin_memory=self.device.type == "cuda")
         rows, cached, device = host.to(self.device, non_blocking=True)

@@ -181,3 +181,18 @@ def test_launches_past_2_to_32_threads_are_refused_before_the_first():
     assert rc == UNSUPPORTED and "total_q * q_heads" in lib.load_library().mla_last_error().decode()
     rc = prompt(T=(1 << 19) - 1, batch=65535, hq=4096, hk=4096, qt=4096 * 128, kr=4096 * 128, vr=4096 * 128, ot=4096 * 128, lt=4096)
     assert rc == UNSUPPORTED and "more than a launch holds" in lib.load_library().mla_last_error().decode()
+
+
+def test_step_refuses_rows_that_are_not_there_and_rows_of_the_padding():
+    """The launch cuts a row index to the table, so that one past it would be another request's row; a row that is filled
+    while padding reads it would be read half filled."""
+    table = PagedTokenTable(4, 16, torch.zeros((3, 64), dtype=torch.int32))
+    one = Req(table_idx=1, cached_len=0, device_len=1)
+    for idx in (3, -1):
+        far = Req(table_idx=idx, cached_len=0, device_len=1)
+        for reqs, padding in (([one, far], []), ([one], [far])):
+            with pytest.raises(AssertionError, match="has 3 rows"):
+                table.allocate_step(reqs, padding)
+    with pytest.raises(AssertionError, match="rows of their own"):
+        table.allocate_step([one], [Req(table_idx=2, cached_len=0, device_len=1), Req(table_idx=1, cached_len=0, device_len=1)])
+    assert table.free_pages == 4
