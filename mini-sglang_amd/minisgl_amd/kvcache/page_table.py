@@ -84,10 +84,10 @@ class PagedTokenTable:
         assert len(taken) == len(reqs) and taken.isdisjoint([r.table_idx for r in padding]), "requests that take pages have rows of their own"
         height, width = self.page_table.shape
         assert all(0 <= r.table_idx < height for r in batch), f"the token table has {height} rows"
-        assert all(r.device_len <= width for r in batch), f"a token table row holds {width} tokens"
         needed = sum(-(-r.device_len // ps) - -(-r.cached_len // ps) for r in reqs)
         if needed > self.free_pages:
             raise RuntimeError(f"out of KV pages: {needed} needed, {self.free_pages} free")
+        assert all(r.device_len <= width for r in batch), f"a token table row holds {width} tokens"
         host = torch.tensor([[r.table_idx for r in batch], [r.cached_len for r in batch], [r.device_len for r in batch]],
                             dtype=torch.int32, pin_memory=self.device.type == "cuda")
         rows, cached, device = host.to(self.device, non_blocking=True)
