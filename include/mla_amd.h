@@ -341,8 +341,7 @@ int mla_q_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, int32
  * not read, and a row that an infinity or a NaN in a later token's value came near (weight zero times it, in the matrix
  * product) is computed again by itself, which is slow (0.13 ms per 1000 keys). So is a row whose finite values add up past
  * fp32's range on the way to a result inside it. Scores, unscaled and scaled, are fp32: one past its range makes its row
- * NaN. Where keys are split, their pieces are weighed by fp32 LSEs, which from 2^24 on do not tell how many keys a piece
- * held.
+ * NaN.
  *
  * mla_gqa_prompt_bf16: whole prompts; k and v are packed like q (row cu_seqlens[b] + j), as many keys as queries.
  */

@@ -16,6 +16,8 @@
 
 namespace mla {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 struct GqaParams {
   const __bf16* q;  // [T, Hq, D]
   int64_t q_stride_t, q_stride_h;
@@ -39,7 +41,7 @@ struct GqaParams {
   float* lse;  // [T, Hq] or null
   int64_t lse_stride_t;
   float* ws_o;    // [slots, rows, D] partial outputs of split requests, normalised
-  float* ws_lse;  // [slots, rows] their log2-domain LSEs
+  f32x2* ws_lse;  // [slots, rows] their log2-domain LSEs: the nearest fp32, and the rest
   int32_t target;  // items that a batch's keys are split into, about (0: no splitting), a power of two
   int32_t log2_target;
   int32_t fit;     // at most `target`, where that can be
@@ -205,6 +207,13 @@ __device__ __forceinline__ bool gqa_find(const GqaParams& p, int item, GqaItem& 
     slots += __builtin_amdgcn_readlane(sincl, 63);
   }
   return false;
+}
+
+// LSE m + t of a row, log2 domain, and what its rounding leaves out (from |m| = 2^24 on as large as the sum's logarithm, by
+// which pieces of like scores differ).
+__device__ __forceinline__ f32x2 gqa_lse(bool some, float m, float t) {
+  const float sum = m + t;
+  return some ? f32x2{sum, (m - sum) + t} : f32x2{-INFINITY, 0.f};
 }
 
 // Token row of key j of request b (packed prompts: q0 + j); page ids are clamped into the pool. The host keeps pools

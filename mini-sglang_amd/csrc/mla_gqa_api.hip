@@ -198,7 +198,7 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
                                 out_stride_t, out_stride_h, lse, lse_stride_t))
     return rc;
   const int64_t most = (int64_t)max_q * p.group;  // rows of a request and KV head
-  const int64_t need = 4 * workspace_rows(most) * (dim + 1);
+  const int64_t need = 4 * workspace_rows(most) * (dim + 2);
   const int64_t keys = (int64_t)pt_cols * page_size;
   // a piece's end, its length rounded up to 64 keys in each of the pieces before it, stays below 2^31
   p.max_keys = (int32_t)(keys < 0x7ff00000 ? keys : 0x7ff00000);
@@ -215,7 +215,7 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
   p.max_q = max_q;
   if (workspace != nullptr) {
     p.ws_o = static_cast<float*>(workspace);
-    p.ws_lse = p.ws_o + workspace_rows(most) * dim;
+    p.ws_lse = reinterpret_cast<f32x2*>(p.ws_o + workspace_rows(most) * dim);
   }
   return launch(who, p, choice, dim, stream);
 }
@@ -229,7 +229,7 @@ int mla_gqa_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads, in
   const char* who = "mla_gqa_workspace_bytes";
   if (bytes == nullptr || max_q < 0) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: bytes is null or max_q %d < 0", who, max_q);
   if (int rc = mla::check_heads(who, q_heads, kv_heads, head_dim)) return rc;
-  *bytes = 4 * mla::workspace_rows((int64_t)max_q * (q_heads / kv_heads)) * (head_dim + 1);
+  *bytes = 4 * mla::workspace_rows((int64_t)max_q * (q_heads / kv_heads)) * (head_dim + 2);
   return mla::done(hipSuccess, who);
 }
 

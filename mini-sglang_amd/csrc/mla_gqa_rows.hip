@@ -424,7 +424,8 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
   // ---- results: a lane holds row c32, dims 32 db + 8 i4 + 4 g32 + 0..3
   const float l = sum_halves(l_run);
   const bool some = l > 0.f || l != l;
-  const float inv = some ? 1.f / l : 0.f, lse2 = some ? m_ref + (d_ref + log2f(l)) : -INFINITY;
+  const float inv = some ? 1.f / l : 0.f;
+  const f32x2 lse2 = gqa_lse(some, m_ref, d_ref + log2f(l));
   const int64_t at = (int64_t)it.slot * kRows + 32 * wave + c32;
   if (it.slot >= 0) {
     if (live) {
@@ -440,7 +441,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gqa_rows_kernel(const GqaPara
       if (g32 == 0) p.ws_lse[at] = lse2;
     }
   } else {
-    if (p.lse != nullptr && g32 == 0 && live) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2 * 0.69314718055994531f;
+    if (p.lse != nullptr && g32 == 0 && live) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2[0] * 0.69314718055994531f;
     auto packed = [&](int db, int i4) __attribute__((always_inline)) {
       return u32x2{pack_bf16x2(O[db][4 * i4] * inv, O[db][4 * i4 + 1] * inv), pack_bf16x2(O[db][4 * i4 + 2] * inv, O[db][4 * i4 + 3] * inv)};
     };

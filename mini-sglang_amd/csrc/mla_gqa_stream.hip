@@ -192,8 +192,9 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
       f[w] = __builtin_amdgcn_exp2f(s_m[w][row] - mt);
       lt += f[w] * s_l[w][row];
     }
-    const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
-    const float lse2 = lt > 0.f || lt != lt ? mt + log2f(lt) : -INFINITY;
+    const bool some = lt > 0.f || lt != lt;
+    const float inv = some ? 1.f / lt : 0.f;
+    const f32x2 lse2 = gqa_lse(some, mt, log2f(lt));
     const int r = it.block * kRows + 16 * nb + row, tok = r / G, head = it.head * G + r % G;
     float zero = 0.f;
 #pragma unroll
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
     }
     if (x == 0 && tok < E) {
       if (it.slot >= 0) p.ws_lse[(int64_t)it.slot * kRows + 16 * nb + row] = lse2;
-      else if (p.lse != nullptr) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2 * 0.69314718055994531f;
+      else if (p.lse != nullptr) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2[0] * 0.69314718055994531f;
     }
     uint64_t bad = __ballot(zero != 0.f && lt < INFINITY);  // finite sums times 0 are 0
     if (__builtin_expect(bad != 0, 0)) {
@@ -228,7 +229,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
   }
 }
 
-// Partial results of requests in pieces, joined: lse = log2 sum_i 2^lse_i, out = sum_i 2^(lse_i - lse) o_i.
+// Partial results of requests in pieces, joined: lse = log2 sum_i 2^lse_i, out = sum_i 2^(lse_i - lse) o_i, with lse_i of two
+// floats each (gqa_lse).
 // One CTA per (query, query head): its waves take every fourth piece (kWaves 4), or a wave per row (kWaves 1).
 // Bound: dependent loads (lengths, the pieces' lse, their rows). 4.3 us for 32 rows, 7 for 4096 rows of 64 requests.
 template <int D, int kRows, int kWaves>
@@ -260,7 +262,7 @@ __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams 
   const int rr = tok * p.group + h % p.group, row = rr % kRows;
   // piece i of the row's block and head: slot0 + i kv_heads
   const int64_t slot0 = slots + (int64_t)(rr / kRows) * pieces * p.kv_heads + h / p.group;
-  const float* lse = p.ws_lse + slot0 * kRows + row;
+  const f32x2* lse = p.ws_lse + slot0 * kRows + row;
   const float* part = p.ws_o + (slot0 * kRows + row) * D + (D / 64) * lane;
   const int64_t ls = (int64_t)p.kv_heads * kRows, os = ls * D;
   typedef float part_t __attribute__((ext_vector_type(D / 64)));
@@ -271,13 +273,24 @@ __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams 
     for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const part_t*>(part + min(i + u * kWaves, pieces - 1) * os);
   };
   load(wave);
-  float mt = kLowest;
-  for (int i = lane; i < pieces; i += 64) mt = fmaxf(mt, lse[i * ls]);
+  // the largest LSE, and of those alike in fp32 the largest rest
+  float mt = kLowest, rest = kLowest;
+  for (int i = lane; i < pieces; i += 64) {
+    const f32x2 x = lse[i * ls];
+    rest = x[0] > mt ? x[1] : x[0] == mt ? fmaxf(rest, x[1]) : rest;
+    mt = fmaxf(mt, x[0]);
+  }
+  const float m_lane = mt;
   mt = wave_max64(mt);
+  rest = wave_max64(m_lane == mt ? rest : kLowest);
   float lt = 0.f;
   part_t o = {};
   for (int i0 = 0; i0 < pieces; i0 += 64) {  // 64 pieces at a time: their weights in the lanes
-    const float f = i0 + lane < pieces ? __builtin_amdgcn_exp2f(lse[(i0 + lane) * ls] - mt) : 0.f;
+    float f = 0.f;
+    if (i0 + lane < pieces) {
+      const f32x2 x = lse[(i0 + lane) * ls];
+      f = __builtin_amdgcn_exp2f((x[0] - mt) + (x[1] - rest));
+    }
     lt += wave_sum64(f);
     const int n = min(64, pieces - i0);
     for (int i = wave; i < n; i += 8 * kWaves) {
@@ -303,7 +316,7 @@ __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams 
   if constexpr (D == 128) *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(o[0] * inv, o[1] * inv);
   else *out = (__bf16)(o[0] * inv);
   if (lane == 0 && p.lse != nullptr)
-    p.lse[(int64_t)t * p.lse_stride_t + h] = lt > 0.f || lt != lt ? (mt + log2f(lt)) * 0.69314718055994531f : -INFINITY;
+    p.lse[(int64_t)t * p.lse_stride_t + h] = lt > 0.f || lt != lt ? (mt + (rest + log2f(lt))) * 0.69314718055994531f : -INFINITY;
 }
 
 template <int D, int NB>

@@ -304,3 +304,28 @@ def test_pieces_enlarged_until_they_run_at_once(dim, lens):
             rel = 2.0 ** -8 + 2 * (dim + 16) * 2.0 ** -24 * 200 + 2 * (n + 16) * 2.0 ** -24
             assert ((out[b : b + 1].double() - ref.out).abs() <= 1.02 * (rel * ref.size + 2.0 ** -8 * ref.out.abs())).all(), (b, n)
             assert ((lse[b : b + 1].double() - ref.lse).abs() <= (dim + 16) * 2.0 ** -24 * 200 + (n + 16) * 2.0 ** -24 + 2.0 ** -22 * ref.lse.abs()).all(), (b, n)
+
+
+@pytest.mark.parametrize("kind,extends,prefixes,heads", [
+    (Paged, [1, 1, 1], [3000, 40, 1999], (8, 2)), (Paged, [3, 2], [5000, 1111], (16, 4)), (InBlocks, [200, 3], [3000, 700], (8, 2)),
+])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_alike_at_far_scores_weigh_alike_in_every_piece(kind, extends, prefixes, heads, dim):
+    """All scores of a row are one number, in most rows past what fp32 adds a sum's logarithm to: the result is the mean
+    of all values, however many keys a piece of them holds."""
+    gen = torch.Generator().manual_seed(dim)
+    c = kind(extends, prefixes, *heads, dim, 16, seed=dim + 1, scale=0.125)
+    made, at = [], 0
+    for b, (e, n) in enumerate(zip(extends, c.lens)):
+        q, k = far(gen, e, heads[0], n, heads[1], dim)
+        k[:] = (k != 0) * 1536.0 if b % 2 else (k != 0) * -640.0
+        v = torch.randn((n, heads[1], dim), generator=gen) + torch.arange(n)[:, None, None] * (4.0 / n)  # pieces differ
+        j = torch.arange(n)
+        rows = c.pt[b].long()[j // 16] * 16 + j % 16
+        c.k.view(-1, heads[1], dim)[rows], c.v.view(-1, heads[1], dim)[rows] = k.to(torch.bfloat16), v.to(torch.bfloat16)
+        c.q[at : at + e] = q
+        made.append((slice(at, at + e), q, k.to(torch.bfloat16), v.to(torch.bfloat16)))
+        at += e
+    out, lse = c.run()
+    for one, q, k, v in made:
+        Exact(q, k, v, 0.125).check(out[one], lse[one])
