@@ -88,11 +88,6 @@ __device__ __forceinline__ T wave_scan(T v, F&& f) {
 __device__ __forceinline__ int wave_iscan(int v) {
   return wave_scan(v, [](int a, int b) { return a + b; });
 }
-__device__ __forceinline__ uint32_t wave_sum_sat(uint32_t v) {
-  v = wave_scan(v, [](uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); });
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
-
 // Keys of a piece, C: the batch's keys, weighted with the row blocks that read them, over `target` items, in whole tiles
 // of 64 and at least gqa_min_split; with `fit`, enlarged until the pieces are at most `target` (the CTAs that run at once:
 // one more piece would be a round of its own). Requests of more keys are cut into ceil(L / C) pieces. Every kernel of a
@@ -100,7 +95,7 @@ __device__ __forceinline__ uint32_t wave_sum_sat(uint32_t v) {
 // lengths; in whole numbers, since the kernels find each other's partial results by it: a sum that one of them rounds
 // otherwise would join foreign ones. C is above cost / target, so a batch has fewer than `target` pieces more than
 // blocks; a request in pieces has L > C, so ceil(L / C) <= 2 L / C, and 2 target slots hold every piece. The cost counts
-// 16 keys as one and stops at 2^32 - 1, where requests stay in one piece.
+// 16 keys as one; requests stay in one piece where it passes 2^26 for one of them (or of every 64th), 2^30 keys of one block.
 // Least keys of a piece: a tile for each wave of the stream kernel; 16 stages of the blocks (their joining takes 6 us).
 template <int kRows>
 constexpr int gqa_min_split() {
@@ -116,14 +111,15 @@ template <int kRows>
 __device__ __forceinline__ int gqa_piece_keys(const GqaParams& p, const GqaRequest& r) {
   if (p.target <= 0) return 0x7fffffff;
   const int lane = threadIdx.x & 63;
+  constexpr uint32_t kMost = (1u << 26) - 1;  // of a lane: the wave's sum fits 32 bits
   auto cost_of = [&](const GqaRequest& x) {
     const uint64_t c = (uint64_t)(uint32_t)gqa_blocks<kRows>(p, x) * (uint32_t)((x.L + 15) >> 4);
-    return c < UINT32_MAX ? (uint32_t)c : UINT32_MAX;
+    return c < kMost ? (uint32_t)c : kMost;
   };
   uint32_t cost = lane < p.batch ? cost_of(r) : 0;
-  for (int b = 64 + lane; b < p.batch; b += 64) cost = __builtin_elementwise_add_sat(cost, cost_of(gqa_request(p, b)));
-  cost = wave_sum_sat(cost);
-  if (cost == UINT32_MAX) return 0x7fffffc0;
+  for (int b = 64 + lane; b < p.batch; b += 64) cost = min(cost + cost_of(gqa_request(p, b)), kMost);
+  if (__ballot(cost == kMost) != 0) return 0x7fffffc0;
+  cost = (uint32_t)__builtin_amdgcn_readlane(wave_iscan((int)cost), 63);
   const uint64_t c = ((uint64_t)cost * (uint32_t)(16 * p.kv_heads) >> p.log2_target) + 64;
   int C = c < 0x7fffffc0 ? (int)c & ~63 : 0x7fffffc0;
   // blocks: `target` items are two CTAs a compute unit; short pieces, half as many. One against two, 64 query and 8 KV

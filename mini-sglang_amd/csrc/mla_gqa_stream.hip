@@ -273,22 +273,27 @@ __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams 
     for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const part_t*>(part + min(i + u * kWaves, pieces - 1) * os);
   };
   load(wave);
-  // the largest LSE, and of those alike in fp32 the largest rest
-  float mt = kLowest, rest = kLowest;
-  for (int i = lane; i < pieces; i += 64) {
-    const f32x2 x = lse[i * ls];
-    rest = x[0] > mt ? x[1] : x[0] == mt ? fmaxf(rest, x[1]) : rest;
-    mt = fmaxf(mt, x[0]);
-  }
-  const float m_lane = mt;
+  f32x2 own{-INFINITY, 0.f};  // of piece `lane`
+  if (lane < pieces) own = lse[lane * ls];
+  float mt = fmaxf(own[0], kLowest);
+  for (int i = 64 + lane; i < pieces; i += 64) mt = fmaxf(mt, lse[i * ls][0]);
   mt = wave_max64(mt);
-  rest = wave_max64(m_lane == mt ? rest : kLowest);
+  // of the largest LSEs that are alike in fp32 the largest rest; below 2^24 at most half a bit, and left in the weights
+  float rest = 0.f;
+  if (__ballot(fabsf(mt) >= 16777216.f) != 0) {
+    rest = own[0] == mt ? own[1] : kLowest;
+    for (int i = 64 + lane; i < pieces; i += 64) {
+      const f32x2 x = lse[i * ls];
+      if (x[0] == mt) rest = fmaxf(rest, x[1]);
+    }
+    rest = wave_max64(rest);
+  }
   float lt = 0.f;
   part_t o = {};
   for (int i0 = 0; i0 < pieces; i0 += 64) {  // 64 pieces at a time: their weights in the lanes
     float f = 0.f;
     if (i0 + lane < pieces) {
-      const f32x2 x = lse[(i0 + lane) * ls];
+      const f32x2 x = i0 == 0 ? own : lse[(i0 + lane) * ls];
       f = __builtin_amdgcn_exp2f((x[0] - mt) + (x[1] - rest));
     }
     lt += wave_sum64(f);
