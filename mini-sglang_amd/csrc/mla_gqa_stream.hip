@@ -231,7 +231,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
 
 // Partial results of requests in pieces, joined: lse = log2 sum_i 2^lse_i, out = sum_i 2^(lse_i - lse) o_i, with lse_i of two
 // floats each (gqa_lse).
-// One CTA per (query, query head): its waves take every fourth piece (kWaves 4), or a wave per row (kWaves 1).
+// One CTA per (query, query head): its waves take every fourth piece (kWaves 4), or a wave per row (kWaves 1). Weights are
+// times 2^-12, exactly: up to 2^12 pieces of the largest values sum up within fp32's range.
 // Bound: dependent loads (lengths, the pieces' lse, their rows). 4.3 us for 32 rows, 7 for 4096 rows of 64 requests.
 template <int D, int kRows, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams p) {
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams 
     float f = 0.f;
     if (i0 + lane < pieces) {
       const f32x2 x = i0 == 0 ? own : lse[(i0 + lane) * ls];
-      f = __builtin_amdgcn_exp2f((x[0] - mt) + (x[1] - rest));
+      f = __builtin_amdgcn_exp2f((x[0] - mt) + (x[1] - rest)) * 0x1p-12f;
     }
     lt += wave_sum64(f);
     const int n = min(64, pieces - i0);
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams 
   if constexpr (D == 128) *reinterpret_cast<uint32_t*>(out) = pack_bf16x2(o[0] * inv, o[1] * inv);
   else *out = (__bf16)(o[0] * inv);
   if (lane == 0 && p.lse != nullptr)
-    p.lse[(int64_t)t * p.lse_stride_t + h] = lt > 0.f || lt != lt ? (mt + (rest + log2f(lt))) * 0.69314718055994531f : -INFINITY;
+    p.lse[(int64_t)t * p.lse_stride_t + h] = lt > 0.f || lt != lt ? (mt + (rest + log2f(lt * 0x1p12f))) * 0.69314718055994531f : -INFINITY;
 }
 
 template <int D, int NB>
