@@ -408,6 +408,85 @@ int mla_page_tables_from_lengths(int32_t *token_table, int32_t token_table_rows,
                                  int32_t *positions, int32_t total_new, int32_t *cu_seqlens_q, int32_t *pages_taken,
                                  void *stream);
 
+/*
+ * Queries, keys and values of grouped heads from a fused projection's output to attention and cache, in one launch. For each
+ * token t and head of q [tokens, q_heads, head_dim] and k [tokens, kv_heads, head_dim] (any strides that are multiples of 8;
+ * 16-byte aligned):
+ *   y = x / sqrt(mean(x^2) + eps) * weight  (q_weight, k_weight [head_dim]; both NULL: y = x), then RoPE of its first
+ *   rotary_dim dims (a multiple of 8, 0 for none) at positions[t], with the conventions and the cos_sin
+ *   [max_position, rotary_dim] of mla_latent_rows_bf16.
+ * fp32 arithmetic, one rounding. Queries go to q_out [tokens, q_heads, head_dim], keys and (v not NULL) the rows of v as
+ * they are to rows slots[t] (index_bits 32 or 64) of k_out and v_out [out_rows, kv_heads, head_dim]: row r, head h at
+ * k_out + r * k_out_stride_row + h * k_out_stride_h; slots outside [0, out_rows) are not written, others must be distinct.
+ * slots NULL: row t. q_out may be q, and without slots k_out k and v_out v, with their strides; other outputs overlap no
+ * input. Replaces the q / k norms and the rotation of python/minisgl/layers/attention.py:40-52 (norm.py, rotary.py:39-51)
+ * and the store of python/minisgl/kvcache/mha_pool.py:45-56.
+ */
+int mla_qk_norm_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_stride_t,
+                          int64_t k_stride_h, const void *v, int64_t v_stride_t, int64_t v_stride_h, const void *q_weight,
+                          const void *k_weight, float eps, const int32_t *positions, const float *cos_sin,
+                          int32_t max_position, int32_t rotary_dim, int32_t interleaved, int32_t tokens, int32_t q_heads,
+                          int32_t kv_heads, int32_t head_dim, void *q_out, int64_t q_out_stride_t, int64_t q_out_stride_h,
+                          void *k_out, int64_t k_out_stride_row, int64_t k_out_stride_h, void *v_out,
+                          int64_t v_out_stride_row, int64_t v_out_stride_h, const void *slots, int32_t index_bits,
+                          int64_t out_rows, void *stream);
+
+/*
+ * A paged pool of keys or values in 4 bits, MXFP4 of the OCP Microscaling Formats 1.0: blocks of 32 dims in order, each value
+ * one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (code 0..7, bit 3 the sign) times its block's power of two.
+ *   codes   [num_pages, page_size, kv_heads, head_dim / 2]: dims 2 i and 2 i + 1 in the low and high half of byte i
+ *   scales  [num_pages, page_size, kv_heads, head_dim / 32]: the exponent plus 127 (254 at most 2^127; a value past bf16's range
+ *           is an infinity); 255: the block is NaN
+ * Strides in bytes: of codes multiples of 16, codes 16-byte aligned; of scales multiples of head_dim / 32, scales aligned by
+ * as much; rows contiguous. page_size a power of two.
+ */
+typedef struct {
+  void *codes, *scales;
+  int64_t code_stride_page, code_stride_token, code_stride_head;
+  int64_t scale_stride_page, scale_stride_token, scale_stride_head;
+} mla_mx4_pool;
+
+/*
+ * mla_mx4_store: rows k, v [rows, kv_heads, head_dim] (bf16; strides multiples of 8, 16-byte aligned) to token rows indices[i]
+ * (index_bits 32 or 64; row r is token r % page_size of page r / page_size) of the pools. Indices outside the pool are skipped;
+ * others must be distinct. A block's exponent is floor(log2 of its largest magnitude) - 2, at least -127; values are rounded
+ * to the nearest, ties to the even code, 6 units at most; a block with an infinity or a NaN gets scale 255 and codes 0.
+ * Bit-exact. Replaces store_kv_cache (python/minisgl/kernel/csrc/jit/store.cu:25-53) for this pool.
+ * mla_mx4_load: the values of rows indices[i] into k, v [rows, kv_heads, head_dim] (exact in bf16); 0 for indices outside.
+ */
+int mla_mx4_store(const mla_mx4_pool *k_pool, const mla_mx4_pool *v_pool, int32_t num_pages, int32_t page_size,
+                  int32_t kv_heads, int32_t head_dim, const void *indices, int32_t index_bits, int32_t rows, const void *k,
+                  int64_t k_stride_t, int64_t k_stride_h, const void *v, int64_t v_stride_t, int64_t v_stride_h, void *stream);
+int mla_mx4_load(const mla_mx4_pool *k_pool, const mla_mx4_pool *v_pool, int32_t num_pages, int32_t page_size,
+                 int32_t kv_heads, int32_t head_dim, const void *indices, int32_t index_bits, int32_t rows, void *k,
+                 int64_t k_stride_t, int64_t k_stride_h, void *v, int64_t v_stride_t, int64_t v_stride_h, void *stream);
+
+/*
+ * mla_gqa_chunk_bf16 and mla_gqa_decode_bf16 over pools of 4 bits, with the same arguments and semantics otherwise: the
+ * result is that of the codes' values, fp32 scores and sums, numerators in bf16 for the product with the values. Both pools
+ * have the same strides. A NaN block reaches the rows that attend its token only. Requests of more than 32 rows (max_q times
+ * q_heads / kv_heads) may have their keys' values laid out in bf16 first: total_keys is at least the sum of seq_lens_k (its
+ * keys past that are not those of the pool), and sizes that part of the workspace. mla_gqa_mx4_workspace_bytes: enough for
+ * every call with at most max_q queries a request, `batch` requests, max_keys = pt_cols * page_size, and total_keys;
+ * NULL with 0 bytes will do where none is used.
+ */
+int mla_gqa_mx4_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t batch,
+                                int64_t max_keys, int64_t total_keys, int64_t *bytes);
+
+int mla_gqa_chunk_mx4(const void *q, int64_t q_stride_t, int64_t q_stride_h, const mla_mx4_pool *k_pool,
+                      const mla_mx4_pool *v_pool, int32_t num_pages, int32_t page_size, const int32_t *page_table,
+                      int32_t pt_cols, int64_t pt_stride, const int32_t *cu_seqlens_q, const int32_t *seq_lens_k,
+                      int32_t batch, int32_t total_q, int32_t max_q, int64_t total_keys, int32_t q_heads, int32_t kv_heads,
+                      int32_t head_dim, float scale, void *workspace, int64_t workspace_bytes, void *out,
+                      int64_t out_stride_t, int64_t out_stride_h, float *lse, int64_t lse_stride_t, void *stream);
+
+int mla_gqa_decode_mx4(const void *q, int64_t q_stride_b, int64_t q_stride_h, const mla_mx4_pool *k_pool,
+                       const mla_mx4_pool *v_pool, int32_t num_pages, int32_t page_size, const int32_t *page_table,
+                       int32_t pt_cols, int64_t pt_stride, const int32_t *seq_lens, int32_t batch, int64_t total_keys,
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, void *workspace,
+                       int64_t workspace_bytes, void *out, int64_t out_stride_b, int64_t out_stride_h, float *lse,
+                       int64_t lse_stride_b, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

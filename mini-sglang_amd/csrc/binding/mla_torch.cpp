@@ -27,6 +27,12 @@ struct {
   decltype(&mla_gqa_chunk_bf16) chunk;
   decltype(&mla_gqa_decode_bf16) decode;
   decltype(&mla_page_tables_from_lengths) tables;
+  decltype(&mla_qk_norm_rope_bf16) norm_rope;
+  decltype(&mla_mx4_store) mx4_store;
+  decltype(&mla_mx4_load) mx4_load;
+  decltype(&mla_gqa_mx4_workspace_bytes) mx4_workspace_bytes;
+  decltype(&mla_gqa_chunk_mx4) chunk_mx4;
+  decltype(&mla_gqa_decode_mx4) decode_mx4;
   PyObject* current_device;
   PyObject* current_stream;
 } g;
@@ -110,33 +116,94 @@ int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 
 // (an expanded dimension has stride 0, and more than one element)
 bool one_apart(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 || t.stride(dim) == 1; }
 
-// What the attention calls share.
-struct Attention {
-  const at::Tensor &q, &k, &v, &out;
+// What the attention calls share of everything but keys and values.
+struct Queries {
+  const at::Tensor &q, &out;
   const at::Tensor* lse = nullptr;
   long device;
-  int64_t T, Hq, Hkv, D;
+  int64_t T, Hq, D;
 
-  Attention(PyObject* q_, PyObject* k_, PyObject* v_, PyObject* out_, PyObject* lse_, int k_dims)
-      : q(tensor(q_, "q")), k(tensor(k_, "k")), v(tensor(v_, "v")), out(tensor(out_, "out")), device(gpu_of(q)) {
+  Queries(PyObject* q_, PyObject* out_, PyObject* lse_) : q(tensor(q_, "q")), out(tensor(out_, "out")), device(gpu_of(q)) {
     if (lse_ != Py_None) lse = &tensor(lse_, "lse");
-    require(q.dim() == 3 && k.dim() == k_dims, "q is [T, Hq, D]; k and v are [T, Hkv, D], or pools [pages, ps, Hkv, D]");
-    T = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(-2);
-    require(k.size(-1) == D && v.sizes() == k.sizes() && Hkv > 0 && Hq % Hkv == 0, "k and v have q's D and heads that divide q's");
-    require(device >= 0 && gpu_of(k) == device && gpu_of(v) == device && gpu_of(out) == device &&
-                (lse == nullptr || gpu_of(*lse) == device),
-            "all tensors must be on one GPU");
-    require(q.scalar_type() == at::kBFloat16 && k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 &&
-                out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes(),
-            "q, k, v and out are bf16, out of q's shape");
+    require(q.dim() == 3, "q is [T, Hq, D]");
+    T = q.size(0), Hq = q.size(1), D = q.size(2);
+    require(device >= 0 && gpu_of(out) == device && (lse == nullptr || gpu_of(*lse) == device), "all tensors must be on one GPU");
+    require(q.scalar_type() == at::kBFloat16 && out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes(), "q and out are bf16, out of q's shape");
     require(lse == nullptr || (lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == T && lse->size(1) == Hq),
             "lse is fp32 [T, Hq]");
-    require(q.stride(2) == 1 && k.stride(-1) == 1 && v.stride(-1) == 1 && out.stride(2) == 1 && (lse == nullptr || one_apart(*lse, 1)),
-            "rows must be contiguous");
-    require(T <= INT32_MAX && Hq <= INT32_MAX && Hkv <= INT32_MAX, "sizes past 32 bits");
+    require(q.stride(2) == 1 && out.stride(2) == 1 && (lse == nullptr || one_apart(*lse, 1)), "rows must be contiguous");
+    require(T <= INT32_MAX && Hq <= INT32_MAX, "sizes past 32 bits");
   }
   float* lse_ptr() const { return lse == nullptr ? nullptr : static_cast<float*>(lse->data_ptr()); }
   int64_t lse_stride() const { return lse == nullptr || T == 1 ? Hq : lse->stride(0); }
+};
+
+// The same with bf16 keys and values.
+struct Attention : Queries {
+  const at::Tensor &k, &v;
+  int64_t Hkv;
+
+  Attention(PyObject* q_, PyObject* k_, PyObject* v_, PyObject* out_, PyObject* lse_, int k_dims)
+      : Queries(q_, out_, lse_), k(tensor(k_, "k")), v(tensor(v_, "v")) {
+    require(k.dim() == k_dims, "k and v are [T, Hkv, D], or pools [pages, ps, Hkv, D]");
+    Hkv = k.size(-2);
+    require(k.size(-1) == D && v.sizes() == k.sizes() && Hkv > 0 && Hq % Hkv == 0, "k and v have q's D and heads that divide q's");
+    require(gpu_of(k) == device && gpu_of(v) == device, "all tensors must be on one GPU");
+    require(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16, "k and v are bf16");
+    require(k.stride(-1) == 1 && v.stride(-1) == 1, "rows must be contiguous");
+    require(Hkv <= INT32_MAX, "sizes past 32 bits");
+  }
+};
+
+// A pool of 4 bits: codes and scales.
+struct Pool4 {
+  int64_t pages, ps, heads, dim;
+  mla_mx4_pool c;
+
+  Pool4(PyObject* codes_, PyObject* scales_, long device) {
+    const at::Tensor &codes = tensor(codes_, "codes"), &scales = tensor(scales_, "scales");
+    require(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && codes.dim() == 4 && scales.dim() == 4 &&
+                gpu_of(codes) == device && gpu_of(scales) == device,
+            "a pool's codes and scales are uint8 [pages, ps, Hkv, D / 2] and [pages, ps, Hkv, D / 32], on the other tensors' GPU");
+    pages = codes.size(0), ps = codes.size(1), heads = codes.size(2), dim = 2 * codes.size(3);
+    require(scales.size(0) == pages && scales.size(1) == ps && scales.size(2) == heads && 32 * scales.size(3) == dim,
+            "a pool's scales have a byte for each 32 dims");
+    require(one_apart(codes, 3) && one_apart(scales, 3), "rows must be contiguous");
+    require(pages <= INT32_MAX && ps <= INT32_MAX && heads <= INT32_MAX && dim <= INT32_MAX, "sizes past 32 bits");
+    c = {codes.data_ptr(), scales.data_ptr(), stride_of(codes, 0), stride_of(codes, 1), stride_of(codes, 2),
+         stride_of(scales, 0), stride_of(scales, 1), stride_of(scales, 2)};
+  }
+  bool like(const Pool4& x) const { return pages == x.pages && ps == x.ps && heads == x.heads && dim == x.dim; }
+};
+
+// Row numbers [n], int32 or int64.
+struct Rows {
+  const void* ptr;
+  int bits;
+  Rows(PyObject* o, const char* name, int64_t n, long device) {
+    const at::Tensor& t = tensor(o, name);
+    if ((t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || t.dim() != 1 || t.size(0) != n || !t.is_contiguous() || gpu_of(t) != device) {
+      PyErr_Format(PyExc_AssertionError, "%s must be int32 or int64 [%lld], contiguous, on the other tensors' GPU", name, (long long)n);
+      throw Refused();
+    }
+    ptr = t.data_ptr();
+    bits = t.scalar_type() == at::kInt ? 32 : 64;
+  }
+};
+
+// bf16 [T, H, D] with contiguous rows
+struct Heads {
+  const at::Tensor& t;
+  Heads(PyObject* o, const char* name, int64_t T, int64_t H, int64_t D, long device) : t(tensor(o, name)) {
+    if (t.scalar_type() != at::kBFloat16 || t.dim() != 3 || t.size(0) != T || (H >= 0 && t.size(1) != H) || t.size(2) != D || t.stride(2) != 1 ||
+        t.size(1) > INT32_MAX || gpu_of(t) != device) {
+      PyErr_Format(PyExc_AssertionError, "%s must be bf16 [%lld, heads, %lld] with the other tensors' heads, rows contiguous, on one GPU", name, (long long)T, (long long)D);
+      throw Refused();
+    }
+  }
+  void* ptr() const { return t.data_ptr(); }
+  int64_t row() const { return stride_of(t, 0); }
+  int64_t head() const { return stride_of(t, 1); }
 };
 
 // A call's body: its value, or the Python error that it or torch has set.
@@ -295,9 +362,162 @@ PyObject* page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// bind(addresses of the five entry points..., torch's current device, torch's current raw stream)
+// gqa_paged_mx4(q, k codes, k scales, v codes, v scales, page_table, cu_seqlens_q or None, seq_lens, max_seqlen_q, scale, out,
+//               lse, workspace, total_keys or None, stream)
+PyObject* gqa_paged_mx4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 15, [&]() -> PyObject* {
+    const Queries x(a[0], a[10], a[11]);
+    const Pool4 k(a[1], a[2], x.device), v(a[3], a[4], x.device);
+    require(k.like(v) && k.dim == x.D && k.heads > 0 && x.Hq % k.heads == 0, "the pools have q's D and heads that divide q's");
+    const at::Tensor& lens = tensor(a[7], "seq_lens");
+    require(lens.dim() == 1, "seq_lens is [B]");
+    const int64_t B = lens.size(0);
+    const int32_t* lens_ptr = index(a[7], "seq_lens", B, x.device);
+    const at::Tensor& pt = tensor(a[5], "page_table");
+    require(pt.scalar_type() == at::kInt && pt.dim() == 2 && pt.size(0) >= B && one_apart(pt, 1) && gpu_of(pt) == x.device,
+            "page_table is int32 [B, cols], on q's GPU");
+    const int64_t pt_row = pt.size(0) == 1 ? pt.size(1) : pt.stride(0);
+    require(B <= INT32_MAX && pt.size(1) <= INT32_MAX, "sizes past 32 bits");
+    const bool decode = a[6] == Py_None;
+    const int32_t* cu = nullptr;
+    if (decode) require(x.T == B, "one token a request");
+    else cu = index(a[6], "cu_seqlens_q", B + 1, x.device);
+    const int32_t max_q = (int32_t)std::max<int64_t>(std::min<int64_t>(integer(a[8]), x.T), -1);
+    const float scale = number(a[9]);
+    const int64_t max_keys = pt.size(1) * k.ps, total = a[13] == Py_None ? B * std::min<int64_t>(max_keys, INT32_MAX) : integer(a[13]);
+    if (!is_current(x.device)) return PyLong_FromLong(kOtherDevice);
+    void* stream = stream_of(a[14], x.device);
+    const int32_t* pt_ptr = static_cast<const int32_t*>(pt.data_ptr());
+    auto call = [&](void* ws, int64_t bytes) {
+      return launched([&] {
+        if (decode)
+          return g.decode_mx4(x.q.data_ptr(), stride_of(x.q, 0), stride_of(x.q, 1), &k.c, &v.c, (int32_t)k.pages, (int32_t)k.ps, pt_ptr,
+                              (int32_t)pt.size(1), pt_row, lens_ptr, (int32_t)B, total, (int32_t)x.Hq, (int32_t)k.heads, (int32_t)x.D, scale,
+                              ws, bytes, x.out.data_ptr(), stride_of(x.out, 0), stride_of(x.out, 1), x.lse_ptr(), x.lse_stride(), stream);
+        return g.chunk_mx4(x.q.data_ptr(), stride_of(x.q, 0), stride_of(x.q, 1), &k.c, &v.c, (int32_t)k.pages, (int32_t)k.ps, pt_ptr,
+                           (int32_t)pt.size(1), pt_row, cu, lens_ptr, (int32_t)B, (int32_t)x.T, max_q, total, (int32_t)x.Hq,
+                           (int32_t)k.heads, (int32_t)x.D, scale, ws, bytes, x.out.data_ptr(), stride_of(x.out, 0), stride_of(x.out, 1),
+                           x.lse_ptr(), x.lse_stride(), stream);
+      });
+    };
+    if (a[12] != Py_None) {
+      const at::Tensor& w = tensor(a[12], "workspace");
+      require(gpu_of(w) == x.device && w.is_contiguous(), "the workspace is one block on q's GPU");
+      return PyLong_FromLong(call(w.data_ptr(), (int64_t)w.nbytes()));
+    }
+    // without one first, as gqa_paged
+    long rc = call(nullptr, 0);
+    if (rc == MLA_ERR_INVALID_ARG) {
+      int64_t bytes = 0;
+      if ((rc = g.mx4_workspace_bytes(max_q, (int32_t)x.Hq, (int32_t)k.heads, (int32_t)x.D, (int32_t)B, max_keys, total, &bytes))) return PyLong_FromLong(rc);
+      if (!allocates_for(a[14], stream, x.device)) return PyLong_FromLong(kOtherStream);
+      const at::Tensor made = at::empty({bytes}, x.q.options().dtype(at::kByte));
+      rc = call(made.data_ptr(), bytes);
+    }
+    return PyLong_FromLong(rc);
+  });
+}
+
+// mx4_store / mx4_load(k codes, k scales, v codes, v scales, indices, k, v, stream)
+PyObject* mx4_rows(PyObject* const* a, Py_ssize_t n, bool load) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    const at::Tensor& indices = tensor(a[4], "indices");
+    const long device = gpu_of(indices);
+    require(device >= 0 && indices.dim() == 1, "indices is [T], on the GPU");
+    const int64_t T = indices.size(0);
+    const Rows rows(a[4], "indices", T, device);
+    const Pool4 kp(a[0], a[1], device), vp(a[2], a[3], device);
+    require(kp.like(vp) && T <= INT32_MAX, "both pools have the same shape");
+    const Heads k(a[5], "k", T, kp.heads, kp.dim, device), v(a[6], "v", T, kp.heads, kp.dim, device);
+    if (!is_current(device)) return PyLong_FromLong(kOtherDevice);
+    void* stream = stream_of(a[7], device);
+    auto call = [&](auto entry) {
+      return entry(&kp.c, &vp.c, (int32_t)kp.pages, (int32_t)kp.ps, (int32_t)kp.heads, (int32_t)kp.dim, rows.ptr, rows.bits, (int32_t)T, k.ptr(),
+                   k.row(), k.head(), v.ptr(), v.row(), v.head(), stream);
+    };
+    return PyLong_FromLong(launched([&] { return load ? call(g.mx4_load) : call(g.mx4_store); }));
+  });
+}
+PyObject* mx4_store(PyObject*, PyObject* const* a, Py_ssize_t n) { return mx4_rows(a, n, false); }
+PyObject* mx4_load(PyObject*, PyObject* const* a, Py_ssize_t n) { return mx4_rows(a, n, true); }
+
+// qk_norm_rope(q, k, v or None, q_weight or None, k_weight or None, eps, positions, cos_sin, interleaved, q_out, k_out,
+//              v_out or None, slots or None, stream)
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 14, [&]() -> PyObject* {
+    const at::Tensor& q0 = tensor(a[0], "q");
+    const long device = gpu_of(q0);
+    require(device >= 0 && q0.dim() == 3, "q is [T, Hq, D], on the GPU");
+    const int64_t T = q0.size(0), Hq = q0.size(1), D = q0.size(2);
+    require(T <= INT32_MAX && D <= INT32_MAX, "sizes past 32 bits");
+    const Heads q(a[0], "q", T, Hq, D, device), k(a[1], "k", T, -1, D, device), q_out(a[9], "q_out", T, Hq, D, device);
+    const int64_t Hkv = k.t.size(1);
+    require((a[2] == Py_None) == (a[11] == Py_None), "v comes with v_out");
+    require((a[3] == Py_None) == (a[4] == Py_None), "both weights, or none");
+    auto weight = [&](PyObject* o, const char* name) -> const void* {
+      if (o == Py_None) return nullptr;
+      const at::Tensor& w = tensor(o, name);
+      require(w.scalar_type() == at::kBFloat16 && w.dim() == 1 && w.size(0) == D && w.is_contiguous() && gpu_of(w) == device, "weights are bf16 [D]");
+      return w.data_ptr();
+    };
+    const void *qw = weight(a[3], "q_weight"), *kw = weight(a[4], "k_weight");
+    const float eps = number(a[5]);
+    const int32_t* positions = index(a[6], "positions", T, device);
+    const at::Tensor& cs = tensor(a[7], "cos_sin");
+    require(cs.scalar_type() == at::kFloat && cs.dim() == 2 && cs.is_contiguous() && gpu_of(cs) == device && cs.size(0) <= INT32_MAX &&
+                cs.size(1) <= D,
+            "cos_sin is fp32 [max_position, R], contiguous, R at most D");
+    const int interleaved = PyObject_IsTrue(a[8]);
+    if (interleaved < 0) throw Refused();
+    struct To {
+      void* ptr;
+      int64_t row, head;
+    } v_in{}, k_to{}, v_to{};
+    if (a[2] != Py_None) {
+      const Heads v(a[2], "v", T, Hkv, D, device);
+      v_in = {v.ptr(), v.row(), v.head()};
+    }
+    const void* slots = nullptr;
+    int bits = 32;
+    int64_t out_rows = T;
+    if (a[12] == Py_None) {
+      const Heads ko(a[10], "k_out", T, Hkv, D, device);
+      k_to = {ko.ptr(), ko.row(), ko.head()};
+      if (a[11] != Py_None) {
+        const Heads vo(a[11], "v_out", T, Hkv, D, device);
+        v_to = {vo.ptr(), vo.row(), vo.head()};
+      }
+    } else {
+      const Rows r(a[12], "slots", T, device);
+      slots = r.ptr, bits = r.bits;
+      out_rows = -1;
+      auto pool = [&](PyObject* o, const char* name) {
+        const at::Tensor& t = tensor(o, name);
+        require(t.scalar_type() == at::kBFloat16 && t.dim() == 4 && t.size(2) == Hkv && t.size(3) == D && t.stride(3) == 1 && gpu_of(t) == device,
+                "with slots, k_out and v_out are bf16 pools [pages, ps, Hkv, D]");
+        const int64_t ps = t.size(1), rows = t.size(0) * ps;
+        require(t.size(0) == 1 || ps == 1 || t.stride(0) == ps * t.stride(1), "pages of the pools must follow one another");
+        require(out_rows == -1 || out_rows == rows, "both pools have as many rows");
+        out_rows = rows;
+        return To{t.data_ptr(), ps == 1 ? stride_of(t, 0) : t.stride(1), stride_of(t, 2)};
+      };
+      k_to = pool(a[10], "k_out");
+      if (a[11] != Py_None) v_to = pool(a[11], "v_out");
+    }
+    if (!is_current(device)) return PyLong_FromLong(kOtherDevice);
+    void* stream = stream_of(a[13], device);
+    return PyLong_FromLong(launched([&] {
+      return g.norm_rope(q.ptr(), q.row(), q.head(), k.ptr(), k.row(), k.head(), v_in.ptr, v_in.row, v_in.head, qw, kw, eps, positions,
+                         static_cast<const float*>(cs.data_ptr()), (int32_t)cs.size(0), (int32_t)cs.size(1), interleaved, (int32_t)T,
+                         (int32_t)Hq, (int32_t)Hkv, (int32_t)D, q_out.ptr(), q_out.row(), q_out.head(), k_to.ptr, k_to.row, k_to.head,
+                         v_to.ptr, v_to.row, v_to.head, slots, bits, out_rows, stream);
+    }));
+  });
+}
+
+// bind(addresses of the eleven entry points..., torch's current device, torch's current raw stream)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 7, [&]() -> PyObject* {
+  return guarded(n, 13, [&]() -> PyObject* {
     auto address = [&](int i) {
       void* p = PyLong_AsVoidPtr(a[i]);
       if (p == nullptr) {
@@ -311,16 +531,23 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     g.chunk = reinterpret_cast<decltype(g.chunk)>(address(2));
     g.decode = reinterpret_cast<decltype(g.decode)>(address(3));
     g.tables = reinterpret_cast<decltype(g.tables)>(address(4));
-    Py_INCREF(a[5]);
-    Py_INCREF(a[6]);
-    g.current_device = a[5];
-    g.current_stream = a[6];
+    g.norm_rope = reinterpret_cast<decltype(g.norm_rope)>(address(5));
+    g.mx4_store = reinterpret_cast<decltype(g.mx4_store)>(address(6));
+    g.mx4_load = reinterpret_cast<decltype(g.mx4_load)>(address(7));
+    g.mx4_workspace_bytes = reinterpret_cast<decltype(g.mx4_workspace_bytes)>(address(8));
+    g.chunk_mx4 = reinterpret_cast<decltype(g.chunk_mx4)>(address(9));
+    g.decode_mx4 = reinterpret_cast<decltype(g.decode_mx4)>(address(10));
+    Py_INCREF(a[11]);
+    Py_INCREF(a[12]);
+    g.current_device = a[11];
+    g.current_stream = a[12];
     Py_RETURN_NONE;
   });
 }
 
 #define MLA_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {MLA_METHOD(bind), MLA_METHOD(gqa_prompt), MLA_METHOD(gqa_paged), MLA_METHOD(page_tables), {}};
+PyMethodDef methods[] = {MLA_METHOD(bind),      MLA_METHOD(gqa_prompt), MLA_METHOD(gqa_paged), MLA_METHOD(page_tables), MLA_METHOD(qk_norm_rope),
+                         MLA_METHOD(mx4_store), MLA_METHOD(mx4_load),   MLA_METHOD(gqa_paged_mx4), {}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mla_torch", nullptr, -1, methods};
 
 }  // namespace

@@ -152,6 +152,24 @@ hipError_t launch_q_rope(const void* q, int64_t qst, int64_t qsh, int32_t tokens
                          const float* cos_sin, int32_t max_pos, int32_t interleaved, void* pe, int64_t pst, int64_t psh,
                          void* nope, int64_t nst, int64_t nsh, hipStream_t stream);
 
+// Queries, keys and values of grouped heads from a projection to attention and cache (mla_rotary.hip).
+struct QkNormRopeParams {
+  const __bf16 *q, *k, *v;  // [T, Hq, D], [T, Hkv, D]; v null: none
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const __bf16 *q_weight, *k_weight;  // [D], or null: no norm
+  float eps;
+  const int32_t* positions;  // [T]
+  const float* cos_sin;      // [max_position, rotary_dim]
+  int32_t max_position, rotary_dim, interleaved;
+  int32_t tokens, q_heads, kv_heads;
+  __bf16 *q_out, *k_out, *v_out;
+  int64_t qo_stride_t, qo_stride_h, ko_stride_row, ko_stride_h, vo_stride_row, vo_stride_h;
+  const void* slots;  // rows of k_out and v_out, or null: the token's
+  int32_t index_bits;
+  int64_t out_rows;
+};
+hipError_t launch_qk_norm_rope(const QkNormRopeParams& p, int dim, hipStream_t stream);
+
 // Tables of a scheduler step (mla_tables.hip).
 struct PageTablesParams {
   int32_t* token_table;

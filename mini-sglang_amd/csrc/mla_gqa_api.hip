@@ -5,6 +5,7 @@
 #include <algorithm>
 
 #include "mla_gqa.h"
+#include "mla_gqa_mx4.h"
 
 namespace mla {
 namespace {
@@ -16,6 +17,10 @@ int done(hipError_t e, const char* who) {
 }
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
+Mx4View mx4_view(const mla_mx4_pool& x) {
+  return {static_cast<uint8_t*>(x.codes), static_cast<uint8_t*>(x.scales), x.code_stride_page, x.code_stride_token, x.code_stride_head,
+          x.scale_stride_page, x.scale_stride_token, x.scale_stride_head};
+}
 
 // A launch's kernel: CTAs of 16 or 32 rows that stream keys, or (rows 128) blocks; how many items a paged batch is cut
 // into (target, fit: mla_gqa.h; 0: requests in one piece), and whether its CTAs are the wide ones.
@@ -113,24 +118,15 @@ int check_heads(const char* who, int32_t q_heads, int32_t kv_heads, int32_t dim)
   return MLA_OK;
 }
 
-// What all three attention entry points check; fills p but for the keys' addressing.
-int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
-                     int64_t k_row_stride, int64_t k_head_stride, const void* v, int64_t v_row_stride,
-                     int64_t v_head_stride, int32_t batch, int32_t total_q, int32_t q_heads, int32_t kv_heads,
-                     int32_t dim, float scale, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
-                     int64_t lse_stride_t) {
-  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr)
-    return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
-  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8))
-    return api_error(MLA_ERR_INVALID_ARG, "%s: q, k and v must be 16-byte and out 8-byte aligned", who);
-  if (k_row_stride > 0x7fffffff || v_row_stride > 0x7fffffff)
-    return api_error(MLA_ERR_UNSUPPORTED, "%s: k and v rows lie more than 4 GiB apart", who);
+// What all attention entry points check of everything but keys and values.
+int query_params(const char* who, GqaParams& p, const void* q, int64_t q_stride_t, int64_t q_stride_h, int32_t batch,
+                 int32_t total_q, int32_t q_heads, int32_t kv_heads, int32_t dim, float scale, void* out,
+                 int64_t out_stride_t, int64_t out_stride_h, float* lse, int64_t lse_stride_t) {
+  if (q == nullptr || out == nullptr) return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (!aligned(q, 16) || !aligned(out, 8)) return api_error(MLA_ERR_INVALID_ARG, "%s: q must be 16-byte and out 8-byte aligned", who);
   if (q_stride_t % 8 || q_stride_h % 8 || q_stride_t < 0 || q_stride_h < 0)
     return api_error(MLA_ERR_INVALID_ARG, "%s: q strides (%lld, %lld) must be non-negative multiples of 8", who,
                      (long long)q_stride_t, (long long)q_stride_h);
-  if (k_row_stride % 8 || k_head_stride % 8 || v_row_stride % 8 || v_head_stride % 8 || k_row_stride < 0 ||
-      k_head_stride < 0 || v_row_stride < 0 || v_head_stride < 0)
-    return api_error(MLA_ERR_INVALID_ARG, "%s: k and v strides must be non-negative multiples of 8", who);
   // rows of out must not overlap, tokens outside heads or heads outside tokens
   const bool by_token = (q_heads == 1 || out_stride_h >= dim) && (total_q == 1 || out_stride_t >= (q_heads - 1) * out_stride_h + dim);
   const bool by_head = (total_q == 1 || out_stride_t >= dim) && (q_heads == 1 || out_stride_h >= (total_q - 1) * out_stride_t + dim);
@@ -145,12 +141,6 @@ int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_str
   p.q = static_cast<const __bf16*>(q);
   p.q_stride_t = q_stride_t;
   p.q_stride_h = q_stride_h;
-  p.k = static_cast<const __bf16*>(k);
-  p.k_row_stride = k_row_stride;
-  p.k_head_stride = k_head_stride;
-  p.v = static_cast<const __bf16*>(v);
-  p.v_row_stride = v_row_stride;
-  p.v_head_stride = v_head_stride;
   p.batch = batch;
   p.total_q = total_q;
   p.kv_heads = kv_heads;
@@ -165,14 +155,66 @@ int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_str
   return MLA_OK;
 }
 
-int launch(const char* who, GqaParams& p, const Choice& c, int dim, void* stream) {
+// What the entry points over bf16 keys and values check; fills p but for the keys' addressing.
+int attention_params(const char* who, GqaParams& p, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                     int64_t k_row_stride, int64_t k_head_stride, const void* v, int64_t v_row_stride,
+                     int64_t v_head_stride, int32_t batch, int32_t total_q, int32_t q_heads, int32_t kv_heads,
+                     int32_t dim, float scale, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                     int64_t lse_stride_t) {
+  if (k == nullptr || v == nullptr) return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (!aligned(k, 16) || !aligned(v, 16)) return api_error(MLA_ERR_INVALID_ARG, "%s: k and v must be 16-byte aligned", who);
+  if (k_row_stride > 0x7fffffff || v_row_stride > 0x7fffffff)
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: k and v rows lie more than 4 GiB apart", who);
+  if (k_row_stride % 8 || k_head_stride % 8 || v_row_stride % 8 || v_head_stride % 8 || k_row_stride < 0 ||
+      k_head_stride < 0 || v_row_stride < 0 || v_head_stride < 0)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: k and v strides must be non-negative multiples of 8", who);
+  p.k = static_cast<const __bf16*>(k);
+  p.k_row_stride = k_row_stride;
+  p.k_head_stride = k_head_stride;
+  p.v = static_cast<const __bf16*>(v);
+  p.v_row_stride = v_row_stride;
+  p.v_head_stride = v_head_stride;
+  return query_params(who, p, q, q_stride_t, q_stride_h, batch, total_q, q_heads, kv_heads, dim, scale, out, out_stride_t,
+                      out_stride_h, lse, lse_stride_t);
+}
+
+int set_choice(const char* who, GqaParams& p, const Choice& c) {
   p.target = c.target;
   for (p.log2_target = 0; (1 << p.log2_target) < c.target;) ++p.log2_target;
   p.fit = c.fit;
   p.wide = c.wide;
   if (!gqa_grids_ok(p, c.rows))
     return api_error(MLA_ERR_UNSUPPORTED, "%s: %d rows of %d heads are more than a launch holds", who, p.total_q, p.kv_heads * p.group);
+  return MLA_OK;
+}
+
+int launch(const char* who, GqaParams& p, const Choice& c, int dim, void* stream) {
+  if (int rc = set_choice(who, p, c)) return rc;
   return done(c.rows >= kBlock ? launch_gqa_rows(p, dim, c.rows, (hipStream_t)stream) : launch_gqa_stream(p, dim, c.rows, (hipStream_t)stream), who);
+}
+
+int check_pages(const char* who, int32_t num_pages, int32_t page_size, const int32_t* page_table, int32_t pt_cols,
+                int64_t pt_stride, const int32_t* seq_lens_k, int32_t batch, const void* workspace, int64_t workspace_bytes) {
+  if (page_table == nullptr || seq_lens_k == nullptr || (workspace == nullptr && workspace_bytes != 0))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (!is_pow2(page_size)) return api_error(MLA_ERR_UNSUPPORTED, "%s: page_size %d must be a power of two", who, page_size);
+  if (num_pages < 1 || pt_cols < 1 || (batch > 1 && pt_stride < pt_cols))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: num_pages %d, pt_cols %d, pt_stride %lld", who, num_pages, pt_cols, (long long)pt_stride);
+  if ((int64_t)num_pages * page_size > 0x7fffffff)
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: a pool of %d pages of %d passes 2^31 rows", who, num_pages, page_size);
+  return MLA_OK;
+}
+
+// The keys' addressing but for the pool's pointers.
+void set_pages(GqaParams& p, int32_t num_pages, int32_t page_size, const int32_t* page_table, int64_t pt_stride,
+               const int32_t* cu_seqlens_q, const int32_t* seq_lens_k, int32_t max_q) {
+  p.num_pages = num_pages;
+  for (p.log2_ps = 0; (1 << p.log2_ps) < page_size;) ++p.log2_ps;
+  p.page_table = page_table;
+  p.pt_stride = pt_stride;
+  p.cu_seqlens_q = cu_seqlens_q;
+  p.seq_lens_k = seq_lens_k;
+  p.max_q = max_q;
 }
 
 int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
@@ -185,13 +227,7 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
     return api_error(MLA_ERR_INVALID_ARG, "%s: batch %d, total_q %d, max_q %d", who, batch, total_q, max_q);
   if (int rc = check_heads(who, q_heads, kv_heads, dim)) return rc;
   if (batch == 0 || total_q == 0 || max_q == 0) return done(hipSuccess, who);
-  if (page_table == nullptr || seq_lens_k == nullptr || (workspace == nullptr && workspace_bytes != 0))
-    return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
-  if (!is_pow2(page_size)) return api_error(MLA_ERR_UNSUPPORTED, "%s: page_size %d must be a power of two", who, page_size);
-  if (num_pages < 1 || pt_cols < 1 || (batch > 1 && pt_stride < pt_cols))
-    return api_error(MLA_ERR_INVALID_ARG, "%s: num_pages %d, pt_cols %d, pt_stride %lld", who, num_pages, pt_cols, (long long)pt_stride);
-  if ((int64_t)num_pages * page_size > 0x7fffffff)
-    return api_error(MLA_ERR_UNSUPPORTED, "%s: a pool of %d pages of %d passes 2^31 rows", who, num_pages, page_size);
+  if (int rc = check_pages(who, num_pages, page_size, page_table, pt_cols, pt_stride, seq_lens_k, batch, workspace, workspace_bytes)) return rc;
   GqaParams p = {};
   if (int rc = attention_params(who, p, q, q_stride_t, q_stride_h, k_pool, k_row_stride, k_head_stride, v_pool,
                                 v_row_stride, v_head_stride, batch, total_q, q_heads, kv_heads, dim, scale, out,
@@ -206,18 +242,144 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
   if (!aligned(workspace, 16) || (workspace_bytes < need && (workspace != nullptr || choice.target > 0)))
     return api_error(MLA_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
                      (long long)need, (long long)workspace_bytes);
-  p.num_pages = num_pages;
-  for (p.log2_ps = 0; (1 << p.log2_ps) < page_size;) ++p.log2_ps;
-  p.page_table = page_table;
-  p.pt_stride = pt_stride;
-  p.cu_seqlens_q = cu_seqlens_q;
-  p.seq_lens_k = seq_lens_k;
-  p.max_q = max_q;
+  set_pages(p, num_pages, page_size, page_table, pt_stride, cu_seqlens_q, seq_lens_k, max_q);
   if (workspace != nullptr) {
     p.ws_o = static_cast<float*>(workspace);
     p.ws_lse = reinterpret_cast<f32x2*>(p.ws_o + workspace_rows(most) * dim);
   }
   return launch(who, p, choice, dim, stream);
+}
+
+// ---- over a cache of 4 bits
+
+// Bytes of a workspace: partial results, and for requests of more than 32 rows their keys' values in pages of 64 and the
+// page table of these.
+struct Mx4Space {
+  int64_t split, table, rows, cols, bytes;
+};
+Mx4Space mx4_space(int64_t most, int32_t kv_heads, int32_t dim, int32_t batch, int64_t max_keys, int64_t total_keys) {
+  Mx4Space s = {};
+  s.split = 4 * workspace_rows(most) * (dim + 2);
+  if (most > 32) {
+    s.cols = (max_keys + 63) / 64;
+    s.rows = 64 * std::min(total_keys / 64 + batch, batch * s.cols);
+    s.table = (4 * batch * s.cols + 15) / 16 * 16;
+  }
+  s.bytes = s.split + s.table + 2 * s.rows * kv_heads * dim * 2;
+  return s;
+}
+
+int check_mx4(const char* who, const Mx4View& k, const Mx4View& v, int32_t dim, int64_t num_pages, int64_t page_size, int32_t kv_heads) {
+  if (k.codes == nullptr || k.scales == nullptr || v.codes == nullptr || v.scales == nullptr)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (!is_pow2(page_size)) return api_error(MLA_ERR_UNSUPPORTED, "%s: page_size %lld must be a power of two", who, (long long)page_size);
+  if (num_pages < 1 || kv_heads < 1) return api_error(MLA_ERR_INVALID_ARG, "%s: num_pages %lld, kv_heads %d", who, (long long)num_pages, kv_heads);
+  if (num_pages * page_size > 0x7fffffff)
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: a pool of %lld pages of %lld passes 2^31 rows", who, (long long)num_pages, (long long)page_size);
+  const int64_t scale_row = dim / 32;
+  if (!aligned(k.codes, 16) || !aligned(v.codes, 16) || !aligned(k.scales, scale_row) || !aligned(v.scales, scale_row))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: codes must be 16-byte aligned, scales by a row's %d bytes", who, dim / 32);
+  for (const Mx4View* x : {&k, &v})
+    if (x->c_page % 16 || x->c_tok % 16 || x->c_head % 16 || x->s_page % scale_row || x->s_tok % scale_row || x->s_head % scale_row ||
+        x->c_page < 0 || x->c_tok < 0 || x->c_head < 0 || x->s_page < 0 || x->s_tok < 0 || x->s_head < 0)
+      return api_error(MLA_ERR_INVALID_ARG, "%s: strides must be non-negative multiples of 16 bytes (codes) and of a row (scales)", who);
+  return MLA_OK;
+}
+
+int paged_mx4(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h, const mla_mx4_pool* k_pool,
+              const mla_mx4_pool* v_pool, int32_t num_pages, int32_t page_size, const int32_t* page_table, int32_t pt_cols,
+              int64_t pt_stride, const int32_t* cu_seqlens_q, const int32_t* seq_lens_k, int32_t batch, int32_t total_q,
+              int32_t max_q, int64_t total_keys, int32_t q_heads, int32_t kv_heads, int32_t dim, float scale, void* workspace,
+              int64_t workspace_bytes, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+              int64_t lse_stride_t, void* stream) {
+  if (batch < 0 || total_q < 0 || max_q < 0 || total_keys < 0)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: batch %d, total_q %d, max_q %d, total_keys %lld", who, batch, total_q, max_q, (long long)total_keys);
+  if (int rc = check_heads(who, q_heads, kv_heads, dim)) return rc;
+  if (batch == 0 || total_q == 0 || max_q == 0) return done(hipSuccess, who);
+  if (k_pool == nullptr || v_pool == nullptr) return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (int rc = check_pages(who, num_pages, page_size, page_table, pt_cols, pt_stride, seq_lens_k, batch, workspace, workspace_bytes)) return rc;
+  const Mx4View k = mx4_view(*k_pool), v = mx4_view(*v_pool);
+  if (int rc = check_mx4(who, k, v, dim, num_pages, page_size, kv_heads)) return rc;
+  if (k.c_page != v.c_page || k.c_tok != v.c_tok || k.c_head != v.c_head || k.s_page != v.s_page || k.s_tok != v.s_tok || k.s_head != v.s_head)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: the pools of keys and values must have the same strides", who);
+  GqaMx4Params mp = {};
+  GqaParams& p = mp.g;
+  if (int rc = query_params(who, p, q, q_stride_t, q_stride_h, batch, total_q, q_heads, kv_heads, dim, scale, out, out_stride_t,
+                            out_stride_h, lse, lse_stride_t))
+    return rc;
+  mp.k_codes = k.codes;
+  mp.k_scales = k.scales;
+  mp.v_codes = v.codes;
+  mp.v_scales = v.scales;
+  mp.c_page = k.c_page, mp.c_tok = k.c_tok, mp.c_head = k.c_head;
+  mp.s_page = k.s_page, mp.s_tok = k.s_tok, mp.s_head = k.s_head;
+  const int64_t most = (int64_t)max_q * p.group, keys = (int64_t)pt_cols * page_size;
+  p.max_keys = (int32_t)(keys < 0x7ff00000 ? keys : 0x7ff00000);
+  const Choice choice = choose(dim, batch, total_q, p.group, kv_heads, most, p.max_keys);
+  const bool laid_out = choice.rows >= kBlock;
+  const Mx4Space space = mx4_space(most, kv_heads, dim, batch, p.max_keys, total_keys);
+  if (!aligned(workspace, 16) || (workspace_bytes < space.bytes && (workspace != nullptr || choice.target > 0 || laid_out)))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
+                     (long long)space.bytes, (long long)workspace_bytes);
+  set_pages(p, num_pages, page_size, page_table, pt_stride, cu_seqlens_q, seq_lens_k, max_q);
+  if (workspace != nullptr) {
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_lse = reinterpret_cast<f32x2*>(p.ws_o + workspace_rows(most) * dim);
+  }
+  if (int rc = set_choice(who, p, choice)) return rc;
+  if (!laid_out) return done(launch_gqa_mx4(mp, dim, choice.rows, (hipStream_t)stream), who);
+  char* at = static_cast<char*>(workspace) + space.split;
+  mp.scratch_table = reinterpret_cast<int32_t*>(at);
+  mp.scratch_cols = (int32_t)space.cols;
+  mp.scratch_rows = space.rows;
+  mp.scratch_k = reinterpret_cast<__bf16*>(at + space.table);
+  mp.scratch_v = mp.scratch_k + space.rows * kv_heads * dim;
+  if (space.rows / 64 * 256 > UINT32_MAX || kv_heads > 65535 || space.rows > 0x7fffffff)
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: %lld keys are more than a launch holds", who, (long long)space.rows);
+  if (hipError_t e = launch_mx4_pages(mp, dim, (hipStream_t)stream); e != hipSuccess) return done(e, who);
+  p.k = mp.scratch_k;
+  p.v = mp.scratch_v;
+  p.k_row_stride = p.v_row_stride = dim;
+  p.k_head_stride = p.v_head_stride = space.rows * dim;
+  p.num_pages = (int32_t)(space.rows / 64);
+  p.log2_ps = 6;
+  p.page_table = mp.scratch_table;
+  p.pt_stride = space.cols;
+  return done(launch_gqa_rows(p, dim, choice.rows, (hipStream_t)stream), who);
+}
+
+int mx4_rows(const char* who, bool load, const mla_mx4_pool* k_pool, const mla_mx4_pool* v_pool, int32_t num_pages, int32_t page_size,
+             int32_t kv_heads, int32_t dim, const void* indices, int32_t index_bits, int32_t rows, const void* k,
+             int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* stream) {
+  if (dim != 64 && dim != 128) return api_error(MLA_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128, got %d", who, dim);
+  if (rows < 0 || (index_bits != 32 && index_bits != 64))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: rows %d, index_bits %d", who, rows, index_bits);
+  if (rows == 0) return done(hipSuccess, who);
+  if (k_pool == nullptr || v_pool == nullptr || indices == nullptr || k == nullptr || v == nullptr)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  Mx4Rows p = {};
+  p.k_pool = mx4_view(*k_pool), p.v_pool = mx4_view(*v_pool);
+  if (int rc = check_mx4(who, p.k_pool, p.v_pool, dim, num_pages, page_size, kv_heads)) return rc;
+  if (!aligned(k, 16) || !aligned(v, 16) || k_stride_t % 8 || k_stride_h % 8 || v_stride_t % 8 || v_stride_h % 8 || k_stride_t < 0 ||
+      k_stride_h < 0 || v_stride_t < 0 || v_stride_h < 0)
+    return api_error(MLA_ERR_INVALID_ARG, "%s: k and v must be 16-byte aligned, with non-negative strides that are multiples of 8", who);
+  if ((int64_t)rows * 2 * kv_heads * (dim / 8) > UINT32_MAX - 256)
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: %d rows of %d heads are more than a launch holds", who, rows, kv_heads);
+  if (load) {
+    p.k_out = static_cast<__bf16*>(const_cast<void*>(k));
+    p.v_out = static_cast<__bf16*>(const_cast<void*>(v));
+  } else {
+    p.k = static_cast<const __bf16*>(k);
+    p.v = static_cast<const __bf16*>(v);
+  }
+  p.k_stride_t = k_stride_t, p.k_stride_h = k_stride_h, p.v_stride_t = v_stride_t, p.v_stride_h = v_stride_h;
+  p.indices = indices;
+  p.index_bits = index_bits;
+  p.rows = rows;
+  p.kv_heads = kv_heads;
+  for (p.log2_ps = 0; (1 << p.log2_ps) < page_size;) ++p.log2_ps;
+  p.pool_rows = (int64_t)num_pages * page_size;
+  return done(launch_mx4_rows(p, dim, load, (hipStream_t)stream), who);
 }
 
 }  // namespace
@@ -327,6 +489,119 @@ int mla_page_tables_from_lengths(int32_t* token_table, int32_t token_table_rows,
   p.cu_seqlens_q = cu_seqlens_q;
   p.pages_taken = pages_taken;
   return mla::done(mla::launch_page_tables(p, max_extend, (hipStream_t)stream), who);
+}
+
+int mla_gqa_mx4_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t batch,
+                                int64_t max_keys, int64_t total_keys, int64_t* bytes) {
+  const char* who = "mla_gqa_mx4_workspace_bytes";
+  if (bytes == nullptr || max_q < 0 || batch < 0 || max_keys < 0 || total_keys < 0)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: bytes is null, or max_q %d, batch %d, max_keys %lld or total_keys %lld < 0", who, max_q,
+                          batch, (long long)max_keys, (long long)total_keys);
+  if (int rc = mla::check_heads(who, q_heads, kv_heads, head_dim)) return rc;
+  *bytes = mla::mx4_space((int64_t)max_q * (q_heads / kv_heads), kv_heads, head_dim, batch, std::min<int64_t>(max_keys, 0x7ff00000), total_keys).bytes;
+  return mla::done(hipSuccess, who);
+}
+
+int mla_gqa_chunk_mx4(const void* q, int64_t q_stride_t, int64_t q_stride_h, const mla_mx4_pool* k_pool,
+                      const mla_mx4_pool* v_pool, int32_t num_pages, int32_t page_size, const int32_t* page_table,
+                      int32_t pt_cols, int64_t pt_stride, const int32_t* cu_seqlens_q, const int32_t* seq_lens_k,
+                      int32_t batch, int32_t total_q, int32_t max_q, int64_t total_keys, int32_t q_heads, int32_t kv_heads,
+                      int32_t head_dim, float scale, void* workspace, int64_t workspace_bytes, void* out,
+                      int64_t out_stride_t, int64_t out_stride_h, float* lse, int64_t lse_stride_t, void* stream) {
+  const char* who = "mla_gqa_chunk_mx4";
+  if (batch > 0 && total_q > 0 && max_q > 0 && cu_seqlens_q == nullptr)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  return mla::paged_mx4(who, q, q_stride_t, q_stride_h, k_pool, v_pool, num_pages, page_size, page_table, pt_cols, pt_stride,
+                        cu_seqlens_q, seq_lens_k, batch, total_q, max_q < total_q ? max_q : total_q, total_keys, q_heads, kv_heads,
+                        head_dim, scale, workspace, workspace_bytes, out, out_stride_t, out_stride_h, lse, lse_stride_t, stream);
+}
+
+int mla_gqa_decode_mx4(const void* q, int64_t q_stride_b, int64_t q_stride_h, const mla_mx4_pool* k_pool,
+                       const mla_mx4_pool* v_pool, int32_t num_pages, int32_t page_size, const int32_t* page_table,
+                       int32_t pt_cols, int64_t pt_stride, const int32_t* seq_lens, int32_t batch, int64_t total_keys,
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, void* workspace,
+                       int64_t workspace_bytes, void* out, int64_t out_stride_b, int64_t out_stride_h, float* lse,
+                       int64_t lse_stride_b, void* stream) {
+  return mla::paged_mx4("mla_gqa_decode_mx4", q, q_stride_b, q_stride_h, k_pool, v_pool, num_pages, page_size, page_table, pt_cols,
+                        pt_stride, nullptr, seq_lens, batch, batch, 1, total_keys, q_heads, kv_heads, head_dim, scale, workspace,
+                        workspace_bytes, out, out_stride_b, out_stride_h, lse, lse_stride_b, stream);
+}
+
+int mla_mx4_store(const mla_mx4_pool* k_pool, const mla_mx4_pool* v_pool, int32_t num_pages, int32_t page_size,
+                  int32_t kv_heads, int32_t head_dim, const void* indices, int32_t index_bits, int32_t rows, const void* k,
+                  int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, void* stream) {
+  return mla::mx4_rows("mla_mx4_store", false, k_pool, v_pool, num_pages, page_size, kv_heads, head_dim, indices, index_bits, rows, k,
+                       k_stride_t, k_stride_h, v, v_stride_t, v_stride_h, stream);
+}
+
+int mla_mx4_load(const mla_mx4_pool* k_pool, const mla_mx4_pool* v_pool, int32_t num_pages, int32_t page_size, int32_t kv_heads,
+                 int32_t head_dim, const void* indices, int32_t index_bits, int32_t rows, void* k, int64_t k_stride_t,
+                 int64_t k_stride_h, void* v, int64_t v_stride_t, int64_t v_stride_h, void* stream) {
+  return mla::mx4_rows("mla_mx4_load", true, k_pool, v_pool, num_pages, page_size, kv_heads, head_dim, indices, index_bits, rows, k,
+                       k_stride_t, k_stride_h, v, v_stride_t, v_stride_h, stream);
+}
+
+int mla_qk_norm_rope_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+                          int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h, const void* q_weight,
+                          const void* k_weight, float eps, const int32_t* positions, const float* cos_sin,
+                          int32_t max_position, int32_t rotary_dim, int32_t interleaved, int32_t tokens, int32_t q_heads,
+                          int32_t kv_heads, int32_t head_dim, void* q_out, int64_t q_out_stride_t, int64_t q_out_stride_h,
+                          void* k_out, int64_t k_out_stride_row, int64_t k_out_stride_h, void* v_out,
+                          int64_t v_out_stride_row, int64_t v_out_stride_h, const void* slots, int32_t index_bits,
+                          int64_t out_rows, void* stream) {
+  const char* who = "mla_qk_norm_rope_bf16";
+  if (tokens < 0 || q_heads < 0 || kv_heads < 0 || q_heads > 4096 || kv_heads > 4096 || out_rows < 0)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: tokens %d, q_heads %d and kv_heads %d (0 to 4096), out_rows %lld", who, tokens, q_heads,
+                          kv_heads, (long long)out_rows);
+  if (head_dim != 64 && head_dim != 128) return mla::api_error(MLA_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128, got %d", who, head_dim);
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 8 != 0 || (rotary_dim > 0 && max_position < 1))
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: rotary_dim %d must be a multiple of 8 in [0, %d], max_position %d positive", who,
+                          rotary_dim, head_dim, max_position);
+  if ((q_weight == nullptr) != (k_weight == nullptr) || (v == nullptr) != (v_out == nullptr))
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: both weights or none, v with v_out", who);
+  if (!(eps >= 0.f) || !isfinite(eps)) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: bad eps", who);
+  if (slots != nullptr && index_bits != 32 && index_bits != 64)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: index_bits %d", who, index_bits);
+  if (slots == nullptr && out_rows < tokens)
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: %lld rows for %d tokens", who, (long long)out_rows, tokens);
+  if (tokens == 0 || q_heads + kv_heads == 0) return mla::done(hipSuccess, who);
+  if ((q_heads > 0 && (q == nullptr || q_out == nullptr)) || (kv_heads > 0 && (k == nullptr || k_out == nullptr)) ||
+      (rotary_dim > 0 && (positions == nullptr || cos_sin == nullptr)))
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: null pointer", who);
+  for (const void* x : {q, k, v, q_weight, k_weight, static_cast<const void*>(cos_sin), static_cast<const void*>(q_out),
+                        static_cast<const void*>(k_out), static_cast<const void*>(v_out)})
+    if (!mla::aligned(x, 16)) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: tensors must be 16-byte aligned", who);
+  for (int64_t x : {q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, q_out_stride_t, q_out_stride_h,
+                    k_out_stride_row, k_out_stride_h, v_out_stride_row, v_out_stride_h})
+    if (x % 8 || x < 0) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: strides must be non-negative multiples of 8", who);
+  if ((int64_t)tokens * (q_heads + 2 * kv_heads + 8) * (head_dim / 8) > UINT32_MAX - 256)
+    return mla::api_error(MLA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads are more than a launch holds", who, tokens, q_heads + 2 * kv_heads);
+  mla::QkNormRopeParams p = {};
+  p.q = static_cast<const __bf16*>(q);
+  p.k = static_cast<const __bf16*>(k);
+  p.v = static_cast<const __bf16*>(v);
+  p.q_stride_t = q_stride_t, p.q_stride_h = q_stride_h, p.k_stride_t = k_stride_t, p.k_stride_h = k_stride_h;
+  p.v_stride_t = v_stride_t, p.v_stride_h = v_stride_h;
+  p.q_weight = static_cast<const __bf16*>(q_weight);
+  p.k_weight = static_cast<const __bf16*>(k_weight);
+  p.eps = eps;
+  p.positions = positions;
+  p.cos_sin = cos_sin;
+  p.max_position = max_position;
+  p.rotary_dim = rotary_dim;
+  p.interleaved = interleaved != 0;
+  p.tokens = tokens;
+  p.q_heads = q_heads;
+  p.kv_heads = kv_heads;
+  p.q_out = static_cast<__bf16*>(q_out);
+  p.k_out = static_cast<__bf16*>(k_out);
+  p.v_out = static_cast<__bf16*>(v_out);
+  p.qo_stride_t = q_out_stride_t, p.qo_stride_h = q_out_stride_h, p.ko_stride_row = k_out_stride_row, p.ko_stride_h = k_out_stride_h;
+  p.vo_stride_row = v_out_stride_row, p.vo_stride_h = v_out_stride_h;
+  p.slots = slots;
+  p.index_bits = index_bits;
+  p.out_rows = out_rows;
+  return mla::done(mla::launch_qk_norm_rope(p, head_dim, (hipStream_t)stream), who);
 }
 
 }  // extern "C"

@@ -1,0 +1,364 @@
+// Grouped-head attention over a cache of 4 bits (mla_mx4.h), with the items, pieces and joining of mla_gqa.h: single tokens
+// and short chunks read the codes here; long chunks have their keys' values laid out first (mx4_pages_kernel), for the bf16
+// kernels.
+//
+// As mla_gqa_stream.hip, one CTA per (request, rows, KV head, piece of the keys), whose waves take tiles of 32 keys in turn,
+// load a tile ahead and share nothing until the end. A tile is 4.3 KB (head_dim 128): codes go through the wave's
+// LDS, and become bf16 in the registers that the matrix instructions read:
+//   scores   S^T = K Q^T: lane (key a16, g) reads the 16 bytes of the key's block g, and so the dims 32 g + 8 s + 0..7 for
+//            step s; the queries lie alike. One scale a lane.
+//   outputs  O^T = V^T P^T: lane (n, g) reads dims 8 n + 0..7 of keys 4 g + 0..3 and 16 + 4 g + 0..3, as the numerators lie;
+//            a conversion gives dims (8 n + 2 c, + 1) of one key, two of them swap halves, and product m of 8 has dim
+//            8 n + m in row n: lane (row a16, g) ends up with the 32 dims 32 g + 8 i + m.
+// At head_dim 64 half as many of each.
+#include <type_traits>
+
+#include "mla_gqa.h"
+#include "mla_gqa_mx4.h"
+
+namespace mla {
+namespace {
+
+constexpr int kTileKeys = 32;
+constexpr float kLowest = -3.4028234663852886e38f;
+// Numerators are times 2^-24: sums of 2^24 values of the largest size (6 2^125) stay in fp32's range
+constexpr float kRoom = 0x1p24f;
+
+__device__ __forceinline__ uint32_t any_ff(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+
+// NB blocks of 16 rows, NW waves
+template <int D, int NB, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params mp) {
+  const GqaParams& p = mp.g;
+  constexpr int kRows = 16 * NB, kRowB = D / 2, kScaleB = D / 32, kKs = D / 32, kDb = D / 16;
+  constexpr int kLoads = kTileKeys * kRowB / 1024;  // 16-byte loads of a lane per K or V tile
+  constexpr int kLanes = kRowB / 16;                // lanes of a row in such a load
+  using scale_t = std::conditional_t<D == 128, uint32_t, uint16_t>;
+  using kword_t = std::conditional_t<D == 128, u32x4, u32x2>;
+  using vword_t = std::conditional_t<D == 128, uint32_t, uint16_t>;
+  struct Tile {
+    char k[kTileKeys * kRowB], v[kTileKeys * kRowB];
+    scale_t ks[kTileKeys], vs[kTileKeys];
+  };
+  union Own {
+    Tile t;
+    char o[16 * D * 4];  // a block's outputs at the end, fp32 [16 rows][D]
+  };
+  __shared__ __attribute__((aligned(16))) Own s_own[NW];
+  __shared__ float s_m[NW][16], s_l[NW][16];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  GqaItem it;
+  if (!gqa_find<kRows, false>(p, blockIdx.x, it)) return;
+  const int C = it.C;
+  const int E = it.r.E, L = it.r.L, P = it.r.P, G = p.group;
+  const int a16 = lane & 15, g = lane >> 4;
+  int limit[NB];
+  bf16x8 qf[NB][kKs];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = it.block * kRows + 16 * nb + a16, tok = r / G;
+    const bool live = tok < E;
+    limit[nb] = live ? P + tok : -1;
+    const __bf16* q = p.q + (int64_t)(it.r.q0 + (live ? tok : 0)) * p.q_stride_t + (int64_t)(it.head * G + (live ? r % G : 0)) * p.q_stride_h;
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks) qf[nb][ks] = *reinterpret_cast<const bf16x8*>(q + (8 * kKs) * g + 8 * ks);
+  }
+  const int last_tok = min(E - 1, (it.block * kRows + kRows - 1) / G);
+  const int first_limit = P + it.block * kRows / G;  // of the item's first row: no key up to it is masked
+  const int k0 = it.piece * C, k1 = min(it.pieces > 1 ? k0 + C : L, P + last_tok + 1);
+  const uint8_t *kh = mp.k_codes + (int64_t)it.head * mp.c_head + lane % kLanes * 16, *vh = mp.v_codes + (int64_t)it.head * mp.c_head + lane % kLanes * 16;
+  const uint8_t* sh = (lane < 32 ? mp.k_scales : mp.v_scales) + (int64_t)it.head * mp.s_head;
+
+  f32x4 O[NB][kDb];
+  float m[NB], l[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb] = kLowest;
+    l[nb] = 0.f;
+#pragma unroll
+    for (int db = 0; db < kDb; ++db) O[nb][db] = f32x4{};
+  }
+  u32x4 kr[kLoads], vr[kLoads];
+  scale_t sr{};
+  // lane t and t + 32: row of token t of the tile
+  auto rows = [&](int t0) __attribute__((always_inline)) { return gqa_row(p, it.b, it.r.q0, min(t0 + (lane & 31), L - 1)); };
+  auto load = [&](int row) __attribute__((always_inline)) {
+    const int64_t page = row >> p.log2_ps, tok = row & ((1 << p.log2_ps) - 1);
+    const int64_t at = page * mp.c_page + tok * mp.c_tok;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t from = __shfl(at, u * (64 / kLanes) + lane / kLanes);
+      kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + from));
+      vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + from));
+    }
+    sr = *reinterpret_cast<const scale_t*>(sh + page * mp.s_page + tok * mp.s_tok);
+  };
+  Tile& tile = s_own[wave].t;
+  // K: 16-byte chunks of a key permuted (head_dim 128), so that the 16 keys of a read lie in different banks. V: key
+  // 16 t + 4 g + i at row 16 t + 4 i + g, so that a read of one (t, i) is one run of bytes.
+  auto kpos = [&](int t, int c) __attribute__((always_inline)) { return t * kRowB + (D == 128 ? c ^ ((t >> 2) & 3) : c) * 16; };
+  auto vpos = [&](int t) __attribute__((always_inline)) { return ((t & 16) | (t & 3) << 2 | (t >> 2 & 3)) * kRowB; };
+  // the byte of block b of a scale word, in bits 30..23; other bits are others'
+  auto scale_at = [](uint32_t w, int b) __attribute__((always_inline)) { return D == 128 ? __builtin_amdgcn_alignbit(w, w, (8 * b + 9) & 31) : w >> 8 * b << 23; };
+
+  constexpr int kStep = NW * kTileKeys;
+  int t0 = k0 + kTileKeys * wave, row_next = 0;
+  if (t0 < k1) {
+    const int row = rows(t0);
+    row_next = rows(t0 + kStep);
+    load(row);
+  }
+  for (; t0 < k1; t0 += kStep) {
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int t = u * (64 / kLanes) + lane / kLanes;
+      *reinterpret_cast<u32x4*>(tile.k + kpos(t, lane % kLanes)) = kr[u];
+      *reinterpret_cast<u32x4*>(tile.v + vpos(t) + lane % kLanes * 16) = vr[u];
+    }
+    (lane < 32 ? tile.ks : tile.vs)[lane & 31] = sr;
+    if (t0 + kStep < k1) load(row_next);
+    if (t0 + 2 * kStep < k1) row_next = rows(t0 + 2 * kStep);
+    f32x4 sc[NB][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = 16 * h + a16;
+      const kword_t kw = *reinterpret_cast<const kword_t*>(D == 128 ? tile.k + kpos(key, g) : tile.k + kpos(key, 0) + 8 * g);
+      const uint32_t ks = scale_at(tile.ks[key], D == 128 ? g : g >> 1);
+#pragma unroll
+      for (int s = 0; s < kKs; ++s) {
+        const bf16x8 kc = __builtin_bit_cast(bf16x8, mx4_values(kw[s], ks));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          sc[nb][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc, qf[nb][s], s == 0 ? f32x4{} : sc[nb][h], 0, 0, 0);
+      }
+    }
+    const bool masked = t0 + kTileKeys - 1 > first_limit || t0 + kTileKeys > k1;
+    u32x4 pb[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      // the scaled scores are rounded before their maximum is taken from them: the largest numerator is 2^-24 at any size
+#pragma clang fp contract(off)
+      f32x4(&s)[2] = sc[nb];
+      // score (h, i) of a lane: row a16, key t0 + 16 h + 4 g + i
+      float top = kLowest;
+      const int lim = min(limit[nb], k1 - 1) - t0 - 4 * g;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[h][i] *= p.scale_log2;
+          if (masked && 16 * h + i > lim) s[h][i] = -INFINITY;
+          top = fmaxf(top, s[h][i]);
+        }
+      top = wave_max_g(top);
+      if (__ballot(top > m[nb]) != 0) {
+        const float m_new = fmaxf(m[nb], top), f = __builtin_amdgcn_exp2f(m[nb] - m_new);
+        m[nb] = m_new;
+        l[nb] *= f;
+#pragma unroll
+        for (int db = 0; db < kDb; ++db) O[nb][db] *= f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(s[h][i] - m[nb]) * (1.f / kRoom);
+          l[nb] += e[i];
+        }
+        pb[nb][2 * h] = pack_bf16x2(e[0], e[1]);
+        pb[nb][2 * h + 1] = pack_bf16x2(e[2], e[3]);
+      }
+    }
+    vword_t vw[2][4];
+    scale_t sw[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        vw[h][i] = *reinterpret_cast<const vword_t*>(tile.v + (16 * h + 4 * i + g) * kRowB + sizeof(vword_t) * a16);
+        sw[h][i] = tile.vs[16 * h + 4 * g + i];
+      }
+    constexpr int kLanesB = 32 / (D / 16);  // lanes n of a block
+    if (__builtin_expect(masked, 0)) {
+      // Blocks of V that are NaN at a key that not every row attends: the product would bring them to rows of weight zero.
+      // They are left out, and added to the rows that attend them.
+      uint32_t any = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) any |= any_ff(sw[h][i]);
+      if (__ballot(any != 0) != 0) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int lim = min(limit[nb], k1 - 1) - t0 - 4 * g;
+          uint32_t hit = 0;  // bit 7 of byte b: of block b, at a key of the lane's that row a16 attends
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (16 * h + i <= lim) hit |= any_ff(sw[h][i]);
+          const auto a = __builtin_amdgcn_permlane16_swap(hit, hit, false, false);
+          hit = a[0] | a[1];
+          const auto b = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
+          hit = b[0] | b[1];
+          const float add = hit >> (8 * (D == 128 ? g : g >> 1) + 7) & 1 ? __builtin_nanf("") : 0.f;
+#pragma unroll
+          for (int db = 0; db < kDb; ++db) O[nb][db] += add;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((sw[h][i] >> 8 * (a16 / kLanesB) & 255) == 255) vw[h][i] = 0, sw[h][i] = 0;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kDb / 2; ++c) {
+      uint32_t x[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f = __uint_as_float(scale_at(sw[h][i], a16 / kLanesB));
+          // (the selector is a constant of the instruction)
+          x[h][i] = __builtin_bit_cast(uint32_t, c == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], f, 0)
+                                                 : c == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], f, 1)
+                                                 : c == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], f, 2)
+                                                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], f, 3));
+        }
+      u32x4 lo, hi;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          lo[2 * h + i] = __builtin_amdgcn_perm(x[h][2 * i + 1], x[h][2 * i], 0x05040100);
+          hi[2 * h + i] = __builtin_amdgcn_perm(x[h][2 * i + 1], x[h][2 * i], 0x07060302);
+        }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        O[nb][2 * c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), __builtin_bit_cast(bf16x8, pb[nb]), O[nb][2 * c], 0, 0, 0);
+        O[nb][2 * c + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, pb[nb]), O[nb][2 * c + 1], 0, 0, 0);
+      }
+    }
+  }
+
+  // ---- the waves' results joined, one block of 16 rows at a time
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const float lw = wave_sum_g(l[nb]);
+    if (nb > 0) __syncthreads();
+    // lane: row a16, dims (kDb * 4) g + kDb i + m, 16-byte chunks rotated by the row
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < kDb / 4; ++c)
+        *reinterpret_cast<f32x4*>(s_own[wave].o + a16 * (D * 4) + ((kDb * g + kDb / 4 * i + c + a16) % (D / 4)) * 16) =
+            f32x4{O[nb][4 * c][i], O[nb][4 * c + 1][i], O[nb][4 * c + 2][i], O[nb][4 * c + 3][i]};
+    if (g == 0) {
+      s_m[wave][a16] = m[nb];
+      s_l[wave][a16] = lw;
+    }
+    __syncthreads();
+    // kTpr threads a row, 4 dims each at a time
+    constexpr int kTpr = 4 * NW;
+    const int row = threadIdx.x / kTpr, x = threadIdx.x % kTpr;
+    float mt = s_m[0][row];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) mt = fmaxf(mt, s_m[w][row]);
+    float f[NW], lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(s_m[w][row] - mt);
+      lt += f[w] * s_l[w][row];
+    }
+    const bool some = lt > 0.f || lt != lt;
+    const float inv = some ? 1.f / lt : 0.f;
+    const f32x2 lse2 = gqa_lse(some, mt, log2f(lt * kRoom));
+    const int r = it.block * kRows + 16 * nb + row, tok = r / G, head = it.head * G + r % G;
+#pragma unroll
+    for (int c = tok < E ? x : D; c < D / 4; c += kTpr) {
+      f32x4 o = f32x4{};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) o += *reinterpret_cast<const f32x4*>(s_own[w].o + row * (D * 4) + ((c + row) % (D / 4)) * 16) * f[w];
+      o *= inv;
+      if (it.slot >= 0) {
+        *reinterpret_cast<f32x4*>(p.ws_o + ((int64_t)it.slot * kRows + 16 * nb + row) * D + 4 * c) = o;
+      } else {
+        u32x2 v{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+        *reinterpret_cast<u32x2*>(p.out + (int64_t)(it.r.q0 + tok) * p.out_stride_t + (int64_t)head * p.out_stride_h + 4 * c) = v;
+      }
+    }
+    if (x == 0 && tok < E) {
+      if (it.slot >= 0) p.ws_lse[(int64_t)it.slot * kRows + 16 * nb + row] = lse2;
+      else if (p.lse != nullptr) p.lse[(int64_t)(it.r.q0 + tok) * p.lse_stride_t + head] = lse2[0] * 0.69314718055994531f;
+    }
+  }
+}
+
+// Values of every key of a batch, in pages of 64 rows for the bf16 kernels: request b's keys take the rows from 64 times the
+// pages of the requests before it on. scratch: K and V [rows] of kv_heads * D each, and the page table.
+template <int D>
+__global__ __launch_bounds__(256) void mx4_pages_kernel(const GqaMx4Params mp) {
+  const GqaParams& p = mp.g;
+  constexpr int kLanes = D / 8;
+  const int lane = threadIdx.x & 63;
+  // the CTA's page of 64 keys: its request, by a scan of the pages
+  int acc = 0, b = -1, first = 0, L = 0;
+  for (int c0 = 0; c0 < p.batch && b < 0; c0 += 64) {
+    int len = 0;
+    if (c0 + lane < p.batch) len = gqa_request(p, c0 + lane).L;
+    const int n = (len + 63) >> 6, incl = wave_iscan(n);
+    const uint64_t hit = __ballot((int)blockIdx.x >= acc + incl - n && (int)blockIdx.x < acc + incl);
+    if (hit != 0) {
+      const int fl = __builtin_ctzll(hit);
+      b = c0 + fl;
+      first = acc + __builtin_amdgcn_readlane(incl - n, fl);
+      L = __builtin_amdgcn_readlane(len, fl);
+    } else {
+      acc += __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  if (b < 0) return;
+  const int page = (int)blockIdx.x - first;
+  if (threadIdx.x == 0 && blockIdx.y == 0) mp.scratch_table[(int64_t)b * mp.scratch_cols + page] = (int)blockIdx.x;
+  const int head = blockIdx.y;
+  for (int i = threadIdx.x; i < 64 * kLanes * 2; i += 256) {
+    const int x = i % kLanes, t = i / kLanes % 64, j = 64 * page + t;
+    const bool v = i >= 64 * kLanes;
+    if (j >= L) continue;
+    const int row = gqa_row(p, b, 0, j);
+    const int64_t pg = row >> p.log2_ps, tok = row & ((1 << p.log2_ps) - 1);
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>((v ? mp.v_codes : mp.k_codes) + pg * mp.c_page + tok * mp.c_tok + head * mp.c_head + 4 * x);
+    const uint32_t scale = (v ? mp.v_scales : mp.k_scales)[pg * mp.s_page + tok * mp.s_tok + head * mp.s_head + x / 4];
+    const int64_t at = ((int64_t)head * mp.scratch_rows + (int64_t)blockIdx.x * 64 + t) * D + 8 * x;
+    *reinterpret_cast<u32x4*>((v ? mp.scratch_v : mp.scratch_k) + at) = mx4_values(codes, scale << 23);
+  }
+}
+
+template <int D, int NB>
+void launch_stream(const GqaMx4Params& p, int64_t grid, hipStream_t stream) {
+  if (p.g.wide) hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 8>), dim3((unsigned)grid), dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 4>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+}
+
+}  // namespace
+
+hipError_t launch_gqa_mx4(const GqaMx4Params& p, int dim, int rows, hipStream_t stream) {
+  const int64_t grid = gqa_ctas(p.g, rows);
+  if (dim == 128) rows == 16 ? launch_stream<128, 1>(p, grid, stream) : launch_stream<128, 2>(p, grid, stream);
+  else rows == 16 ? launch_stream<64, 1>(p, grid, stream) : launch_stream<64, 2>(p, grid, stream);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && p.g.target > 0) e = launch_gqa_merge(p.g, dim, rows, stream);
+  return e;
+}
+
+hipError_t launch_mx4_pages(const GqaMx4Params& p, int dim, hipStream_t stream) {
+  const dim3 grid((unsigned)(p.scratch_rows / 64), (unsigned)p.g.kv_heads);
+  if (dim == 128) hipLaunchKernelGGL(mx4_pages_kernel<128>, grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL(mx4_pages_kernel<64>, grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace mla

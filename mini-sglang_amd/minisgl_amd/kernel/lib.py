@@ -24,6 +24,8 @@ _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 
 # symbol -> (restype, argtypes); must match include/mla_amd.h
+_pool = ctypes.c_void_p  # const mla_mx4_pool*
+
 SIGNATURES = {
     "mla_last_error": (ctypes.c_char_p, []),
     "mla_abi_version": (ctypes.c_int, []),
@@ -98,9 +100,33 @@ SIGNATURES = {
         [_vp, _i32, _i32, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _i32, _i64, _vp, _vp, _i32,
          _vp, _vp, _vp],
     ),
+    "mla_qk_norm_rope_bf16": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _vp, _i32, _i32, _i32, _i32,
+         _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i64, _vp],
+    ),
+    "mla_mx4_store": (
+        ctypes.c_int,
+        [_pool, _pool, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp],
+    ),
+    "mla_mx4_load": (
+        ctypes.c_int,
+        [_pool, _pool, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp],
+    ),
+    "mla_gqa_mx4_workspace_bytes": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _i64, _i64, ctypes.POINTER(_i64)]),
+    "mla_gqa_chunk_mx4": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _pool, _pool, _i32, _i32, _vp, _i32, _i64, _vp, _vp, _i32, _i32, _i32, _i64, _i32, _i32, _i32,
+         ctypes.c_float, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
+    ),
+    "mla_gqa_decode_mx4": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _pool, _pool, _i32, _i32, _vp, _i32, _i64, _vp, _i32, _i64, _i32, _i32, _i32, ctypes.c_float,
+         _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
+    ),
 }
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 PLAN_BLOCK = 64
 PLAN_CTA_INTS = 4
 PLAN_REQ_INTS = 3
@@ -554,7 +580,8 @@ def load_binding():
         raise MLAKernelError(f"minisgl_amd.kernel._mla_torch was built for {binding.built_for}, this is {now}: build it with "
                              "`python mini-sglang_amd/build.py`")
     entry_points = (lib.mla_gqa_prompt_bf16, lib.mla_gqa_workspace_bytes, lib.mla_gqa_chunk_bf16, lib.mla_gqa_decode_bf16,
-                    lib.mla_page_tables_from_lengths)
+                    lib.mla_page_tables_from_lengths, lib.mla_qk_norm_rope_bf16, lib.mla_mx4_store, lib.mla_mx4_load,
+                    lib.mla_gqa_mx4_workspace_bytes, lib.mla_gqa_chunk_mx4, lib.mla_gqa_decode_mx4)
     binding.bind(*(ctypes.cast(f, _vp).value for f in entry_points), torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
     return binding
 
@@ -661,3 +688,95 @@ def page_tables_from_lengths(token_table, table_idx, cached_lens, device_lens, f
         got = _again(got, token_table.device, call, "mla_page_tables_from_lengths", token_table, table_idx, cached_lens, device_lens,
                      free_slots, page_size, max_device_len, max_extend, total_new, alloc_reqs, stream)
     return PageTables(*got)
+
+
+def qk_norm_rope(q, k, v, q_weight, k_weight, eps: float, positions, cos_sin, interleaved: bool, q_out, k_out, v_out=None,
+                 slots=None, stream=None) -> None:
+    """The norm of each head of ``q [T, Hq, D]`` and ``k [T, Hkv, D]`` (D 64 or 128; any strides that are multiples of 8: the
+    parts of a fused projection's output) with ``q_weight``, ``k_weight [D]`` (both None: none), the rotation of their first
+    R dims at ``positions [T]`` (int32) from the fp32 ``cos_sin [max_position, R]`` table, and the rows of K and V into a
+    cache, in one launch. Queries go to ``q_out [T, Hq, D]`` (may be ``q``). ``slots [T]`` (int32 or int64): keys and the rows
+    of ``v`` go to the token rows ``slots`` of the pools ``k_out``, ``v_out [pages, ps, Hkv, D]``; slots outside are skipped.
+    Without ``slots``, ``k_out`` and ``v_out`` are ``[T, Hkv, D]`` (``k_out`` may be ``k``). ``v`` None: keys alone."""
+    call = load_binding().qk_norm_rope
+    rc = call(q, k, v, q_weight, k_weight, eps, positions, cos_sin, interleaved, q_out, k_out, v_out, slots, stream)
+    if rc != 0:
+        _again(rc, q.device, call, "mla_qk_norm_rope_bf16", q, k, v, q_weight, k_weight, eps, positions, cos_sin, interleaved,
+               q_out, k_out, v_out, slots, stream)
+
+
+class MX4Pool(NamedTuple):
+    """A paged pool of keys or values in 4 bits (OCP MXFP4: blocks of 32 dims; ``include/mla_amd.h``)."""
+
+    codes: "torch.Tensor"  # uint8 [pages, ps, Hkv, D / 2], two dims a byte, the even one in the low half
+    scales: "torch.Tensor"  # uint8 [pages, ps, Hkv, D / 32], a power of two's exponent plus 127; 255: NaN
+
+
+def mx4_pool(num_pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> MX4Pool:
+    """A pool with each head's rows of a page next to each other."""
+    import torch
+
+    def part(width):
+        return torch.empty((num_pages, kv_heads, page_size, width), dtype=torch.uint8, device=device).transpose(1, 2)
+
+    assert head_dim in (64, 128), "head_dim is 64 or 128"
+    return MX4Pool(part(head_dim // 2), part(head_dim // 32))
+
+
+def mx4_store(k_pool: MX4Pool, v_pool: MX4Pool, indices, k, v, stream=None) -> None:
+    """Rows ``k``, ``v [T, Hkv, D]`` (bf16) to the token rows ``indices [T]`` (int32 or int64) of the pools, each block of 32
+    dims rounded to 4 bits and a power of two; indices outside the pools are skipped, others must be distinct."""
+    call = load_binding().mx4_store
+    rc = call(*k_pool, *v_pool, indices, k, v, stream)
+    if rc != 0:
+        _again(rc, k.device, call, "mla_mx4_store", *k_pool, *v_pool, indices, k, v, stream)
+
+
+def mx4_load(k_pool: MX4Pool, v_pool: MX4Pool, indices, k=None, v=None, stream=None):
+    """The values of token rows ``indices [T]`` as bf16 ``k``, ``v [T, Hkv, D]`` (exact; 0 for indices outside the pools)."""
+    import torch
+
+    rows, (_, _, heads, width) = indices.shape[0], k_pool.codes.shape
+
+    def made():
+        return _made(stream, lambda: torch.empty((rows, heads, 2 * width), dtype=torch.bfloat16, device=k_pool.codes.device))
+
+    k, v = made() if k is None else k, made() if v is None else v
+    call = load_binding().mx4_load
+    rc = call(*k_pool, *v_pool, indices, k, v, stream)
+    if rc != 0:
+        _again(rc, k.device, call, "mla_mx4_load", *k_pool, *v_pool, indices, k, v, stream)
+    return k, v
+
+
+def gqa_mx4_workspace_bytes(max_seqlen_q: int, q_heads: int, kv_heads: int, head_dim: int, batch: int, max_keys: int,
+                            total_keys: int) -> int:
+    """Bytes of the workspace that ``gqa_chunk_mx4`` (``gqa_decode_mx4``: ``max_seqlen_q`` 1) needs for up to ``batch`` requests
+    of up to ``max_keys`` keys by the page table's width, ``total_keys`` in all."""
+    out = _i64(0)
+    check(load_library().mla_gqa_mx4_workspace_bytes(max_seqlen_q, q_heads, kv_heads, head_dim, batch, max_keys, total_keys,
+                                                     ctypes.byref(out)), "mla_gqa_mx4_workspace_bytes")
+    return int(out.value)
+
+
+def gqa_chunk_mx4(q, k_pool: MX4Pool, v_pool: MX4Pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q: int, scale: float, out,
+                  lse=None, workspace=None, total_keys: int | None = None, stream=None) -> None:
+    """``gqa_chunk`` over pools of 4 bits. ``total_keys``: at least the sum of ``seq_lens_k`` (the host's; None: all that the page
+    table can hold), which bounds the memory where chunks of more than 32 rows (tokens times ``Hq // Hkv``) have their keys'
+    values laid out in bf16. ``workspace``: uint8, of ``gqa_mx4_workspace_bytes``, or None."""
+    assert cu_seqlens_q is not None, "cu_seqlens_q is [B + 1]"
+    call = load_binding().gqa_paged_mx4
+    args = (q, *k_pool, *v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q, scale, out, lse, workspace, total_keys, stream)
+    rc = call(*args)
+    if rc != 0:
+        _again(rc, q.device, call, "mla_gqa_chunk_mx4", *args)
+
+
+def gqa_decode_mx4(q, k_pool: MX4Pool, v_pool: MX4Pool, page_table, seq_lens, scale: float, out, lse=None, workspace=None,
+                   total_keys: int | None = None, stream=None) -> None:
+    """``gqa_chunk_mx4`` with one new token a request: ``q [B, Hq, D]`` -> ``out [B, Hq, D]`` (+ ``lse [B, Hq]``)."""
+    call = load_binding().gqa_paged_mx4
+    args = (q, *k_pool, *v_pool, page_table, None, seq_lens, 1, scale, out, lse, workspace, total_keys, stream)
+    rc = call(*args)
+    if rc != 0:
+        _again(rc, q.device, call, "mla_gqa_decode_mx4", *args)
