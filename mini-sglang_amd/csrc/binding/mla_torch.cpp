@@ -125,10 +125,14 @@ struct Queries {
 
   Queries(PyObject* q_, PyObject* out_, PyObject* lse_) : q(tensor(q_, "q")), out(tensor(out_, "out")), device(gpu_of(q)) {
     if (lse_ != Py_None) lse = &tensor(lse_, "lse");
-    require(q.dim() == 3, "q is [T, Hq, D]");
+    require(q.dim() == 3, "q is [T, Hq, D]; k and v are [T, Hkv, D], or pools [pages, ps, Hkv, D]");
     T = q.size(0), Hq = q.size(1), D = q.size(2);
+  }
+  // once keys and values have q's heads and width
+  void check() const {
     require(device >= 0 && gpu_of(out) == device && (lse == nullptr || gpu_of(*lse) == device), "all tensors must be on one GPU");
-    require(q.scalar_type() == at::kBFloat16 && out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes(), "q and out are bf16, out of q's shape");
+    require(q.scalar_type() == at::kBFloat16 && out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes(),
+            "q, k, v and out are bf16, out of q's shape");
     require(lse == nullptr || (lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == T && lse->size(1) == Hq),
             "lse is fp32 [T, Hq]");
     require(q.stride(2) == 1 && out.stride(2) == 1 && (lse == nullptr || one_apart(*lse, 1)), "rows must be contiguous");
@@ -149,7 +153,8 @@ struct Attention : Queries {
     Hkv = k.size(-2);
     require(k.size(-1) == D && v.sizes() == k.sizes() && Hkv > 0 && Hq % Hkv == 0, "k and v have q's D and heads that divide q's");
     require(gpu_of(k) == device && gpu_of(v) == device, "all tensors must be on one GPU");
-    require(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16, "k and v are bf16");
+    check();
+    require(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16, "q, k, v and out are bf16, out of q's shape");
     require(k.stride(-1) == 1 && v.stride(-1) == 1, "rows must be contiguous");
     require(Hkv <= INT32_MAX, "sizes past 32 bits");
   }
@@ -367,6 +372,7 @@ PyObject* page_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* gqa_paged_mx4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 15, [&]() -> PyObject* {
     const Queries x(a[0], a[10], a[11]);
+    x.check();
     const Pool4 k(a[1], a[2], x.device), v(a[3], a[4], x.device);
     require(k.like(v) && k.dim == x.D && k.heads > 0 && x.Hq % k.heads == 0, "the pools have q's D and heads that divide q's");
     const at::Tensor& lens = tensor(a[7], "seq_lens");
