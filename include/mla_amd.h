@@ -464,7 +464,7 @@ int mla_mx4_load(const mla_mx4_pool *k_pool, const mla_mx4_pool *v_pool, int32_t
 /*
  * mla_gqa_chunk_bf16 and mla_gqa_decode_bf16 over pools of 4 bits, with the same arguments and semantics otherwise: the
  * result is that of the codes' values, fp32 scores and sums, numerators in bf16 for the product with the values. Both pools
- * have the same strides. A NaN block reaches the rows that attend its token only. Requests of more than 32 rows (max_q times
+ * have the same strides. A NaN block reaches the rows that attend its token only. Requests of more than 512 rows (max_q times
  * q_heads / kv_heads) may have their keys' values laid out in bf16 first: total_keys is at least the sum of seq_lens_k (its
  * keys past that are not those of the pool), and sizes that part of the workspace. mla_gqa_mx4_workspace_bytes: enough for
  * every call with at most max_q queries a request, `batch` requests, max_keys = pt_cols * page_size, and total_keys;

@@ -424,28 +424,92 @@ PyObject* gqa_paged_mx4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// mx4_store / mx4_load(k codes, k scales, v codes, v scales, indices, k, v, stream)
-PyObject* mx4_rows(PyObject* const* a, Py_ssize_t n, bool load) {
+// What mx4_store and mx4_load share: the pools, and their rows' numbers.
+struct PoolRows {
+  const at::Tensor& indices;
+  long device;
+  int64_t T;
+  Rows rows;
+  Pool4 k, v;
+  explicit PoolRows(PyObject* const* a)
+      : indices(tensor(a[4], "indices")), device(gpu_of(indices)), T((check(indices, device), indices.size(0))), rows(a[4], "indices", T, device),
+        k(a[0], a[1], device), v(a[2], a[3], device) {
+    require(k.like(v) && T <= INT32_MAX, "both pools have the same shape");
+  }
+  static void check(const at::Tensor& t, long device) { require(device >= 0 && t.dim() == 1, "indices is [T], on the GPU"); }
+  template <typename Entry, typename Ptr>
+  long call(Entry entry, Ptr* kp, int64_t kt, int64_t kh, Ptr* vp, int64_t vt, int64_t vh, void* stream) const {
+    return launched([&] {
+      return entry(&k.c, &v.c, (int32_t)k.pages, (int32_t)k.ps, (int32_t)k.heads, (int32_t)k.dim, rows.ptr, rows.bits, (int32_t)T, kp, kt, kh,
+                   vp, vt, vh, stream);
+    });
+  }
+};
+
+// mx4_store(k codes, k scales, v codes, v scales, indices, k, v, stream)
+PyObject* mx4_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 8, [&]() -> PyObject* {
-    const at::Tensor& indices = tensor(a[4], "indices");
-    const long device = gpu_of(indices);
-    require(device >= 0 && indices.dim() == 1, "indices is [T], on the GPU");
-    const int64_t T = indices.size(0);
-    const Rows rows(a[4], "indices", T, device);
-    const Pool4 kp(a[0], a[1], device), vp(a[2], a[3], device);
-    require(kp.like(vp) && T <= INT32_MAX, "both pools have the same shape");
-    const Heads k(a[5], "k", T, kp.heads, kp.dim, device), v(a[6], "v", T, kp.heads, kp.dim, device);
-    if (!is_current(device)) return PyLong_FromLong(kOtherDevice);
-    void* stream = stream_of(a[7], device);
-    auto call = [&](auto entry) {
-      return entry(&kp.c, &vp.c, (int32_t)kp.pages, (int32_t)kp.ps, (int32_t)kp.heads, (int32_t)kp.dim, rows.ptr, rows.bits, (int32_t)T, k.ptr(),
-                   k.row(), k.head(), v.ptr(), v.row(), v.head(), stream);
-    };
-    return PyLong_FromLong(launched([&] { return load ? call(g.mx4_load) : call(g.mx4_store); }));
+    const PoolRows x(a);
+    const Heads k(a[5], "k", x.T, x.k.heads, x.k.dim, x.device), v(a[6], "v", x.T, x.k.heads, x.k.dim, x.device);
+    if (!is_current(x.device)) return PyLong_FromLong(kOtherDevice);
+    return PyLong_FromLong(x.call(g.mx4_store, k.ptr(), k.row(), k.head(), v.ptr(), v.row(), v.head(), stream_of(a[7], x.device)));
   });
 }
-PyObject* mx4_store(PyObject*, PyObject* const* a, Py_ssize_t n) { return mx4_rows(a, n, false); }
-PyObject* mx4_load(PyObject*, PyObject* const* a, Py_ssize_t n) { return mx4_rows(a, n, true); }
+
+// mx4_load(k codes, k scales, v codes, v scales, indices, k or None, v or None, stream) -> code, or (k, v)
+PyObject* mx4_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    const PoolRows x(a);
+    const int64_t width = x.k.heads * x.k.dim;
+    struct {
+      void* ptr;
+      int64_t row, head;
+    } to[2];
+    int missing = 0;
+    for (int i = 0; i < 2; ++i) {
+      if (a[5 + i] == Py_None) {
+        ++missing;
+      } else {
+        const Heads h(a[5 + i], i ? "v" : "k", x.T, x.k.heads, x.k.dim, x.device);
+        to[i] = {h.ptr(), h.row(), h.head()};
+      }
+    }
+    if (!is_current(x.device)) return PyLong_FromLong(kOtherDevice);
+    void* stream = stream_of(a[7], x.device);
+    at::Tensor made;
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (missing > 0) {
+      if (!allocates_for(a[7], stream, x.device)) return PyLong_FromLong(kOtherStream);
+      made = at::empty({missing * x.T * width}, x.indices.options().dtype(at::kBFloat16));  // one allocation for both
+      int64_t at = 0;
+      for (int i = 0; i < 2; ++i)
+        if (a[5 + i] == Py_None) {
+          to[i] = {static_cast<char*>(made.data_ptr()) + 2 * at, width, x.k.dim};
+          at += x.T * width;
+        }
+    }
+    const long rc = x.call(g.mx4_load, to[0].ptr, to[0].row, to[0].head, to[1].ptr, to[1].row, to[1].head, stream);
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject* r = PyTuple_New(2);
+    if (r == nullptr) return nullptr;
+    int64_t at = 0;
+    for (int i = 0; i < 2; ++i) {
+      PyObject* o = a[5 + i];
+      if (o == Py_None) {
+        o = THPVariable_Wrap(made.as_strided({x.T, x.k.heads, x.k.dim}, {width, x.k.dim, 1}, at));
+        at += x.T * width;
+      } else {
+        Py_INCREF(o);
+      }
+      if (o == nullptr) {
+        Py_DECREF(r);
+        return nullptr;
+      }
+      PyTuple_SET_ITEM(r, i, o);
+    }
+    return r;
+  });
+}
 
 // qk_norm_rope(q, k, v or None, q_weight or None, k_weight or None, eps, positions, cos_sin, interleaved, q_out, k_out,
 //              v_out or None, slots or None, stream)

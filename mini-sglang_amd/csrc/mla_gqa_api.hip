@@ -252,7 +252,9 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
 
 // ---- over a cache of 4 bits
 
-// Bytes of a workspace: partial results, and for requests of more than 32 rows their keys' values in pages of 64 and the
+// Rows of a request that are streamed from the codes at most.
+constexpr int64_t kStreamRows = 512;
+// Bytes of a workspace: partial results, and for requests of more rows than that their keys' values in pages of 64 and the
 // page table of these.
 struct Mx4Space {
   int64_t split, table, rows, cols, bytes;
@@ -260,7 +262,7 @@ struct Mx4Space {
 Mx4Space mx4_space(int64_t most, int32_t kv_heads, int32_t dim, int32_t batch, int64_t max_keys, int64_t total_keys) {
   Mx4Space s = {};
   s.split = 4 * workspace_rows(most) * (dim + 2);
-  if (most > 32) {
+  if (most > kStreamRows) {
     s.cols = (max_keys + 63) / 64;
     s.rows = 64 * std::min(total_keys / 64 + batch, batch * s.cols);
     s.table = (4 * batch * s.cols + 15) / 16 * 16;
@@ -283,6 +285,8 @@ int check_mx4(const char* who, const Mx4View& k, const Mx4View& v, int32_t dim, 
     if (x->c_page % 16 || x->c_tok % 16 || x->c_head % 16 || x->s_page % scale_row || x->s_tok % scale_row || x->s_head % scale_row ||
         x->c_page < 0 || x->c_tok < 0 || x->c_head < 0 || x->s_page < 0 || x->s_tok < 0 || x->s_head < 0)
       return api_error(MLA_ERR_INVALID_ARG, "%s: strides must be non-negative multiples of 16 bytes (codes) and of a row (scales)", who);
+    else if (x->c_tok > (1 << 24) || x->s_tok > (1 << 24))
+      return api_error(MLA_ERR_UNSUPPORTED, "%s: tokens lie more than 16 MiB apart", who);
   return MLA_OK;
 }
 
@@ -315,7 +319,15 @@ int paged_mx4(const char* who, const void* q, int64_t q_stride_t, int64_t q_stri
   mp.s_page = k.s_page, mp.s_tok = k.s_tok, mp.s_head = k.s_head;
   const int64_t most = (int64_t)max_q * p.group, keys = (int64_t)pt_cols * page_size;
   p.max_keys = (int32_t)(keys < 0x7ff00000 ? keys : 0x7ff00000);
-  const Choice choice = choose(dim, batch, total_q, p.group, kv_heads, most, p.max_keys);
+  Choice choice = choose(dim, batch, total_q, p.group, kv_heads, most, p.max_keys);
+  // Blocks read values that are laid out first, 512 bytes for every 136 of the cache: worth it where many rows read them. 32-row
+  // CTAs / laid out, us, 64 and 8 heads of 128: six chunks of 32 on 8000 109 / 147, of 64 181 / 207, of 96 254 / 270, of 128 329 /
+  // 288; four of 64 on 2000 64 / 54, on 500 15 / 28; 32 and 8 heads of 64, of 64 on 2000 16 / 16, of 128 51 / 48.
+  if (choice.rows >= kBlock && most <= kStreamRows) {
+    const int64_t ctas = std::max<int64_t>((total_q * (int64_t)p.group + 31) / 32, batch) * kv_heads;
+    const bool few = 2 * ctas <= kFit;
+    choice = {32, few ? kFit : p.max_keys <= kOnePieceMany || ctas >= kTarget ? 0 : kTarget, few, false};
+  }
   const bool laid_out = choice.rows >= kBlock;
   const Mx4Space space = mx4_space(most, kv_heads, dim, batch, p.max_keys, total_keys);
   if (!aligned(workspace, 16) || (workspace_bytes < space.bytes && (workspace != nullptr || choice.target > 0 || laid_out)))

@@ -21,13 +21,15 @@ namespace {
 
 constexpr int kTileKeys = 32;
 constexpr float kLowest = -3.4028234663852886e38f;
-// Numerators are times 2^-24: sums of 2^24 values of the largest size (6 2^125) stay in fp32's range
-constexpr float kRoom = 0x1p24f;
+// References are 24 above the largest score (log2 domain), so numerators at most 2^-24: sums of 2^24 values of the largest
+// size (6 2^125) stay in fp32's range
+constexpr float kRoom = 24.f;
 
 __device__ __forceinline__ uint32_t any_ff(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
 
-// NB blocks of 16 rows, NW waves
-template <int D, int NB, int NW>
+// NB blocks of 16 rows, NW waves. kBig: pages of 32 tokens or more, so that a tile lies in one page and its addresses are
+// the wave's (scalar), where they are a lane's otherwise.
+template <int D, int NB, int NW, bool kBig>
 __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params mp) {
   const GqaParams& p = mp.g;
   constexpr int kRows = 16 * NB, kRowB = D / 2, kScaleB = D / 32, kKs = D / 32, kDb = D / 16;
@@ -67,8 +69,6 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   const int last_tok = min(E - 1, (it.block * kRows + kRows - 1) / G);
   const int first_limit = P + it.block * kRows / G;  // of the item's first row: no key up to it is masked
   const int k0 = it.piece * C, k1 = min(it.pieces > 1 ? k0 + C : L, P + last_tok + 1);
-  const uint8_t *kh = mp.k_codes + (int64_t)it.head * mp.c_head + lane % kLanes * 16, *vh = mp.v_codes + (int64_t)it.head * mp.c_head + lane % kLanes * 16;
-  const uint8_t* sh = (lane < 32 ? mp.k_scales : mp.v_scales) + (int64_t)it.head * mp.s_head;
 
   f32x4 O[NB][kDb];
   float m[NB], l[NB];
@@ -81,18 +81,40 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   }
   u32x4 kr[kLoads], vr[kLoads];
   scale_t sr{};
-  // lane t and t + 32: row of token t of the tile
-  auto rows = [&](int t0) __attribute__((always_inline)) { return gqa_row(p, it.b, it.r.q0, min(t0 + (lane & 31), L - 1)); };
-  auto load = [&](int row) __attribute__((always_inline)) {
-    const int64_t page = row >> p.log2_ps, tok = row & ((1 << p.log2_ps) - 1);
-    const int64_t at = page * mp.c_page + tok * mp.c_tok;
+  // What a tile's addresses come from, read a tile ahead: the page's id (rows past the length in a page are read, and left
+  // out), or the row of token t in lanes t and t + 32.
+  auto rows = [&](int t0) __attribute__((always_inline)) {
+    if constexpr (kBig) return p.page_table[(int64_t)it.b * p.pt_stride + (min(t0, L - 1) >> p.log2_ps)];
+    else return gqa_row(p, it.b, it.r.q0, min(t0 + (lane & 31), L - 1));
+  };
+  // of the lane in a tile: codes by load, scales
+  uint32_t code_at[kLoads], scale_off;
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const int64_t from = __shfl(at, u * (64 / kLanes) + lane / kLanes);
-      kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + from));
-      vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + from));
+  for (int u = 0; u < kLoads; ++u) code_at[u] = (kBig ? (u * (64 / kLanes) + lane / kLanes) * (uint32_t)mp.c_tok : 0) + lane % kLanes * 16;
+  scale_off = kBig ? (lane & 31) * (uint32_t)mp.s_tok : 0;
+  const uint8_t *kh = mp.k_codes + (int64_t)it.head * mp.c_head, *vh = mp.v_codes + (int64_t)it.head * mp.c_head;
+  const uint8_t *ksh = mp.k_scales + (int64_t)it.head * mp.s_head, *vsh = mp.v_scales + (int64_t)it.head * mp.s_head;
+  auto load = [&](int t0, int row) __attribute__((always_inline)) {
+    if constexpr (kBig) {
+      const int64_t page = min(max(__builtin_amdgcn_readfirstlane(row), 0), p.num_pages - 1), tok = t0 & ((1 << p.log2_ps) - 1);
+      const int64_t at = page * mp.c_page + tok * mp.c_tok, sat = page * mp.s_page + tok * mp.s_tok;
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + at + code_at[u]));
+        vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + at + code_at[u]));
+      }
+      sr = *reinterpret_cast<const scale_t*>((lane < 32 ? ksh : vsh) + sat + scale_off);
+    } else {
+      const int64_t page = row >> p.log2_ps, tok = row & ((1 << p.log2_ps) - 1);
+      const int64_t at = page * mp.c_page + tok * mp.c_tok;
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int64_t from = __shfl(at, u * (64 / kLanes) + lane / kLanes) + code_at[u];
+        kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + from));
+        vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + from));
+      }
+      sr = *reinterpret_cast<const scale_t*>((lane < 32 ? ksh : vsh) + page * mp.s_page + tok * mp.s_tok);
     }
-    sr = *reinterpret_cast<const scale_t*>(sh + page * mp.s_page + tok * mp.s_tok);
   };
   Tile& tile = s_own[wave].t;
   // K: 16-byte chunks of a key permuted (head_dim 128), so that the 16 keys of a read lie in different banks. V: key
@@ -101,40 +123,29 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   auto vpos = [&](int t) __attribute__((always_inline)) { return ((t & 16) | (t & 3) << 2 | (t >> 2 & 3)) * kRowB; };
   // the byte of block b of a scale word, in bits 30..23; other bits are others'
   auto scale_at = [](uint32_t w, int b) __attribute__((always_inline)) { return D == 128 ? __builtin_amdgcn_alignbit(w, w, (8 * b + 9) & 31) : w >> 8 * b << 23; };
+  constexpr int kLanesB = 32 / (D / 16);  // lanes n of a block of V
 
-  constexpr int kStep = NW * kTileKeys;
-  int t0 = k0 + kTileKeys * wave, row_next = 0;
-  if (t0 < k1) {
-    const int row = rows(t0);
-    row_next = rows(t0 + kStep);
-    load(row);
-  }
-  for (; t0 < k1; t0 += kStep) {
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const int t = u * (64 / kLanes) + lane / kLanes;
-      *reinterpret_cast<u32x4*>(tile.k + kpos(t, lane % kLanes)) = kr[u];
-      *reinterpret_cast<u32x4*>(tile.v + vpos(t) + lane % kLanes * 16) = vr[u];
-    }
-    (lane < 32 ? tile.ks : tile.vs)[lane & 31] = sr;
-    if (t0 + kStep < k1) load(row_next);
-    if (t0 + 2 * kStep < k1) row_next = rows(t0 + 2 * kStep);
+  // kMasked: some row does not attend some key of the tile
+  auto step = [&](int t0, auto kMasked) __attribute__((always_inline)) {
     f32x4 sc[NB][2];
+    kword_t kw[2];
+    uint32_t ks[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int key = 16 * h + a16;
-      const kword_t kw = *reinterpret_cast<const kword_t*>(D == 128 ? tile.k + kpos(key, g) : tile.k + kpos(key, 0) + 8 * g);
-      const uint32_t ks = scale_at(tile.ks[key], D == 128 ? g : g >> 1);
+      kw[h] = *reinterpret_cast<const kword_t*>(D == 128 ? tile.k + kpos(key, g) : tile.k + kpos(key, 0) + 8 * g);
+      ks[h] = scale_at(tile.ks[key], D == 128 ? g : g >> 1);
+    }
 #pragma unroll
-      for (int s = 0; s < kKs; ++s) {
-        const bf16x8 kc = __builtin_bit_cast(bf16x8, mx4_values(kw[s], ks));
+    for (int s = 0; s < kKs; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bf16x8 kc = __builtin_bit_cast(bf16x8, mx4_values(kw[h][s], ks[h]));
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
           sc[nb][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc, qf[nb][s], s == 0 ? f32x4{} : sc[nb][h], 0, 0, 0);
       }
-    }
-    const bool masked = t0 + kTileKeys - 1 > first_limit || t0 + kTileKeys > k1;
-    u32x4 pb[NB];
+    float e[NB][2][4];  // numerators
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       // the scaled scores are rounded before their maximum is taken from them: the largest numerator is 2^-24 at any size
@@ -148,10 +159,10 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s[h][i] *= p.scale_log2;
-          if (masked && 16 * h + i > lim) s[h][i] = -INFINITY;
+          if (decltype(kMasked)::value && 16 * h + i > lim) s[h][i] = -INFINITY;
           top = fmaxf(top, s[h][i]);
         }
-      top = wave_max_g(top);
+      top = wave_max_g(top) + kRoom;
       if (__ballot(top > m[nb]) != 0) {
         const float m_new = fmaxf(m[nb], top), f = __builtin_amdgcn_exp2f(m[nb] - m_new);
         m[nb] = m_new;
@@ -160,16 +171,12 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
         for (int db = 0; db < kDb; ++db) O[nb][db] *= f;
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float e[4];
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(s[h][i] - m[nb]) * (1.f / kRoom);
-          l[nb] += e[i];
+          e[nb][h][i] = __builtin_amdgcn_exp2f(s[h][i] - m[nb]);
+          l[nb] += e[nb][h][i];
         }
-        pb[nb][2 * h] = pack_bf16x2(e[0], e[1]);
-        pb[nb][2 * h + 1] = pack_bf16x2(e[2], e[3]);
-      }
     }
     vword_t vw[2][4];
     scale_t sw[2][4];
@@ -180,8 +187,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
         vw[h][i] = *reinterpret_cast<const vword_t*>(tile.v + (16 * h + 4 * i + g) * kRowB + sizeof(vword_t) * a16);
         sw[h][i] = tile.vs[16 * h + 4 * g + i];
       }
-    constexpr int kLanesB = 32 / (D / 16);  // lanes n of a block
-    if (__builtin_expect(masked, 0)) {
+    if constexpr (decltype(kMasked)::value) {
       // Blocks of V that are NaN at a key that not every row attends: the product would bring them to rows of weight zero.
       // They are left out, and added to the rows that attend them.
       uint32_t any = 0;
@@ -214,35 +220,72 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
             if ((sw[h][i] >> 8 * (a16 / kLanesB) & 255) == 255) vw[h][i] = 0, sw[h][i] = 0;
       }
     }
+    float vs[2][4];
 #pragma unroll
-    for (int c = 0; c < kDb / 2; ++c) {
-      uint32_t x[2][4];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int i = 0; i < 4; ++i) vs[h][i] = __uint_as_float(scale_at(sw[h][i], a16 / kLanesB));
+    // two dims of V's word c of key (h, i)
+    auto two = [&](auto c, int h, int i) __attribute__((always_inline)) {
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], vs[h][i], decltype(c)::value));
+    };
+    auto mfma = [](u32x4 a, u32x4 b, f32x4& o) __attribute__((always_inline)) {
+      o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), o, 0, 0, 0);
+    };
+    auto products = [&](auto c) __attribute__((always_inline)) {
+      constexpr int kC = decltype(c)::value;
+      if constexpr (kC < kDb / 2) {
+          u32x4 lo, hi;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float f = __uint_as_float(scale_at(sw[h][i], a16 / kLanesB));
-          // (the selector is a constant of the instruction)
-          x[h][i] = __builtin_bit_cast(uint32_t, c == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], f, 0)
-                                                 : c == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], f, 1)
-                                                 : c == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], f, 2)
-                                                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(vw[h][i], f, 3));
-        }
-      u32x4 lo, hi;
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x = two(c, h, 2 * i), y = two(c, h, 2 * i + 1);
+              lo[2 * h + i] = __builtin_amdgcn_perm(y, x, 0x05040100);
+              hi[2 * h + i] = __builtin_amdgcn_perm(y, x, 0x07060302);
+            }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          lo[2 * h + i] = __builtin_amdgcn_perm(x[h][2 * i + 1], x[h][2 * i], 0x05040100);
-          hi[2 * h + i] = __builtin_amdgcn_perm(x[h][2 * i + 1], x[h][2 * i], 0x07060302);
-        }
+          for (int nb = 0; nb < NB; ++nb) {
+            u32x4 pb;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        O[nb][2 * c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), __builtin_bit_cast(bf16x8, pb[nb]), O[nb][2 * c], 0, 0, 0);
-        O[nb][2 * c + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, pb[nb]), O[nb][2 * c + 1], 0, 0, 0);
+            for (int h = 0; h < 2; ++h) {
+              pb[2 * h] = pack_bf16x2(e[nb][h][0], e[nb][h][1]);
+              pb[2 * h + 1] = pack_bf16x2(e[nb][h][2], e[nb][h][3]);
+            }
+            mfma(lo, pb, O[nb][2 * kC]);
+            mfma(hi, pb, O[nb][2 * kC + 1]);
+          }
       }
-    }
+    };
+    products(std::integral_constant<int, 0>{});
+    products(std::integral_constant<int, 1>{});
+    products(std::integral_constant<int, 2>{});
+    products(std::integral_constant<int, 3>{});
+  };
+
+  constexpr int kStep = NW * kTileKeys;
+  int t0 = k0 + kTileKeys * wave, row_next = 0;
+  if (t0 < k1) {
+    const int row = rows(t0);
+    row_next = rows(t0 + kStep);
+    load(t0, row);
   }
+  auto tiles = [&](int end, auto kMasked) __attribute__((always_inline)) {
+    for (; t0 < end; t0 += kStep) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int t = u * (64 / kLanes) + lane / kLanes;
+        *reinterpret_cast<u32x4*>(tile.k + kpos(t, lane % kLanes)) = kr[u];
+        *reinterpret_cast<u32x4*>(tile.v + vpos(t) + lane % kLanes * 16) = vr[u];
+      }
+      (lane < 32 ? tile.ks : tile.vs)[lane & 31] = sr;
+      if (t0 + kStep < k1) load(t0 + kStep, row_next);
+      if (t0 + 2 * kStep < k1) row_next = rows(t0 + 2 * kStep);
+      step(t0, kMasked);
+    }
+  };
+  tiles(min(k1, first_limit + 1) - kTileKeys + 1, std::false_type{});
+  tiles(k1, std::true_type{});
 
   // ---- the waves' results joined, one block of 16 rows at a time
 #pragma unroll
@@ -275,7 +318,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
     }
     const bool some = lt > 0.f || lt != lt;
     const float inv = some ? 1.f / lt : 0.f;
-    const f32x2 lse2 = gqa_lse(some, mt, log2f(lt * kRoom));
+    const f32x2 lse2 = gqa_lse(some, mt - kRoom, log2f(lt * 0x1p24f));
     const int r = it.block * kRows + 16 * nb + row, tok = r / G, head = it.head * G + r % G;
 #pragma unroll
     for (int c = tok < E ? x : D; c < D / 4; c += kTpr) {
@@ -321,26 +364,43 @@ __global__ __launch_bounds__(256) void mx4_pages_kernel(const GqaMx4Params mp) {
     }
   }
   if (b < 0) return;
-  const int page = (int)blockIdx.x - first;
-  if (threadIdx.x == 0 && blockIdx.y == 0) mp.scratch_table[(int64_t)b * mp.scratch_cols + page] = (int)blockIdx.x;
-  const int head = blockIdx.y;
-  for (int i = threadIdx.x; i < 64 * kLanes * 2; i += 256) {
-    const int x = i % kLanes, t = i / kLanes % 64, j = 64 * page + t;
-    const bool v = i >= 64 * kLanes;
-    if (j >= L) continue;
-    const int row = gqa_row(p, b, 0, j);
-    const int64_t pg = row >> p.log2_ps, tok = row & ((1 << p.log2_ps) - 1);
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>((v ? mp.v_codes : mp.k_codes) + pg * mp.c_page + tok * mp.c_tok + head * mp.c_head + 4 * x);
-    const uint32_t scale = (v ? mp.v_scales : mp.k_scales)[pg * mp.s_page + tok * mp.s_tok + head * mp.s_head + x / 4];
-    const int64_t at = ((int64_t)head * mp.scratch_rows + (int64_t)blockIdx.x * 64 + t) * D + 8 * x;
-    *reinterpret_cast<u32x4*>((v ? mp.scratch_v : mp.scratch_k) + at) = mx4_values(codes, scale << 23);
+  const int page = (int)blockIdx.x - first, head = blockIdx.y;
+  if (threadIdx.x == 0 && head == 0) mp.scratch_table[(int64_t)b * mp.scratch_cols + page] = (int)blockIdx.x;
+  constexpr int kRowsAtOnce = 256 / kLanes, kN = 64 / kRowsAtOnce;
+  const int x = threadIdx.x % kLanes, t0 = threadIdx.x / kLanes;
+  int64_t pg[kN], tok[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const int row = gqa_row(p, b, 0, min(64 * page + t0 + i * kRowsAtOnce, L - 1));
+    pg[i] = row >> p.log2_ps;
+    tok[i] = row & ((1 << p.log2_ps) - 1);
   }
+  uint32_t codes[kN][2], scales[kN][2];
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      codes[i][v] = *reinterpret_cast<const uint32_t*>((v ? mp.v_codes : mp.k_codes) + pg[i] * mp.c_page + tok[i] * mp.c_tok + head * mp.c_head + 4 * x);
+      scales[i][v] = (v ? mp.v_scales : mp.k_scales)[pg[i] * mp.s_page + tok[i] * mp.s_tok + head * mp.s_head + x / 4];
+    }
+  // (rows past the request's last in its last page are its last again: nothing reads them)
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const int64_t at = ((int64_t)head * mp.scratch_rows + (int64_t)blockIdx.x * 64 + t0 + i * kRowsAtOnce) * D + 8 * x;
+      *reinterpret_cast<u32x4*>((v ? mp.scratch_v : mp.scratch_k) + at) = mx4_values(codes[i][v], scales[i][v] << 23);
+    }
 }
 
+template <int D, int NB, bool kBig>
+void launch_stream(const GqaMx4Params& p, int64_t grid, hipStream_t stream) {
+  if (p.g.wide) hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 8, kBig>), dim3((unsigned)grid), dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 4, kBig>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+}
 template <int D, int NB>
 void launch_stream(const GqaMx4Params& p, int64_t grid, hipStream_t stream) {
-  if (p.g.wide) hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 8>), dim3((unsigned)grid), dim3(512), 0, stream, p);
-  else hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 4>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+  p.g.log2_ps >= 5 ? launch_stream<D, NB, true>(p, grid, stream) : launch_stream<D, NB, false>(p, grid, stream);
 }
 
 }  // namespace

@@ -14,13 +14,13 @@ struct Piece {
   bool v;
 };
 template <int D>
-__device__ __forceinline__ Piece mx4_piece(const Mx4Rows& p, int64_t i) {
+__device__ __forceinline__ Piece mx4_piece(const Mx4Rows& p, uint32_t i) {
   constexpr int kLanes = D / 8;
   Piece r;
   r.x = (int)(i % kLanes);
-  const int64_t row = i / kLanes;
-  const int h = (int)(row % (2 * p.kv_heads));
-  r.t = (int)(row / (2 * p.kv_heads));
+  const uint32_t row = i / kLanes, heads = 2 * p.kv_heads;
+  r.t = (int)(row / heads);
+  const int h = (int)(row - r.t * heads);
   r.v = h >= p.kv_heads;
   r.head = r.v ? h - p.kv_heads : h;
   return r;
@@ -32,8 +32,8 @@ __device__ __forceinline__ int64_t mx4_index(const Mx4Rows& p, int t) {
 
 template <int D>
 __global__ __launch_bounds__(256) void mx4_store_kernel(const Mx4Rows p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)p.rows * 2 * p.kv_heads * (D / 8)) return;  // whole rows: a block's four lanes leave together
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;  // 32 bits by the host
+  if (i >= (uint32_t)p.rows * 2 * p.kv_heads * (D / 8)) return;  // whole rows: a block's four lanes leave together
   const Piece c = mx4_piece<D>(p, i);
   const int64_t row = mx4_index(p, c.t);
   const __bf16* in = c.v ? p.v + (int64_t)c.t * p.v_stride_t + (int64_t)c.head * p.v_stride_h
@@ -63,8 +63,8 @@ __global__ __launch_bounds__(256) void mx4_store_kernel(const Mx4Rows p) {
 
 template <int D>
 __global__ __launch_bounds__(256) void mx4_load_kernel(const Mx4Rows p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)p.rows * 2 * p.kv_heads * (D / 8)) return;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;  // 32 bits by the host
+  if (i >= (uint32_t)p.rows * 2 * p.kv_heads * (D / 8)) return;
   const Piece c = mx4_piece<D>(p, i);
   const int64_t row = mx4_index(p, c.t);
   u32x4 w{};

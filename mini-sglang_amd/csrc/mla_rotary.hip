@@ -41,9 +41,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRopeParam
   constexpr int kLanes = D / 8, kRows = 64 / kLanes, kStep = kRows * U;
   const int lane = threadIdx.x & 63, x = lane % kLanes;
   const int heads = p.q_heads + p.kv_heads, rows = heads + (p.v != nullptr ? p.kv_heads : 0);
-  const int groups = (rows + kStep - 1) / kStep;
-  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= (int64_t)p.tokens * groups) return;
+  const uint32_t groups = (rows + kStep - 1) / kStep;  // waves of a token
+  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= p.tokens * groups) return;
   const int t = (int)(item / groups), r0 = (int)(item % groups) * kStep + lane / kLanes;
   int64_t slot = t;
   if (p.slots != nullptr) slot = p.index_bits == 32 ? ((const int32_t*)p.slots)[t] : ((const int64_t*)p.slots)[t];
@@ -110,8 +110,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRopeParam
     __bf16* out = r < p.q_heads ? p.q_out + (int64_t)t * p.qo_stride_t + (int64_t)r * p.qo_stride_h
                   : r < heads   ? p.k_out + slot * p.ko_stride_row + (int64_t)(r - p.q_heads) * p.ko_stride_h
                                 : p.v_out + slot * p.vo_stride_row + (int64_t)(r - heads) * p.vo_stride_h;
-    *reinterpret_cast<u32x2*>(out + a) = xa[u];
-    *reinterpret_cast<u32x2*>(out + b) = xb[u];
+    if constexpr (U == 1) {
+      *reinterpret_cast<u32x2*>(out + a) = xa[u];
+      *reinterpret_cast<u32x2*>(out + b) = xb[u];
+    } else {
+      __builtin_nontemporal_store(xa[u], reinterpret_cast<u32x2*>(out + a));
+      __builtin_nontemporal_store(xb[u], reinterpret_cast<u32x2*>(out + b));
+    }
   }
 }
 
@@ -119,11 +124,23 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRopeParam
 
 hipError_t launch_qk_norm_rope(const QkNormRopeParams& p, int dim, hipStream_t stream) {
   const int rows = p.q_heads + p.kv_heads + (p.v != nullptr ? p.kv_heads : 0);
-  const int step = 512 / dim;
-  const int64_t items = (int64_t)p.tokens * ((rows + step - 1) / step);
-  const dim3 grid((unsigned)((items + 3) / 4));
-  if (dim == 128) hipLaunchKernelGGL((qk_norm_rope_kernel<128, 1>), grid, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((qk_norm_rope_kernel<64, 1>), grid, dim3(256), 0, stream, p);
+  // Rows of a lane: one while all waves run at once, more where their loads should be in flight together. us for 1 / 2 / 4, 64
+  // and 8 heads of 128 with V: 128 tokens (2560 waves of one row) 3.7 / 4.0 / 4.8; 256 4.5 / 4.4 / 5.1; 2048 20.4 / 16.0 / 16.0;
+  // 8192 (163840) 88 / 66.9 / 63.4. Non-temporal stores with more than one: 68.8 and 66.6 without. (Loads stay temporal: a
+  // projection's output lies in the caches; 2048 tokens 16.0, 19.9 with non-temporal ones.)
+  const int step = 512 / dim;  // rows of a wave
+  const int64_t waves = (int64_t)p.tokens * ((rows + step - 1) / step);
+  const int u = waves <= 4096 ? 1 : waves <= 98304 ? 2 : 4;
+  const dim3 grid((unsigned)(((int64_t)p.tokens * ((rows + step * u - 1) / (step * u)) + 3) / 4));
+#define MLA_ROTARY(D, U) \
+  if (dim == D && u == U) hipLaunchKernelGGL((qk_norm_rope_kernel<D, U>), grid, dim3(256), 0, stream, p);
+  MLA_ROTARY(64, 1)
+  MLA_ROTARY(64, 2)
+  MLA_ROTARY(64, 4)
+  MLA_ROTARY(128, 1)
+  MLA_ROTARY(128, 2)
+  MLA_ROTARY(128, 4)
+#undef MLA_ROTARY
   return hipGetLastError();
 }
 

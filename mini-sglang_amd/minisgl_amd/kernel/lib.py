@@ -734,19 +734,11 @@ def mx4_store(k_pool: MX4Pool, v_pool: MX4Pool, indices, k, v, stream=None) -> N
 
 def mx4_load(k_pool: MX4Pool, v_pool: MX4Pool, indices, k=None, v=None, stream=None):
     """The values of token rows ``indices [T]`` as bf16 ``k``, ``v [T, Hkv, D]`` (exact; 0 for indices outside the pools)."""
-    import torch
-
-    rows, (_, _, heads, width) = indices.shape[0], k_pool.codes.shape
-
-    def made():
-        return _made(stream, lambda: torch.empty((rows, heads, 2 * width), dtype=torch.bfloat16, device=k_pool.codes.device))
-
-    k, v = made() if k is None else k, made() if v is None else v
     call = load_binding().mx4_load
-    rc = call(*k_pool, *v_pool, indices, k, v, stream)
-    if rc != 0:
-        _again(rc, k.device, call, "mla_mx4_load", *k_pool, *v_pool, indices, k, v, stream)
-    return k, v
+    got = call(*k_pool, *v_pool, indices, k, v, stream)
+    if isinstance(got, int):
+        got = _again(got, indices.device, call, "mla_mx4_load", *k_pool, *v_pool, indices, k, v, stream)
+    return got
 
 
 def gqa_mx4_workspace_bytes(max_seqlen_q: int, q_heads: int, kv_heads: int, head_dim: int, batch: int, max_keys: int,
@@ -762,7 +754,7 @@ def gqa_mx4_workspace_bytes(max_seqlen_q: int, q_heads: int, kv_heads: int, head
 def gqa_chunk_mx4(q, k_pool: MX4Pool, v_pool: MX4Pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q: int, scale: float, out,
                   lse=None, workspace=None, total_keys: int | None = None, stream=None) -> None:
     """``gqa_chunk`` over pools of 4 bits. ``total_keys``: at least the sum of ``seq_lens_k`` (the host's; None: all that the page
-    table can hold), which bounds the memory where chunks of more than 32 rows (tokens times ``Hq // Hkv``) have their keys'
+    table can hold), which bounds the memory where chunks of more than 512 rows (tokens times ``Hq // Hkv``) have their keys'
     values laid out in bf16. ``workspace``: uint8, of ``gqa_mx4_workspace_bytes``, or None."""
     assert cu_seqlens_q is not None, "cu_seqlens_q is [B + 1]"
     call = load_binding().gqa_paged_mx4

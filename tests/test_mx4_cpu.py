@@ -105,14 +105,14 @@ def test_empty_calls_do_nothing():
 
 
 def test_workspace_bytes():
-    """Partial results alone for up to 32 rows a request; past that the values of total_keys keys and a table, not more than the
+    """Partial results alone for up to 512 rows a request; past that the values of total_keys keys and a table, not more than the
     page table holds, and never less for more."""
-    assert lib.gqa_mx4_workspace_bytes(1, 32, 1, 128, 100, 1 << 17, 1 << 24) == lib.gqa_workspace_bytes(1, 32, 1, 128)
-    at = lib.gqa_mx4_workspace_bytes(5, 64, 8, 128, 4, 8192, 20000)
-    split = lib.gqa_workspace_bytes(5, 64, 8, 128)
+    assert lib.gqa_mx4_workspace_bytes(16, 32, 1, 128, 100, 1 << 17, 1 << 24) == lib.gqa_workspace_bytes(16, 32, 1, 128)
+    at = lib.gqa_mx4_workspace_bytes(65, 64, 8, 128, 4, 8192, 20000)
+    split = lib.gqa_workspace_bytes(65, 64, 8, 128)
     assert split + 2 * 20000 * 8 * 128 * 2 <= at <= split + 4 * 4 * 128 + 2 * (20000 + 4 * 64) * 8 * 128 * 2
-    assert lib.gqa_mx4_workspace_bytes(5, 64, 8, 128, 4, 8192, 1 << 40) == lib.gqa_mx4_workspace_bytes(5, 64, 8, 128, 4, 8192, 4 * 8192)
-    assert at <= lib.gqa_mx4_workspace_bytes(6, 64, 8, 128, 4, 8192, 20000) and at <= lib.gqa_mx4_workspace_bytes(5, 64, 8, 128, 5, 8192, 20001)
+    assert lib.gqa_mx4_workspace_bytes(65, 64, 8, 128, 4, 8192, 1 << 40) == lib.gqa_mx4_workspace_bytes(65, 64, 8, 128, 4, 8192, 4 * 8192)
+    assert at <= lib.gqa_mx4_workspace_bytes(66, 64, 8, 128, 4, 8192, 20000) and at <= lib.gqa_mx4_workspace_bytes(65, 64, 8, 128, 5, 8192, 20001)
     for bad in ((-1, 8, 2, 128, 1, 1, 1), (1, 8, 3, 128, 1, 1, 1), (1, 8, 2, 96, 1, 1, 1), (1, 8, 2, 128, -1, 1, 1), (1, 8, 2, 128, 1, -1, 1), (1, 8, 2, 128, 1, 1, -1)):
         with pytest.raises(lib.MLAKernelError):
             lib.gqa_mx4_workspace_bytes(*bad)
