@@ -125,9 +125,10 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   auto scale_at = [](uint32_t w, int b) __attribute__((always_inline)) { return D == 128 ? __builtin_amdgcn_alignbit(w, w, (8 * b + 9) & 31) : w >> 8 * b << 23; };
   constexpr int kLanesB = 32 / (D / 16);  // lanes n of a block of V
 
-  // kMasked: some row does not attend some key of the tile
-  auto step = [&](int t0, auto kMasked) __attribute__((always_inline)) {
-    f32x4 sc[NB][2];
+  // kMasked: some row does not attend some key of the tile. The item's first `active` blocks of rows have rows.
+  auto step = [&](int t0, auto kMasked, auto active) __attribute__((always_inline)) {
+    constexpr int kAct = decltype(active)::value;
+    f32x4 sc[kAct][2];
     kword_t kw[2];
     uint32_t ks[2];
 #pragma unroll
@@ -142,12 +143,12 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
       for (int h = 0; h < 2; ++h) {
         const bf16x8 kc = __builtin_bit_cast(bf16x8, mx4_values(kw[h][s], ks[h]));
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < kAct; ++nb)
           sc[nb][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc, qf[nb][s], s == 0 ? f32x4{} : sc[nb][h], 0, 0, 0);
       }
-    float e[NB][2][4];  // numerators
+    u32x4 pb[kAct];  // numerators of a row, in pairs of keys
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+    for (int nb = 0; nb < kAct; ++nb) {
       // the scaled scores are rounded before their maximum is taken from them: the largest numerator is 2^-24 at any size
 #pragma clang fp contract(off)
       f32x4(&s)[2] = sc[nb];
@@ -171,12 +172,16 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
         for (int db = 0; db < kDb; ++db) O[nb][db] *= f;
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[nb][h][i] = __builtin_amdgcn_exp2f(s[h][i] - m[nb]);
-          l[nb] += e[nb][h][i];
+          e[i] = __builtin_amdgcn_exp2f(s[h][i] - m[nb]);
+          l[nb] += e[i];
         }
+        pb[nb][2 * h] = pack_bf16x2(e[0], e[1]);
+        pb[nb][2 * h + 1] = pack_bf16x2(e[2], e[3]);
+      }
     }
     vword_t vw[2][4];
     scale_t sw[2][4];
@@ -197,7 +202,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
         for (int i = 0; i < 4; ++i) any |= any_ff(sw[h][i]);
       if (__ballot(any != 0) != 0) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
+        for (int nb = 0; nb < kAct; ++nb) {
           const int lim = min(limit[nb], k1 - 1) - t0 - 4 * g;
           uint32_t hit = 0;  // bit 7 of byte b: of block b, at a key of the lane's that row a16 attends
 #pragma unroll
@@ -245,15 +250,9 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
               hi[2 * h + i] = __builtin_amdgcn_perm(y, x, 0x07060302);
             }
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            u32x4 pb;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              pb[2 * h] = pack_bf16x2(e[nb][h][0], e[nb][h][1]);
-              pb[2 * h + 1] = pack_bf16x2(e[nb][h][2], e[nb][h][3]);
-            }
-            mfma(lo, pb, O[nb][2 * kC]);
-            mfma(hi, pb, O[nb][2 * kC + 1]);
+          for (int nb = 0; nb < kAct; ++nb) {
+            mfma(lo, pb[nb], O[nb][2 * kC]);
+            mfma(hi, pb[nb], O[nb][2 * kC + 1]);
           }
       }
     };
@@ -270,7 +269,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
     row_next = rows(t0 + kStep);
     load(t0, row);
   }
-  auto tiles = [&](int end, auto kMasked) __attribute__((always_inline)) {
+  auto tiles = [&](int end, auto kMasked, auto active) __attribute__((always_inline)) {
     for (; t0 < end; t0 += kStep) {
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
@@ -281,11 +280,15 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
       (lane < 32 ? tile.ks : tile.vs)[lane & 31] = sr;
       if (t0 + kStep < k1) load(t0 + kStep, row_next);
       if (t0 + 2 * kStep < k1) row_next = rows(t0 + 2 * kStep);
-      step(t0, kMasked);
+      step(t0, kMasked, active);
     }
   };
-  tiles(min(k1, first_limit + 1) - kTileKeys + 1, std::false_type{});
-  tiles(k1, std::true_type{});
+  auto stream = [&](auto active) __attribute__((always_inline)) {
+    tiles(min(k1, first_limit + 1) - kTileKeys + 1, std::false_type{}, active);
+    tiles(k1, std::true_type{}, active);
+  };
+  if (NB == 1 || it.block * kRows + 16 < E * G) stream(std::integral_constant<int, NB>{});
+  else stream(std::integral_constant<int, 1>{});
 
   // ---- the waves' results joined, one block of 16 rows at a time
 #pragma unroll
