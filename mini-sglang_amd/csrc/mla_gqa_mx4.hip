@@ -21,11 +21,16 @@ namespace {
 
 constexpr int kTileKeys = 32;
 constexpr float kLowest = -3.4028234663852886e38f;
-// References are 24 above the largest score (log2 domain), so numerators at most 2^-24: sums of 2^24 values of the largest
-// size (6 2^125) stay in fp32's range
+// Numerators are relative to a reference that a row's largest score (log2 domain) may pass by kLag before it follows: sums are
+// rescaled seldom (16 drafts of 1 to 8 on 1k to 16k, 32 and 8 heads: 40.0 us with 0, 37.3).
+constexpr float kLag = 6.f;
+// Once a wave has seen values of 2^101 and more (scales from kLarge), its references are kRoom higher: sums of 2^18 values of
+// the largest size, 6 2^125, stay in fp32's range. Smaller ones need no such room (and the smallest would fall out of the range).
 constexpr float kRoom = 24.f;
-
+constexpr uint32_t kLarge = 228;
+// whether a byte of w is 255; at least kLarge
 __device__ __forceinline__ uint32_t any_ff(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+__device__ __forceinline__ uint32_t any_large(uint32_t w) { return ((w & 0x7f7f7f7fu) + (256 - kLarge) * 0x01010101u) & w & 0x80808080u; }
 
 // NB blocks of 16 rows, NW waves. kBig: pages of 32 tokens or more, so that a tile lies in one page and its addresses are
 // the wave's (scalar), where they are a lane's otherwise.
@@ -71,7 +76,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   const int k0 = it.piece * C, k1 = min(it.pieces > 1 ? k0 + C : L, P + last_tok + 1);
 
   f32x4 O[NB][kDb];
-  float m[NB], l[NB];
+  float m[NB], l[NB], room = 0.f;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     m[nb] = kLowest;
@@ -149,7 +154,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
     u32x4 pb[kAct];  // numerators of a row, in pairs of keys
 #pragma unroll
     for (int nb = 0; nb < kAct; ++nb) {
-      // the scaled scores are rounded before their maximum is taken from them: the largest numerator is 2^-24 at any size
+      // the scaled scores are rounded before their maximum is taken from them: the largest numerator is 1 to 2^kLag at any size
 #pragma clang fp contract(off)
       f32x4(&s)[2] = sc[nb];
       // score (h, i) of a lane: row a16, key t0 + 16 h + 4 g + i
@@ -163,8 +168,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
           if (decltype(kMasked)::value && 16 * h + i > lim) s[h][i] = -INFINITY;
           top = fmaxf(top, s[h][i]);
         }
-      top = wave_max_g(top) + kRoom;
-      if (__ballot(top > m[nb]) != 0) {
+      top = wave_max_g(top) + room;
+      if (__ballot(top > m[nb] + kLag) != 0) {
         const float m_new = fmaxf(m[nb], top), f = __builtin_amdgcn_exp2f(m[nb] - m_new);
         m[nb] = m_new;
         l[nb] *= f;
@@ -278,6 +283,16 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
         *reinterpret_cast<u32x4*>(tile.v + vpos(t) + lane % kLanes * 16) = vr[u];
       }
       (lane < 32 ? tile.ks : tile.vs)[lane & 31] = sr;
+      if (__builtin_expect(__ballot(lane >= 32 && any_large(sr) != 0) != 0, 0) && room == 0.f) {
+        room = kRoom;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          m[nb] += kRoom;
+          l[nb] *= 0x1p-24f;
+#pragma unroll
+          for (int db = 0; db < kDb; ++db) O[nb][db] *= 0x1p-24f;
+        }
+      }
       if (t0 + kStep < k1) load(t0 + kStep, row_next);
       if (t0 + 2 * kStep < k1) row_next = rows(t0 + 2 * kStep);
       step(t0, kMasked, active);
@@ -321,7 +336,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
     }
     const bool some = lt > 0.f || lt != lt;
     const float inv = some ? 1.f / lt : 0.f;
-    const f32x2 lse2 = gqa_lse(some, mt - kRoom, log2f(lt * 0x1p24f));
+    const f32x2 lse2 = gqa_lse(some, mt, log2f(lt));
     const int r = it.block * kRows + 16 * nb + row, tok = r / G, head = it.head * G + r % G;
 #pragma unroll
     for (int c = tok < E ? x : D; c < D / 4; c += kTpr) {

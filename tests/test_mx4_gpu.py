@@ -175,12 +175,12 @@ class Paged:
             whole.view(-1, *whole.shape[2:])[rows] = some
 
     def ref(self):
-        """The bounds hold while numerators are bf16's normal numbers, 2^-126 at least. They are times 2^-24 (room for sums of
-        the largest values), so one below 2^-102 of the row's largest may come out as anything from 0 to twice itself: such
-        keys, fewer than L, bring an error of at most 2^-102 L max |v| together (the sum of numerators is 1 at least)."""
+        """The bounds of oracle/ref_gqa.py are for sums within fp32's normal range. A numerator below it, 2^-126, may come out as
+        anything up to twice itself, and so may its product with a value: at most L of each, over a sum of numerators that is at
+        least 1 (the largest's), bring 2^-126 L (max |v| + 1) to a result."""
         v = M.values(*self.v)
         ref = R.chunk(self.q, M.values(*self.k), v, self.pt, self.extends, self.lens, self.scale)
-        return ref._replace(out_bound=ref.out_bound + 2.0 ** -102 * max(self.lens) * v.nan_to_num().abs().max())
+        return ref._replace(out_bound=ref.out_bound + 2.0 ** -126 * max(self.lens) * (v.nan_to_num(posinf=0.0, neginf=0.0).abs().max() + 1))
 
     def run(self, max_q=None, workspace=None, total_keys=-1, decode=False):
         q = self.q.to(DEV)
@@ -206,7 +206,7 @@ def test_decode_heads(dim, heads):
 
 @pytest.mark.parametrize("by_head", [False, True])
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("page_size", [1, 2, 8, 64, 256])
+@pytest.mark.parametrize("page_size", [1, 2, 8, 16, 32, 64, 256])
 def test_decode_pages(dim, page_size, by_head):
     c = Paged([1] * 7, [0, 1, 62, 63, 64, 300, 1999], 8, 2, dim, page_size, page_size + dim, by_head=by_head)
     check(*c.run(decode=True), c.ref())
@@ -284,16 +284,58 @@ def test_nan_reaches_rows_that_attend_it(dim, extends, prefixes):
         assert over.max() <= 0, what
 
 
-def test_largest_values():
+@pytest.mark.parametrize("extends,prefixes", [([1, 1], [3000, 70]), ([3, 20], [200, 100]), ([140], [1000])])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_largest_values(dim, extends, prefixes):
     """Sums on the way to a result pass fp32's range unless the numerators leave room."""
-    c = Paged([1, 1], [3000, 70], 4, 2, 128, 16, 12, scale=2.0 ** -30)  # weights alike
-    for pool in (c.v,):
-        pool[0].fill_(0x77)  # 6 and 6
-        pool[1].fill_(252)
-    out, lse = c.run(decode=True)
+    c = Paged(extends, prefixes, 4, 2, dim, 16, 12, scale=2.0 ** -30)  # weights alike
+    c.v[0].fill_(0x77)  # 6 and 6
+    c.v[1].fill_(252)
+    out, lse = c.run()
     want = torch.tensor(6 * 2.0 ** 125, dtype=torch.float64)
     # 2^-8 for the numerators and for the result
     assert ((out.double().cpu() - want).abs() <= 2.02 * 2.0 ** -8 * want).all()
+    assert ((lse.double().cpu() - c.ref().lse).abs() <= c.ref().lse_bound + 2.0 ** -19).all()  # a sum of 24 and more, rounded
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("order", ["falling", "rising"])
+def test_values_of_every_size(dim, order):
+    """Blocks from next to the largest to the smallest that a result can hold, by token: in tiles before and after one another."""
+    c = Paged([1, 40], [700, 300], 4, 2, dim, 32, 14, scale=1.0)
+    gen = torch.Generator().manual_seed(15)
+    for b, L in enumerate(c.lens):
+        for j in range(L):
+            e = 122 - (240 * j) // L if order == "falling" else -118 + (240 * j) // L
+            c.put(c.v, b, [j], (torch.randn((1, 2, dim), generator=gen).clamp(-8, 8) * 2.0 ** e).to(torch.bfloat16))
+    check(*c.run(), c.ref())
+
+
+@pytest.mark.parametrize("size", [2.0 ** -120, 2.0 ** -60, 2.0 ** 60, 2.0 ** 120])
+def test_values_of_a_size(size):
+    c = Paged([1, 9], [2000, 100], 8, 2, 128, 64, 16)
+    gen = torch.Generator().manual_seed(17)
+    for b, L in enumerate(c.lens):
+        c.put(c.v, b, range(L), (torch.randn((L, 2, 128), generator=gen).clamp(-8, 8) * size).to(torch.bfloat16))
+    check(*c.run(), c.ref())
+
+
+def test_pages_and_lengths_outside():
+    """Page ids outside the pool are taken as its first and last page, lengths past the page table as its width, and queries past
+    total_q are left out: what the arrays hold is never followed out of the tensors."""
+    c = Paged([1, 1, 1], [90, 40, 20], 4, 2, 128, 32, 18)
+    pages = c.pt.shape[1]
+    c.v[0].copy_(torch.randint(0, 256, c.v[0].shape, generator=torch.Generator().manual_seed(1), dtype=torch.uint8))
+    c.k[1].fill_(126)
+    c.v[1].fill_(127)
+    c.pt[0, 1], c.pt[1, 0], c.pt[2, 0] = 1 << 30, -(1 << 31), c.k[0].shape[0]
+    given = list(c.lens)
+    c.lens[2] = 1 << 30
+    c.pt[2, 1:] = -1
+    out, lse = c.run(decode=True, total_keys=1000)
+    c.pt.clamp_(0, c.k[0].shape[0] - 1)
+    c.lens = given[:2] + [pages * 32]
+    check(out, lse, c.ref())
 
 
 @pytest.mark.parametrize("scale", [1e-6, 3.0, 100.0])
