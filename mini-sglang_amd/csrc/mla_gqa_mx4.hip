@@ -24,13 +24,13 @@ constexpr float kLowest = -3.4028234663852886e38f;
 // Numerators are relative to a reference that a row's largest score (log2 domain) may pass by kLag before it follows: sums are
 // rescaled seldom (16 drafts of 1 to 8 on 1k to 16k, 32 and 8 heads: 40.0 us with 0, 37.3).
 constexpr float kLag = 6.f;
-// Once a wave has seen values of 2^101 and more (scales from kLarge), its references are kRoom higher: sums of 2^18 values of
-// the largest size, 6 2^125, stay in fp32's range. Smaller ones need no such room (and the smallest would fall out of the range).
+// A wave whose sums of values did not come out finite takes its keys again with numerators times 2^-kRoom: sums of 2^18 values of
+// the largest size, 6 2^125, stay in fp32's range then, and what is not finite now is the result. (Smaller values would fall
+// out of the range at the other end, and what tells large ones apart costs every tile 5 %.) The factor is kept beside the
+// reference: a far score's spacing is more than kRoom.
 constexpr float kRoom = 24.f;
-constexpr uint32_t kLarge = 228;
-// whether a byte of w is 255; at least kLarge
+// whether a byte of w is 255
 __device__ __forceinline__ uint32_t any_ff(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
-__device__ __forceinline__ uint32_t any_large(uint32_t w) { return ((w & 0x7f7f7f7fu) + (256 - kLarge) * 0x01010101u) & w & 0x80808080u; }
 
 // NB blocks of 16 rows, NW waves. kBig: pages of 32 tokens or more, so that a tile lies in one page and its addresses are
 // the wave's (scalar), where they are a lane's otherwise.
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
     char o[16 * D * 4];  // a block's outputs at the end, fp32 [16 rows][D]
   };
   __shared__ __attribute__((aligned(16))) Own s_own[NW];
-  __shared__ float s_m[NW][16], s_l[NW][16];
+  __shared__ float s_m[NW][16], s_l[NW][16], s_room[NW];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GqaItem it;
@@ -76,14 +76,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   const int k0 = it.piece * C, k1 = min(it.pieces > 1 ? k0 + C : L, P + last_tok + 1);
 
   f32x4 O[NB][kDb];
-  float m[NB], l[NB], room = 0.f;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    m[nb] = kLowest;
-    l[nb] = 0.f;
-#pragma unroll
-    for (int db = 0; db < kDb; ++db) O[nb][db] = f32x4{};
-  }
+  float m[NB], l[NB];
   u32x4 kr[kLoads], vr[kLoads];
   scale_t sr{};
   // What a tile's addresses come from, read a tile ahead: the page's id (rows past the length in a page are read, and left
@@ -131,7 +124,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   constexpr int kLanesB = 32 / (D / 16);  // lanes n of a block of V
 
   // kMasked: some row does not attend some key of the tile. The item's first `active` blocks of rows have rows.
-  auto step = [&](int t0, auto kMasked, auto active) __attribute__((always_inline)) {
+  auto step = [&](int t0, auto kMasked, auto active, auto roomy) __attribute__((always_inline)) {
     constexpr int kAct = decltype(active)::value;
     f32x4 sc[kAct][2];
     kword_t kw[2];
@@ -168,7 +161,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
           if (decltype(kMasked)::value && 16 * h + i > lim) s[h][i] = -INFINITY;
           top = fmaxf(top, s[h][i]);
         }
-      top = wave_max_g(top) + room;
+      top = wave_max_g(top);
       if (__ballot(top > m[nb] + kLag) != 0) {
         const float m_new = fmaxf(m[nb], top), f = __builtin_amdgcn_exp2f(m[nb] - m_new);
         m[nb] = m_new;
@@ -182,6 +175,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           e[i] = __builtin_amdgcn_exp2f(s[h][i] - m[nb]);
+          if constexpr (decltype(roomy)::value) e[i] *= 0x1p-24f;
           l[nb] += e[i];
         }
         pb[nb][2 * h] = pack_bf16x2(e[0], e[1]);
@@ -267,43 +261,51 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
     products(std::integral_constant<int, 3>{});
   };
 
-  constexpr int kStep = NW * kTileKeys;
-  int t0 = k0 + kTileKeys * wave, row_next = 0;
-  if (t0 < k1) {
-    const int row = rows(t0);
-    row_next = rows(t0 + kStep);
-    load(t0, row);
-  }
-  auto tiles = [&](int end, auto kMasked, auto active) __attribute__((always_inline)) {
-    for (; t0 < end; t0 += kStep) {
+  auto stream = [&](auto active, auto roomy) __attribute__((always_inline)) {
+    constexpr int kStep = NW * kTileKeys;
 #pragma unroll
-      for (int u = 0; u < kLoads; ++u) {
-        const int t = u * (64 / kLanes) + lane / kLanes;
-        *reinterpret_cast<u32x4*>(tile.k + kpos(t, lane % kLanes)) = kr[u];
-        *reinterpret_cast<u32x4*>(tile.v + vpos(t) + lane % kLanes * 16) = vr[u];
-      }
-      (lane < 32 ? tile.ks : tile.vs)[lane & 31] = sr;
-      if (__builtin_expect(__ballot(lane >= 32 && any_large(sr) != 0) != 0, 0) && room == 0.f) {
-        room = kRoom;
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb] = kLowest;
+      l[nb] = 0.f;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          m[nb] += kRoom;
-          l[nb] *= 0x1p-24f;
-#pragma unroll
-          for (int db = 0; db < kDb; ++db) O[nb][db] *= 0x1p-24f;
-        }
-      }
-      if (t0 + kStep < k1) load(t0 + kStep, row_next);
-      if (t0 + 2 * kStep < k1) row_next = rows(t0 + 2 * kStep);
-      step(t0, kMasked, active);
+      for (int db = 0; db < kDb; ++db) O[nb][db] = f32x4{};
     }
+    int t0 = k0 + kTileKeys * wave, row_next = 0;
+    if (t0 < k1) {
+      const int row = rows(t0);
+      row_next = rows(t0 + kStep);
+      load(t0, row);
+    }
+    auto tiles = [&](int end, auto kMasked) __attribute__((always_inline)) {
+      for (; t0 < end; t0 += kStep) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+          const int t = u * (64 / kLanes) + lane / kLanes;
+          *reinterpret_cast<u32x4*>(tile.k + kpos(t, lane % kLanes)) = kr[u];
+          *reinterpret_cast<u32x4*>(tile.v + vpos(t) + lane % kLanes * 16) = vr[u];
+        }
+        (lane < 32 ? tile.ks : tile.vs)[lane & 31] = sr;
+        if (t0 + kStep < k1) load(t0 + kStep, row_next);
+        if (t0 + 2 * kStep < k1) row_next = rows(t0 + 2 * kStep);
+        step(t0, kMasked, active, roomy);
+      }
+    };
+    tiles(min(k1, first_limit + 1) - kTileKeys + 1, std::false_type{});
+    tiles(k1, std::true_type{});
   };
-  auto stream = [&](auto active) __attribute__((always_inline)) {
-    tiles(min(k1, first_limit + 1) - kTileKeys + 1, std::false_type{}, active);
-    tiles(k1, std::true_type{}, active);
-  };
-  if (NB == 1 || it.block * kRows + 16 < E * G) stream(std::integral_constant<int, NB>{});
-  else stream(std::integral_constant<int, 1>{});
+  if (NB == 1 || it.block * kRows + 16 < E * G) stream(std::integral_constant<int, NB>{}, std::false_type{});
+  else stream(std::integral_constant<int, 1>{}, std::false_type{});
+  float zero = 0.f, room = 0.f;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int db = 0; db < kDb; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zero = fmaf(O[nb][db][i], 0.f, zero);  // finite sums times 0 are 0
+  if (__builtin_expect(__ballot(zero != 0.f) != 0, 0)) {
+    room = kRoom;
+    stream(std::integral_constant<int, NB>{}, std::true_type{});
+  }
 
   // ---- the waves' results joined, one block of 16 rows at a time
 #pragma unroll
@@ -321,22 +323,26 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
       s_m[wave][a16] = m[nb];
       s_l[wave][a16] = lw;
     }
+    if (lane == 0) s_room[wave] = room;
     __syncthreads();
     // kTpr threads a row, 4 dims each at a time
     constexpr int kTpr = 4 * NW;
     const int row = threadIdx.x / kTpr, x = threadIdx.x % kTpr;
-    float mt = s_m[0][row];
+    float mt = s_m[0][row], rt = s_room[0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) mt = fmaxf(mt, s_m[w][row]);
+    for (int w = 1; w < NW; ++w) {
+      mt = fmaxf(mt, s_m[w][row]);
+      rt = fmaxf(rt, s_room[w]);
+    }
     float f[NW], lt = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      f[w] = __builtin_amdgcn_exp2f(s_m[w][row] - mt);
+      f[w] = __builtin_amdgcn_exp2f(s_m[w][row] - mt) * __builtin_amdgcn_exp2f(s_room[w] - rt) * 0x1p-4f;  // their sum is finite too
       lt += f[w] * s_l[w][row];
     }
     const bool some = lt > 0.f || lt != lt;
     const float inv = some ? 1.f / lt : 0.f;
-    const f32x2 lse2 = gqa_lse(some, mt, log2f(lt));
+    const f32x2 lse2 = gqa_lse(some, mt, log2f(lt * (__builtin_amdgcn_exp2f(rt) * 0x1p4f)));
     const int r = it.block * kRows + 16 * nb + row, tok = r / G, head = it.head * G + r % G;
 #pragma unroll
     for (int c = tok < E ? x : D; c < D / 4; c += kTpr) {
