@@ -1,6 +1,6 @@
 // Grouped-head attention over a cache of 4 bits (mla_mx4.h), with the items, pieces and joining of mla_gqa.h: single tokens
-// and short chunks read the codes here; long chunks have their keys' values laid out first (mx4_pages_kernel), for the bf16
-// kernels.
+// and chunks of up to 512 rows read the codes here; longer ones have their keys' values laid out first (mx4_pages_kernel), for
+// the bf16 kernels.
 //
 // As mla_gqa_stream.hip, one CTA per (request, rows, KV head, piece of the keys), whose waves take tiles of 32 keys in turn,
 // load a tile ahead and share nothing until the end. A tile is 4.3 KB (head_dim 128): codes go through the wave's
@@ -11,6 +11,15 @@
 //            a conversion gives dims (8 n + 2 c, + 1) of one key, two of them swap halves, and product m of 8 has dim
 //            8 n + m in row n: lane (row a16, g) ends up with the 32 dims 32 g + 8 i + m.
 // At head_dim 64 half as many of each.
+// Bound: with 16 rows, reading (64 requests of 1k to 8k tokens, 64 and 8 heads of 128: 321 MB in 66 us, 4.9 TB/s; its loads alone, the
+// rest left out, take 63); vector instructions, some 150 a tile, and the matrix instructions, which hardly overlap with them
+// (measured: 1.8 ns and 7 ns each a SIMD, 9.5 for one of the latter with two of the former), take 45 us of it, hidden. With 32
+// rows they are the bound: 16 chunks of 1 to 8 tokens on 1k to 16k, 32 and 8 heads, 154 MB in 35 us. Below some 20 MB: dependent
+// loads (lengths, page, tile) and the joining's launch: one request of 1500, 5.7 us and 4.2.
+// What did not pay, us for the 64 requests: two tiles ahead in registers 77 for 75, in a ring of LDS tiles that loads fill by
+// themselves 66 for 66 at any depth; more waves (128 registers) 72 for 66; pairs of dims in place of pairs of keys, without the
+// swaps and with twice the matrix instructions, 66 for 66; equal shares of the batch's keys for as many CTAs as run at once
+// 61 for 66, but 20 for 18.5 (8 of 32k to 128k) and 41 for 37 (the drafts).
 #include <type_traits>
 
 #include "mla_gqa.h"
@@ -56,7 +65,9 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GqaItem it;
-  if (!gqa_find<kRows, false>(p, blockIdx.x, it)) return;
+  // long requests first where items of a length differ in work (one block of rows or two): 16 drafts 37.3 -> 35.3 us; with one
+  // block the order gains nothing and its search costs (64 requests of 1k to 8k 66.1 -> 68.4)
+  if (!gqa_find<kRows, (NB > 1)>(p, blockIdx.x, it)) return;
   const int C = it.C;
   const int E = it.r.E, L = it.r.L, P = it.r.P, G = p.group;
   const int a16 = lane & 15, g = lane >> 4;

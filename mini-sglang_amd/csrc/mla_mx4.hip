@@ -3,6 +3,8 @@
 // A lane takes 8 dims: 16 bytes of bf16, 4 of codes. Four lanes share a block of 32; its largest magnitude is found in two
 // DPP steps on the bits (bf16 magnitudes order like whole numbers, infinities and NaN above all of them). The power of two
 // is exact to divide by, so rounding to the nearest code is the only rounding, in one instruction for two values.
+// Bound: HBM for many rows, a launch for few. 8192 rows of 8 heads of 128, 43 MB: in 11.0 us, out 9.6 (13.3 and 12.6 with a
+// thread for K and one for V); 64 rows 3 us each.
 #include "mla_mx4.h"
 
 namespace mla {

@@ -8,6 +8,8 @@
 // A row is D / 8 lanes' (a wave holds 4 rows of 128 or 8 of 64), 8 dims a lane in two chunks of 4 that hold both halves of
 // its pairs: no lane needs another's values but for the sum of squares, which is 3 or 4 DPP steps. Rows of one token are
 // next to each other in a wave, so they share the angles.
+// Bound: HBM for many tokens (8192 of 64 and 8 heads of 128, with V: 340 MB in 63 us, 5.4 TB/s), a launch and three dependent
+// loads for few (64 tokens 3.7 us).
 #include "mla_common.h"
 #include "mla_device.h"
 
