@@ -41,12 +41,17 @@ constexpr float kRoom = 24.f;
 // whether a byte of w is 255
 __device__ __forceinline__ uint32_t any_ff(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
 
-// NB blocks of 16 rows, NW waves. kBig: pages of 32 tokens or more, so that a tile lies in one page and its addresses are
-// the wave's (scalar), where they are a lane's otherwise.
-template <int D, int NB, int NW, bool kBig>
+// How a tile's codes are addressed: kPage, it lies in one page (of 32 tokens or more), by scalars of the wave's; kRow, a row a
+// lane. kShared: as kRow, and a cache line holds codes of more than one head, so it should stay for the others; else codes
+// are read once (non-temporal).
+enum Mx4Tile { kPage, kRow, kShared };
+
+// NB blocks of 16 rows, NW waves
+template <int D, int NB, int NW, Mx4Tile kTile>
 __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params mp) {
   const GqaParams& p = mp.g;
-  constexpr int kRows = 16 * NB, kRowB = D / 2, kScaleB = D / 32, kKs = D / 32, kDb = D / 16;
+  constexpr bool kBig = kTile == kPage;
+  constexpr int kRows = 16 * NB, kRowB = D / 2, kKs = D / 32, kDb = D / 16;
   constexpr int kLoads = kTileKeys * kRowB / 1024;  // 16-byte loads of a lane per K or V tile
   constexpr int kLanes = kRowB / 16;                // lanes of a row in such a load
   using scale_t = std::conditional_t<D == 128, uint32_t, uint16_t>;
@@ -65,9 +70,14 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GqaItem it;
+  // A round of the chip's 8 dies takes 8 (block, piece)s with all their heads, a die each: with small pages the heads of a token
+  // share cache lines. 64 requests of 1k to 8k, 64 and 8 heads of 128, us with / without: pages of 1 token 135 / 193, of 2 92 / 109, of
+  // 4 84 / 88, of 16 and 64 alike.
+  const uint32_t per = 8 * p.kv_heads, in = blockIdx.x % per;
+  const int item = (int)(blockIdx.x - in + in % 8 * p.kv_heads + in / 8);
   // long requests first where items of a length differ in work (one block of rows or two): 16 drafts 37.3 -> 35.3 us; with one
   // block the order gains nothing and its search costs (64 requests of 1k to 8k 66.1 -> 68.4)
-  if (!gqa_find<kRows, (NB > 1)>(p, blockIdx.x, it)) return;
+  if (!gqa_find<kRows, (NB > 1)>(p, item, it)) return;
   const int C = it.C;
   const int E = it.r.E, L = it.r.L, P = it.r.P, G = p.group;
   const int a16 = lane & 15, g = lane >> 4;
@@ -103,14 +113,23 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   scale_off = kBig ? (lane & 31) * (uint32_t)mp.s_tok : 0;
   const uint8_t *kh = mp.k_codes + (int64_t)it.head * mp.c_head, *vh = mp.v_codes + (int64_t)it.head * mp.c_head;
   const uint8_t *ksh = mp.k_scales + (int64_t)it.head * mp.s_head, *vsh = mp.v_scales + (int64_t)it.head * mp.s_head;
+  auto codes = [&](const uint8_t* k, const uint8_t* v, int u) __attribute__((always_inline)) {
+    const u32x4 *kp = reinterpret_cast<const u32x4*>(k), *vp = reinterpret_cast<const u32x4*>(v);
+    if constexpr (kTile == kShared) {
+      kr[u] = *kp;
+      vr[u] = *vp;
+    } else {
+      kr[u] = __builtin_nontemporal_load(kp);
+      vr[u] = __builtin_nontemporal_load(vp);
+    }
+  };
   auto load = [&](int t0, int row) __attribute__((always_inline)) {
     if constexpr (kBig) {
       const int64_t page = min(max(__builtin_amdgcn_readfirstlane(row), 0), p.num_pages - 1), tok = t0 & ((1 << p.log2_ps) - 1);
       const int64_t at = page * mp.c_page + tok * mp.c_tok, sat = page * mp.s_page + tok * mp.s_tok;
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
-        kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + at + code_at[u]));
-        vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + at + code_at[u]));
+        codes(kh + at + code_at[u], vh + at + code_at[u], u);
       }
       sr = *reinterpret_cast<const scale_t*>((lane < 32 ? ksh : vsh) + sat + scale_off);
     } else {
@@ -119,8 +138,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
         const int64_t from = __shfl(at, u * (64 / kLanes) + lane / kLanes) + code_at[u];
-        kr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kh + from));
-        vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vh + from));
+        codes(kh + from, vh + from, u);
       }
       sr = *reinterpret_cast<const scale_t*>((lane < 32 ? ksh : vsh) + page * mp.s_page + tok * mp.s_tok);
     }
@@ -428,20 +446,25 @@ __global__ __launch_bounds__(256) void mx4_pages_kernel(const GqaMx4Params mp) {
     }
 }
 
-template <int D, int NB, bool kBig>
+template <int D, int NB, Mx4Tile kTile>
 void launch_stream(const GqaMx4Params& p, int64_t grid, hipStream_t stream) {
-  if (p.g.wide) hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 8, kBig>), dim3((unsigned)grid), dim3(512), 0, stream, p);
-  else hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 4, kBig>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+  if (p.g.wide) hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 8, kTile>), dim3((unsigned)grid), dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL((gqa_mx4_kernel<D, NB, 4, kTile>), dim3((unsigned)grid), dim3(256), 0, stream, p);
 }
 template <int D, int NB>
 void launch_stream(const GqaMx4Params& p, int64_t grid, hipStream_t stream) {
-  p.g.log2_ps >= 5 ? launch_stream<D, NB, true>(p, grid, stream) : launch_stream<D, NB, false>(p, grid, stream);
+  // a head's run of codes in a page against a line of 128 bytes. us with temporal / non-temporal loads, 64 requests of 1k to 8k, 8 KV
+  // heads: head_dim 128, pages of 1 token 112 / 135, of 2 (whole lines) 95 / 92; 64, of 1 81 / 116, of 2 67 / 74, of 4 59 / 58
+  const int64_t run = p.c_tok == D / 2 ? (int64_t)(D / 2) << p.g.log2_ps : D / 2;
+  if (run < 128 && p.g.kv_heads > 1) launch_stream<D, NB, kShared>(p, grid, stream);
+  else if (p.g.log2_ps >= 5) launch_stream<D, NB, kPage>(p, grid, stream);
+  else launch_stream<D, NB, kRow>(p, grid, stream);
 }
 
 }  // namespace
 
 hipError_t launch_gqa_mx4(const GqaMx4Params& p, int dim, int rows, hipStream_t stream) {
-  const int64_t grid = gqa_ctas(p.g, rows);
+  const int64_t per = 8 * p.g.kv_heads, grid = (gqa_ctas(p.g, rows) + per - 1) / per * per;  // whole rounds
   if (dim == 128) rows == 16 ? launch_stream<128, 1>(p, grid, stream) : launch_stream<128, 2>(p, grid, stream);
   else rows == 16 ? launch_stream<64, 1>(p, grid, stream) : launch_stream<64, 2>(p, grid, stream);
   hipError_t e = hipGetLastError();
