@@ -346,7 +346,7 @@ int paged_mx4(const char* who, const void* q, int64_t q_stride_t, int64_t q_stri
   mp.scratch_rows = space.rows;
   mp.scratch_k = reinterpret_cast<__bf16*>(at + space.table);
   mp.scratch_v = mp.scratch_k + space.rows * kv_heads * dim;
-  if (space.rows / 64 * 256 > UINT32_MAX || kv_heads > 65535 || space.rows > 0x7fffffff)
+  if ((space.rows / 64 + 8) * kv_heads * 256 > UINT32_MAX || space.rows > 0x7fffffff)
     return api_error(MLA_ERR_UNSUPPORTED, "%s: %lld keys are more than a launch holds", who, (long long)space.rows);
   if (hipError_t e = launch_mx4_pages(mp, dim, (hipStream_t)stream); e != hipSuccess) return done(e, who);
   p.k = mp.scratch_k;

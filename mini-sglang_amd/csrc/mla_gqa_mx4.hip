@@ -41,6 +41,15 @@ constexpr float kRoom = 24.f;
 // whether a byte of w is 255
 __device__ __forceinline__ uint32_t any_ff(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
 
+// The CTA's item, of which the heads come fastest: CTAs go to the chip's 8 dies in turn, and a round of 8 heads' CTAs takes 8 (block,
+// piece)s with all their heads, a die each, since with small pages the heads of a token share cache lines. 64 requests of 1k
+// to 8k, 64 and 8 heads of 128, us with / without: pages of 1 token 135 / 193, of 2 92 / 109, of 4 84 / 88, of 16 and 64 alike.
+__device__ __forceinline__ int mx4_item(int heads) {
+  const uint32_t per = 8 * heads, in = blockIdx.x % per;
+  return (int)(blockIdx.x - in + in % 8 * heads + in / 8);
+}
+inline int64_t mx4_rounds(int64_t ctas, int heads) { return (ctas + 8 * heads - 1) / (8 * heads) * (8 * heads); }
+
 // How a tile's codes are addressed: kPage, it lies in one page (of 32 tokens or more), by scalars of the wave's; kRow, a row a
 // lane. kShared: as kRow, and a cache line holds codes of more than one head, so it should stay for the others; else codes
 // are read once (non-temporal).
@@ -70,11 +79,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GqaItem it;
-  // A round of the chip's 8 dies takes 8 (block, piece)s with all their heads, a die each: with small pages the heads of a token
-  // share cache lines. 64 requests of 1k to 8k, 64 and 8 heads of 128, us with / without: pages of 1 token 135 / 193, of 2 92 / 109, of
-  // 4 84 / 88, of 16 and 64 alike.
-  const uint32_t per = 8 * p.kv_heads, in = blockIdx.x % per;
-  const int item = (int)(blockIdx.x - in + in % 8 * p.kv_heads + in / 8);
+  const int item = mx4_item(p.kv_heads);
   // long requests first where items of a length differ in work (one block of rows or two): 16 drafts 37.3 -> 35.3 us; with one
   // block the order gains nothing and its search costs (64 requests of 1k to 8k 66.1 -> 68.4)
   if (!gqa_find<kRows, (NB > 1)>(p, item, it)) return;
@@ -400,13 +405,14 @@ __global__ __launch_bounds__(256) void mx4_pages_kernel(const GqaMx4Params mp) {
   const GqaParams& p = mp.g;
   constexpr int kLanes = D / 8;
   const int lane = threadIdx.x & 63;
-  // the CTA's page of 64 keys: its request, by a scan of the pages
+  // the CTA's head and page of 64 keys: its request, by a scan of the pages
+  const int item = mx4_item(p.kv_heads), head = item % p.kv_heads, to = item / p.kv_heads;
   int acc = 0, b = -1, first = 0, L = 0;
   for (int c0 = 0; c0 < p.batch && b < 0; c0 += 64) {
     int len = 0;
     if (c0 + lane < p.batch) len = gqa_request(p, c0 + lane).L;
     const int n = (len + 63) >> 6, incl = wave_iscan(n);
-    const uint64_t hit = __ballot((int)blockIdx.x >= acc + incl - n && (int)blockIdx.x < acc + incl);
+    const uint64_t hit = __ballot(to >= acc + incl - n && to < acc + incl);
     if (hit != 0) {
       const int fl = __builtin_ctzll(hit);
       b = c0 + fl;
@@ -416,9 +422,9 @@ __global__ __launch_bounds__(256) void mx4_pages_kernel(const GqaMx4Params mp) {
       acc += __builtin_amdgcn_readlane(incl, 63);
     }
   }
-  if (b < 0) return;
-  const int page = (int)blockIdx.x - first, head = blockIdx.y;
-  if (threadIdx.x == 0 && head == 0) mp.scratch_table[(int64_t)b * mp.scratch_cols + page] = (int)blockIdx.x;
+  if (b < 0 || to >= mp.scratch_rows / 64) return;
+  const int page = to - first;
+  if (threadIdx.x == 0 && head == 0) mp.scratch_table[(int64_t)b * mp.scratch_cols + page] = to;
   constexpr int kRowsAtOnce = 256 / kLanes, kN = 64 / kRowsAtOnce;
   const int x = threadIdx.x % kLanes, t0 = threadIdx.x / kLanes;
   int64_t pg[kN], tok[kN];
@@ -441,7 +447,7 @@ __global__ __launch_bounds__(256) void mx4_pages_kernel(const GqaMx4Params mp) {
   for (int i = 0; i < kN; ++i)
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      const int64_t at = ((int64_t)head * mp.scratch_rows + (int64_t)blockIdx.x * 64 + t0 + i * kRowsAtOnce) * D + 8 * x;
+      const int64_t at = ((int64_t)head * mp.scratch_rows + (int64_t)to * 64 + t0 + i * kRowsAtOnce) * D + 8 * x;
       *reinterpret_cast<u32x4*>((v ? mp.scratch_v : mp.scratch_k) + at) = mx4_values(codes[i][v], scales[i][v] << 23);
     }
 }
@@ -464,7 +470,7 @@ void launch_stream(const GqaMx4Params& p, int64_t grid, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_gqa_mx4(const GqaMx4Params& p, int dim, int rows, hipStream_t stream) {
-  const int64_t per = 8 * p.g.kv_heads, grid = (gqa_ctas(p.g, rows) + per - 1) / per * per;  // whole rounds
+  const int64_t grid = mx4_rounds(gqa_ctas(p.g, rows), p.g.kv_heads);
   if (dim == 128) rows == 16 ? launch_stream<128, 1>(p, grid, stream) : launch_stream<128, 2>(p, grid, stream);
   else rows == 16 ? launch_stream<64, 1>(p, grid, stream) : launch_stream<64, 2>(p, grid, stream);
   hipError_t e = hipGetLastError();
@@ -473,7 +479,7 @@ hipError_t launch_gqa_mx4(const GqaMx4Params& p, int dim, int rows, hipStream_t 
 }
 
 hipError_t launch_mx4_pages(const GqaMx4Params& p, int dim, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.scratch_rows / 64), (unsigned)p.g.kv_heads);
+  const dim3 grid((unsigned)mx4_rounds(p.scratch_rows / 64 * p.g.kv_heads, p.g.kv_heads));
   if (dim == 128) hipLaunchKernelGGL(mx4_pages_kernel<128>, grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL(mx4_pages_kernel<64>, grid, dim3(256), 0, stream, p);
   return hipGetLastError();
