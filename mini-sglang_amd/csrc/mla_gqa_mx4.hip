@@ -11,7 +11,7 @@
 //            a conversion gives dims (8 n + 2 c, + 1) of one key, two of them swap halves, and product m of 8 has dim
 //            8 n + m in row n: lane (row a16, g) ends up with the 32 dims 32 g + 8 i + m.
 // At head_dim 64 half as many of each.
-// Bound: with 16 rows, reading (64 requests of 1k to 8k tokens, 64 and 8 heads of 128: 321 MB in 66 us, 4.9 TB/s; its loads alone, the
+// Bound: with 16 rows, reading (64 requests of 1k to 8k tokens, 64 and 8 heads of 128: 344 MB in 66 us, 5.2 TB/s; its loads alone, the
 // rest left out, take 63); vector instructions, some 150 a tile, and the matrix instructions, which hardly overlap with them
 // (measured: 1.8 ns and 7 ns each a SIMD, 9.5 for one of the latter with two of the former), take 45 us of it, hidden. With 32
 // rows they are the bound: 16 chunks of 1 to 8 tokens on 1k to 16k, 32 and 8 heads, 154 MB in 35 us. Below some 20 MB: dependent
