@@ -419,7 +419,7 @@ int mla_page_tables_from_lengths(int32_t *token_table, int32_t token_table_rows,
  * they are to rows slots[t] (index_bits 32 or 64) of k_out and v_out [out_rows, kv_heads, head_dim]: row r, head h at
  * k_out + r * k_out_stride_row + h * k_out_stride_h; slots outside [0, out_rows) are not written, others must be distinct.
  * slots NULL: row t. q_out may be q, and without slots k_out k and v_out v, with their strides; other outputs overlap no
- * input. Replaces the q / k norms and the rotation of python/minisgl/layers/attention.py:40-52 (norm.py, rotary.py:39-51)
+ * input. Replaces the q / k norms and the rotation of python/minisgl/layers/attention.py:17-57 (norm.py, rotary.py:39-51)
  * and the store of python/minisgl/kvcache/mha_pool.py:45-56.
  */
 int mla_qk_norm_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_stride_t,

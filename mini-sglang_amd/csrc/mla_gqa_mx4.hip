@@ -273,20 +273,20 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
     auto products = [&](auto c) __attribute__((always_inline)) {
       constexpr int kC = decltype(c)::value;
       if constexpr (kC < kDb / 2) {
-          u32x4 lo, hi;
+        u32x4 lo, hi;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t x = two(c, h, 2 * i), y = two(c, h, 2 * i + 1);
-              lo[2 * h + i] = __builtin_amdgcn_perm(y, x, 0x05040100);
-              hi[2 * h + i] = __builtin_amdgcn_perm(y, x, 0x07060302);
-            }
-#pragma unroll
-          for (int nb = 0; nb < kAct; ++nb) {
-            mfma(lo, pb[nb], O[nb][2 * kC]);
-            mfma(hi, pb[nb], O[nb][2 * kC + 1]);
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x = two(c, h, 2 * i), y = two(c, h, 2 * i + 1);
+            lo[2 * h + i] = __builtin_amdgcn_perm(y, x, 0x05040100);
+            hi[2 * h + i] = __builtin_amdgcn_perm(y, x, 0x07060302);
           }
+#pragma unroll
+        for (int nb = 0; nb < kAct; ++nb) {
+          mfma(lo, pb[nb], O[nb][2 * kC]);
+          mfma(hi, pb[nb], O[nb][2 * kC + 1]);
+        }
       }
     };
     products(std::integral_constant<int, 0>{});

@@ -1,7 +1,7 @@
 """64-bit oracle of the 4-bit cache and of the norms and rotation of grouped heads. TEST INFRASTRUCTURE ONLY.
 
 4 bits: MXFP4 of the OCP Microscaling Formats 1.0, by its tables: E2M1 elements, E8M0 scales, blocks of 32.
-Norms and rotation: python/minisgl/layers/attention.py:40-52, norm.py and rotary.py:22-51 of the reference.
+Norms and rotation: python/minisgl/layers/attention.py:17-57, norm.py and rotary.py:22-51 of the reference.
 """
 
 from __future__ import annotations
