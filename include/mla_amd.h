@@ -419,7 +419,7 @@ int mla_page_tables_from_lengths(int32_t *token_table, int32_t token_table_rows,
  * they are to rows slots[t] (index_bits 32 or 64) of k_out and v_out [out_rows, kv_heads, head_dim]: row r, head h at
  * k_out + r * k_out_stride_row + h * k_out_stride_h; slots outside [0, out_rows) are not written, others must be distinct.
  * slots NULL: row t. q_out may be q, and without slots k_out k and v_out v, with their strides; other outputs overlap no
- * input. Replaces the q / k norms and the rotation of python/minisgl/layers/attention.py:17-57 (norm.py, rotary.py:39-51)
+ * input, and rows of outputs not one another. Replaces the q / k norms and the rotation of python/minisgl/layers/attention.py:17-57 (norm.py, rotary.py:39-51)
  * and the store of python/minisgl/kvcache/mha_pool.py:45-56.
  */
 int mla_qk_norm_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_stride_t,
@@ -436,9 +436,9 @@ int mla_qk_norm_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h,
  * one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (code 0..7, bit 3 the sign) times its block's power of two.
  *   codes   [num_pages, page_size, kv_heads, head_dim / 2]: dims 2 i and 2 i + 1 in the low and high half of byte i
  *   scales  [num_pages, page_size, kv_heads, head_dim / 32]: the exponent plus 127 (254 at most 2^127; a value past bf16's range
- *           is an infinity); 255: the block is NaN
+ *           is an infinity: attention over such a block may give NaN; mla_mx4_store writes 252 at most); 255: the block is NaN
  * Strides in bytes: of codes multiples of 16, codes 16-byte aligned; of scales multiples of head_dim / 32, scales aligned by
- * as much; rows contiguous. page_size a power of two.
+ * as much; rows contiguous, none over another. page_size a power of two.
  */
 typedef struct {
   void *codes, *scales;
@@ -452,7 +452,8 @@ typedef struct {
  * others must be distinct. A block's exponent is floor(log2 of its largest magnitude) - 2, at least -127; values are rounded
  * to the nearest, ties to the even code, 6 units at most; a block with an infinity or a NaN gets scale 255 and codes 0.
  * Bit-exact. Replaces store_kv_cache (python/minisgl/kernel/csrc/jit/store.cu:25-53) for this pool.
- * mla_mx4_load: the values of rows indices[i] into k, v [rows, kv_heads, head_dim] (exact in bf16); 0 for indices outside.
+ * mla_mx4_load: the values of rows indices[i] into k, v [rows, kv_heads, head_dim] (exact in bf16), whose rows do not overlap;
+ * 0 for indices outside.
  */
 int mla_mx4_store(const mla_mx4_pool *k_pool, const mla_mx4_pool *v_pool, int32_t num_pages, int32_t page_size,
                   int32_t kv_heads, int32_t head_dim, const void *indices, int32_t index_bits, int32_t rows, const void *k,

@@ -110,6 +110,14 @@ int64_t workspace_rows(int64_t most) {
   return 2 * (int64_t)kTarget * (most <= 16 ? 16 : 32);
 }
 
+// Whether rows of `width` elements do not overlap: `outer` of them outer_stride apart, each of `inner` inner_stride apart, in
+// either order.
+bool rows_apart(int64_t outer, int64_t outer_stride, int64_t inner, int64_t inner_stride, int64_t width) {
+  const bool by_outer = (inner <= 1 || inner_stride >= width) && (outer <= 1 || outer_stride >= (inner - 1) * inner_stride + width);
+  const bool by_inner = (outer <= 1 || outer_stride >= width) && (inner <= 1 || inner_stride >= (outer - 1) * outer_stride + width);
+  return by_outer || by_inner;
+}
+
 int check_heads(const char* who, int32_t q_heads, int32_t kv_heads, int32_t dim) {
   if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0)
     return api_error(MLA_ERR_INVALID_ARG, "%s: %d query heads are no multiple of %d KV heads", who, q_heads, kv_heads);
@@ -127,10 +135,8 @@ int query_params(const char* who, GqaParams& p, const void* q, int64_t q_stride_
   if (q_stride_t % 8 || q_stride_h % 8 || q_stride_t < 0 || q_stride_h < 0)
     return api_error(MLA_ERR_INVALID_ARG, "%s: q strides (%lld, %lld) must be non-negative multiples of 8", who,
                      (long long)q_stride_t, (long long)q_stride_h);
-  // rows of out must not overlap, tokens outside heads or heads outside tokens
-  const bool by_token = (q_heads == 1 || out_stride_h >= dim) && (total_q == 1 || out_stride_t >= (q_heads - 1) * out_stride_h + dim);
-  const bool by_head = (total_q == 1 || out_stride_t >= dim) && (q_heads == 1 || out_stride_h >= (total_q - 1) * out_stride_t + dim);
-  if (out_stride_t % 4 || out_stride_h % 4 || out_stride_t < 0 || out_stride_h < 0 || !(by_token || by_head))
+  if (out_stride_t % 4 || out_stride_h % 4 || out_stride_t < 0 || out_stride_h < 0 ||
+      !rows_apart(total_q, out_stride_t, q_heads, out_stride_h, dim))
     return api_error(MLA_ERR_INVALID_ARG, "%s: out strides (%lld, %lld) must be multiples of 4 and hold %d tokens of %d heads of %d",
                      who, (long long)out_stride_t, (long long)out_stride_h, total_q, q_heads, dim);
   if (lse != nullptr && total_q > 1 && lse_stride_t < q_heads)
@@ -264,7 +270,7 @@ Mx4Space mx4_space(int64_t most, int32_t kv_heads, int32_t dim, int32_t batch, i
   s.split = 4 * workspace_rows(most) * (dim + 2);
   if (most > kStreamRows) {
     s.cols = (max_keys + 63) / 64;
-    s.rows = 64 * std::min(total_keys / 64 + batch, batch * s.cols);
+    s.rows = std::min<int64_t>(64 * std::min(total_keys / 64 + batch, batch * s.cols), int64_t{1} << 31);  // (more are refused)
     s.table = (4 * batch * s.cols + 15) / 16 * 16;
   }
   s.bytes = s.split + s.table + 2 * s.rows * kv_heads * dim * 2;
@@ -287,6 +293,9 @@ int check_mx4(const char* who, const Mx4View& k, const Mx4View& v, int32_t dim, 
       return api_error(MLA_ERR_INVALID_ARG, "%s: strides must be non-negative multiples of 16 bytes (codes) and of a row (scales)", who);
     else if (x->c_tok > (1 << 24) || x->s_tok > (1 << 24))
       return api_error(MLA_ERR_UNSUPPORTED, "%s: tokens lie more than 16 MiB apart", who);
+    else if ((num_pages > 1 && (x->c_page < dim / 2 || x->s_page < scale_row)) || (page_size > 1 && (x->c_tok < dim / 2 || x->s_tok < scale_row)) ||
+             (kv_heads > 1 && (x->c_head < dim / 2 || x->s_head < scale_row)))
+      return api_error(MLA_ERR_INVALID_ARG, "%s: rows of a pool lie over one another: strides below a row", who);
   return MLA_OK;
 }
 
@@ -339,6 +348,8 @@ int paged_mx4(const char* who, const void* q, int64_t q_stride_t, int64_t q_stri
     p.ws_lse = reinterpret_cast<f32x2*>(p.ws_o + workspace_rows(most) * dim);
   }
   if (int rc = set_choice(who, p, choice)) return rc;
+  if (!laid_out && (gqa_ctas(p, choice.rows) + 8 * kv_heads) * (choice.wide ? 512 : 256) > UINT32_MAX)  // in whole rounds of heads
+    return api_error(MLA_ERR_UNSUPPORTED, "%s: %d rows of %d heads are more than a launch holds", who, total_q, q_heads);
   if (!laid_out) return done(launch_gqa_mx4(mp, dim, choice.rows, (hipStream_t)stream), who);
   char* at = static_cast<char*>(workspace) + space.split;
   mp.scratch_table = reinterpret_cast<int32_t*>(at);
@@ -377,6 +388,8 @@ int mx4_rows(const char* who, bool load, const mla_mx4_pool* k_pool, const mla_m
     return api_error(MLA_ERR_INVALID_ARG, "%s: k and v must be 16-byte aligned, with non-negative strides that are multiples of 8", who);
   if ((int64_t)rows * 2 * kv_heads * (dim / 8) > UINT32_MAX - 256)
     return api_error(MLA_ERR_UNSUPPORTED, "%s: %d rows of %d heads are more than a launch holds", who, rows, kv_heads);
+  if (load && (!rows_apart(rows, k_stride_t, kv_heads, k_stride_h, dim) || !rows_apart(rows, v_stride_t, kv_heads, v_stride_h, dim)))
+    return api_error(MLA_ERR_INVALID_ARG, "%s: rows of k or v overlap", who);
   if (load) {
     p.k_out = static_cast<__bf16*>(const_cast<void*>(k));
     p.v_out = static_cast<__bf16*>(const_cast<void*>(v));
@@ -509,6 +522,7 @@ int mla_gqa_mx4_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads
   if (bytes == nullptr || max_q < 0 || batch < 0 || max_keys < 0 || total_keys < 0)
     return mla::api_error(MLA_ERR_INVALID_ARG, "%s: bytes is null, or max_q %d, batch %d, max_keys %lld or total_keys %lld < 0", who, max_q,
                           batch, (long long)max_keys, (long long)total_keys);
+  if (batch > 65535) return mla::api_error(MLA_ERR_UNSUPPORTED, "%s: at most 65535 requests, got %d", who, batch);
   if (int rc = mla::check_heads(who, q_heads, kv_heads, head_dim)) return rc;
   *bytes = mla::mx4_space((int64_t)max_q * (q_heads / kv_heads), kv_heads, head_dim, batch, std::min<int64_t>(max_keys, 0x7ff00000), total_keys).bytes;
   return mla::done(hipSuccess, who);
@@ -588,6 +602,18 @@ int mla_qk_norm_rope_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h,
     if (x % 8 || x < 0) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: strides must be non-negative multiples of 8", who);
   if ((int64_t)tokens * (q_heads + 2 * kv_heads + 8) * (head_dim / 8) > UINT32_MAX - 256)
     return mla::api_error(MLA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads are more than a launch holds", who, tokens, q_heads + 2 * kv_heads);
+  auto moved = [&](const void* in, int64_t in_t, int64_t in_h, const void* to, int64_t to_t, int64_t to_h, int32_t heads) {
+    return heads > 0 && in == to && ((tokens > 1 && in_t != to_t) || (heads > 1 && in_h != to_h));
+  };
+  if (moved(q, q_stride_t, q_stride_h, q_out, q_out_stride_t, q_out_stride_h, q_heads) ||
+      moved(k, k_stride_t, k_stride_h, k_out, k_out_stride_row, k_out_stride_h, kv_heads) ||
+      (v != nullptr && moved(v, v_stride_t, v_stride_h, v_out, v_out_stride_row, v_out_stride_h, kv_heads)) ||
+      (slots != nullptr && kv_heads > 0 && (k == k_out || (v != nullptr && v == v_out))))
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: outputs in the place of inputs take their strides, and no slots", who);
+  if ((q_heads > 0 && !mla::rows_apart(tokens, q_out_stride_t, q_heads, q_out_stride_h, head_dim)) ||
+      (kv_heads > 0 && !mla::rows_apart(out_rows, k_out_stride_row, kv_heads, k_out_stride_h, head_dim)) ||
+      (kv_heads > 0 && v != nullptr && !mla::rows_apart(out_rows, v_out_stride_row, kv_heads, v_out_stride_h, head_dim)))
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: rows of q_out, k_out or v_out overlap", who);
   mla::QkNormRopeParams p = {};
   p.q = static_cast<const __bf16*>(q);
   p.k = static_cast<const __bf16*>(k);

@@ -592,7 +592,7 @@ _OTHER_DEVICE, _OTHER_STREAM = -1, -2
 def _again(rc: int, device, call, name: str, *args):
     """The rest of a call (its last argument the stream) that did not go through at once: with the tensors' GPU current, with
     the stream current that memory is allocated for (only there is a block's last use ordered before the launch), or its
-    error. Results of such an allocation are marked as used on the caller's stream, for when they are freed."""
+    error. Results of such a call are marked as used on the caller's stream, for when they are freed."""
     import torch
 
     with torch.cuda.device(device):
@@ -604,7 +604,8 @@ def _again(rc: int, device, call, name: str, *args):
             with torch.cuda.stream(stream):
                 rc = call(*args)
             if isinstance(rc, tuple):
-                rc[0].record_stream(callers)  # of the block that all of them lie in
+                for t in rc:
+                    t.record_stream(callers)
     if isinstance(rc, int) and rc != 0:
         check(rc, name)
     return rc

@@ -64,6 +64,8 @@ POOLS = [
     (dict(kp=pool(ct=72)), INVALID, "strides"), (dict(kp=pool(ch=-64)), INVALID, "strides"), (dict(vp=pool(sh=2)), INVALID, "strides"), (dict(vp=pool(st=-8)), INVALID, "strides"),
     (dict(ps=24), UNSUPPORTED, "page_size"), (dict(ps=0), UNSUPPORTED, "page_size"), (dict(pages=0), INVALID, "num_pages"),
     (dict(pages=1 << 20, ps=1 << 12), UNSUPPORTED, "2^31 rows"), (dict(d=96), UNSUPPORTED, "head_dim"), (dict(d=256), UNSUPPORTED, "head_dim"),
+    (dict(kp=pool(ct=1 << 25)), UNSUPPORTED, "16 MiB"), (dict(vp=pool(st=1 << 25)), UNSUPPORTED, "16 MiB"),
+    (dict(kp=pool(cp=0)), INVALID, "over one another"), (dict(kp=pool(st=0)), INVALID, "over one another"), (dict(vp=pool(ch=48)), INVALID, "over one another"),
 ]
 ROWS = POOLS + [
     (dict(n=-1), INVALID, "rows"), (dict(bits=16), INVALID, "index_bits"), (dict(idx=None), INVALID, "null"), (dict(k=None), INVALID, "null"), (dict(v=None), INVALID, "null"),
@@ -89,8 +91,15 @@ ROPE = [
 ]
 
 
+LOAD = ROWS + [(dict(kt=0), INVALID, "overlap"), (dict(vt=128), INVALID, "overlap"), (dict(kh=0), INVALID, "overlap")]
+ROPE += [(dict(qot=2048), INVALID, "in the place"), (dict(qo=16 * P, ko=16 * P), INVALID, "no slots"), (dict(qo=16 * P, vo=16 * P), INVALID, "no slots"),
+         (dict(slots=None, rows=5, kor=512), INVALID, "in the place")]
+ELSE = dict(qo=16 * P, ko=32 * P, vo=48 * P)
+ROPE += [({**ELSE, **kw}, INVALID, "overlap") for kw in (dict(qot=0), dict(qoh=64), dict(kor=128), dict(voh=0))]
+
+
 @pytest.mark.parametrize("call,cases", [
-    (lambda **kw: rows("mla_mx4_store", **kw), ROWS), (lambda **kw: rows("mla_mx4_load", **kw), ROWS), (decode, ATTENTION),
+    (lambda **kw: rows("mla_mx4_store", **kw), ROWS), (lambda **kw: rows("mla_mx4_load", **kw), LOAD), (decode, ATTENTION),
     (chunk, ATTENTION + [(dict(cu=None), INVALID, "null"), (dict(max_q=-1), INVALID, "max_q"), (dict(T=-1), INVALID, "total_q")]), (rope, ROPE)])
 def test_refusals(call, cases):
     for kw, code, text in cases:
@@ -113,7 +122,8 @@ def test_workspace_bytes():
     assert split + 2 * 20000 * 8 * 128 * 2 <= at <= split + 4 * 4 * 128 + 2 * (20000 + 4 * 64) * 8 * 128 * 2
     assert lib.gqa_mx4_workspace_bytes(65, 64, 8, 128, 4, 8192, 1 << 40) == lib.gqa_mx4_workspace_bytes(65, 64, 8, 128, 4, 8192, 4 * 8192)
     assert at <= lib.gqa_mx4_workspace_bytes(66, 64, 8, 128, 4, 8192, 20000) and at <= lib.gqa_mx4_workspace_bytes(65, 64, 8, 128, 5, 8192, 20001)
-    for bad in ((-1, 8, 2, 128, 1, 1, 1), (1, 8, 3, 128, 1, 1, 1), (1, 8, 2, 96, 1, 1, 1), (1, 8, 2, 128, -1, 1, 1), (1, 8, 2, 128, 1, -1, 1), (1, 8, 2, 128, 1, 1, -1)):
+    assert lib.gqa_mx4_workspace_bytes(1 << 20, 4096, 4096, 128, 65535, 1 << 31, 1 << 62) > 0  # no overflow
+    for bad in ((1, 8, 2, 128, 70000, 1, 1), (-1, 8, 2, 128, 1, 1, 1), (1, 8, 3, 128, 1, 1, 1), (1, 8, 2, 96, 1, 1, 1), (1, 8, 2, 128, -1, 1, 1), (1, 8, 2, 128, 1, -1, 1), (1, 8, 2, 128, 1, 1, -1)):
         with pytest.raises(lib.MLAKernelError):
             lib.gqa_mx4_workspace_bytes(*bad)
 

@@ -392,6 +392,91 @@ def test_another_stream(decode):
         check(out, lse, ref)
 
 
+def test_rows_on_another_stream():
+    """In and out on a stream that is not the current one, results made for it, alone or beside a given one."""
+    gen = torch.Generator().manual_seed(26)
+    T, heads, dim = 500, 4, 128
+    x, y = randn(gen, T, heads, dim), randn(gen, T, heads, dim)
+    want = [M.values(*M.rounded(z)).to(torch.bfloat16) for z in (x, y)]
+    pools = [lib.mx4_pool(40, 16, heads, dim, DEV) for _ in "kv"]
+    slots = torch.randperm(640, generator=gen)[:T].to(DEV)
+    side, xd, yd = torch.cuda.Stream(), x.to(DEV), y.to(DEV)
+    torch.cuda.synchronize()
+    for given in (False, True):
+        late = torch.zeros_like(xd)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(1_000_000)
+            late.copy_(xd)
+        lib.mx4_store(*pools, slots, late, yd, stream=side)
+        k = torch.zeros_like(xd) if given else None
+        side.wait_stream(torch.cuda.current_stream())
+        k, v = lib.mx4_load(*pools, slots, k=k, stream=side)
+        torch.full((1 << 20,), NAN, device=DEV)
+        side.synchronize()
+        assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+        for p in pools:
+            p.codes.zero_()
+        torch.cuda.synchronize()
+
+
+def test_rows_captured():
+    """Stores and loads in a graph follow what their tensors hold at each replay; slots of -1 are skipped."""
+    gen = torch.Generator().manual_seed(27)
+    T, heads, dim = 33, 2, 64
+    pools = [lib.mx4_pool(5, 16, heads, dim, DEV) for _ in "kv"]
+    x, y = (torch.zeros((T, heads, dim), dtype=torch.bfloat16, device=DEV) for _ in "kv")
+    k, v = torch.empty_like(x), torch.empty_like(x)
+    slots = torch.arange(T, dtype=torch.int32, device=DEV)
+
+    def call():
+        lib.mx4_store(*pools, slots, x, y)
+        lib.mx4_load(*pools, slots, k, v)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for new in (33, 20, 33):
+        a, b = randn(gen, T, heads, dim), randn(gen, T, heads, dim)
+        s = torch.randperm(80, generator=gen)[:T].int()
+        s[new:] = -1
+        x.copy_(a), y.copy_(b), slots.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, z in ((k, a), (v, b)):
+            want = M.values(*M.rounded(z)).to(torch.bfloat16)
+            want[new:] = 0
+            assert torch.equal(got.cpu(), want)
+
+
+def test_tensors_that_do_not_fit():
+    x = torch.zeros((2, 4, 128), dtype=torch.bfloat16, device=DEV)
+    p = lib.mx4_pool(2, 4, 4, 128, DEV)
+    i = torch.zeros(2, dtype=torch.int32, device=DEV)
+    half = lib.mx4_pool(2, 4, 2, 128, DEV)
+    refused = [
+        (lambda: lib.mx4_store(p, half, i, x, x), "same shape"), (lambda: lib.mx4_store(p, p, i, x[:, :2], x), "k must be"),
+        (lambda: lib.mx4_store(p, p, i, x, x.float()), "v must be"), (lambda: lib.mx4_store(p, p, i.float(), x, x), "indices must be"),
+        (lambda: lib.mx4_store(p, p, i[:1], x, x), "k must be"), (lambda: lib.mx4_store(lib.MX4Pool(p.codes, p.scales[..., :3]), p, i, x, x), "for each 32 dims"),
+        (lambda: lib.mx4_store(lib.MX4Pool(p.codes.int(), p.scales), p, i, x, x), "uint8"),
+        (lambda: lib.gqa_decode_mx4(x[..., :64], p, p, i.view(2, 1), i, 0.1, x[..., :64]), "q's D"),
+        (lambda: lib.gqa_decode_mx4(x[:, :3].contiguous(), p, p, i.view(2, 1), i, 0.1, x[:, :3].contiguous()), "heads that divide"),
+        (lambda: lib.gqa_decode_mx4(x, p, p, i.view(2, 1), i[:1], 0.1, x), "one token"), (lambda: lib.gqa_decode_mx4(x, p, p, i, i, 0.1, x), "page_table"),
+        (lambda: lib.gqa_chunk_mx4(x, p, p, i.view(2, 1), i, i, 1, 0.1, x), "cu_seqlens_q"),
+        (lambda: lib.gqa_chunk_mx4(x, p, p, i.view(2, 1), None, i, 1, 0.1, x), "cu_seqlens_q"),
+    ]
+    for call, text in refused:
+        with pytest.raises(AssertionError, match=text):
+            call()
+    other = lib.MX4Pool(torch.zeros((2, 4, 4, 64), dtype=torch.uint8, device=DEV), torch.zeros((2, 4, 4, 4), dtype=torch.uint8, device=DEV))
+    with pytest.raises(lib.MLAKernelError, match="same strides"):
+        lib.gqa_decode_mx4(x, p, other, i.view(2, 1), i, 0.1, torch.empty_like(x))
+    with pytest.raises(lib.MLAKernelError, match="overlap"):
+        lib.mx4_load(p, p, i, k=x[:1].expand(2, 4, 128))
+
+
 @pytest.mark.parametrize("decode", [True, False])
 def test_captured(decode):
     """Two graphs with workspaces of their own, replayed by turns with eager calls between, following their lengths."""

@@ -164,3 +164,38 @@ def test_captured():
         near(q_out, *M.norm_rope(raw_q, w, EPS, p, cs, False))
         near(pools[0].view(80, hk, dim)[s.to(DEV).long()], *M.norm_rope(raw_k, w, EPS, p, cs, False))
         assert torch.equal(pools[1].view(80, hk, dim)[s.to(DEV).long()].cpu(), raw_v)
+
+
+def test_another_stream():
+    gen = torch.Generator().manual_seed(9)
+    T, hq, hk, dim = 700, 4, 2, 128
+    q, k, w = randn(gen, T, hq, dim), randn(gen, T, hk, dim), randn(gen, dim)
+    pos, cs = torch.arange(T, dtype=torch.int32) % 300, table(dim)
+    qd, kd, wd, pd, cd = q.to(DEV), k.to(DEV), w.to(DEV), pos.to(DEV), cs.to(DEV)
+    late, q_out, k_out, side = torch.zeros_like(qd), torch.zeros_like(qd), torch.zeros_like(kd), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000)
+        late.copy_(qd)
+    lib.qk_norm_rope(late, kd, None, wd, wd, EPS, pd, cd, False, q_out, k_out, stream=side)
+    side.synchronize()
+    near(q_out, *M.norm_rope(q, w, EPS, pos, cs, False))
+    near(k_out, *M.norm_rope(k, w, EPS, pos, cs, False))
+
+
+def test_tensors_that_do_not_fit():
+    x, k, w = (torch.zeros(s, dtype=torch.bfloat16, device=DEV) for s in ((3, 4, 128), (3, 2, 128), (128,)))
+    i, cs = torch.zeros(3, dtype=torch.int32, device=DEV), table(128).to(DEV)
+    pool = torch.zeros((2, 4, 2, 128), dtype=torch.bfloat16, device=DEV)
+    call = lambda q=x, k=k, v=None, qw=w, kw=w, pos=i, cs=cs, q_out=x, k_out=k, v_out=None, **kv: lib.qk_norm_rope(  # noqa: E731
+        q, k, v, qw, kw, EPS, pos, cs, False, q_out, k_out, v_out, **kv)
+    for kw, text in ((dict(v=k), "v comes with"), (dict(qw=None), "both weights"), (dict(qw=w[:64]), "weights"), (dict(pos=i.long()), "positions"),
+                     (dict(cs=cs.double()), "cos_sin"), (dict(cs=cs[:, :64]), "cos_sin"), (dict(q_out=k), "q_out"), (dict(k_out=x), "k_out"), (dict(k=k[:2]), "k must"),
+                     (dict(k_out=pool), "k_out"), (dict(slots=i), "pools"), (dict(slots=i.float(), k_out=pool), "slots"), (dict(q=x.float()), "q must"),
+                     (dict(slots=i, k_out=pool, v=k, v_out=pool[:1]), "as many rows")):
+        with pytest.raises(AssertionError, match=text):
+            call(**kw)
+    with pytest.raises(lib.MLAKernelError, match="overlap"):
+        call(q_out=x[:1].expand(3, 4, 128))
+    with pytest.raises(lib.MLAKernelError, match="rotary_dim"):
+        call(cs=cs[:, :12].contiguous())
