@@ -602,6 +602,10 @@ int mla_qk_norm_rope_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h,
     if (x % 8 || x < 0) return mla::api_error(MLA_ERR_INVALID_ARG, "%s: strides must be non-negative multiples of 8", who);
   if ((int64_t)tokens * (q_heads + 2 * kv_heads + 8) * (head_dim / 8) > UINT32_MAX - 256)
     return mla::api_error(MLA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads are more than a launch holds", who, tokens, q_heads + 2 * kv_heads);
+  if ((q_heads > 0 && !mla::rows_apart(tokens, q_out_stride_t, q_heads, q_out_stride_h, head_dim)) ||
+      (kv_heads > 0 && !mla::rows_apart(out_rows, k_out_stride_row, kv_heads, k_out_stride_h, head_dim)) ||
+      (kv_heads > 0 && v != nullptr && !mla::rows_apart(out_rows, v_out_stride_row, kv_heads, v_out_stride_h, head_dim)))
+    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: rows of q_out, k_out or v_out overlap", who);
   auto moved = [&](const void* in, int64_t in_t, int64_t in_h, const void* to, int64_t to_t, int64_t to_h, int32_t heads) {
     return heads > 0 && in == to && ((tokens > 1 && in_t != to_t) || (heads > 1 && in_h != to_h));
   };
@@ -610,10 +614,6 @@ int mla_qk_norm_rope_bf16(const void* q, int64_t q_stride_t, int64_t q_stride_h,
       (v != nullptr && moved(v, v_stride_t, v_stride_h, v_out, v_out_stride_row, v_out_stride_h, kv_heads)) ||
       (slots != nullptr && kv_heads > 0 && (k == k_out || (v != nullptr && v == v_out))))
     return mla::api_error(MLA_ERR_INVALID_ARG, "%s: outputs in the place of inputs take their strides, and no slots", who);
-  if ((q_heads > 0 && !mla::rows_apart(tokens, q_out_stride_t, q_heads, q_out_stride_h, head_dim)) ||
-      (kv_heads > 0 && !mla::rows_apart(out_rows, k_out_stride_row, kv_heads, k_out_stride_h, head_dim)) ||
-      (kv_heads > 0 && v != nullptr && !mla::rows_apart(out_rows, v_out_stride_row, kv_heads, v_out_stride_h, head_dim)))
-    return mla::api_error(MLA_ERR_INVALID_ARG, "%s: rows of q_out, k_out or v_out overlap", who);
   mla::QkNormRopeParams p = {};
   p.q = static_cast<const __bf16*>(q);
   p.k = static_cast<const __bf16*>(k);
