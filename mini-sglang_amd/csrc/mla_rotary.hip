@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRopeParam
         unpack4(*reinterpret_cast<const u32x2*>(w + a), g);
         unpack4(*reinterpret_cast<const u32x2*>(w + b), g + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= inv * g[i];
+        for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * g[i];  // (at most sqrt(D) times the weight: nothing between passes the range)
       }
       if (turns) {
 #pragma unroll

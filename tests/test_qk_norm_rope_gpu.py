@@ -199,3 +199,17 @@ def test_tensors_that_do_not_fit():
         call(q_out=x[:1].expand(3, 4, 128))
     with pytest.raises(lib.MLAKernelError, match="rotary_dim"):
         call(cs=cs[:, :12].contiguous())
+
+
+def test_factors_past_the_range():
+    """1 / norm times the weight may leave fp32's range where the result does not."""
+    gen = torch.Generator().manual_seed(10)
+    T, hq, hk, dim = 9, 3, 1, 128
+    pos, cs = torch.arange(T, dtype=torch.int32), table(dim)
+    for x, w in ((1e18, 1e-30), (1e-9, 3e36)):
+        q, k = randn(gen, T, hq, dim) * x, randn(gen, T, hk, dim) * x
+        qw, kw = randn(gen, dim) * w, randn(gen, dim) * w
+        q_out, k_out = (torch.full(z.shape, NAN, dtype=torch.bfloat16, device=DEV) for z in (q, k))
+        lib.qk_norm_rope(q.to(DEV), k.to(DEV), None, qw.to(DEV), kw.to(DEV), EPS, pos.to(DEV), cs.to(DEV), False, q_out, k_out)
+        near(q_out, *M.norm_rope(q, qw, EPS, pos, cs, False))
+        near(k_out, *M.norm_rope(k, kw, EPS, pos, cs, False))
