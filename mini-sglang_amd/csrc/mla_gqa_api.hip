@@ -77,9 +77,14 @@ bool wide_blocks(int dim, int64_t blocks, int64_t avg, int64_t keys) {
 // Few rows on longer keys are cut in CTAs of 16 rows: a chunk of 100 on 2000, 8 heads and 1, 17 in blocks 21; on 4000 20,
 // 22; on 8000 26, 24. Else up to 32 rows are streamed, bound by reading K and V: 64 chunks of 8 on 1k to 8k, 32 and 8
 // heads, 256, in blocks 277; with 64 and 8 heads (64 rows) 432, 297.
-Choice choose(int dim, int32_t batch, int64_t total_q, int32_t group, int32_t kv_heads, int64_t most, int64_t keys) {
+//
+// A cache of 4 bits costs instructions, as many at head_dim 64 as at 128, rather than bytes. One piece / cut, us, requests of
+// one token of up to n keys (an eighth of it at least), head_dim 128: 8 CTAs 700 6.0 / 9.3, 1000 10.4 / 9.6; 32 900 8.9 / 9.9,
+// 1200 10.8 / 9.9; 64 1200 10.4 / 11.9, 2000 12.9 / 13.0, 3000 20 / 15; 128 2000 15.6 / 16.4, 3000 20.5 / 19.8; 256 2000 17 / 21,
+// 3000 23 / 29; 64: 8 1000 8.9 / 8.8; 32 1200 9.2 / 9.1; 128 2000 13.6 / 14.4, 3000 17.7 / 16.9; 256 3000 19 / 25.
+Choice choose(int dim, int32_t batch, int64_t total_q, int32_t group, int32_t kv_heads, int64_t most, int64_t keys, bool mx4 = false) {
   auto ctas = [&](int rows) { return std::max<int64_t>((total_q * group + rows - 1) / rows, batch) * kv_heads; };
-  auto one_piece = [&](int64_t n) { return 2 * n <= kFit && (keys == 0 || keys * dim <= (512 + 4 * n) * 128); };
+  auto one_piece = [&](int64_t n) { return 2 * n <= kFit && (keys == 0 || (mx4 ? keys <= 850 + 10 * n : keys * dim <= (512 + 4 * n) * 128)); };
   for (int rows : {16, 32}) {
     if (one_piece(ctas(rows))) return {rows, 0, false, true};
     if (most <= rows) break;
@@ -328,7 +333,7 @@ int paged_mx4(const char* who, const void* q, int64_t q_stride_t, int64_t q_stri
   mp.s_page = k.s_page, mp.s_tok = k.s_tok, mp.s_head = k.s_head;
   const int64_t most = (int64_t)max_q * p.group, keys = (int64_t)pt_cols * page_size;
   p.max_keys = (int32_t)(keys < 0x7ff00000 ? keys : 0x7ff00000);
-  Choice choice = choose(dim, batch, total_q, p.group, kv_heads, most, p.max_keys);
+  Choice choice = choose(dim, batch, total_q, p.group, kv_heads, most, p.max_keys, true);
   // Blocks read values that are laid out first, 512 bytes for every 136 of the cache: worth it where many rows read them. 32-row
   // CTAs / laid out, us, 64 and 8 heads of 128: six chunks of 32 on 8000 109 / 147, of 64 181 / 207, of 96 254 / 270, of 128 329 /
   // 288; four of 64 on 2000 64 / 54, on 500 15 / 28; 32 and 8 heads of 64, of 64 on 2000 16 / 16, of 128 51 / 48.
