@@ -219,6 +219,17 @@ def test_decode_split(dim, lens):
     check(*c.run(decode=True), c.ref())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("most", [3200, 3500])
+def test_many_keys_in_one_piece_or_not(dim, most):
+    """Either side of the most keys that as many CTAs as compute units take in one piece."""
+    lens = [most, 1, 33, 0, 255, 256, 257, 2900] + [(37 * i) % 700 for i in range(22)]
+    c = Paged([1] * 30, [n - 1 for n in lens], 16, 8, dim, 16, most)
+    check(*c.run(decode=True), c.ref())
+    c = Paged([2, 1, 5] * 10, lens, 16, 8, dim, 16, most)
+    check(*c.run(), c.ref())
+
+
 def test_decode_without_keys():
     c = Paged([1] * 4, [9, -1, 33, -1], 4, 2, 128, 16, 3)
     out, lse = c.run(decode=True)
