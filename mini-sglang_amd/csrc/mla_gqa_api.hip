@@ -40,6 +40,12 @@ constexpr int kBlock = 128;
 constexpr int kBlocksEnough = 1024;
 constexpr int kOnePieceBlocks = 1024;
 constexpr int kOnePieceMany = 1600;
+// Of a cache of 4 bits joining costs more than reading. One piece / cut, us, of 4 heads a KV head, up to n keys (an eighth at
+// least), head_dim 128: 320 CTAs of 16 rows 1600 21.6 / 25.5, 2400 30 / 28; 512 2400 32 / 37, 3200 40 / 44, 6000 70 / 67; 1024
+// 3200 65 / 71, 6000 113 / 113; 2048 3200 112 / 129; 320 of 32 rows 1600 27 / 49, 3200 46 / 63, 6000 80 / 91; 512 2400 44 / 74,
+// 6000 85 / 118; 1024 2400 90 / 119, 6000 200 / 212. Few long requests among many short ones would wait for the longest: not
+// past 3200 and 6144.
+int64_t one_piece_mx4(int rows, int64_t ctas) { return rows == 16 ? std::min<int64_t>(6 * ctas, 3200) : std::min<int64_t>(12 * ctas, 6144); }
 // Prompts of at least this many tokens on average (head_dim 128), in blocks alone on their compute units: two halves of a
 // block's keys side by side. With / without, us: 3000, 8 heads and 1 46 / 51; 4000, 4 and 1 57 / 65, at head_dim 64 42 / 52;
 // 1000, 16 and 2 23 / 23, at head_dim 64 17 / 18; four of 300, 8 and 2 15 / 12.
@@ -82,16 +88,22 @@ bool wide_blocks(int dim, int64_t blocks, int64_t avg, int64_t keys) {
 // one token of up to n keys (an eighth of it at least), head_dim 128: 8 CTAs 700 6.0 / 9.3, 1000 10.4 / 9.6; 32 900 8.9 / 9.9,
 // 1200 10.8 / 9.9; 64 1200 10.4 / 11.9, 2000 12.9 / 13.0, 3000 20 / 15; 128 2000 15.6 / 16.4, 3000 20.5 / 19.8; 256 2000 17 / 21,
 // 3000 23 / 29; 64: 8 1000 8.9 / 8.8; 32 1200 9.2 / 9.1; 128 2000 13.6 / 14.4, 3000 17.7 / 16.9; 256 3000 19 / 25.
+// Four waves have a tile each by 128 keys, eight by 256: up to 200 keys 8 CTAs 4.8 / 5.0, 256 6.1 / 6.3, up to 400 5.5 / 5.8, 8.5 / 7.4.
+// More than 16 rows, more CTAs than compute units: 16 rows of four waves / 32 of eight, 24 requests of 8 to 48 rows, 8 KV heads,
+// up to 100 6.8 / 13.9, 500 10.6 / 16.1, 1000 16.2 / 17.7; at head_dim 64 5.9 / 11.4, 9.1 / 12.9, 13.7 / 14.5.
+// More CTAs of 16 rows than run at once, 16 / 32 rows of four waves: 64 requests, up to 250 14.2 / 17.3, 750 25.9 / 24.6; 128, up to 250
+// 24.8 / 27.2; requests of 64 rows, which fill 32: 200 of 4 KV heads on 190 42 / 38, at head_dim 64 30 / 25.
 Choice choose(int dim, int32_t batch, int64_t total_q, int32_t group, int32_t kv_heads, int64_t most, int64_t keys, bool mx4 = false) {
   auto ctas = [&](int rows) { return std::max<int64_t>((total_q * group + rows - 1) / rows, batch) * kv_heads; };
   auto one_piece = [&](int64_t n) { return 2 * n <= kFit && (keys == 0 || (mx4 ? keys <= 850 + 10 * n : keys * dim <= (512 + 4 * n) * 128)); };
+  const bool at_once = ctas(16) <= (dim == 64 ? kAtOnce64 : kAtOnce128);
   for (int rows : {16, 32}) {
-    if (one_piece(ctas(rows))) return {rows, 0, false, true};
+    if (one_piece(ctas(rows))) return {rows, 0, false, !mx4 || keys > 256};
     if (most <= rows) break;
+    if (mx4 && (at_once ? keys <= 1000 : keys <= 256 && total_q * group <= 32 * (int64_t)batch)) return {16, 0, false, false};
   }
   const int64_t blocks = (total_q * group + kBlock - 1) / kBlock * kv_heads;
   const int64_t avg = total_q / batch;
-  const bool at_once = ctas(16) <= (dim == 64 ? kAtOnce64 : kAtOnce128);
   if (keys == 0) {
     if (wide_blocks(dim, blocks, avg, avg)) return {2 * kBlock, 0, false, false};
     const bool halves = 2 * ctas(kBlock) <= kFit && avg * 128 >= kAloneTokens * dim;
@@ -102,7 +114,7 @@ Choice choose(int dim, int32_t batch, int64_t total_q, int32_t group, int32_t kv
   if (most <= 32) {
     const int rows = most <= 16 ? 16 : 32;
     if (2 * ctas(rows) <= kFit) return {rows, kFit, true, false};
-    return {rows, keys <= kOnePieceMany ? 0 : kTarget, false, false};
+    return {rows, keys <= (mx4 ? one_piece_mx4(rows, ctas(rows)) : kOnePieceMany) ? 0 : kTarget, false, false};
   }
   if (blocks >= kBlocksEnough || keys <= kOnePieceBlocks) return {wide_blocks(dim, blocks, avg, keys) ? 2 * kBlock : kBlock, 0, false, false};
   return {kBlock, kBlocksTarget, false, false};
@@ -340,7 +352,7 @@ int paged_mx4(const char* who, const void* q, int64_t q_stride_t, int64_t q_stri
   if (choice.rows >= kBlock && most <= kStreamRows) {
     const int64_t ctas = std::max<int64_t>((total_q * (int64_t)p.group + 31) / 32, batch) * kv_heads;
     const bool few = 2 * ctas <= kFit;
-    choice = {32, few ? kFit : p.max_keys <= kOnePieceMany || ctas >= kTarget ? 0 : kTarget, few, false};
+    choice = {32, few ? kFit : p.max_keys <= one_piece_mx4(32, ctas) || ctas >= kTarget ? 0 : kTarget, few, false};
   }
   const bool laid_out = choice.rows >= kBlock;
   const Mx4Space space = mx4_space(most, kv_heads, dim, batch, p.max_keys, total_keys);

@@ -230,6 +230,25 @@ def test_many_keys_in_one_piece_or_not(dim, most):
     check(*c.run(), c.ref())
 
 
+@pytest.mark.parametrize("batch,kv_heads,group,most,extend", [
+    (24, 8, 8, 500, 6),     # more CTAs of 16 rows than compute units, up to 1000 keys
+    (24, 8, 8, 1300, 6),    # and past it
+    (70, 8, 8, 200, 6),     # more than run at once, up to 256 keys
+    (40, 8, 8, 150, 12),    # of fuller requests
+    (20, 2, 4, 120, 3),     # up to 256 keys in one piece: four waves
+    (40, 8, 4, 1700, 1),    # one piece of more CTAs than run at once
+    (40, 8, 4, 2100, 1),    # cut
+    (40, 8, 8, 3000, 5),    # 32 rows, in one piece
+    (40, 8, 8, 4200, 5)])   # cut
+def test_every_choice(batch, kv_heads, group, most, extend):
+    gen = torch.Generator().manual_seed(batch + most)
+    extends = torch.randint(1, extend + 1, (batch,), generator=gen).tolist()
+    prefixes = [most] + torch.randint(0, 200, (batch - 1,), generator=gen).tolist()
+    extends[-1] = extend
+    c = Paged(extends, prefixes, kv_heads * group, kv_heads, 64, 16, most)
+    check(*c.run(), c.ref())
+
+
 def test_decode_without_keys():
     c = Paged([1] * 4, [9, -1, 33, -1], 4, 2, 128, 16, 3)
     out, lse = c.run(decode=True)
