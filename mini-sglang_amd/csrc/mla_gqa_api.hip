@@ -349,11 +349,13 @@ int paged_mx4(const char* who, const void* q, int64_t q_stride_t, int64_t q_stri
   // Blocks read values that are laid out first, 512 bytes for every 136 of the cache: worth it where many rows read them. 32-row
   // CTAs / laid out, us, 64 and 8 heads of 128: six chunks of 32 on 8000 109 / 147, of 64 181 / 207, of 96 254 / 270, of 128 329 /
   // 288; four of 64 on 2000 64 / 54, on 500 15 / 28; 32 and 8 heads of 64, of 64 on 2000 16 / 16, of 128 51 / 48.
-  if (choice.rows >= kBlock && most <= kStreamRows) {
-    const int64_t ctas = std::max<int64_t>((total_q * (int64_t)p.group + 31) / 32, batch) * kv_heads;
-    const bool few = 2 * ctas <= kFit;
+  // Where blocks are too few to fill the chip, more rows as well. 32-row CTAs / laid out, 512 CTAs, on 500, 2000, 4000, 6000 keys: a
+  // chunk of 256, 64 and 8 heads 19 / 25, 41 / 52, 70 / 66, 128 / 82; of 1000, 16 and 2 24 / 43, 43 / 56, 68 / 72, 142 / 88; 320, four of
+  // 160, 16 and 4 16 / 24, 29 / 40, 49 / 51; 960 31 / 28, 63 / 66, 108 / 108. (Up to 256 CTAs choose() streams what is short.)
+  const int64_t ctas = std::max<int64_t>((total_q * (int64_t)p.group + 31) / 32, batch) * kv_heads;
+  const bool few = 2 * ctas <= kFit;
+  if (choice.rows >= kBlock && (most <= kStreamRows || (!few && ctas <= kFit && p.max_keys <= 4096)))
     choice = {32, few ? kFit : p.max_keys <= one_piece_mx4(32, ctas) || ctas >= kTarget ? 0 : kTarget, few, false};
-  }
   const bool laid_out = choice.rows >= kBlock;
   const Mx4Space space = mx4_space(most, kv_heads, dim, batch, p.max_keys, total_keys);
   if (!aligned(workspace, 16) || (workspace_bytes < space.bytes && (workspace != nullptr || choice.target > 0 || laid_out)))

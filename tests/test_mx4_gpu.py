@@ -279,6 +279,17 @@ def test_chunk_long(dim, total):
     check(*c.run(total_keys=total), c.ref())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("extends,prefixes,heads", [
+    ([256], [600], (64, 8)),           # streamed: blocks would be few
+    ([256], [3900], (64, 8)),          # laid out: long
+    ([530], [40], (32, 4)),            # laid out: more
+    ([160, 3, 0, 300], [9, 2000, 30, 0], (16, 4))])
+def test_more_rows_streamed_or_laid_out(extends, prefixes, heads, dim):
+    c = Paged(extends, prefixes, *heads, dim, 16, dim + len(extends))
+    check(*c.run(), c.ref())
+
+
 def test_chunk_many_requests():
     r = random.Random(6)
     extends = [r.choice([0, 1, 2, 17, 70]) for _ in range(140)]
