@@ -436,7 +436,7 @@ int mla_qk_norm_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h,
  * one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (code 0..7, bit 3 the sign) times its block's power of two.
  *   codes   [num_pages, page_size, kv_heads, head_dim / 2]: dims 2 i and 2 i + 1 in the low and high half of byte i
  *   scales  [num_pages, page_size, kv_heads, head_dim / 32]: the exponent plus 127 (254 at most 2^127; a value past bf16's range
- *           is an infinity: attention over such a block may give NaN; mla_mx4_store writes 252 at most); 255: the block is NaN
+ *           is an infinity: rows that attend it may give NaN there; mla_mx4_store writes 252 at most); 255: the block is NaN
  * Strides in bytes: of codes multiples of 16, codes 16-byte aligned; of scales multiples of head_dim / 32, scales aligned by
  * as much; rows contiguous, none over another. page_size a power of two.
  */
@@ -465,7 +465,8 @@ int mla_mx4_load(const mla_mx4_pool *k_pool, const mla_mx4_pool *v_pool, int32_t
 /*
  * mla_gqa_chunk_bf16 and mla_gqa_decode_bf16 over pools of 4 bits, with the same arguments and semantics otherwise: the
  * result is that of the codes' values, fp32 scores and sums, numerators in bf16 for the product with the values. Both pools
- * have the same strides. A NaN block reaches the rows that attend its token only. Requests of more than 512 rows (max_q times
+ * have the same strides. What is not finite reaches the rows that attend its token only, whatever pool rows hold that no
+ * request attends. Requests of more than 512 rows (max_q times
  * q_heads / kv_heads) may have their keys' values laid out in bf16 first: total_keys is at least the sum of seq_lens_k (its
  * keys past that are not those of the pool), and sizes that part of the workspace. mla_gqa_mx4_workspace_bytes: enough for
  * every call with at most max_q queries a request, `batch` requests, max_keys = pt_cols * page_size, and total_keys;

@@ -38,8 +38,12 @@ constexpr float kLag = 6.f;
 // out of the range at the other end, and what tells large ones apart costs every tile 5 %.) The factor is kept beside the
 // reference: a far score's spacing is more than kRoom.
 constexpr float kRoom = 24.f;
-// whether a byte of w is 255
-__device__ __forceinline__ uint32_t any_ff(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+// whether a byte of w is 253 or more
+__device__ __forceinline__ uint32_t any_fd(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x03030303u) & w & 0x80808080u; }
+// bit 2 of the codes of w that a scale of 253 or more puts past bf16's range: 4 and 6 2^126, 2 and more 2^127; all of 255
+__device__ __forceinline__ uint32_t past_range(uint32_t w, uint32_t scale) {
+  return (scale == 255 ? ~0u : scale == 254 ? w : scale == 253 ? w & w << 1 : 0) & 0x44444444u;
+}
 
 // The CTA's item, of which the heads come fastest: CTAs go to the chip's 8 dies in turn, and a round of 8 heads' CTAs takes 8 (block,
 // piece)s with all their heads, a die each, since with small pages the heads of a token share cache lines. 64 requests of 1k
@@ -76,6 +80,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   };
   __shared__ __attribute__((aligned(16))) Own s_own[NW];
   __shared__ float s_m[NW][16], s_l[NW][16], s_room[NW];
+  __shared__ __attribute__((aligned(NW))) uint8_t s_left_out[NW];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   GqaItem it;
@@ -100,9 +105,12 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   const int last_tok = min(E - 1, (it.block * kRows + kRows - 1) / G);
   const int first_limit = P + it.block * kRows / G;  // of the item's first row: no key up to it is masked
   const int k0 = it.piece * C, k1 = min(it.pieces > 1 ? k0 + C : L, P + last_tok + 1);
+  const int whole = min(k1, first_limit + 1);  // tiles that end past it have keys that some row does not attend
+  const int masked0 = k0 + (max(whole - k0, 0) & -kTileKeys);
 
   f32x4 O[NB][kDb];
   float m[NB], l[NB];
+  bool left_out = false;
   u32x4 kr[kLoads], vr[kLoads];
   scale_t sr{};
   // What a tile's addresses come from, read a tile ahead: the page's id (rows past the length in a page are read, and left
@@ -226,36 +234,25 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
         sw[h][i] = tile.vs[16 * h + 4 * g + i];
       }
     if constexpr (decltype(kMasked)::value) {
-      // Blocks of V that are NaN at a key that not every row attends: the product would bring them to rows of weight zero.
-      // They are left out, and added to the rows that attend them.
+      // What is not finite at a key that not every row attends, or past the item's keys (rows that nobody wrote): the product would
+      // bring it to rows of weight zero. It is left out, and added to the rows that attend it at the end.
       uint32_t any = 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) any |= any_ff(sw[h][i]);
+        for (int i = 0; i < 4; ++i) any |= any_fd(sw[h][i]);
       if (__ballot(any != 0) != 0) {
-#pragma unroll
-        for (int nb = 0; nb < kAct; ++nb) {
-          const int lim = min(limit[nb], k1 - 1) - t0 - 4 * g;
-          uint32_t hit = 0;  // bit 7 of byte b: of block b, at a key of the lane's that row a16 attends
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (16 * h + i <= lim) hit |= any_ff(sw[h][i]);
-          const auto a = __builtin_amdgcn_permlane16_swap(hit, hit, false, false);
-          hit = a[0] | a[1];
-          const auto b = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
-          hit = b[0] | b[1];
-          const float add = hit >> (8 * (D == 128 ? g : g >> 1) + 7) & 1 ? __builtin_nanf("") : 0.f;
-#pragma unroll
-          for (int db = 0; db < kDb; ++db) O[nb][db] += add;
-        }
+        uint32_t ours = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if ((sw[h][i] >> 8 * (a16 / kLanesB) & 255) == 255) vw[h][i] = 0, sw[h][i] = 0;
+          for (int i = 0; i < 4; ++i) {
+            if (16 * h + i < k1 - t0 - 4 * g) ours |= any_fd(sw[h][i]);
+            const uint32_t scale = sw[h][i] >> (8 * (a16 / kLanesB)) & 255;
+            vw[h][i] &= (vword_t)~((past_range(vw[h][i], scale) >> 2) * 15);
+            if (scale == 255) sw[h][i] = 0;
+          }
+        left_out = left_out || __ballot(ours != 0) != 0;
       }
     }
     float vs[2][4];
@@ -324,7 +321,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
         step(t0, kMasked, active, roomy);
       }
     };
-    tiles(min(k1, first_limit + 1) - kTileKeys + 1, std::false_type{});
+    tiles(whole - kTileKeys + 1, std::false_type{});
     tiles(k1, std::true_type{});
   };
   if (NB == 1 || it.block * kRows + 16 < E * G) stream(std::integral_constant<int, NB>{}, std::false_type{});
@@ -357,7 +354,10 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
       s_m[wave][a16] = m[nb];
       s_l[wave][a16] = lw;
     }
-    if (lane == 0) s_room[wave] = room;
+    if (lane == 0) {
+      s_room[wave] = room;
+      s_left_out[wave] = left_out;
+    }
     __syncthreads();
     // kTpr threads a row, 4 dims each at a time
     constexpr int kTpr = 4 * NW;
@@ -368,6 +368,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
       mt = fmaxf(mt, s_m[w][row]);
       rt = fmaxf(rt, s_room[w]);
     }
+    const bool add = *reinterpret_cast<const std::conditional_t<NW == 8, uint64_t, uint32_t>*>(s_left_out) != 0;
     float f[NW], lt = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
@@ -384,6 +385,18 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
 #pragma unroll
       for (int w = 0; w < NW; ++w) o += *reinterpret_cast<const f32x4*>(s_own[w].o + row * (D * 4) + ((c + row) % (D / 4)) * 16) * f[w];
       o *= inv;
+      if (__builtin_expect(add, 0)) {  // what the row attends of the masked tiles and their products left out
+        for (int j = masked0; j < min(k1, P + tok + 1); ++j) {
+          const int from = gqa_row(p, it.b, it.r.q0, j), in_page = from & ((1 << p.log2_ps) - 1);
+          const int64_t page = from >> p.log2_ps;
+          const uint32_t scale = vsh[page * mp.s_page + in_page * mp.s_tok + c / 8];
+          if (scale < 253) continue;
+          const uint32_t w = *reinterpret_cast<const uint16_t*>(vh + page * mp.c_page + in_page * mp.c_tok + 2 * c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (past_range(w, scale) >> (4 * i + 2) & 1) o[i] += scale == 255 ? __builtin_nanf("") : w >> (4 * i + 3) & 1 ? -INFINITY : INFINITY;
+        }
+      }
       if (it.slot >= 0) {
         *reinterpret_cast<f32x4*>(p.ws_o + ((int64_t)it.slot * kRows + 16 * nb + row) * D + 4 * c) = o;
       } else {
