@@ -8,8 +8,8 @@
 // A row is D / 8 lanes' (a wave holds 4 rows of 128 or 8 of 64), 8 dims a lane in two chunks of 4 that hold both halves of
 // its pairs: no lane needs another's values but for the sum of squares, which is 3 or 4 DPP steps. Rows of one token are
 // next to each other in a wave, so they share the angles.
-// Bound: HBM for many tokens (8192 of 64 and 8 heads of 128, with V: 340 MB in 63 us, 5.4 TB/s), a launch and three dependent
-// loads for few (64 tokens 3.7 us).
+// Bound: HBM for many tokens (8192 of 64 and 8 heads of 128, with V: 340 MB in 63 us, 5.4 TB/s), a launch and two dependent
+// loads (position, angles) for few (64 tokens 3.7 us).
 #include "mla_common.h"
 #include "mla_device.h"
 
@@ -86,12 +86,28 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRopeParam
     if (r >= rows) continue;
     if (r < heads) {
       if (w != nullptr) {
-        const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+        const float mean = ss * (1.f / D) + p.eps;
+        float inv = rsqrtf(mean);
+        // Squares of 2^64 and more pass fp32's range, those of 2^-63 and less are not exact: the row is taken again, times a power of two.
+        // (All lanes of the row have the same sum. Large values stay themselves for the product, as 1 / norm is at least 2^-128.)
+        if (__builtin_expect(!(mean >= 0x1p-100f && mean <= 3.4028234663852886e38f), 0)) {
+          const bool small = mean < 0x1p-100f;
+          const float by = small ? 0x1p86f : 0x1p-80f;
+          ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float x = f[i] * by;
+            ss = fmaf(x, x, ss);
+            if (small) f[i] = x;
+          }
+          inv = rsqrtf(row_sum<kLanes>(ss) * (1.f / D) + p.eps * by * by);
+          if (!small) inv *= by;
+        }
         float g[8];
         unpack4(*reinterpret_cast<const u32x2*>(w + a), g);
         unpack4(*reinterpret_cast<const u32x2*>(w + b), g + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * g[i];  // (at most sqrt(D) times the weight: nothing between passes the range)
+        for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * g[i];  // (at most sqrt(D) times the weight)
       }
       if (turns) {
 #pragma unroll
