@@ -204,7 +204,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
           top = fmaxf(top, s[h][i]);
         }
       top = wave_max_g(top);
-      if (__ballot(top > m[nb] + kLag) != 0) {
+      if (__ballot(top - m[nb] > kLag) != 0) {  // (a sum of the two would round up where their spacing is more than kLag)
         const float m_new = fmaxf(m[nb], top), f = __builtin_amdgcn_exp2f(m[nb] - m_new);
         m[nb] = m_new;
         l[nb] *= f;
