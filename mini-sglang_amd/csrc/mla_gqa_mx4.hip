@@ -33,11 +33,11 @@ constexpr float kLowest = -3.4028234663852886e38f;
 // Numerators are relative to a reference that a row's largest score (log2 domain) may pass by kLag before it follows: sums are
 // rescaled seldom (16 drafts of 1 to 8 on 1k to 16k, 32 and 8 heads: 40.0 us with 0, 37.3).
 constexpr float kLag = 6.f;
-// A wave whose sums of values did not come out finite takes its keys again with numerators times 2^-kRoom: sums of 2^18 values of
-// the largest size, 6 2^125, stay in fp32's range then, and what is not finite now is the result. (Smaller values would fall
-// out of the range at the other end, and what tells large ones apart costs every tile 5 %.) The factor is kept beside the
-// reference: a far score's spacing is more than kRoom.
-constexpr float kRoom = 24.f;
+// A wave whose sums of values did not come out finite takes its keys again with numerators times 2^-room: numerators of at most
+// 2^kLag of as many keys as the item has, of values of the largest size, 6 2^125, sum up within fp32's range then, and what is not finite
+// now is the result. At least kRoom: up to 2^18 keys. (Smaller values would fall out of the range at the other end, and what tells large
+// ones apart costs every tile 5 %.) The factor is kept beside the reference: a far score's spacing is more than kRoom.
+constexpr int kRoom = 24;
 // whether a byte of w is 253 or more
 __device__ __forceinline__ uint32_t any_fd(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x03030303u) & w & 0x80808080u; }
 // bit 2 of the codes of w that a scale of 253 or more puts past bf16's range: 4 and 6 2^126, 2 and more 2^127; all of 255
@@ -111,6 +111,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   f32x4 O[NB][kDb];
   float m[NB], l[NB];
   bool left_out = false;
+  int room = 0;
   u32x4 kr[kLoads], vr[kLoads];
   scale_t sr{};
   // What a tile's addresses come from, read a tile ahead: the page's id (rows past the length in a page are read, and left
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           e[i] = __builtin_amdgcn_exp2f(s[h][i] - m[nb]);
-          if constexpr (decltype(roomy)::value) e[i] *= 0x1p-24f;
+          if constexpr (decltype(roomy)::value) e[i] *= __uint_as_float((uint32_t)(127 - room) << 23);
           l[nb] += e[i];
         }
         pb[nb][2 * h] = pack_bf16x2(e[0], e[1]);
@@ -326,7 +327,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
   };
   if (NB == 1 || it.block * kRows + 16 < E * G) stream(std::integral_constant<int, NB>{}, std::false_type{});
   else stream(std::integral_constant<int, 1>{}, std::false_type{});
-  float zero = 0.f, room = 0.f;
+  float zero = 0.f;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
 #pragma unroll
       for (int i = 0; i < 4; ++i) zero = fmaf(O[nb][db][i], 0.f, zero);  // finite sums times 0 are 0
   if (__builtin_expect(__ballot(zero != 0.f) != 0, 0)) {
-    room = kRoom;
+    room = max(kRoom, (int)kLag + 32 - __builtin_clz(max(k1 - k0, 1)));
     stream(std::integral_constant<int, NB>{}, std::true_type{});
   }
 
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
       s_l[wave][a16] = lw;
     }
     if (lane == 0) {
-      s_room[wave] = room;
+      s_room[wave] = (float)room;
       s_left_out[wave] = left_out;
     }
     __syncthreads();

@@ -44,3 +44,13 @@ def test_scores_whose_spacing_is_more_than_the_lag(length):
     bound = (length / 128 / 32 + 16) * 2.0 ** -23 + 2.0 ** -8
     assert ((out - want).abs() <= bound * want).all()
     assert ((lse - (1.5 * 2 ** 26 + 8) * math.log(2) - math.log(n)).abs() <= 16).all()  # two steps of fp32 there
+
+
+@pytest.mark.parametrize("length", [1 << 16, 3 << 25])
+def test_more_keys_than_fit_a_fixed_room(length):
+    """Scores of 0 and 6: the higher ones are at the lag's end, numerators 2^6, and up to 786,432 of them a wave."""
+    out, lse, n = run(length, (0, 127, 0, 127), (0, 127, 7, 127))
+    want = 6 * 2.0 ** 125
+    bound = (length / 128 / 32 + 16) * 2.0 ** -23 + 2.0 ** -8
+    assert ((out - want).abs() <= bound * want).all()
+    assert ((lse - math.log(64.0 * n + (length - n))).abs() <= bound + 2.0 ** -18).all()
