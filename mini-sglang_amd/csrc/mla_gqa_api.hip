@@ -405,7 +405,7 @@ int mx4_rows(const char* who, bool load, const mla_mx4_pool* k_pool, const mla_m
   if (!aligned(k, 16) || !aligned(v, 16) || k_stride_t % 8 || k_stride_h % 8 || v_stride_t % 8 || v_stride_h % 8 || k_stride_t < 0 ||
       k_stride_h < 0 || v_stride_t < 0 || v_stride_h < 0)
     return api_error(MLA_ERR_INVALID_ARG, "%s: k and v must be 16-byte aligned, with non-negative strides that are multiples of 8", who);
-  if ((int64_t)rows * 2 * kv_heads * (dim / 8) > UINT32_MAX - 256)
+  if ((int64_t)rows * kv_heads * (dim / 8) > UINT32_MAX - 256)  // a thread for 8 dims of K and of V
     return api_error(MLA_ERR_UNSUPPORTED, "%s: %d rows of %d heads are more than a launch holds", who, rows, kv_heads);
   if (load && (!rows_apart(rows, k_stride_t, kv_heads, k_stride_h, dim) || !rows_apart(rows, v_stride_t, kv_heads, v_stride_h, dim)))
     return api_error(MLA_ERR_INVALID_ARG, "%s: rows of k or v overlap", who);
