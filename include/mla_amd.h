@@ -438,7 +438,7 @@ int mla_qk_norm_rope_bf16(const void *q, int64_t q_stride_t, int64_t q_stride_h,
  *   scales  [num_pages, page_size, kv_heads, head_dim / 32]: the exponent plus 127 (254 at most 2^127; a value past bf16's range
  *           is an infinity: rows that attend it may give NaN there; mla_mx4_store writes 252 at most); 255: the block is NaN
  * Strides in bytes: of codes multiples of 16, codes 16-byte aligned; of scales multiples of head_dim / 32, scales aligned by
- * as much; rows contiguous, none over another. page_size a power of two.
+ * as much; rows contiguous, none over another (mla_mx4_store refuses such). page_size a power of two.
  */
 typedef struct {
   void *codes, *scales;

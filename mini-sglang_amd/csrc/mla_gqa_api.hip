@@ -135,6 +135,22 @@ bool rows_apart(int64_t outer, int64_t outer_stride, int64_t inner, int64_t inne
   return by_outer || by_inner;
 }
 
+// The same of a pool's rows, by dimensions of n and a stride each in any order: each lies outside all that those of smaller strides hold.
+struct Steps {
+  int64_t n, stride;
+};
+bool rows_apart(Steps a, Steps b, Steps c, int64_t width) {
+  Steps x[] = {a, b, c};
+  std::sort(x, x + 3, [](const Steps& p, const Steps& q) { return p.stride < q.stride; });
+  __int128 held = width;
+  for (const Steps& s : x) {
+    if (s.n <= 1) continue;
+    if (s.stride < held) return false;
+    held += (__int128)(s.n - 1) * s.stride;
+  }
+  return true;
+}
+
 int check_heads(const char* who, int32_t q_heads, int32_t kv_heads, int32_t dim) {
   if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0)
     return api_error(MLA_ERR_INVALID_ARG, "%s: %d query heads are no multiple of %d KV heads", who, q_heads, kv_heads);
@@ -407,6 +423,10 @@ int mx4_rows(const char* who, bool load, const mla_mx4_pool* k_pool, const mla_m
     return api_error(MLA_ERR_INVALID_ARG, "%s: k and v must be 16-byte aligned, with non-negative strides that are multiples of 8", who);
   if ((int64_t)rows * kv_heads * (dim / 8) > UINT32_MAX - 256)  // a thread for 8 dims of K and of V
     return api_error(MLA_ERR_UNSUPPORTED, "%s: %d rows of %d heads are more than a launch holds", who, rows, kv_heads);
+  for (const Mx4View* x : {&p.k_pool, &p.v_pool})
+    if (!load && (!rows_apart({num_pages, x->c_page}, {page_size, x->c_tok}, {kv_heads, x->c_head}, dim / 2) ||
+                  !rows_apart({num_pages, x->s_page}, {page_size, x->s_tok}, {kv_heads, x->s_head}, dim / 32)))
+      return api_error(MLA_ERR_INVALID_ARG, "%s: rows of a pool lie over one another", who);
   if (load && (!rows_apart(rows, k_stride_t, kv_heads, k_stride_h, dim) || !rows_apart(rows, v_stride_t, kv_heads, v_stride_h, dim)))
     return api_error(MLA_ERR_INVALID_ARG, "%s: rows of k or v overlap", who);
   if (load) {

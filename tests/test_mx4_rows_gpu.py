@@ -1,6 +1,8 @@
-"""Rows into the 4-bit cache: as many as a launch holds."""
+"""Rows into the 4-bit cache: as many as a launch holds, and pools of every order of their dimensions."""
 
 from __future__ import annotations
+
+import itertools
 
 import pytest
 import torch
@@ -37,3 +39,26 @@ def test_store_of_more_than_two_to_the_31_pieces():
         rest = torch.ones(2 * ps, dtype=torch.bool)
         rest[mine] = False
         assert (codes[rest] == 0x5A).all() and (scales[rest] == 0x5A).all()
+
+
+@pytest.mark.parametrize("order", itertools.permutations(range(3)))
+@pytest.mark.parametrize("room", [0, 1])
+def test_pools_of_every_order(order, room):
+    """Pages, tokens and heads with strides in any order, with and without room between them; codes and scales not alike."""
+    gen = torch.Generator().manual_seed(2)
+    pages, ps, heads, dim = 3, 8, 2, 64
+
+    def part(width, order):
+        sizes = [(pages, ps, heads)[i] + room for i in order]
+        made = torch.full((*sizes, width), 0x5A, dtype=torch.uint8, device=DEV)
+        return made.permute(*(order.index(i) for i in range(3)), 3)[:pages, :ps, :heads]
+
+    pools = [lib.MX4Pool(part(dim // 2, order), part(dim // 32, o)) for o in (order[::-1], order)]
+    slots = torch.randperm(pages * ps, generator=gen)
+    x, y = (torch.randn((pages * ps, heads, dim), generator=gen).to(torch.bfloat16) for _ in "kv")
+    lib.mx4_store(*pools, slots.to(DEV), x.to(DEV), y.to(DEV))
+    for p, z in zip(pools, (x, y)):
+        codes, scales = M.rounded(z)
+        assert torch.equal(p.codes.cpu().flatten(0, 1)[slots], codes) and torch.equal(p.scales.cpu().flatten(0, 1)[slots], scales)
+    k, v = lib.mx4_load(*pools, slots.to(DEV))
+    assert torch.equal(k.cpu().double(), M.values(*M.rounded(x))) and torch.equal(v.cpu().double(), M.values(*M.rounded(y)))
