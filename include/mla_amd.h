@@ -466,11 +466,11 @@ int mla_mx4_load(const mla_mx4_pool *k_pool, const mla_mx4_pool *v_pool, int32_t
  * mla_gqa_chunk_bf16 and mla_gqa_decode_bf16 over pools of 4 bits, with the same arguments and semantics otherwise: the
  * result is that of the codes' values, fp32 scores and sums, numerators in bf16 for the product with the values. Both pools
  * have the same strides. What is not finite reaches the rows that attend its token only, whatever pool rows hold that no
- * request attends. Requests of more than 512 rows (max_q times
- * q_heads / kv_heads) may have their keys' values laid out in bf16 first: total_keys is at least the sum of seq_lens_k (its
- * keys past that are not those of the pool), and sizes that part of the workspace. mla_gqa_mx4_workspace_bytes: enough for
- * every call with at most max_q queries a request, `batch` requests, max_keys = pt_cols * page_size, and total_keys;
- * NULL with 0 bytes will do where none is used.
+ * request attends. Requests of more than 512 rows (max_q times q_heads / kv_heads) may have their keys' values laid out in
+ * bf16 first: total_keys is at least the sum of seq_lens_k (its keys past that are not those of the pool), and sizes that
+ * part of the workspace. mla_gqa_mx4_workspace_bytes: enough for every call with at most max_q queries a request, `batch`
+ * requests, max_keys = pt_cols * page_size, and total_keys; a call that lays nothing out takes as many as with max_keys and
+ * total_keys 0, and NULL with 0 bytes will do where none is used.
  */
 int mla_gqa_mx4_workspace_bytes(int32_t max_q, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t batch,
                                 int64_t max_keys, int64_t total_keys, int64_t *bytes);

@@ -411,11 +411,13 @@ PyObject* gqa_paged_mx4(PyObject*, PyObject* const* a, Py_ssize_t n) {
       require(gpu_of(w) == x.device && w.is_contiguous(), "the workspace is one block on q's GPU");
       return PyLong_FromLong(call(w.data_ptr(), (int64_t)w.nbytes()));
     }
-    // without one first, as gqa_paged
+    // without one first, as gqa_paged; then with one for partial results alone, and last with room for the keys' values
     long rc = call(nullptr, 0);
-    if (rc == MLA_ERR_INVALID_ARG) {
+    for (const bool values : {false, true}) {
+      if (rc != MLA_ERR_INVALID_ARG) break;
       int64_t bytes = 0;
-      if ((rc = g.mx4_workspace_bytes(max_q, (int32_t)x.Hq, (int32_t)k.heads, (int32_t)x.D, (int32_t)B, max_keys, total, &bytes))) return PyLong_FromLong(rc);
+      if ((rc = g.mx4_workspace_bytes(max_q, (int32_t)x.Hq, (int32_t)k.heads, (int32_t)x.D, (int32_t)B, values ? max_keys : 0, values ? total : 0, &bytes)))
+        return PyLong_FromLong(rc);
       if (!allocates_for(a[14], stream, x.device)) return PyLong_FromLong(kOtherStream);
       const at::Tensor made = at::empty({bytes}, x.q.options().dtype(at::kByte));
       rc = call(made.data_ptr(), bytes);

@@ -291,10 +291,10 @@ int paged(const char* who, const void* q, int64_t q_stride_t, int64_t q_stride_h
 
 // ---- over a cache of 4 bits
 
-// Rows of a request that are streamed from the codes at most.
+// Requests of up to this many rows are streamed from the codes, never laid out.
 constexpr int64_t kStreamRows = 512;
-// Bytes of a workspace: partial results, and for requests of more rows than that their keys' values in pages of 64 and the
-// page table of these.
+// Bytes of a workspace: partial results (`split`), and for calls with requests of more rows, which may have them laid out, their keys'
+// values in pages of 64 and the page table of these.
 struct Mx4Space {
   int64_t split, table, rows, cols, bytes;
 };
@@ -374,9 +374,10 @@ int paged_mx4(const char* who, const void* q, int64_t q_stride_t, int64_t q_stri
     choice = {32, few ? kFit : p.max_keys <= one_piece_mx4(32, ctas) || ctas >= kTarget ? 0 : kTarget, few, false};
   const bool laid_out = choice.rows >= kBlock;
   const Mx4Space space = mx4_space(most, kv_heads, dim, batch, p.max_keys, total_keys);
-  if (!aligned(workspace, 16) || (workspace_bytes < space.bytes && (workspace != nullptr || choice.target > 0 || laid_out)))
+  const int64_t need = laid_out ? space.bytes : space.split;
+  if (!aligned(workspace, 16) || (workspace_bytes < need && (workspace != nullptr || choice.target > 0 || laid_out)))
     return api_error(MLA_ERR_INVALID_ARG, "%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
-                     (long long)space.bytes, (long long)workspace_bytes);
+                     (long long)need, (long long)workspace_bytes);
   set_pages(p, num_pages, page_size, page_table, pt_stride, cu_seqlens_q, seq_lens_k, max_q);
   if (workspace != nullptr) {
     p.ws_o = static_cast<float*>(workspace);

@@ -1,6 +1,6 @@
 // Grouped-head attention over a cache of 4 bits (mla_mx4.h), with the items, pieces and joining of mla_gqa.h: single tokens
-// and chunks of up to 512 rows read the codes here; longer ones have their keys' values laid out first (mx4_pages_kernel), for
-// the bf16 kernels.
+// and chunks of up to 512 rows read the codes here, and longer ones where their blocks would be too few to fill the chip; others have
+// their keys' values laid out first (mx4_pages_kernel), for the bf16 kernels.
 //
 // As mla_gqa_stream.hip, one CTA per (request, rows, KV head, piece of the keys), whose waves take tiles of 32 keys in turn,
 // load a tile ahead and share nothing until the end. A tile is 4.3 KB (head_dim 128): codes go through the wave's
