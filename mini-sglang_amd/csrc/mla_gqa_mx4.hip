@@ -12,7 +12,7 @@
 //            8 n + m in row n: lane (row a16, g) ends up with the 32 dims 32 g + 8 i + m.
 // At head_dim 64 half as many of each.
 // Bound: with 16 rows, reading (64 requests of 1k to 8k tokens, 64 and 8 heads of 128: 344 MB in 66 us, 5.2 TB/s; its loads alone, the
-// rest left out, take 63); vector instructions, some 150 a tile, and the matrix instructions, which hardly overlap with them
+// rest left out, take 63, and a plain stream 49 with one CTA a compute unit, 54 to 77 with more); vector instructions, some 150 a tile, and the matrix instructions, which hardly overlap with them
 // (measured: 1.8 ns and 7 ns each a SIMD, 9.5 for one of the latter with two of the former), take 45 us of it, hidden. With 32
 // rows they are the bound: 16 chunks of 1 to 8 tokens on 1k to 16k, 32 and 8 heads, 154 MB in 35 us. Below some 20 MB: dependent
 // loads (lengths, page, tile) and the joining's launch: one request of 1500, 5.7 us and 4.2.
@@ -187,7 +187,10 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_mx4_kernel(const GqaMx4Params 
         for (int nb = 0; nb < kAct; ++nb)
           sc[nb][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kc, qf[nb][s], s == 0 ? f32x4{} : sc[nb][h], 0, 0, 0);
       }
-    u32x4 pb[kAct];  // numerators of a row, in pairs of keys
+    // Numerators of a row, in pairs of keys, in bf16 as the matrix instruction takes them (their sum l is of the unrounded ones): each is
+    // off by 2^-8 at most, independently, and results by 1.2 to 1.4 times what their own rounding costs. A second product with what
+    // the rounding leaves out would be twice the matrix instructions.
+    u32x4 pb[kAct];
 #pragma unroll
     for (int nb = 0; nb < kAct; ++nb) {
       // the scaled scores are rounded before their maximum is taken from them: the largest numerator is 1 to 2^kLag at any size

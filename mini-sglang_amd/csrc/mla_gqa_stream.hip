@@ -232,7 +232,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gqa_stream_kernel(const GqaParams 
 // Partial results of requests in pieces, joined: lse = log2 sum_i 2^lse_i, out = sum_i 2^(lse_i - lse) o_i, with lse_i of two
 // floats each (gqa_lse).
 // One CTA per (query, query head): its waves take every fourth piece (kWaves 4), or a wave per row (kWaves 1). Weights are
-// times 2^-12, exactly: up to 2^12 pieces of the largest values sum up within fp32's range.
+// times 2^-12: up to 2^12 pieces of the largest values sum up within fp32's range. (Exact but for products below its normal
+// range: results of 2^-126 are as far off as larger ones, measured over 131,072 keys.)
 // Bound: dependent loads (lengths, the pieces' lse, their rows). 4.3 us for 32 rows, 7 for 4096 rows of 64 requests.
 template <int D, int kRows, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void gqa_merge_kernel(const GqaParams p) {

@@ -756,7 +756,7 @@ def gqa_chunk_mx4(q, k_pool: MX4Pool, v_pool: MX4Pool, page_table, cu_seqlens_q,
                   lse=None, workspace=None, total_keys: int | None = None, stream=None) -> None:
     """``gqa_chunk`` over pools of 4 bits. ``total_keys``: at least the sum of ``seq_lens_k`` (the host's; None: all that the page
     table can hold), which bounds the memory where chunks of more than 512 rows (tokens times ``Hq // Hkv``) have their keys'
-    values laid out in bf16. ``workspace``: uint8, of ``gqa_mx4_workspace_bytes``, or None."""
+    values laid out in bf16: 4 D bytes for each KV head and key, so a wide table needs it. ``workspace``: uint8, of ``gqa_mx4_workspace_bytes``, or None."""
     assert cu_seqlens_q is not None, "cu_seqlens_q is [B + 1]"
     call = load_binding().gqa_paged_mx4
     args = (q, *k_pool, *v_pool, page_table, cu_seqlens_q, seq_lens_k, max_seqlen_q, scale, out, lse, workspace, total_keys, stream)
