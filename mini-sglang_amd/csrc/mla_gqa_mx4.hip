@@ -12,10 +12,11 @@
 //            8 n + m in row n: lane (row a16, g) ends up with the 32 dims 32 g + 8 i + m.
 // At head_dim 64 half as many of each.
 // Bound: with 16 rows, reading (64 requests of 1k to 8k tokens, 64 and 8 heads of 128: 344 MB in 66 us, 5.2 TB/s; its loads alone, the
-// rest left out, take 63, and a plain stream 49 with one CTA a compute unit, 54 to 77 with more); vector instructions, some 150 a tile, and the matrix instructions, which hardly overlap with them
-// (measured: 1.8 ns and 7 ns each a SIMD, 9.5 for one of the latter with two of the former), take 45 us of it, hidden. With 32
-// rows they are the bound: 16 chunks of 1 to 8 tokens on 1k to 16k, 32 and 8 heads, 154 MB in 35 us. Below some 20 MB: dependent
-// loads (lengths, page, tile) and the joining's launch: one request of 1500, 5.7 us and 4.2.
+// rest left out, take 63, and a plain stream 49 with one CTA a compute unit, 54 to 77 with more); vector instructions, some 150 a
+// tile, and the matrix instructions, which hardly overlap with them (measured: 1.8 ns and 7 ns each a SIMD, 9.5 for one of the
+// latter with two of the former), take 45 us of it, hidden. With 32 rows they are the bound: 16 chunks of 1 to 8 tokens on 1k to
+// 16k, 32 and 8 heads, 154 MB in 35 us. Below some 20 MB: dependent loads (lengths, page, tile) and the joining's launch: one
+// request of 1500, 5.9 us and 4.2.
 // What did not pay, us for the 64 requests: two tiles ahead in registers 77 for 75, in a ring of LDS tiles that loads fill by
 // themselves 66 for 66 at any depth; more waves (128 registers) 72 for 66; pairs of dims in place of pairs of keys, without the
 // swaps and with twice the matrix instructions, 66 for 66; equal shares of the batch's keys for as many CTAs as run at once

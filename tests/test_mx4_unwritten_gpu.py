@@ -59,15 +59,12 @@ def test_rows_that_nobody_attends_of_values_laid_out(page_size):
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("page_size", [32, 64])
 def test_new_pool_in_used_memory(dim, page_size):
-    """A pool made where the allocator had other bytes, a prompt stored to it, and its next token."""
+    """A pool of memory with other bytes, a prompt stored to it, and its next token."""
     gen = torch.Generator().manual_seed(page_size)
     L, hq, hk = 75, 8, 2
     pages = -(-L // page_size)
-    used = torch.full((4 * pages * page_size * hk * dim,), 253, dtype=torch.uint8, device=DEV)
-    torch.cuda.synchronize()
-    del used
     k, v = lib.mx4_pool(pages, page_size, hk, dim, DEV), lib.mx4_pool(pages, page_size, hk, dim, DEV)
-    for p in (k, v):  # whatever the allocator gave
+    for p in (k, v):  # as the allocator may give it
         p.codes.fill_(0x77), p.scales.fill_(253)
     x, y, q = randn(gen, L, hk, dim), randn(gen, L, hk, dim), randn(gen, 1, hq, dim)
     lib.mx4_store(k, v, torch.arange(L, device=DEV), x.to(DEV), y.to(DEV))
